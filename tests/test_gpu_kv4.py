@@ -1,0 +1,342 @@
+"""Kernels of the 4-bit KV cache against plain implementations in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import kv4_ref
+from xixi_vllm_b200.ops import cpu_ref, kv4
+from xixi_vllm_b200.runtime.staging import AttnBatch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+D = 128
+HALF_BF16 = 2.0 ** -8          # largest relative error of one rounding to bf16
+
+
+def _ops():
+    from xixi_vllm_b200.ops import dispatch
+    return dispatch
+
+
+def _cuda():
+    from xixi_vllm_b200.ops import cuda
+    return cuda
+
+
+def _empty(nb, hkv, bs):
+    return [torch.zeros(nb, hkv, bs, kv4.row_bytes(D), dtype=torch.uint8, device=DEV) for _ in range(2)]
+
+
+def _random(nb, hkv, bs, seed, scale=1.0):
+    """A cache whose every row holds quantised normal values (made on the CPU by the oracle)."""
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for _ in range(2):
+        c = torch.zeros(nb, hkv, bs, kv4.row_bytes(D), dtype=torch.uint8)
+        kv4.write_rows(c, torch.arange(nb * bs), torch.randn(nb * bs, hkv, D, generator=g) * scale)
+        out.append(c.to(DEV))
+    return out
+
+
+# ---- writing and reading ----
+
+def _write_case(T, hq, hkv, bs, seed, skip=(), parts=0):
+    g = torch.Generator().manual_seed(seed)
+    nb = -(-T // bs) + 2
+    qkv = (torch.randn(T, (hq + 2 * hkv) * D, generator=g) * torch.exp(torch.randn(1, (hq + 2 * hkv) * D, generator=g))).bfloat16()
+    qw, kw = (torch.exp(0.3 * torch.randn(D, generator=g)).bfloat16() for _ in range(2))
+    cs = cpu_ref.build_cos_sin_cache(D, 5000, 1e6)
+    pos = torch.randint(0, 5000, (T,), generator=g, dtype=torch.int32)
+    slots = torch.randperm(nb * bs, generator=g)[:T].to(torch.int32)
+    for i in skip:
+        slots[i] = -1
+    return nb, qkv, qw, kw, cs, pos, slots
+
+
+def _rotated(x, w, cs, pos, eps):
+    x = x.double().numpy()
+    x = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w.double().numpy()
+    a, b = x[..., :D // 2], x[..., D // 2:]
+    c, s = np.split(cs[pos.long()].double().numpy()[:, None], 2, -1)
+    return np.concatenate([a * c - b * s, b * c + a * s], -1)
+
+
+@pytest.mark.parametrize("T,hq,hkv,bs,skip", [(1, 16, 8, 16, ()), (2, 3, 1, 16, (0,)), (33, 32, 8, 48, (0, 5, 32)),
+                                              (130, 40, 8, 128, ()), (7, 0, 2, 16, ())])
+def test_write_then_read(T, hq, hkv, bs, skip):
+    nb, qkv, qw, kw, cs, pos, slots = _write_case(T, hq, hkv, bs, T, skip)
+    k, v = _empty(nb, hkv, bs)
+    q = _ops().qk_norm_rope_cache(qkv.to(DEV), qw.to(DEV), kw.to(DEV), 1e-6, cs.to(DEV), pos.to(DEV), slots.to(DEV), k, v,
+                                  hq, hkv, D)
+    _cuda().check_status()
+    x = qkv.view(T, hq + 2 * hkv, D)
+    live = np.array([s >= 0 for s in slots.tolist()])
+    # V: the kernel and the definition do the same exact or correctly rounded steps, so the levels are equal
+    want_v = kv4_ref.levels(x[:, hq + hkv:].double().numpy()) * live[:, None, None]
+    got_v, _ = kv4_ref.rows(v, slots.tolist())
+    np.testing.assert_allclose(got_v, want_v, rtol=1e-12)
+    # K: 64-bit norm and rotation, rounded to fp32 and bf16 alike
+    want_k = kv4_ref.levels(kv4_ref.to_bf16(_rotated(x[:, hq:hq + hkv], kw, cs, pos, 1e-6))) * live[:, None, None]
+    got_k, _ = kv4_ref.rows(k, slots.tolist())
+    np.testing.assert_allclose(got_k, want_k, rtol=1e-12)
+    # q: fp32 (a dozen roundings of 2^-24 on terms no larger than the pair's norm), then one rounding to bf16
+    if hq:
+        want_q = _rotated(x[:, :hq], qw, cs, pos, 1e-6)
+        norm = np.sqrt(want_q ** 2 + np.roll(want_q, D // 2, -1) ** 2)
+        assert (np.abs(q.double().cpu().numpy().reshape(T, hq, D) - want_q) <= HALF_BF16 * np.abs(want_q) + 2.0 ** -19 * norm + 1e-30).all()
+    kk, vv = _ops().read_cache(k, v, slots.to(DEV), D)
+    _cuda().check_status()
+    for got, want in ((kk, got_k), (vv, got_v)):
+        assert got.shape == (T, hkv, D)
+        assert (np.abs(got.double().cpu().numpy() - want) <= HALF_BF16 * np.abs(want) * (1 + 2.0 ** -14)).all()
+    # nothing else was written
+    used = torch.zeros(nb * bs, dtype=torch.bool)
+    used[slots[slots >= 0].long()] = True
+    rest = [s for s in range(nb * bs) if not used[s]]
+    for c in (k, v):
+        vals, swing = kv4_ref.rows(c, rest)
+        assert not vals.any() and not swing.any()
+
+
+def test_write_sums_split_k_planes():
+    T, hq, hkv, bs = 5, 4, 2, 16
+    nb, qkv, qw, kw, cs, pos, slots = _write_case(T, hq, hkv, bs, 3)
+    cuda = _cuda()
+    planes = torch.randn(3, *qkv.shape, generator=torch.Generator().manual_seed(4)).to(DEV)
+    part = cuda.SplitKPartial(planes.view(torch.uint8).flatten(), 3, *qkv.shape)
+    # ((p0 + p1) + p2) in fp32, then bf16: the kernel's order
+    whole = ((planes[0] + planes[1]) + planes[2]).bfloat16()
+    a, b = _empty(nb, hkv, bs), _empty(nb, hkv, bs)
+    args = (qw.to(DEV), kw.to(DEV), 1e-6, cs.to(DEV), pos.to(DEV), slots.to(DEV))
+    qa = cuda.qk_norm_rope_cache(part, *args, *a, hq, hkv, D)
+    qb = cuda.qk_norm_rope_cache(whole, *args, *b, hq, hkv, D)
+    cuda.check_status()
+    assert torch.equal(qa, qb) and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_write_matches_the_cpu_backend_byte_for_byte():
+    T, hq, hkv, bs = 70, 8, 4, 32
+    nb, qkv, qw, kw, cs, pos, slots = _write_case(T, hq, hkv, bs, 9, (3,))
+    qkv[11, 5] = float("nan")
+    qkv[12, (hq + hkv) * D + 20] = float("inf")                # one group of a V row
+    qkv[13] = 0.0                                              # constant groups
+    qkv[14, (hq + hkv) * D:] = 1.5
+    gpu = _empty(nb, hkv, bs)
+    cpu = [c.cpu() for c in gpu]
+    _ops().qk_norm_rope_cache(qkv.to(DEV), qw.to(DEV), kw.to(DEV), 1e-6, cs.to(DEV), pos.to(DEV), slots.to(DEV), *gpu, hq, hkv, D)
+    cpu_ref.qk_norm_rope_cache(qkv, qw, kw, 1e-6, cs, pos, slots, *cpu, hq, hkv, D)
+    _cuda().check_status()
+    live = slots[slots >= 0].long()
+    for a, b in zip(gpu, cpu):
+        torch.testing.assert_close(kv4.read_rows(a.cpu(), live), kv4.read_rows(b, live), rtol=0, atol=0, equal_nan=True)
+
+
+def test_bad_slots_and_positions_are_reported_and_not_followed():
+    T, hq, hkv, bs = 4, 2, 1, 16
+    nb, qkv, qw, kw, cs, pos, slots = _write_case(T, hq, hkv, bs, 5)
+    k, v = _empty(nb, hkv, bs)
+    args = (qkv.to(DEV), qw.to(DEV), kw.to(DEV), 1e-6, cs.to(DEV))
+    slots[1] = nb * bs
+    _ops().qk_norm_rope_cache(*args, pos.to(DEV), slots.to(DEV), k, v, hq, hkv, D)
+    with pytest.raises(RuntimeError, match="status 5"):
+        _cuda().check_status()
+    kk, _ = _ops().read_cache(k, v, slots.to(DEV), D)
+    assert not kk[1].any() and bool(kk[0].any())
+    with pytest.raises(RuntimeError, match="status 5"):
+        _cuda().check_status()
+    pos[2] = 5000
+    slots[1] = -1
+    _ops().qk_norm_rope_cache(*args, pos.to(DEV), slots.to(DEV), k, v, hq, hkv, D)
+    with pytest.raises(RuntimeError, match="status 5"):
+        _cuda().check_status()
+
+
+# ---- attention ----
+
+def _attend(q_lens, kv_lens, hq, hkv, bs=16, n_decode=0, seed=0, poison=False, q_scale=1.0, extra_pages=1, v_scale=1.0):
+    B = len(kv_lens)
+    maxb = max(1, max(-(-n // bs) for n in kv_lens)) + extra_pages
+    nb = sum(-(-n // bs) for n in kv_lens) + 2
+    g = torch.Generator().manual_seed(seed + 100)
+    perm = torch.randperm(nb, generator=g).tolist()
+    table = torch.zeros(B, maxb, dtype=torch.int32)
+    for b, n in enumerate(kv_lens):
+        for i in range(-(-n // bs)):
+            table[b, i] = perm.pop()
+    k, v = _random(nb, hkv, bs, seed, v_scale)
+    if poison:                     # parameters of every row that no sequence holds are NaN
+        live = torch.zeros(nb * bs, dtype=torch.bool)
+        for b, n in enumerate(kv_lens):
+            for t in range(n):
+                live[int(table[b, t // bs]) * bs + t % bs] = True
+        dead = (~live).nonzero().flatten()
+        if len(dead):
+            for c in (k, v):
+                host = c.cpu()
+                kv4.write_rows(host, dead, torch.full((len(dead), hkv, D), float("nan")))
+                c.copy_(host)
+    T = sum(q_lens)
+    q = (torch.randn(T, hq * D, generator=g) * q_scale).bfloat16()
+    cu = torch.tensor([0] + list(np.cumsum(q_lens)), dtype=torch.int32)
+    scale = D ** -0.5
+    attn = AttnBatch(cu_q=cu.to(DEV), kv_lens=torch.tensor(kv_lens, dtype=torch.int32, device=DEV), block_tables=table.to(DEV),
+                     num_seqs=B, num_decode=n_decode, max_q_len=max(q_lens), max_kv_len=max(kv_lens), num_tokens=T)
+    out = _ops().paged_attention(q.to(DEV), k, v, attn, scale, hq, hkv, D)
+    torch.cuda.synchronize()
+    _cuda().check_status()
+    ref, mag, swing, qk = kv4_ref.attention(q, k, v, q_lens, kv_lens, table, scale, hq)
+    got = out.double().cpu().numpy().reshape(T, hq, D)
+    qk = qk[..., None]
+    # Decode rows: the output and P s_g are each rounded to bf16 once; scores are fp32 sums of at most 2 * 64 products
+    # no larger than 17 times those of q and k (codes biased by 136), so 2^-24 * 17 * 8 bounds their relative error.
+    tol = HALF_BF16 * (np.abs(ref) + swing) + 2 * (2.0 ** -24 * 17 * 8 * qk + 2.0 ** -20) * mag
+    # Chunks: K, V and P are rounded to bf16 (K: the score moves by 2^-8 of sum |q| |k|, a probability by twice that).
+    chunk = HALF_BF16 * (np.abs(ref) + 2 * mag) * (1 + HALF_BF16) + (np.exp(2 * HALF_BF16 * qk) - 1) * mag + 2.0 ** -18 * mag
+    tol[n_decode:] = chunk[n_decode:]
+    worst = (np.abs(got - ref) - tol).max()
+    assert worst <= 0, worst
+    if ref.any():
+        rel = np.linalg.norm(got - ref) / np.linalg.norm(ref)
+        assert rel <= HALF_BF16, rel
+    return out
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 8), (16, 8), (3, 1), (32, 8), (5, 1), (8, 1), (9, 1), (32, 2)])
+def test_decode_groups(hq, hkv):
+    _attend([1] * 5, [1, 15, 16, 17, 150], hq, hkv, n_decode=5, seed=hq)
+
+
+@pytest.mark.parametrize("bs", [16, 48, 128])
+def test_decode_page_sizes_and_empty_rows(bs):
+    _attend([1] * 6, [0, 1, bs, bs + 1, 2 * bs - 1, 0], 8, 2, bs=bs, n_decode=6, seed=bs)
+
+
+def test_decode_all_rows_empty():
+    assert not _attend([1] * 2, [0, 0], 4, 2, n_decode=2).any()
+
+
+def test_decode_many_splits_and_long_tables():
+    _attend([1, 1], [1100, 513], 8, 2, n_decode=2, extra_pages=2000)       # most splits see nothing
+
+
+def test_decode_growing_maxima():
+    _attend([1, 1], [400, 700], 8, 1, n_decode=2, q_scale=8.0, seed=4)
+
+
+def test_rows_beyond_the_sequence_may_hold_nan():
+    _attend([1, 1, 1, 20, 70], [1, 15, 33, 20, 100], 8, 2, n_decode=3, poison=True)
+    _attend([1, 65], [47, 130], 4, 2, bs=48, n_decode=1, poison=True)
+
+
+def test_nan_inside_a_sequence_reaches_its_rows_only():
+    k, v = _random(4, 1, 16, 1)
+    host = k.cpu()
+    kv4.write_rows(host, torch.arange(16), torch.full((16, 1, D), float("nan")))
+    k.copy_(host)
+    q = torch.ones(2, 2 * D, device=DEV).bfloat16()
+    i32 = dict(dtype=torch.int32, device=DEV)
+    attn = AttnBatch(cu_q=torch.tensor([0, 1, 2], **i32), kv_lens=torch.tensor([16, 20], **i32),
+                     block_tables=torch.tensor([[0, 0], [1, 2]], **i32), num_seqs=2, num_decode=2, max_q_len=1,
+                     max_kv_len=20, num_tokens=2)
+    out = _ops().paged_attention(q, k, v, attn, 0.1, 2, 1, D)
+    assert bool(out[0].isnan().all()) and bool(out[1].isfinite().all())
+
+
+@pytest.mark.parametrize("hq,hkv,bs", [(8, 2, 16), (3, 1, 48), (4, 4, 64)])
+def test_chunks(hq, hkv, bs):
+    _attend([1, 15, 64, 65, 33], [1, 15, 64, 65, 33 + 40], hq, hkv, bs=bs, seed=hq)
+
+
+def test_chunk_with_no_context_is_zero_and_mixed_batch():
+    _attend([1, 1, 40, 70], [33, 1, 40, 16 + 70], 8, 2, n_decode=2, seed=7)
+
+
+@pytest.mark.parametrize("q_len,kv_len", [(130, 130), (200, 333), (128, 512)])
+def test_long_chunks(q_len, kv_len):
+    _attend([q_len, 67], [kv_len, 67], 4, 2, seed=q_len)
+
+
+def test_small_and_large_values():
+    _attend([1, 30], [40, 60], 4, 2, n_decode=1, v_scale=2.0 ** -60, q_scale=2.0 ** 60)
+    _attend([1, 30], [40, 60], 4, 2, n_decode=1, v_scale=2.0 ** 40, q_scale=2.0 ** -40)
+
+
+def _small(n_decode=2):
+    k, v = _random(4, 2, 16, 0)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    attn = AttnBatch(cu_q=torch.tensor([0, 1, 2], **i32), kv_lens=torch.tensor([20, 7], **i32),
+                     block_tables=torch.tensor([[0, 1], [2, 0]], **i32), num_seqs=2, num_decode=n_decode, max_q_len=1,
+                     max_kv_len=20, num_tokens=2)
+    return torch.randn(2, 4 * D, generator=torch.Generator().manual_seed(1)).bfloat16().to(DEV), k, v, attn
+
+
+@pytest.mark.parametrize("n_decode", [2, 0])
+def test_bad_pages_lengths_and_ranges_are_reported_and_not_followed(n_decode):
+    ops, cuda = _ops(), _cuda()
+    for field, value in (("block_tables", [[0, 9], [2, 0]]), ("block_tables", [[0, -1], [2, 0]]), ("kv_lens", [33, 7])):
+        q, k, v, attn = _small(n_decode)
+        setattr(attn, field, torch.tensor(value, dtype=torch.int32, device=DEV))
+        out = ops.paged_attention(q, k, v, attn, 0.1, 4, 2, D)
+        with pytest.raises(RuntimeError, match="status 5"):
+            cuda.check_status()
+        assert bool(out[1].isfinite().all())
+    if n_decode == 0:
+        q, k, v, attn = _small(0)
+        attn.cu_q = torch.tensor([0, 1, 3], dtype=torch.int32, device=DEV)
+        ops.paged_attention(q, k, v, attn, 0.1, 4, 2, D)
+        with pytest.raises(RuntimeError, match="status 5"):
+            cuda.check_status()
+
+
+def test_refusals():
+    ops = _ops()
+    q, k, v, attn = _small()
+    for bad, args in ((TypeError, (q.float(), k, v)), (ValueError, (q.t().contiguous().t(), k, v)),
+                      (TypeError, (q, k, v.float())), (ValueError, (q, k[:, :1], v[:, :1])), (ValueError, (q[:1], k, v)),
+                      (ValueError, (q, k.cpu(), v.cpu()))):
+        with pytest.raises(bad):
+            ops.paged_attention(*args, attn, 0.1, 4, 2, D)
+    with pytest.raises(ValueError, match="16 to one"):
+        ops.paged_attention(torch.zeros(2, 34 * D, device=DEV).bfloat16(), k, v, attn, 0.1, 34, 2, D)
+    with pytest.raises(ValueError, match="head_dim 128"):
+        ops.read_cache(torch.zeros(1, 1, 16, 40, dtype=torch.uint8, device=DEV),
+                       torch.zeros(1, 1, 16, 40, dtype=torch.uint8, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV), 64)
+    with pytest.raises(ValueError, match="slots"):
+        ops.read_cache(k, v, torch.zeros(1, dtype=torch.int64, device=DEV), D)
+    attn.kv_lens = attn.kv_lens.long()
+    with pytest.raises(ValueError, match="kv_lens"):
+        ops.paged_attention(q, k, v, attn, 0.1, 4, 2, D)
+    e = ops.paged_attention(q[:0], k, v, AttnBatch(attn.cu_q[:1], attn.kv_lens[:0].int(), attn.block_tables[:0], 0, 0, 0, 0, 0),
+                            0.1, 4, 2, D)
+    assert e.shape == (0, 4 * D)
+
+
+def test_two_streams_and_graph_replay_do_not_share_scratch():
+    """Two captured decode calls with splits, replayed at the same time on two streams, and an eager one between."""
+    ops = _ops()
+    runs = []
+    for seed in (1, 2):
+        k, v = _random(70, 2, 16, seed)
+        g = torch.Generator().manual_seed(seed)
+        q = torch.randn(1, 8 * D, generator=g).bfloat16().to(DEV)
+        i32 = dict(dtype=torch.int32, device=DEV)
+        table = torch.randperm(70, generator=g).to(**i32)[None]
+        attn = AttnBatch(torch.tensor([0, 1], **i32), torch.tensor([1100], **i32), table, 1, 1, 1, 1100, 1)
+        want = ops.paged_attention(q, k, v, attn, 0.09, 8, 2, D).clone()
+        torch.cuda.synchronize()
+        gr, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(gr, stream=s):
+            out = ops.paged_attention(q, k, v, attn, 0.09, 8, 2, D)
+        runs.append((gr, s, out, want, (q, k, v, attn)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for gr, s, out, want, _ in runs:
+            with torch.cuda.stream(s):
+                gr.replay()
+        q, k, v, attn = runs[0][4]
+        eager = ops.paged_attention(q, k, v, attn, 0.09, 8, 2, D)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, runs[0][3])
+        for _, _, out, want, _ in runs:
+            assert torch.equal(out, want)
+    _cuda().check_status()

@@ -1,0 +1,124 @@
+"""4-bit KV cache on the CPU backend: byte format, quantiser, refusals and the engine that uses it."""
+import numpy as np
+import pytest
+import torch
+
+import kv4_ref
+from xixi_vllm_b200.ops import cpu_ref, dispatch as ops, kv4
+from xixi_vllm_b200.runtime.staging import AttnBatch
+
+
+def caches(nb, heads, bs, d):
+    return tuple(torch.zeros(nb, heads, bs, kv4.row_bytes(d), dtype=torch.uint8) for _ in range(2))
+
+
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_quantise_matches_the_definition_in_64_bits(d):
+    g = torch.Generator().manual_seed(d)
+    x = torch.randn(200, d, generator=g) * torch.exp(2 * torch.randn(200, 1, generator=g))
+    x[3], x[4, ::2], x[5] = 0.7, 5.0, 0.0
+    x = x.bfloat16()
+    got = kv4.dequantize(*kv4.quantize(x)).double().numpy()
+    want = kv4_ref.levels(x.double().numpy())
+    # c + s (n - 8) in fp32 rounds once
+    np.testing.assert_allclose(got, want, rtol=2.0 ** -23, atol=0)
+
+
+def test_quantise_error_is_half_a_step_and_constant_groups_are_exact():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(500, 128, generator=g).bfloat16()
+    x[0] = -3.25
+    codes, par = kv4.quantize(x)
+    err = kv4._to_groups((kv4.dequantize(codes, par) - x.float()).abs())
+    step = par[..., 0:1].float()
+    centre = par[..., 1:2].float().abs()
+    # half a step; the ends of the range move by the rounding of s (7.5 steps of 2^-8) and of c
+    assert bool((err <= step * (0.5 + 7.5 * 2.0 ** -8) + centre * 2.0 ** -8 + 1e-6).all())
+    assert torch.equal(kv4.dequantize(codes, par)[0], x[0].float())
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_a_group_with_a_non_finite_value_reads_back_as_nan_and_the_other_group_does_not(value):
+    x = torch.randn(2, 128, generator=torch.Generator().manual_seed(2))
+    x[0, 9] = value                              # word 1: group 1
+    y = kv4.dequantize(*kv4.quantize(x))
+    odd = (torch.arange(128) // 8) % 2 == 1
+    assert bool(y[0, odd].isnan().all()) and bool(y[0, ~odd].isfinite().all()) and bool(y[1].isfinite().all())
+
+
+def test_largest_and_smallest_values():
+    big = 2.0 ** 126                             # eight steps of the largest bf16 would leave fp32
+    x = torch.zeros(3, 128)
+    x[0, 0], x[0, 1] = big, -big
+    x[1, 0] = 1e-38                              # a step below the smallest normal number counts as 0
+    x[2] = 2.0 ** -126
+    y = kv4.dequantize(*kv4.quantize(x))
+    assert bool(y.isfinite().all())
+    assert float((y[0, :2] - x[0, :2]).abs().max()) <= big / 15
+    assert float((y[1] - x[1]).abs().max()) <= 1e-38
+    assert torch.equal(y[2], x[2])
+
+
+@pytest.mark.parametrize("d,bs", [(64, 16), (128, 48)])
+def test_rows_land_where_the_format_says(d, bs):
+    k, _ = caches(3, 2, bs, d)
+    x = torch.randn(5, 2, d, generator=torch.Generator().manual_seed(3))
+    slots = torch.tensor([0, bs + 15, 2 * bs + 1, bs - 1, 2 * bs + 10])
+    kv4.write_rows(k, slots, x)
+    want = kv4_ref.levels(x.bfloat16().double().numpy())
+    got, _ = kv4_ref.rows(k, slots.tolist())
+    np.testing.assert_allclose(got, want, rtol=1e-12)
+    np.testing.assert_allclose(kv4.read_rows(k, slots).numpy(), want, rtol=2.0 ** -23)
+    untouched, _ = kv4_ref.rows(k, [1, bs, 2 * bs])
+    assert not untouched.any()
+
+
+def test_read_cache_negative_slots_and_repeats():
+    k, v = caches(2, 1, 16, 64)
+    kv4.write_rows(k, torch.tensor([5]), torch.ones(1, 1, 64))
+    kv4.write_rows(v, torch.tensor([5]), torch.full((1, 1, 64), 2.0))
+    kk, vv = ops.read_cache(k, v, torch.tensor([5, -1, 5], dtype=torch.int32), 64)
+    assert kk.dtype == torch.bfloat16 and kk.shape == (3, 1, 64)
+    assert kk[:, 0, 0].tolist() == [1, 0, 1] and vv[:, 0, 0].tolist() == [2, 0, 2]
+    e, _ = ops.read_cache(k, v, torch.zeros(0, dtype=torch.int32), 64)
+    assert e.shape == (0, 1, 64)
+
+
+def test_refusals():
+    k, v = caches(2, 1, 16, 64)
+    s = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(TypeError, match="uint8"):
+        ops.read_cache(k, v.float(), s, 64)
+    with pytest.raises(TypeError, match="uint8"):
+        ops.read_cache(torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16), torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16), s, 64)
+    with pytest.raises(ValueError, match="expected"):
+        ops.read_cache(k, v, s, 128)                              # row size of another head_dim
+    with pytest.raises(ValueError, match="one 4-d shape"):
+        ops.read_cache(k, v[:1], s, 64)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.read_cache(k.repeat(1, 2, 1, 1).transpose(0, 1), v.repeat(1, 2, 1, 1).transpose(0, 1), s, 64)
+    with pytest.raises(ValueError, match="expected"):
+        kv4.check_caches(k[:, :, :8], v[:, :, :8], 64)            # a page of half a unit
+    with pytest.raises(ValueError, match="head_dim % 16"):
+        kv4.row_bytes(72)
+
+
+def test_append_then_attend_matches_64_bits():
+    torch.manual_seed(0)
+    hq, hkv, d, bs = 4, 2, 64, 32
+    k, v = caches(6, hkv, bs, d)
+    T = 41
+    qkv = torch.randn(T, (hq + 2 * hkv) * d)
+    cs = cpu_ref.build_cos_sin_cache(d, 100, 1e4)
+    w = torch.ones(d)
+    table = torch.tensor([[4, 2]], dtype=torch.int32)
+    slots = torch.tensor([int(table[0, t // bs]) * bs + t % bs for t in range(T)], dtype=torch.int32)
+    slots_w = slots.clone()
+    q = ops.qk_norm_rope_cache(qkv, w, w, 1e-6, cs, torch.arange(T, dtype=torch.int32), slots_w, k, v, hq, hkv, d)
+    want_v = kv4_ref.levels(qkv[:, (hq + hkv) * d:].view(T, hkv, d).bfloat16().double().numpy())
+    np.testing.assert_allclose(kv4_ref.rows(v, slots.tolist())[0], want_v, rtol=1e-12)
+    attn = AttnBatch(cu_q=torch.tensor([0, T], dtype=torch.int32), kv_lens=torch.tensor([T], dtype=torch.int32),
+                     block_tables=table, num_seqs=1, num_decode=0, max_q_len=T, max_kv_len=T, num_tokens=T)
+    out = ops.paged_attention(q, k, v, attn, d ** -0.5, hq, hkv, d)
+    ref, *_ = kv4_ref.attention(q, k, v, [T], [T], table, d ** -0.5, hq)
+    np.testing.assert_allclose(out.view(T, hq, d).numpy(), ref, atol=1e-5)

@@ -147,6 +147,30 @@ int xv_attn_prefill_tc_profile(const void* q, const void* k_cache, const void* v
                                int max_blocks, float scale, int* status, unsigned long long* prof,
                                cudaStream_t stream);
 
+// ---- KV cache held in 4 bits (kv4.cu, attn_kv4.cu; byte format: common/kv4.cuh), head_dim 128, page sizes that are
+// multiples of 16 ----
+// As xv_qk_norm_rope_cache[_partials], the rows quantised as they are written. `qkv` or `partials` is given. A slot of
+// num_blocks * block_size or more is not written and a position outside cos_sin's max_pos rows uses row 0; both are
+// reported through `status`.
+int xv_kv4_write(const void* qkv, const float* partials, int splits, long long split_stride, const void* q_w,
+                 const void* k_w, float eps, const float* cos_sin, int max_pos, const int* positions, const int* slots,
+                 void* q_out, void* k_cache, void* v_cache, int tokens, int hq, int hkv, int d, int block_size,
+                 int num_blocks, int* status, cudaStream_t stream);
+// bf16 values [tokens, hkv, d] of the rows at `slots` (negative or out of range: zeros, the latter reported).
+int xv_kv4_read(const void* k_cache, const void* v_cache, const int* slots, void* k_out, void* v_out, int tokens, int hkv,
+                int d, int block_size, int num_blocks, int* status, cudaStream_t stream);
+// As xv_attn_decode / xv_attn_prefill. Block-table entries outside [0, num_blocks), lengths beyond the table and query
+// ranges beyond total_rows are reported through `status`, never followed.
+int xv_kv4_decode_splits(int num_seqs, int hkv, int num_sms, int max_tokens_per_seq);
+long long xv_kv4_decode_workspace_bytes(int num_seqs, int hq, int splits);
+int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* kv_lens,
+                  void* out, int num_seqs, int hq, int hkv, int d, int block_size, int max_blocks, int num_blocks,
+                  float scale, int splits, void* workspace, long long workspace_bytes, int* status, cudaStream_t stream);
+int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_q,
+                   const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq,
+                   int hkv, int d, int block_size, int max_blocks, int num_blocks, float scale, int* status,
+                   cudaStream_t stream);
+
 // Input ids < 0 are references into the previous step's samples: ids[i] = prev[-ids[i] - 1] (elementwise.cu).
 int xv_resolve_token_refs(int* ids, int n, const long long* prev, int n_prev, cudaStream_t stream);
 

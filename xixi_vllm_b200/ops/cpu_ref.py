@@ -7,7 +7,7 @@ import (reference: src/compute/layers/ops.py:14-17, src/compute/layers/attention
 
 KV cache layout per layer: ``k_cache, v_cache: [num_blocks, kv_heads, block_size, head_dim]``
 (head-major inside a page, so one page of one head is a contiguous run). Slot ``s`` is
-page ``s // block_size``, offset ``s % block_size``.
+page ``s // block_size``, offset ``s % block_size``. A uint8 cache holds its rows in 4 bits (``ops.kv4``).
 """
 
 from __future__ import annotations
@@ -15,9 +15,11 @@ from __future__ import annotations
 
 import torch
 
+from . import kv4
+
 __all__ = [
     "rmsnorm", "add_rmsnorm", "linear", "silu_mul", "embedding", "build_cos_sin_cache",
-    "qk_norm_rope_cache", "paged_attention", "sample", "argmax",
+    "qk_norm_rope_cache", "read_cache", "paged_attention", "sample", "argmax",
 ]
 
 
@@ -88,19 +90,43 @@ def qk_norm_rope_cache(qkv: torch.Tensor, q_w: torch.Tensor, k_w: torch.Tensor, 
     k = qkv[:, nq:nq + nk].reshape(T, num_kv_heads, D).float()
     v = qkv[:, nq + nk:nq + 2 * nk].reshape(T, num_kv_heads, D)
     q = q * torch.rsqrt(q.pow(2).mean(-1, keepdim=True) + eps) * q_w.float()
+    if kv4.is_kv4(k_cache):
+        k = k.double()          # a code is a choice between levels: values next to a border must fall alike everywhere
     k = k * torch.rsqrt(k.pow(2).mean(-1, keepdim=True) + eps) * k_w.float()
     cs = cos_sin[positions.long()].float()
     cos, sin = cs[:, : D // 2], cs[:, D // 2:]
     q = _rope_neox(q, cos, sin).to(qkv.dtype)
-    k = _rope_neox(k, cos, sin).to(qkv.dtype)
+    k = _rope_neox(k, cos, sin).float().to(qkv.dtype)
     bs = k_cache.shape[2]
     keep = slots >= 0
-    if bool(keep.any()):
+    if kv4.is_kv4(k_cache):
+        if bool(keep.any()):
+            kv4.write_rows(k_cache, slots[keep], k[keep])
+            kv4.write_rows(v_cache, slots[keep], v[keep])
+    elif bool(keep.any()):
         s = slots[keep].long()
         blk, off = s // bs, s % bs
         k_cache[blk, :, off, :] = k[keep].to(k_cache.dtype)
         v_cache[blk, :, off, :] = v[keep].to(v_cache.dtype)
     return q.reshape(T, nq)
+
+
+def read_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 rows ``[T, kv_heads, D]`` of a 4-bit cache; rows whose slot is negative are zero."""
+    out = []
+    for cache in (k_cache, v_cache):
+        rows = kv4.read_rows(cache, slots.clamp_min(0))
+        out.append((rows * (slots >= 0)[:, None, None]).to(torch.bfloat16))
+    return out[0], out[1]
+
+
+def _context(cache: torch.Tensor, blocks: torch.Tensor, length: int) -> torch.Tensor:
+    """fp32 ``[kv_heads, length, D]`` of the first ``length`` tokens in ``blocks``."""
+    bs = cache.shape[2]
+    if kv4.is_kv4(cache):
+        slots = (blocks[:, None] * bs + torch.arange(bs, device=cache.device)).flatten()[:length]
+        return kv4.read_rows(cache, slots).transpose(0, 1)
+    return cache[blocks].permute(1, 0, 2, 3).reshape(cache.shape[1], -1, cache.shape[3])[:, :length].float()
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -125,8 +151,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             continue
         nb = -(-L // bs)
         blocks = block_tables[b, :nb].long()
-        k = k_cache[blocks].permute(1, 0, 2, 3).reshape(num_kv_heads, nb * bs, D)[:, :L].float()
-        v = v_cache[blocks].permute(1, 0, 2, 3).reshape(num_kv_heads, nb * bs, D)[:, :L].float()
+        k, v = _context(k_cache, blocks, L), _context(v_cache, blocks, L)
         qb = q[q0:q1].reshape(n, num_kv_heads, group, D).permute(1, 2, 0, 3).float()   # [Hkv,G,n,D]
         s = torch.einsum("hgnd,hld->hgnl", qb, k) * scale
         qpos = torch.arange(L - n, L, device=q.device)[:, None]

@@ -17,10 +17,11 @@ import os
 import torch
 
 from . import build as _build
+from . import kv4 as _kv4
 
 __all__ = [
     "lib", "rmsnorm", "add_rmsnorm", "linear", "silu_mul", "embedding", "gather_rows",
-    "qk_norm_rope_cache", "paged_attention", "prefill_pair_heads", "prefill_phase_profile", "argmax", "sample", "check_status", "gemm_plan",
+    "qk_norm_rope_cache", "read_cache", "paged_attention", "prefill_pair_heads", "prefill_phase_profile", "argmax", "sample", "check_status", "gemm_plan",
     "decode_splits", "launch_count",
 ]
 
@@ -80,6 +81,16 @@ def lib():
                                      _i32, _i32, _i32, _f32, _vp, _vp]
     L.xv_attn_prefill_tc_profile.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                              _i32, _i32, _i32, _f32, _vp, _vp, _vp]
+    L.xv_kv4_write.argtypes = [_vp, _vp, _i32, _i64, _vp, _vp, _f32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32,
+                               _i32, _i32, _i32, _vp, _vp]
+    L.xv_kv4_read.argtypes = [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp]
+    L.xv_kv4_decode_splits.argtypes = [_i32, _i32, _i32, _i32]
+    L.xv_kv4_decode_workspace_bytes.argtypes = [_i32, _i32, _i32]
+    L.xv_kv4_decode_workspace_bytes.restype = _i64
+    L.xv_kv4_decode.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp,
+                                _i64, _vp, _vp]
+    L.xv_kv4_prefill.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                                 _i32, _f32, _vp, _vp]
     L.xv_argmax.argtypes = [_vp, _vp, _i32, _i32, _i64, _vp]
     L.xv_sample.argtypes = [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp]
     L.xv_tp_reduce_norm.argtypes = [_vp, _vp, _vp, _vp, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _f32,
@@ -334,6 +345,9 @@ def resolve_token_refs(ids, prev) -> None:
 
 def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads,
                        num_kv_heads, head_dim, prefill_begin: int = 0):
+    if _kv4.is_kv4(k_cache):
+        return _kv4_write(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads, num_kv_heads,
+                          head_dim)
     if isinstance(qkv, SplitKPartial):
         _bf16(q_w, k_w, k_cache, v_cache)
         T = qkv.shape[0]
@@ -354,6 +368,105 @@ def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v
                                        v_cache.data_ptr(), T, num_q_heads, num_kv_heads, head_dim,
                                        k_cache.shape[2], prefill_begin, _stream()), "qk_norm_rope_cache")
     return q
+
+
+def _vector(t, n: int, dtype, device, what: str) -> None:
+    """``t`` must hold at least ``n`` contiguous elements of ``dtype`` on ``device``."""
+    if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{what}: needs {n} contiguous {dtype} values on {device}, got {tuple(t.shape)} {t.dtype} on "
+                         f"{t.device}")
+
+
+def _kv4_caches(k_cache, v_cache, head_dim: int, num_kv_heads: int | None = None) -> None:
+    _kv4.check_caches(k_cache, v_cache, head_dim, num_kv_heads)
+    if head_dim != 128:
+        raise ValueError(f"4-bit caches on the GPU need head_dim 128, got {head_dim}")
+
+
+def _kv4_write(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads, num_kv_heads, head_dim):
+    dev = k_cache.device
+    _kv4_caches(k_cache, v_cache, head_dim, num_kv_heads)
+    _bf16(q_w, k_w)
+    part = isinstance(qkv, SplitKPartial)
+    cols = (num_q_heads + 2 * num_kv_heads) * head_dim
+    if len(qkv.shape) != 2 or qkv.shape[1] != cols or qkv.device != dev:
+        raise ValueError(f"qk_norm_rope_cache: qkv must be [T, {cols}] on {dev}, got {tuple(qkv.shape)} on {qkv.device}")
+    if not part:
+        _bf16(qkv)
+        if not qkv.is_contiguous():
+            raise ValueError("qk_norm_rope_cache needs contiguous qkv and cache tensors")
+    T = qkv.shape[0]
+    _vector(q_w, head_dim, torch.bfloat16, dev, "q_w")
+    _vector(k_w, head_dim, torch.bfloat16, dev, "k_w")
+    _vector(cos_sin, head_dim, torch.float32, dev, "cos_sin")
+    _vector(positions, T, torch.int32, dev, "positions")
+    _vector(slots, T, torch.int32, dev, "slots")
+    with torch.cuda.device(dev):
+        q = torch.empty((T, num_q_heads * head_dim), dtype=torch.bfloat16, device=dev)
+        if T:
+            _check(lib().xv_kv4_write(
+                None if part else qkv.data_ptr(), qkv.ws.data_ptr() if part else None, qkv.splits if part else 0,
+                qkv.stride_elems if part else 0, q_w.data_ptr(), k_w.data_ptr(), eps, cos_sin.data_ptr(),
+                cos_sin.numel() // head_dim, positions.data_ptr(), slots.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
+                v_cache.data_ptr(), T, num_q_heads, num_kv_heads, head_dim, k_cache.shape[2], k_cache.shape[0],
+                _state(k_cache).status.data_ptr(), _stream()), "kv4_write")
+    return q
+
+
+def read_cache(k_cache, v_cache, slots, head_dim):
+    """bf16 rows of a 4-bit cache (see ``dispatch.read_cache``). A slot beyond the cache gives zeros and status 5."""
+    dev = k_cache.device
+    _kv4_caches(k_cache, v_cache, head_dim)
+    T, hkv = slots.numel(), k_cache.shape[1]
+    _vector(slots, T, torch.int32, dev, "slots")
+    with torch.cuda.device(dev):
+        out = torch.empty((2, T, hkv, head_dim), dtype=torch.bfloat16, device=dev)
+        if T:
+            _check(lib().xv_kv4_read(k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), out[0].data_ptr(),
+                                     out[1].data_ptr(), T, hkv, head_dim, k_cache.shape[2], k_cache.shape[0],
+                                     _state(k_cache).status.data_ptr(), _stream()), "kv4_read")
+    return out[0], out[1]
+
+
+def _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
+    dev = k_cache.device
+    _kv4_caches(k_cache, v_cache, head_dim, num_kv_heads)
+    _bf16(q)
+    bt, n_d, n_p = attn.block_tables, attn.num_decode, attn.num_seqs - attn.num_decode
+    if q.dim() != 2 or q.shape[1] != num_q_heads * head_dim or not q.is_contiguous() or q.device != dev:
+        raise ValueError(f"paged_attention: q must be a contiguous [T, {num_q_heads * head_dim}] tensor on {dev}")
+    if num_q_heads % num_kv_heads or num_q_heads // num_kv_heads > 16:
+        raise ValueError(f"paged_attention: {num_q_heads} query heads over {num_kv_heads} KV heads (at most 16 to one)")
+    if n_d < 0 or n_p < 0 or n_d > q.shape[0] or bt.dim() != 2 or bt.shape[0] < attn.num_seqs:
+        raise ValueError(f"paged_attention: {n_d} decode rows and {n_p} chunks for {q.shape[0]} query rows and a block "
+                         f"table of {tuple(bt.shape)}")
+    if attn.num_seqs > 65535:
+        raise ValueError("paged_attention: at most 65535 sequences")
+    _vector(bt, attn.num_seqs * bt.shape[1], torch.int32, dev, "block_tables")
+    _vector(attn.kv_lens, attn.num_seqs, torch.int32, dev, "kv_lens")
+    if n_p:
+        _vector(attn.cu_q, attn.num_seqs + 1, torch.int32, dev, "cu_q")
+    L, bs, nb, maxb = lib(), k_cache.shape[2], k_cache.shape[0], bt.shape[1]
+    with torch.cuda.device(dev):
+        st = _state(q)
+        out = torch.empty_like(q)
+        if maxb == 0 or nb == 0:        # nothing is cached: every row is empty
+            return out.zero_()
+        if n_d:
+            splits = L.xv_kv4_decode_splits(n_d, num_kv_heads, st.num_sms, maxb * bs)
+            need = L.xv_kv4_decode_workspace_bytes(n_d, num_q_heads, splits)
+            # from torch's allocator, call by call: calls on two streams, or two captured graphs, never share it
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            _check(L.xv_kv4_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(),
+                                   attn.kv_lens.data_ptr(), out.data_ptr(), n_d, num_q_heads, num_kv_heads, head_dim, bs,
+                                   maxb, nb, scale, splits, ws.data_ptr() if need else None, need, st.status.data_ptr(),
+                                   _stream()), "kv4_decode")
+        if n_p:
+            _check(L.xv_kv4_prefill(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(),
+                                    attn.cu_q.data_ptr(), attn.kv_lens.data_ptr(), out.data_ptr(), n_d, n_p,
+                                    attn.max_q_len, q.shape[0], num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale,
+                                    st.status.data_ptr(), _stream()), "kv4_prefill")
+    return out
 
 
 def decode_splits(num_seqs: int, num_kv_heads: int, num_sms: int, max_blocks_tokens: int) -> int:
@@ -384,6 +497,8 @@ def prefill_pair_heads(on: bool) -> None:
 
 def paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
     """Decode rows (the first ``attn.num_decode`` sequences) and prefill chunks of one packed batch."""
+    if _kv4.is_kv4(k_cache):
+        return _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim)
     _bf16(q, k_cache, v_cache)
     st = _state(q)
     L = lib()

@@ -7,11 +7,11 @@ from __future__ import annotations
 
 import torch
 
-from . import cpu_ref
+from . import cpu_ref, kv4
 
 __all__ = [
     "rmsnorm", "add_rmsnorm", "linear", "linear_silu_mul", "silu_mul", "embedding", "qk_norm_rope_cache",
-    "paged_attention", "sample", "argmax", "build_cos_sin_cache", "gather_rows",
+    "read_cache", "paged_attention", "sample", "argmax", "build_cos_sin_cache", "gather_rows",
     "resolve_token_refs",
 ]
 
@@ -66,7 +66,9 @@ def embedding(ids, w, vocab_start=0, out=None):
 def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache,
                        num_q_heads, num_kv_heads, head_dim, prefill_begin: int = 0):
     """``prefill_begin``: index of the first prefill row of the packed batch (decode rows come first).
-    The GPU kernel clears the V rows that follow a prefill chunk's last row inside its page."""
+    The GPU kernel clears the V rows that follow a prefill chunk's last row inside its page.
+    uint8 caches (``ops.kv4``) receive the rows quantised to 4 bits; every other argument is the same. Slots that are
+    not negative must be distinct: of two rows for one slot, either may be stored, or a mixture."""
     if qkv.is_cuda:
         return _cuda().qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache,
                                           num_q_heads, num_kv_heads, head_dim, prefill_begin)
@@ -74,8 +76,18 @@ def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v
                                       num_q_heads, num_kv_heads, head_dim)
 
 
+def read_cache(k_cache, v_cache, slots, head_dim):
+    """What a 4-bit cache holds at ``slots [T]`` (int32, as ``qk_norm_rope_cache`` takes them): bf16 ``k, v`` of shape
+    ``[T, kv_heads, head_dim]``. Rows whose slot is negative are zero. A slot may be named any number of times."""
+    kv4.check_caches(k_cache, v_cache, head_dim)
+    if k_cache.is_cuda:
+        return _cuda().read_cache(k_cache, v_cache, slots, head_dim)
+    return cpu_ref.read_cache(k_cache, v_cache, slots)
+
+
 def paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
-    """``attn`` is a ``runtime.staging.AttnBatch`` (cu_q, kv_lens, block_tables, decode split)."""
+    """``attn`` is a ``runtime.staging.AttnBatch`` (cu_q, kv_lens, block_tables, decode split). The caches are bf16
+    pages or, as uint8, pages held in 4 bits (``ops.kv4``)."""
     if q.is_cuda:
         return _cuda().paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim)
     return cpu_ref.paged_attention(q, k_cache, v_cache, attn.cu_q, attn.kv_lens, attn.block_tables,
