@@ -124,6 +124,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--load-format", choices=("auto", "dummy"), default=None)
     p.add_argument("--device", choices=("cuda", "cpu"), default=None)
     p.add_argument("--tp-comm", choices=("auto", "fused", "nccl"), default=None)
+    p.add_argument("--kv-cache-dtype", choices=("auto", "int4"), default=None,
+                   help="how the KV cache is held: the model's dtype, or 4 bits a value")
     p.add_argument("--async-scheduling", choices=("auto", "on", "off"), default=None,
                    help="launch step n+1 before step n's samples are read (auto: on for CUDA without pipeline stages)")
     p.add_argument("--batch", action="store_true", help="run the four-prompt batch demo")
@@ -136,7 +138,8 @@ def config_from_args(args) -> dict:
     path = Path(args.config) if args.config else HERE / "config.yaml"
     cfg = load_config(path, DEFAULTS)
     merge_cli(cfg, args, ("model", "prompt", "max_new_tokens", "temperature", "top_p", "top_k", "prefix_backend",
-                          "max_num_seqs", "load_format", "device", "tp_comm", "async_scheduling"))
+                          "max_num_seqs", "load_format", "device", "tp_comm", "async_scheduling",
+                          "kv_cache_dtype"))
     for flag, key in (("tp", "tp_size"), ("pp", "pp_size"), ("dp", "dp_size")):
         if getattr(args, flag) is not None:
             cfg[key] = getattr(args, flag)

@@ -340,3 +340,84 @@ def test_two_streams_and_graph_replay_do_not_share_scratch():
         for _, _, out, want, _ in runs:
             assert torch.equal(out, want)
     _cuda().check_status()
+
+
+# ---- the operators together, as the engine runs them ----
+
+def _engine(model_dir, prompts, max_tokens, **kw):
+    from xixi_vllm_b200 import Engine, EngineConfig, SamplingParams
+    base = dict(device="cuda", dtype="bfloat16", num_kvcache_blocks=256, max_num_seqs=16, max_num_batched_tokens=256,
+                context_len=512, kv_cache_dtype="int4")
+    base.update(kw)
+    eng = Engine(EngineConfig(model=model_dir, **base))
+    try:
+        seqs = [eng.add_request(p, SamplingParams(max_tokens=max_tokens, ignore_eos=True)) for p in prompts]
+        while eng.has_unfinished():
+            eng.step()
+        return [s.token_ids[s.num_prompt_tokens:] for s in seqs]
+    finally:
+        eng.destroy()
+
+
+@pytest.fixture(scope="module")
+def model_dir(tmp_path_factory):
+    from xixi_vllm_b200.models.synth import make_model_dir
+    return make_model_dir(str(tmp_path_factory.mktemp("kv4_model")), "tiny", std=0.08, num_hidden_layers=2, hidden_size=512,
+                          num_attention_heads=4, num_key_value_heads=2, head_dim=128, intermediate_size=1024,
+                          vocab_size=2048, torch_dtype="bfloat16", tie_word_embeddings=False)
+
+
+def _prompts(lens, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, 2048, (n,), generator=g).tolist() for n in lens]
+
+
+def test_engine_native_and_module_forwards_agree_on_a_4_bit_cache(model_dir, monkeypatch):
+    """Graph-replayed native executor against the Python forward: the same kernels, so identical tokens. Four sequences
+    are a graph bucket of their own and 240 tokens of context one KV split, so both run the same launch shapes (another
+    split count adds in another order)."""
+    prompts = _prompts((7, 33, 120, 200), 2)
+    kw = dict(context_len=240)
+    native = _engine(model_dir, prompts, 10, enforce_eager=False, **kw)
+    late = _engine(model_dir, prompts, 10, enforce_eager=False, async_scheduling="off", **kw)
+    monkeypatch.setenv("XV_NATIVE_FORWARD", "0")
+    assert native == _engine(model_dir, prompts, 10, enforce_eager=True, **kw) == late
+
+
+def test_engine_on_a_4_bit_cache_follows_the_cpu_backend(model_dir):
+    """First sampled token of every prompt: one forward from equal inputs. Later ones depend on it."""
+    prompts = _prompts((5, 16, 17, 40, 100, 3, 230), 0)
+    gpu = _engine(model_dir, prompts, 12)
+    cpu = _engine(model_dir, prompts, 12, device="cpu")
+    assert sum(a[0] == b[0] for a, b in zip(gpu, cpu)) >= len(prompts) - 1, (gpu, cpu)
+
+
+def test_append_attend_and_read_back_as_one_run():
+    """Prompt chunk, two more chunks on top of it, then decode steps: every output against 64-bit attention over the
+    bytes that the steps before it wrote."""
+    ops, cuda = _ops(), _cuda()
+    hq, hkv, bs = 8, 2, 16
+    g = torch.Generator().manual_seed(11)
+    k, v = _empty(12, hkv, bs)
+    table = torch.randperm(12, generator=g)[None].to(torch.int32)
+    cs = cpu_ref.build_cos_sin_cache(D, 400, 1e6).to(DEV)
+    w = torch.ones(D).bfloat16().to(DEV)
+    have = 0
+    for n in (70, 37, 1, 1, 2, 1):
+        qkv = torch.randn(n, (hq + 2 * hkv) * D, generator=g).bfloat16().to(DEV)
+        pos = torch.arange(have, have + n, dtype=torch.int32)
+        slots = torch.tensor([int(table[0, t // bs]) * bs + t % bs for t in range(have, have + n)], dtype=torch.int32)
+        q = ops.qk_norm_rope_cache(qkv, w, w, 1e-6, cs, pos.to(DEV), slots.to(DEV), k, v, hq, hkv, D)
+        have += n
+        i32 = dict(dtype=torch.int32, device=DEV)
+        attn = AttnBatch(torch.tensor([0, n], **i32), torch.tensor([have], **i32), table.to(DEV), 1, 1 if n == 1 else 0, n, have, n)
+        out = ops.paged_attention(q, k, v, attn, D ** -0.5, hq, hkv, D)
+        cuda.check_status()
+        ref, *_ = kv4_ref.attention(q, k, v, [n], [have], table, D ** -0.5, hq)
+        got = out.double().cpu().numpy().reshape(n, hq, D)
+        assert np.linalg.norm(got - ref) <= HALF_BF16 * 2 * np.linalg.norm(ref)
+    every = torch.tensor([int(table[0, t // bs]) * bs + t % bs for t in range(have)], dtype=torch.int32, device=DEV)
+    kk, vv = ops.read_cache(k, v, every, D)
+    for got, cache in ((kk, k), (vv, v)):
+        want, _ = kv4_ref.rows(cache, every.tolist())
+        assert (np.abs(got.double().cpu().numpy() - want) <= HALF_BF16 * np.abs(want) * (1 + 2.0 ** -14)).all()

@@ -122,3 +122,87 @@ def test_append_then_attend_matches_64_bits():
     out = ops.paged_attention(q, k, v, attn, d ** -0.5, hq, hkv, d)
     ref, *_ = kv4_ref.attention(q, k, v, [T], [T], table, d ** -0.5, hq)
     np.testing.assert_allclose(out.view(T, hq, d).numpy(), ref, atol=1e-5)
+
+
+# ---- the engine with kv_cache_dtype="int4" ----
+
+def _generate(model_dir, prompts, max_tokens=8, **kw):
+    from xixi_vllm_b200 import Engine, EngineConfig, SamplingParams
+    base = dict(device="cpu", dtype="float32", num_kvcache_blocks=128, max_num_seqs=8, max_num_batched_tokens=64,
+                context_len=256, kv_cache_dtype="int4")
+    base.update(kw)
+    eng = Engine(EngineConfig(model=model_dir, **base))
+    try:
+        seqs = [eng.add_request(p, SamplingParams(max_tokens=max_tokens, ignore_eos=True)) for p in prompts]
+        while eng.has_unfinished():
+            eng.step()
+        return [s.token_ids[s.num_prompt_tokens:] for s in seqs]
+    finally:
+        eng.destroy()
+
+
+def _prompts(lens, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, 1024, (n,), generator=g).tolist() for n in lens]
+
+
+def test_engine_runs_on_a_4_bit_cache_and_scheduling_does_not_change_tokens(tiny_model_dir):
+    """Chunked prefill, a shared prefix and preemption read pages that other steps wrote."""
+    shared = _prompts([40], 5)[0]
+    prompts = [shared + p for p in _prompts([9, 30, 3, 17], 6)]
+    whole = _generate(tiny_model_dir, prompts, prefix_backend="none", max_num_batched_tokens=512)
+    assert all(len(t) == 8 for t in whole)
+    assert _generate(tiny_model_dir, prompts, prefix_backend="radix", max_num_batched_tokens=32) == whole
+    assert _generate(tiny_model_dir, prompts, prefix_backend="none", num_kvcache_blocks=14) == whole
+    assert _generate(tiny_model_dir, prompts, kvcache_block_size=48, async_scheduling="on") == whole
+
+
+def test_engine_tp2_on_a_4_bit_cache_equals_one_rank(tiny_model_dir):
+    prompts = _prompts([16, 5, 33], 7)
+    assert _generate(tiny_model_dir, prompts, tp_size=2, nccl_port=29911) == _generate(tiny_model_dir, prompts)
+
+
+def test_pool_sizes_and_reads_its_tokens(tiny_model_dir):
+    from xixi_vllm_b200.config import load_model_config
+    from xixi_vllm_b200.parallel import groups
+    from xixi_vllm_b200.runtime.kv_pool import KVPool
+    groups.single_process_groups()
+    try:
+        cfg = load_model_config(tiny_model_dir)
+        pools = {t: KVPool(cfg, num_blocks=4, block_size=32, device="cpu", dtype=torch.bfloat16, cache_dtype=t)
+                 for t in ("auto", "int4")}
+        assert pools["auto"].bytes_per_block == 2 * 2 * 2 * 32 * 128
+        assert pools["int4"].bytes_per_block == 2 * 2 * 2 * 32 * 40
+        assert all(p.kv_cache.numel() * p.kv_cache.element_size() == 4 * p.bytes_per_block for p in pools.values())
+        n = {t: KVPool.auto_num_blocks(cfg, block_size=32, dtype=torch.bfloat16, device="cpu", gpu_memory_utilization=0.9,
+                                       cache_dtype=t) for t in pools}
+        assert n["int4"] == n["auto"] * 128 // 40
+        slots = torch.tensor([33, 2], dtype=torch.int32)
+        x = torch.randn(2, 2, 64).bfloat16()
+        for name, p in pools.items():
+            for c in (p.k_cache(1), p.v_cache(1)):
+                if name == "int4":
+                    kv4.write_rows(c, slots, x)
+                else:
+                    c[slots.long() // 32, :, slots.long() % 32] = x
+            k, v = p.read_tokens(1, slots)
+            assert k.shape == x.shape and torch.equal(k, v)
+            assert float((k - x).float().abs().max()) <= (0 if name == "auto" else 0.3)
+    finally:
+        groups.destroy_model_parallel()
+
+
+def test_configuration_and_command_lines(tiny_model_dir, tmp_path):
+    import run
+    from xixi_vllm_b200 import EngineConfig
+    from xixi_vllm_b200.models.synth import make_model_dir
+    from xixi_vllm_b200.utils.run_utils import engine_config_from
+    assert EngineConfig(model=tiny_model_dir, device="cpu").kv_cache_dtype == "auto"
+    with pytest.raises(ValueError, match="kv_cache_dtype must be"):
+        EngineConfig(model=tiny_model_dir, device="cpu", kv_cache_dtype="int8")
+    with pytest.raises(ValueError, match="head_dim 128"):
+        EngineConfig(model=tiny_model_dir, device="cuda", kv_cache_dtype="int4")      # head_dim 64
+    with pytest.raises(ValueError, match="head_dim"):
+        EngineConfig(model=make_model_dir(str(tmp_path), "tiny", weights=False, head_dim=40), device="cpu", kv_cache_dtype="int4")
+    args = run.build_parser().parse_args(["--model", tiny_model_dir, "--device", "cpu", "--kv-cache-dtype", "int4"])
+    assert engine_config_from(run.config_from_args(args), tiny_model_dir).kv_cache_dtype == "int4"

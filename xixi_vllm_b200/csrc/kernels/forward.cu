@@ -186,8 +186,12 @@ int xv_qwen3_forward(const XvModelDesc* m, const XvBatchDesc* b, const XvArena* 
   }
 
   const int n_dec = b->num_decode, n_pre = b->num_seqs - b->num_decode;
-  const int splits_attn = n_dec > 0 ? decode_splits(n_dec, m->hkv, a->num_sms, b->max_blocks * m->block_size) : 1;
-  if (n_dec > 0 && xv_attn_decode_workspace_bytes(n_dec, m->hq, D, splits_attn) > a->attn_ws_bytes) {
+  const int max_kv = b->max_blocks * m->block_size;
+  const int splits_attn = n_dec <= 0 ? 1
+                          : m->kv4   ? xv_kv4_decode_splits(n_dec, m->hkv, a->num_sms, max_kv)
+                                     : decode_splits(n_dec, m->hkv, a->num_sms, max_kv);
+  if (n_dec > 0 && (m->kv4 ? xv_kv4_decode_workspace_bytes(n_dec, m->hq, splits_attn)
+                           : xv_attn_decode_workspace_bytes(n_dec, m->hq, D, splits_attn)) > a->attn_ws_bytes) {
     g_failed_op = 20;
     return XV_ERR_WORKSPACE;
   }
@@ -203,7 +207,12 @@ int xv_qwen3_forward(const XvModelDesc* m, const XvBatchDesc* b, const XvArena* 
     await_rows_in_next_gemm(c);
     XV_TRY(30, xv_gemm_bf16_defer(a->h, w.qkv, a->qkv, T, m->qkv_rows, H, H, H, m->qkv_rows, a->gemm_ws,
                                   a->gemm_ws_bytes, a->num_sms, a->status, stream, &splits));
-    if (splits > 1) {
+    if (m->kv4) {
+      XV_TRY(36, xv_kv4_write(a->qkv, splits > 1 ? static_cast<const float*>(a->gemm_ws) : nullptr, splits,
+                              static_cast<long long>(T) * m->qkv_rows, w.q_norm, w.k_norm, m->eps, m->cos_sin, m->max_pos,
+                              b->positions, b->slots, a->q, w.k_cache, w.v_cache, T, m->hq, m->hkv, D, m->block_size,
+                              m->num_kv_blocks, a->status, stream));
+    } else if (splits > 1) {
       XV_TRY(31, xv_qk_norm_rope_cache_partials(static_cast<const float*>(a->gemm_ws), splits,
                                                 static_cast<long long>(T) * m->qkv_rows, w.q_norm, w.k_norm, m->eps,
                                                 m->cos_sin, b->positions, b->slots, a->q, w.k_cache, w.v_cache, T,
@@ -212,17 +221,28 @@ int xv_qwen3_forward(const XvModelDesc* m, const XvBatchDesc* b, const XvArena* 
       XV_TRY(32, xv_qk_norm_rope_cache(a->qkv, w.q_norm, w.k_norm, m->eps, m->cos_sin, b->positions, b->slots, a->q,
                                        w.k_cache, w.v_cache, T, m->hq, m->hkv, D, m->block_size, n_dec, stream));
     }
-    if (n_dec > 0)
-      XV_TRY(33, xv_attn_decode(a->q, w.k_cache, w.v_cache, b->block_tables, b->kv_lens, a->attn, n_dec, m->hq, m->hkv,
-                                D, m->block_size, b->max_blocks, m->attn_scale, splits_attn, a->attn_ws, stream));
-    if (n_pre > 0 && prefill_tc)
-      XV_TRY(35, xv_attn_prefill_tc(a->q, w.k_cache, w.v_cache, b->block_tables, b->cu_q, b->kv_lens, a->attn, n_dec,
-                                    n_pre, b->max_q_len, T, m->num_kv_blocks, m->hq, m->hkv, D, m->block_size,
-                                    b->max_blocks, m->attn_scale, a->status, stream));
-    else if (n_pre > 0)
-      XV_TRY(34, xv_attn_prefill(a->q, w.k_cache, w.v_cache, b->block_tables, b->cu_q, b->kv_lens, a->attn, n_dec,
-                                 n_pre, b->max_q_len, m->hq, m->hkv, D, m->block_size, b->max_blocks, m->attn_scale,
-                                 stream));
+    if (m->kv4) {
+      if (n_dec > 0)
+        XV_TRY(37, xv_kv4_decode(a->q, w.k_cache, w.v_cache, b->block_tables, b->kv_lens, a->attn, n_dec, m->hq, m->hkv, D,
+                                 m->block_size, b->max_blocks, m->num_kv_blocks, m->attn_scale, splits_attn, a->attn_ws,
+                                 a->attn_ws_bytes, a->status, stream));
+      if (n_pre > 0)
+        XV_TRY(38, xv_kv4_prefill(a->q, w.k_cache, w.v_cache, b->block_tables, b->cu_q, b->kv_lens, a->attn, n_dec, n_pre,
+                                  b->max_q_len, T, m->hq, m->hkv, D, m->block_size, b->max_blocks, m->num_kv_blocks,
+                                  m->attn_scale, a->status, stream));
+    } else {
+      if (n_dec > 0)
+        XV_TRY(33, xv_attn_decode(a->q, w.k_cache, w.v_cache, b->block_tables, b->kv_lens, a->attn, n_dec, m->hq, m->hkv,
+                                  D, m->block_size, b->max_blocks, m->attn_scale, splits_attn, a->attn_ws, stream));
+      if (n_pre > 0 && prefill_tc)
+        XV_TRY(35, xv_attn_prefill_tc(a->q, w.k_cache, w.v_cache, b->block_tables, b->cu_q, b->kv_lens, a->attn, n_dec,
+                                      n_pre, b->max_q_len, T, m->num_kv_blocks, m->hq, m->hkv, D, m->block_size,
+                                      b->max_blocks, m->attn_scale, a->status, stream));
+      else if (n_pre > 0)
+        XV_TRY(34, xv_attn_prefill(a->q, w.k_cache, w.v_cache, b->block_tables, b->cu_q, b->kv_lens, a->attn, n_dec,
+                                   n_pre, b->max_q_len, m->hq, m->hkv, D, m->block_size, b->max_blocks, m->attn_scale,
+                                   stream));
+    }
     {
       int rc = row_linear_reduce_norm(c, a->attn, w.o, q_cols, w.post_norm, false);
       if (rc) return rc;

@@ -293,6 +293,8 @@ typedef struct XvModelDesc {
   int is_first, is_last;              // pipeline stage: the first owns the embedding, the last the LM head; on
                                       // other stages `final_norm` is the next stage's first input norm and the
                                       // arena's h / residual are received from / sent to the neighbours
+  int kv4;                            // 1: k_cache / v_cache hold 4-bit rows (common/kv4.cuh)
+  int max_pos;                        // rows of cos_sin
 } XvModelDesc;
 
 typedef struct XvBatchDesc {

@@ -37,7 +37,8 @@ class ModelDesc(ctypes.Structure):
                 ("h_offset", _i64), ("buf_bytes", _i64), ("slots_offset", _i64), ("spin_us", ctypes.c_uint),
                 ("num_kv_blocks", _i32), ("prefill_tc", _i32), ("tp_push", _i32), ("tp_push_max", _i32),
                 ("tp_one_shot_max", _i32), ("tp_pull_two_shot", _i32), ("tp_defer_row_wait", _i32), ("is_first", _i32),
-                ("is_last", _i32)]
+                ("is_last", _i32),
+                ("kv4", _i32), ("max_pos", _i32)]
 
 
 class BatchDesc(ctypes.Structure):
@@ -95,6 +96,7 @@ class NativeForward:
         d.qkv_rows = attn0.qkv_proj.weight.shape[0]
         d.block_size = kv.block_size
         d.num_kv_blocks = kv.k_cache(0).shape[0]
+        d.kv4 = 1 if kv.int4 else 0
         d.prefill_tc = int(os.environ.get("XV_ATTN_PREFILL", "tc") != "mma")
         d.eps, d.attn_scale = float(cfg.rms_norm_eps), float(attn0.scale)
         d.gate_up_interleaved = 1 if first.mlp.gate_up_proj.interleave else 0
@@ -108,6 +110,7 @@ class NativeForward:
             d.lm_head = head.weight.data_ptr()
         else:
             d.final_norm = m.boundary_norm.weight.data_ptr()    # the next stage's first input norm
+        d.max_pos = attn0.rotary.cos_sin.shape[0]
         d.cos_sin = attn0.rotary.cos_sin.data_ptr()
         d.layers = ctypes.cast(self.layers, ctypes.POINTER(LayerWeights))
         comm = model.comm
@@ -154,16 +157,24 @@ class NativeForward:
         if not d.gate_up_interleaved:
             self.t["gu"] = buf(T, 2 * d.inter_local)
         st = cuda._state(self.t["h"])
-        need = L.xv_attn_decode_workspace_bytes(max_samples, d.hq, d.head_dim, 16)
-        if need > st.attn_ws.numel():
-            st.attn_ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        if d.kv4:
+            # splits shrink as the batch grows, so the largest need is looked for, up to the longest block table
+            tokens = -(-cfg.max_position_embeddings // d.block_size) * d.block_size
+            need = max(L.xv_kv4_decode_workspace_bytes(n, d.hq, L.xv_kv4_decode_splits(n, d.hkv, st.num_sms, tokens))
+                       for n in range(1, max_samples + 1))
+            attn_ws = self.t["attn_ws"] = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        else:
+            need = L.xv_attn_decode_workspace_bytes(max_samples, d.hq, d.head_dim, 16)
+            if need > st.attn_ws.numel():
+                st.attn_ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            attn_ws = st.attn_ws
         self._state = st
         a = Arena()
         for name in ("h", "qkv", "q", "attn", "act", "residual", "partial", "hidden_out", "logits", "tokens"):
             setattr(a, name, self.t[name].data_ptr())
         a.gu = self.t["gu"].data_ptr() if "gu" in self.t else None
         a.gemm_ws, a.gemm_ws_bytes = st.gemm_ws.data_ptr(), st.gemm_ws.numel()
-        a.attn_ws, a.attn_ws_bytes = st.attn_ws.data_ptr(), st.attn_ws.numel()
+        a.attn_ws, a.attn_ws_bytes = attn_ws.data_ptr(), attn_ws.numel()
         a.status, a.num_sms = st.status.data_ptr(), st.num_sms
         self.arena = a
         self.launches_per_call = 0

@@ -109,9 +109,11 @@ class Worker:
             n = KVPool.auto_num_blocks(cfg.hf_config, block_size=cfg.block_size, dtype=self.dtype,
                                        device=self.device, gpu_memory_utilization=cfg.gpu_memory_utilization,
                                        reserve_bytes=reserve if self.on_cuda else 0,
-                                       max_useful_tokens=cfg.max_num_seqs * cfg.context_len)
+                                       max_useful_tokens=cfg.max_num_seqs * cfg.context_len,
+                                       cache_dtype=cfg.kv_cache_dtype)
             cfg.num_kvcache_blocks = n
-        pool = KVPool(cfg.hf_config, num_blocks=n, block_size=cfg.block_size, device=self.device, dtype=self.dtype)
+        pool = KVPool(cfg.hf_config, num_blocks=n, block_size=cfg.block_size, device=self.device, dtype=self.dtype,
+                      cache_dtype=cfg.kv_cache_dtype)
         if self.rank == 0:
             gib = n * pool.bytes_per_block / 2**30
             print(f"[kv] {n} pages x {cfg.block_size} tokens = {n * cfg.block_size} tokens, {gib:.2f} GiB per rank")
