@@ -370,11 +370,12 @@ def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v
     return q
 
 
-def _vector(t, n: int, dtype, device, what: str) -> None:
-    """``t`` must hold at least ``n`` contiguous elements of ``dtype`` on ``device``."""
+def _vector(t, n: int, dtype, device, what: str) -> int:
+    """Address of ``t``, which must hold at least ``n`` contiguous elements of ``dtype`` on ``device``."""
     if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < n:
         raise ValueError(f"{what}: needs {n} contiguous {dtype} values on {device}, got {tuple(t.shape)} {t.dtype} on "
                          f"{t.device}")
+    return t.data_ptr()
 
 
 def _kv4_caches(k_cache, v_cache, head_dim: int, num_kv_heads: int | None = None) -> None:
@@ -383,89 +384,102 @@ def _kv4_caches(k_cache, v_cache, head_dim: int, num_kv_heads: int | None = None
         raise ValueError(f"4-bit caches on the GPU need head_dim 128, got {head_dim}")
 
 
+def _elsewhere(dev: torch.device) -> bool:
+    """Whether ``dev`` is not the current device: the caller then enters it (1.4 us that the usual call does not pay)."""
+    return dev.index != torch.cuda.current_device()
+
+
 def _kv4_write(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads, num_kv_heads, head_dim):
-    dev = k_cache.device
     _kv4_caches(k_cache, v_cache, head_dim, num_kv_heads)
-    _bf16(q_w, k_w)
+    dev = k_cache.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _kv4_write(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads, num_kv_heads,
+                              head_dim)
     part = isinstance(qkv, SplitKPartial)
-    cols = (num_q_heads + 2 * num_kv_heads) * head_dim
-    if len(qkv.shape) != 2 or qkv.shape[1] != cols or qkv.device != dev:
-        raise ValueError(f"qk_norm_rope_cache: qkv must be [T, {cols}] on {dev}, got {tuple(qkv.shape)} on {qkv.device}")
+    T, cols = qkv.shape if len(qkv.shape) == 2 else (0, -1)
+    if cols != (num_q_heads + 2 * num_kv_heads) * head_dim or qkv.device != dev:
+        raise ValueError(f"qk_norm_rope_cache: qkv must be [T, {(num_q_heads + 2 * num_kv_heads) * head_dim}] on {dev}, got "
+                         f"{tuple(qkv.shape)} on {qkv.device}")
     if not part:
         _bf16(qkv)
         if not qkv.is_contiguous():
             raise ValueError("qk_norm_rope_cache needs contiguous qkv and cache tensors")
-    T = qkv.shape[0]
-    _vector(q_w, head_dim, torch.bfloat16, dev, "q_w")
-    _vector(k_w, head_dim, torch.bfloat16, dev, "k_w")
-    _vector(cos_sin, head_dim, torch.float32, dev, "cos_sin")
-    _vector(positions, T, torch.int32, dev, "positions")
-    _vector(slots, T, torch.int32, dev, "slots")
-    with torch.cuda.device(dev):
-        q = torch.empty((T, num_q_heads * head_dim), dtype=torch.bfloat16, device=dev)
-        if T:
-            _check(lib().xv_kv4_write(
-                None if part else qkv.data_ptr(), qkv.ws.data_ptr() if part else None, qkv.splits if part else 0,
-                qkv.stride_elems if part else 0, q_w.data_ptr(), k_w.data_ptr(), eps, cos_sin.data_ptr(),
-                cos_sin.numel() // head_dim, positions.data_ptr(), slots.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
-                v_cache.data_ptr(), T, num_q_heads, num_kv_heads, head_dim, k_cache.shape[2], k_cache.shape[0],
-                _state(k_cache).status.data_ptr(), _stream()), "kv4_write")
+    _bf16(q_w, k_w)
+    rows = cos_sin.numel() // head_dim
+    args = (None if part else qkv.data_ptr(), qkv.ws.data_ptr() if part else None, qkv.splits if part else 0,
+            qkv.stride_elems if part else 0, _vector(q_w, head_dim, torch.bfloat16, dev, "q_w"),
+            _vector(k_w, head_dim, torch.bfloat16, dev, "k_w"), eps,
+            _vector(cos_sin, head_dim, torch.float32, dev, "cos_sin"), rows,
+            _vector(positions, T, torch.int32, dev, "positions"), _vector(slots, T, torch.int32, dev, "slots"))
+    q = q_w.new_empty((T, num_q_heads * head_dim))
+    if T:
+        nb, _, bs, _ = k_cache.shape
+        _check(lib().xv_kv4_write(*args, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), T, num_q_heads, num_kv_heads,
+                                  head_dim, bs, nb, _state(k_cache).status.data_ptr(),
+                                  torch._C._cuda_getCurrentRawStream(dev.index)), "kv4_write")
     return q
 
 
 def read_cache(k_cache, v_cache, slots, head_dim):
     """bf16 rows of a 4-bit cache (see ``dispatch.read_cache``). A slot beyond the cache gives zeros and status 5."""
-    dev = k_cache.device
     _kv4_caches(k_cache, v_cache, head_dim)
-    T, hkv = slots.numel(), k_cache.shape[1]
-    _vector(slots, T, torch.int32, dev, "slots")
-    with torch.cuda.device(dev):
-        out = torch.empty((2, T, hkv, head_dim), dtype=torch.bfloat16, device=dev)
-        if T:
-            _check(lib().xv_kv4_read(k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), out[0].data_ptr(),
-                                     out[1].data_ptr(), T, hkv, head_dim, k_cache.shape[2], k_cache.shape[0],
-                                     _state(k_cache).status.data_ptr(), _stream()), "kv4_read")
-    return out[0], out[1]
+    dev = k_cache.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return read_cache(k_cache, v_cache, slots, head_dim)
+    T = slots.numel()
+    nb, hkv, bs, _ = k_cache.shape
+    at = _vector(slots, T, torch.int32, dev, "slots")
+    k = k_cache.new_empty((T, hkv, head_dim), dtype=torch.bfloat16)
+    v = torch.empty_like(k)
+    if T:
+        _check(lib().xv_kv4_read(k_cache.data_ptr(), v_cache.data_ptr(), at, k.data_ptr(), v.data_ptr(), T, hkv, head_dim,
+                                 bs, nb, _state(k_cache).status.data_ptr(),
+                                 torch._C._cuda_getCurrentRawStream(dev.index)), "kv4_read")
+    return k, v
 
 
 def _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
-    dev = k_cache.device
     _kv4_caches(k_cache, v_cache, head_dim, num_kv_heads)
+    dev = k_cache.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim)
     _bf16(q)
-    bt, n_d, n_p = attn.block_tables, attn.num_decode, attn.num_seqs - attn.num_decode
+    bt, B, n_d = attn.block_tables, attn.num_seqs, attn.num_decode
+    n_p = B - n_d
     if q.dim() != 2 or q.shape[1] != num_q_heads * head_dim or not q.is_contiguous() or q.device != dev:
         raise ValueError(f"paged_attention: q must be a contiguous [T, {num_q_heads * head_dim}] tensor on {dev}")
-    if num_q_heads % num_kv_heads or num_q_heads // num_kv_heads > 16:
+    if num_q_heads % num_kv_heads or num_q_heads > 16 * num_kv_heads:
         raise ValueError(f"paged_attention: {num_q_heads} query heads over {num_kv_heads} KV heads (at most 16 to one)")
-    if n_d < 0 or n_p < 0 or n_d > q.shape[0] or bt.dim() != 2 or bt.shape[0] < attn.num_seqs:
-        raise ValueError(f"paged_attention: {n_d} decode rows and {n_p} chunks for {q.shape[0]} query rows and a block "
-                         f"table of {tuple(bt.shape)}")
-    if attn.num_seqs > 65535:
+    T = q.shape[0]
+    if n_d < 0 or n_p < 0 or n_d > T or bt.dim() != 2 or bt.shape[0] < B:
+        raise ValueError(f"paged_attention: {n_d} decode rows and {n_p} chunks for {T} query rows and a block table of "
+                         f"{tuple(bt.shape)}")
+    if B > 65535:
         raise ValueError("paged_attention: at most 65535 sequences")
-    _vector(bt, attn.num_seqs * bt.shape[1], torch.int32, dev, "block_tables")
-    _vector(attn.kv_lens, attn.num_seqs, torch.int32, dev, "kv_lens")
+    maxb = bt.shape[1]
+    tables = _vector(bt, B * maxb, torch.int32, dev, "block_tables")
+    lens = _vector(attn.kv_lens, B, torch.int32, dev, "kv_lens")
+    nb, _, bs, _ = k_cache.shape
+    out = torch.empty_like(q)
+    if maxb == 0 or nb == 0:        # nothing is cached: every row is empty
+        return out.zero_()
+    L, st, stream = lib(), _state(q), torch._C._cuda_getCurrentRawStream(dev.index)
+    if n_d:
+        splits = L.xv_kv4_decode_splits(n_d, num_kv_heads, st.num_sms, maxb * bs)
+        need = L.xv_kv4_decode_workspace_bytes(n_d, num_q_heads, splits) if splits > 1 else 0
+        # from torch's allocator, call by call: calls on two streams, or two captured graphs, never share it
+        ws = k_cache.new_empty(need) if need else None
+        _check(L.xv_kv4_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), tables, lens, out.data_ptr(), n_d,
+                               num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale, splits,
+                               ws.data_ptr() if need else None, need, st.status.data_ptr(), stream), "kv4_decode")
     if n_p:
-        _vector(attn.cu_q, attn.num_seqs + 1, torch.int32, dev, "cu_q")
-    L, bs, nb, maxb = lib(), k_cache.shape[2], k_cache.shape[0], bt.shape[1]
-    with torch.cuda.device(dev):
-        st = _state(q)
-        out = torch.empty_like(q)
-        if maxb == 0 or nb == 0:        # nothing is cached: every row is empty
-            return out.zero_()
-        if n_d:
-            splits = L.xv_kv4_decode_splits(n_d, num_kv_heads, st.num_sms, maxb * bs)
-            need = L.xv_kv4_decode_workspace_bytes(n_d, num_q_heads, splits)
-            # from torch's allocator, call by call: calls on two streams, or two captured graphs, never share it
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            _check(L.xv_kv4_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(),
-                                   attn.kv_lens.data_ptr(), out.data_ptr(), n_d, num_q_heads, num_kv_heads, head_dim, bs,
-                                   maxb, nb, scale, splits, ws.data_ptr() if need else None, need, st.status.data_ptr(),
-                                   _stream()), "kv4_decode")
-        if n_p:
-            _check(L.xv_kv4_prefill(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(),
-                                    attn.cu_q.data_ptr(), attn.kv_lens.data_ptr(), out.data_ptr(), n_d, n_p,
-                                    attn.max_q_len, q.shape[0], num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale,
-                                    st.status.data_ptr(), _stream()), "kv4_prefill")
+        _check(L.xv_kv4_prefill(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), tables,
+                                _vector(attn.cu_q, B + 1, torch.int32, dev, "cu_q"), lens, out.data_ptr(), n_d, n_p,
+                                attn.max_q_len, T, num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale,
+                                st.status.data_ptr(), stream), "kv4_prefill")
     return out
 
 
