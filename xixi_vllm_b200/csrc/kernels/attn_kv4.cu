@@ -1,20 +1,26 @@
 // Paged causal GQA attention over a KV cache held in 4 bits (format: common/kv4.cuh), head_dim 128.
 //
-//   kv4_decode_kernel  - one query row per sequence; a CTA owns (sequence, KV head, KV split), its 4 warps take 16-token
-//                        units in turn. Tokens are the M rows of both products and the group's query heads (up to 8, or
-//                        16 as two column tiles) the N columns, so one MMA covers 16 x 16 cache values:
+//   kv4_decode_kernel  - one query row per sequence; a cluster of CTAs, one per KV split, owns (sequence, KV head). Each
+//                        of a CTA's 8 warps streams its own 16-token units through a ring of shared-memory slots (five
+//                        16-byte cp.async a lane for K and V; no block-wide barrier in the loop). Tokens
+//                        are the M rows of both products and the group's query heads (up to 8, or 16 as two column
+//                        tiles) the N columns, so one MMA covers 16 x 16 cache values:
 //                          S^T[token, head] = s_g * (n Q^T) + c_g * sum(Q)   per channel group g
 //                          O^T[channel, head] = (n - 8)^T (s_g P) + c_g^T P
 //                        The MMAs see the codes as exact bf16 integers; scales and centres stay in fp32 (the scale of V
-//                        is folded into P before its one rounding to bf16). Codes go from global memory to MMA operands
-//                        in registers: K's lanes own 16-byte pieces of a row, V's lanes pair two tokens with PRMT.
-//   kv4_combine_kernel - joins the splits.
+//                        is folded into P before its one rounding to bf16). K's lanes own 16-byte pieces of a row, V's
+//                        lanes pair two tokens with PRMT, so codes go from shared memory to MMA operands in registers.
+//                        Warps are merged through shared memory, splits through the cluster's distributed shared
+//                        memory: one launch, no workspace.
 //   kv4_prefill_kernel - packed query chunks: 64 query rows of one head per CTA, KV tiles of 64 tokens dequantised to
 //                        bf16 in shared memory.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
+
+#include <algorithm>
+#include <atomic>
 
 #include "../common/kv4.cuh"
 #include "../common/launch.cuh"
@@ -28,7 +34,6 @@ using namespace xv;
 constexpr int kD = kv4::kD;
 constexpr int kIdDecode = 10, kIdPrefill = 11;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kDecWarps = 4;
 
 struct Params {
   const __nv_bfloat16* q;
@@ -38,8 +43,8 @@ struct Params {
   const int* cu_q;
   const int* kv_lens;
   __nv_bfloat16* out;
-  float* ws_o;      // [seq, hq, split, 128]
-  float* ws_lse;    // [seq, hq, split]
+  float* ws_o;      // [seq, hq, split, 128], when the splits do not fit a cluster
+  float* ws_ml;     // [seq, hq, split, 2]: maximum (log2 units), sum
   int* status;
   int hq, hkv, block_size, max_blocks, num_blocks, splits, seq_begin, total_rows;
   float scale_log2;
@@ -72,36 +77,123 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   return d;
 }
 
-// NT: column tiles of 8 query heads.
-template <int NT>
-__global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Params p) {
+// Token of row r (0..7) of an 8-row group of the MMAs. V's lanes read the tokens of rows 2t and 2t + 1: with this order
+// their four 64-byte rows start on alternating halves of the 128-byte bank line (two-way conflicts, not four-way).
+__device__ __forceinline__ int token_of_row(int r) { return ((r >> 1) ^ (r & 1)) + 4 * (r & 1); }
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void cp_async16_u32(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+constexpr int kStages = 3;               // ring slots of a warp
+constexpr int kPair = 2;                 // units per slot: two independent chains of work per iteration of a warp
+constexpr int kUnitSlot = 2 * kv4::kUnitBytes;
+constexpr int kSlot = kPair * kUnitSlot;
+constexpr float kNoMax = -3.0e38f;       // finite, so that "nothing seen yet" needs no case of its own
+constexpr float kLazy = 8.f;             // log2 units a running maximum may lag behind
+
+constexpr int decode_smem(int warps) { return warps * kStages * kSlot; }
+
+// D = A B: the first product of an accumulation.
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// NT: column tiles of 8 query heads; W: warps.
+template <int NT, int W>
+__global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_kernel(const Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float sm_m[W][8 * NT], sm_l[W][8 * NT];
+  __shared__ float part_o[8 * NT][kD], part_m[8 * NT], part_l[8 * NT];     // this CTA's result, read by the cluster
   grid_dep_launch();
-  grid_dep_wait();
-  __shared__ float sm_o[kDecWarps][8 * NT][kD];
-  __shared__ float sm_m[kDecWarps][8 * NT], sm_l[kDecWarps][8 * NT];
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int G = p.hq / p.hkv;
+  uint8_t* ring = smem + warp * kStages * kSlot;
+  grid_dep_wait();
   const int kv_len = kv_len_of(p, b, kIdDecode);
+  // Consecutive units per warp, so that a page and a place in it follow from the ones before without a division.
   const int tiles = (kv_len + 15) / 16;
-  const int per = (tiles + p.splits - 1) / p.splits;
-  const int tile1 = min((split + 1) * per, tiles);
-  const int units_per_page = p.block_size / kv4::kUnit;
+  const int per = (tiles + p.splits * W - 1) / (p.splits * W);
+  const int tile0 = min((split * W + warp) * per, tiles);
+  const int n_tiles = min(per, tiles - tile0);
+  const int upp = p.block_size / kv4::kUnit;
+
+  // Pages are looked up 32 at a time, one batch ahead of use.
+  const int page0 = tile0 / upp, last_page = max(0, (tiles - 1) / upp);
+  auto lookup = [&](int i) { return page_of(p, b, min(page0 + i, last_page), kIdDecode); };
+  int pages = 0, pages_next = 0;
+  if (n_tiles > 0) {
+    pages = lookup(lane);
+    pages_next = lookup(32 + lane);
+  }
+  // A unit in a slot: K's 1152 bytes, then V's. Five copies of 16 bytes a lane: K's codes, V's codes, and both parameter
+  // blocks by half a warp.
+  const uint32_t page_bytes = static_cast<uint32_t>(p.hkv) * upp * kv4::kUnitBytes;
+  const uint8_t* k_src = p.k_cache + static_cast<size_t>(h) * upp * kv4::kUnitBytes + lane * 16;
+  const uint8_t* v_src = p.v_cache + static_cast<size_t>(h) * upp * kv4::kUnitBytes + lane * 16;
+  const uint8_t* par_src = (lane < 8 ? k_src : v_src - 128) + kv4::kParBase;
+  const uint32_t ring_u32 = smem_u32(ring) + lane * 16;
+  const uint32_t par_dst = (lane < 8 ? 0 : kv4::kUnitBytes - 128) + kv4::kParBase;
+  int page_i = 0, place = tile0 - page0 * upp;               // of the next unit to fetch
+  unsigned fetched = 0, slot_in = 0;
+  auto issue = [&]() {                                       // the next kPair units into the next slot
+#pragma unroll
+    for (int u = 0; u < kPair; ++u) {
+      if (fetched < static_cast<unsigned>(n_tiles)) {
+        if (place == upp) {
+          place = 0;
+          if ((++page_i & 31) == 0) {
+            pages = pages_next;
+            pages_next = lookup(page_i + 32 + lane);
+          }
+        }
+        const uint32_t blk = __shfl_sync(0xffffffffu, pages, page_i & 31);
+        const uint64_t at = static_cast<uint64_t>(blk) * page_bytes + static_cast<uint32_t>(place * kv4::kUnitBytes);
+        const uint32_t dst = ring_u32 + slot_in * kSlot + u * kUnitSlot;
+        cp_async16_u32(dst, k_src + at);
+        cp_async16_u32(dst + 512, k_src + at + 512);
+        cp_async16_u32(dst + kv4::kUnitBytes, v_src + at);
+        cp_async16_u32(dst + kv4::kUnitBytes + 512, v_src + at + 512);
+        if (lane < 16) cp_async16_u32(dst + par_dst, par_src + at);
+        ++place;
+        ++fetched;
+      }
+    }
+    cp_async_commit();                                       // one group per call, empty ones included
+    slot_in = slot_in == kStages - 1 ? 0 : slot_in + 1;
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue();
 
   // Q as the B operand: MMA (word w, half hf) of lane (g, t) multiplies channels 32 t + 8 w + 2 hf + {0, 4, 1, 5}.
   uint32_t qf[NT][4][2][2];
-  float qs[NT][2][2];      // sum of Q over each group for heads 2t, 2t + 1 of the tile
+  // The centres' share of a score, sum over groups of c_g Qs_g - 136 s_g Qs_g with Qs_g the group's sum of Q, is one more
+  // MMA: its A operand is the parameter words as stored, its B operand {-136 Qs_g, Qs_g} as three bf16 terms (24 bits).
+  uint32_t qc[NT][2];
+  // A negative scale is Q's sign, so the running maxima need not know it; zero becomes a scale too small to matter.
+  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+  const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int head = nt * 8 + g;
-    uint4 raw[4];
     const uint4* src = reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(b) * p.hq + h * G + head) * kD + 32 * t);
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      raw[w] = head < G ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
-      const uint32_t r[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
+      const uint4 raw = head < G ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
+      const uint32_t r[4] = {raw.x ^ flip, raw.y ^ flip, raw.z ^ flip, raw.w ^ flip};
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         qf[nt][w][hf][0] = __byte_perm(r[hf], r[hf + 2], 0x5410);     // channels 2 hf, 2 hf + 4
@@ -114,14 +206,19 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Params
     for (int gr = 0; gr < 2; ++gr) {
       sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
       sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
-      qs[nt][gr][0] = __shfl_sync(0xffffffffu, sum[gr], (2 * t) * 4);
-      qs[nt][gr][1] = __shfl_sync(0xffffffffu, sum[gr], (2 * t + 1) * 4);
     }
+    // Lane (g, t) holds K rows 2t, 2t + 1 of B (first register) and 2t + 8, 2t + 9 (second): group t & 1; the first term
+    // for t < 2, the second for t >= 2, the third in the second register for t < 2.
+    const float qs = (t & 1) ? sum[1] : sum[0], bs = -kv4::kBias * qs;
+    const float q1 = __bfloat162float(__float2bfloat16(qs)), b1 = __bfloat162float(__float2bfloat16(bs));
+    const float q2 = __bfloat162float(__float2bfloat16(qs - q1)), b2 = __bfloat162float(__float2bfloat16(bs - b1));
+    qc[nt][0] = t < 2 ? pack_bf16(b1, q1) : pack_bf16(b2, q2);
+    qc[nt][1] = t < 2 ? pack_bf16(bs - b1 - b2, qs - q1 - q2) : 0u;
   }
 
   float o[NT][2][4][4];            // [group][MMA]: rows g, g + 8 = channels 16 g + 8 group + 2 i + {0, 1}; heads 2t, 2t+1
   float cen[NT][2][2];             // sum of P * centre, this lane's tokens
-  float m[NT][2], l[NT][2];
+  float m[NT][2], l[NT][2];        // running maximum of the unscaled scores, sum of P
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -130,106 +227,158 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Params
       for (int i = 0; i < 4; ++i) o[nt][gr][i][0] = o[nt][gr][i][1] = o[nt][gr][i][2] = o[nt][gr][i][3] = 0.f;
       cen[nt][gr][0] = cen[nt][gr][1] = 0.f;
     }
-    m[nt][0] = m[nt][1] = -CUDART_INF_F;
+    m[nt][0] = m[nt][1] = kNoMax;
     l[nt][0] = l[nt][1] = 0.f;
   }
+  const float lag = kLazy / scale;
 
-  for (int tile = split * per + warp; tile < tile1; tile += kDecWarps) {
-    const int blk = page_of(p, b, tile / units_per_page, kIdDecode);
-    const size_t unit = (static_cast<size_t>(blk) * p.hkv + h) * units_per_page * kv4::kUnitBytes +
-                        static_cast<size_t>(tile % units_per_page) * kv4::kUnitBytes;
-    const uint8_t* ku = p.k_cache + unit;
-    const uint8_t* vu = p.v_cache + unit;
-    const uint4 k0 = __ldg(reinterpret_cast<const uint4*>(ku + g * 64 + t * 16));
-    const uint4 k1 = __ldg(reinterpret_cast<const uint4*>(ku + (g + 8) * 64 + t * 16));
-    const uint2 kp0 = __ldg(reinterpret_cast<const uint2*>(ku + kv4::kParBase + g * 8));
-    const uint2 kp1 = __ldg(reinterpret_cast<const uint2*>(ku + kv4::kParBase + (g + 8) * 8));
-    uint2 vp0 = __ldg(reinterpret_cast<const uint2*>(vu + kv4::kParBase + g * 8));
-    uint2 vp1 = __ldg(reinterpret_cast<const uint2*>(vu + kv4::kParBase + (g + 8) * 8));
-    uint2 vw[4];
+  const int tok = token_of_row(g);
+  const uint8_t* const lane_k = ring + tok * 64 + t * 16;
+  const uint8_t* const lane_p = ring + kv4::kParBase + tok * 8;
+  const uint8_t* const lane_v0 = ring + kv4::kUnitBytes + token_of_row(2 * t) * 64 + g * 8;
+  const uint8_t* const lane_v1 = ring + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8;
+  int left = kv_len - tile0 * 16;        // tokens from the slot's first unit on
+  unsigned slot = 0;
+  for (int i = 0; i < n_tiles; i += kPair, left -= 16 * kPair) {
+    cp_async_wait<kStages - 2>();
+    __syncwarp();                        // everyone's part of the slot has landed, and everyone has read the slot filled next
+    issue();
+    const unsigned at = slot * kSlot;
+    slot = slot == kStages - 1 ? 0 : slot + 1;
+    // With an odd number of units the second half of the last slot is an old unit whose tokens are all past the end of
+    // this warp's range.
+    const int mine = min(left, (n_tiles - i) * 16);
+    float x[kPair][NT][4];               // (row g: heads 2t, 2t + 1), (row g + 8: the same)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)      // tokens 2t, 2t + 1, 2t + 8, 2t + 9
-      vw[i] = __ldg(reinterpret_cast<const uint2*>(vu + (2 * t + (i & 1) + 8 * (i >> 1)) * 64 + g * 8));
-
-    const uint32_t ka[4] = {k0.x, k0.y, k0.z, k0.w}, kb[4] = {k1.x, k1.y, k1.z, k1.w};
-    const bool in0 = tile * 16 + g < kv_len, in1 = tile * 16 + g + 8 < kv_len;
-    if (!in0) vp0 = make_uint2(0u, 0u);      // rows past the end: P is 0 and whatever parameters an earlier owner of the
-    if (!in1) vp1 = make_uint2(0u, 0u);      // page left (NaN among them) must not reach the sums; codes are always finite
-    const uint32_t kpar[2][2] = {{kp0.x, kp1.x}, {kp0.y, kp1.y}}, vpar[2][2] = {{vp0.x, vp1.x}, {vp0.y, vp1.y}};
-    uint32_t pf[NT][2][2];           // P * s_g as the B operand of the second product
+    for (int u = 0; u < kPair; ++u) {
+      const uint4 k0 = *reinterpret_cast<const uint4*>(lane_k + at + u * kUnitSlot);
+      const uint4 k1 = *reinterpret_cast<const uint4*>(lane_k + at + u * kUnitSlot + 8 * 64);
+      const uint2 kp0 = *reinterpret_cast<const uint2*>(lane_p + at + u * kUnitSlot);
+      const uint2 kp1 = *reinterpret_cast<const uint2*>(lane_p + at + u * kUnitSlot + 64);
+      const uint32_t ka[4] = {k0.x, k0.y, k0.z, k0.w}, kb[4] = {k1.x, k1.y, k1.z, k1.w};
+      const uint32_t w0 = (t & 1) ? kp0.y : kp0.x, w1 = (t & 1) ? kp1.y : kp1.x;
+      const uint32_t ac[4] = {w0, w1, w0, w1};
+      float s[NT][2][4], sc[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      for (int nt = 0; nt < NT; ++nt) mma_first(sc[nt], ac, qc[nt][0], qc[nt][1]);
 #pragma unroll
       for (int w = 0; w < 4; ++w)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const uint32_t a[4] = {kv4::biased(ka[w], 8 * hf), kv4::biased(kb[w], 8 * hf), kv4::biased(ka[w], 8 * hf + 4),
                                  kv4::biased(kb[w], 8 * hf + 4)};
-          mma_bf16_16816(s[w & 1], a, qf[nt][w][hf][0], qf[nt][w][hf][1]);
-        }
-      float x[4];                    // (token g: heads 2t, 2t+1), (token g + 8: the same)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = e >> 1, hd = e & 1;
-        const float s0 = kv4::par_s(kpar[0][row]), s1 = kv4::par_s(kpar[1][row]);
-        const float c0 = kv4::par_c(kpar[0][row]) - kv4::kBias * s0, c1 = kv4::par_c(kpar[1][row]) - kv4::kBias * s1;
-        x[e] = (s0 * s[0][e] + c0 * qs[nt][0][hd]) + (s1 * s[1][e] + c1 * qs[nt][1][hd]);
-        x[e] = (row ? in1 : in0) ? x[e] * p.scale_log2 : -CUDART_INF_F;
-      }
-#pragma unroll
-      for (int hd = 0; hd < 2; ++hd) {
-        float mx = fmaxf(x[hd], x[2 + hd]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float mn = fmaxf(m[nt][hd], mx), base = mn == -CUDART_INF_F ? 0.f : mn;
-        const float cr = exp2f(m[nt][hd] - base);
-        m[nt][hd] = mn;
-        l[nt][hd] *= cr;
-#pragma unroll
-        for (int gr = 0; gr < 2; ++gr) {
-          cen[nt][gr][hd] *= cr;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            o[nt][gr][i][hd] *= cr;
-            o[nt][gr][i][2 + hd] *= cr;
+          for (int nt = 0; nt < NT; ++nt) {
+            if (w < 2 && hf == 0) mma_first(s[nt][w], a, qf[nt][w][hf][0], qf[nt][w][hf][1]);
+            else mma_bf16_16816(s[nt][w & 1], a, qf[nt][w][hf][0], qf[nt][w][hf][1]);
           }
         }
-        x[hd] = exp2f(x[hd] - base);
-        x[2 + hd] = exp2f(x[2 + hd] - base);
-        l[nt][hd] += x[hd] + x[2 + hd];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint2 kp = e < 2 ? kp0 : kp1;
+          x[u][nt][e] = fmaf(kv4::par_s(kp.x), s[nt][0][e], fmaf(kv4::par_s(kp.y), s[nt][1][e], sc[nt][e]));
+        }
+    }
+    const bool ragged = mine < 16 * kPair;               // warp-uniform
+    if (ragged) {
+#pragma unroll
+      for (int u = 0; u < kPair; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (16 * u + tok >= mine) x[u][nt][0] = x[u][nt][1] = -CUDART_INF_F;
+          if (16 * u + tok + 8 >= mine) x[u][nt][2] = x[u][nt][3] = -CUDART_INF_F;
+        }
+    }
+    bool grow = false;
+    float mx[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int hd = 0; hd < 2; ++hd) {
+        mx[nt][hd] = fmaxf(fmaxf(x[0][nt][hd], x[0][nt][2 + hd]), fmaxf(x[1][nt][hd], x[1][nt][2 + hd]));
+        grow |= mx[nt][hd] > m[nt][hd] + lag;
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int hd = 0; hd < 2; ++hd) {
+          float mn = fmaxf(m[nt][hd], mx[nt][hd]);
+          mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 4));
+          mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 8));
+          mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 16));
+          const float cr = exp2f((m[nt][hd] - mn) * scale);
+          m[nt][hd] = mn;
+          l[nt][hd] *= cr;
+#pragma unroll
+          for (int gr = 0; gr < 2; ++gr) {
+            cen[nt][gr][hd] *= cr;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o[nt][gr][j][hd] *= cr;
+              o[nt][gr][j][2 + hd] *= cr;
+            }
+          }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kPair; ++u) {
+      uint2 vp0 = *reinterpret_cast<const uint2*>(lane_p + at + u * kUnitSlot + kv4::kUnitBytes);
+      uint2 vp1 = *reinterpret_cast<const uint2*>(lane_p + at + u * kUnitSlot + kv4::kUnitBytes + 64);
+      uint2 vw[4];                       // tokens of rows 2t, 2t + 1, then the same 8 further
+      vw[0] = *reinterpret_cast<const uint2*>(lane_v0 + at + u * kUnitSlot);
+      vw[1] = *reinterpret_cast<const uint2*>(lane_v1 + at + u * kUnitSlot);
+      vw[2] = *reinterpret_cast<const uint2*>(lane_v0 + at + u * kUnitSlot + 8 * 64);
+      vw[3] = *reinterpret_cast<const uint2*>(lane_v1 + at + u * kUnitSlot + 8 * 64);
+      if (ragged) {                      // P is 0 there, and whatever parameters an earlier owner of the page left (NaN
+        if (16 * u + tok >= mine) vp0 = make_uint2(0u, 0u);        // among them) must not reach the sums; codes are
+        if (16 * u + tok + 8 >= mine) vp1 = make_uint2(0u, 0u);    // always finite
+      }
+      const uint32_t vpar[2][2] = {{vp0.x, vp1.x}, {vp0.y, vp1.y}};
+      uint32_t pf[NT][2][2];             // P * s_g as the B operand of the second product
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float pr[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][nt][e], scale, -m[nt][e & 1] * scale));
+        l[nt][0] += pr[0] + pr[2];
+        l[nt][1] += pr[1] + pr[3];
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr) {
+          const float s0 = kv4::par_s(vpar[gr][0]), s1 = kv4::par_s(vpar[gr][1]);
+          pf[nt][gr][0] = movmatrix_trans(pack_bf16(pr[0] * s0, pr[1] * s0));
+          pf[nt][gr][1] = movmatrix_trans(pack_bf16(pr[2] * s1, pr[3] * s1));
+          const float c0 = kv4::par_c(vpar[gr][0]), c1 = kv4::par_c(vpar[gr][1]);
+          cen[nt][gr][0] += pr[0] * c0 + pr[2] * c1;
+          cen[nt][gr][1] += pr[1] * c0 + pr[3] * c1;
+        }
       }
 #pragma unroll
       for (int gr = 0; gr < 2; ++gr) {
-        const float s0 = kv4::par_s(vpar[gr][0]), s1 = kv4::par_s(vpar[gr][1]);
-        pf[nt][gr][0] = movmatrix_trans(pack_bf16(x[0] * s0, x[1] * s0));
-        pf[nt][gr][1] = movmatrix_trans(pack_bf16(x[2] * s1, x[3] * s1));
-        const float c0 = kv4::par_c(vpar[gr][0]), c1 = kv4::par_c(vpar[gr][1]);
-        cen[nt][gr][0] += x[0] * c0 + x[2] * c1;
-        cen[nt][gr][1] += x[1] * c0 + x[3] * c1;
-      }
-    }
+        const uint32_t w0 = gr ? vw[0].y : vw[0].x, w1 = gr ? vw[1].y : vw[1].x, w2 = gr ? vw[2].y : vw[2].x,
+                       w3 = gr ? vw[3].y : vw[3].x;
 #pragma unroll
-    for (int gr = 0; gr < 2; ++gr) {
-      const uint32_t w0 = gr ? vw[0].y : vw[0].x, w1 = gr ? vw[1].y : vw[1].x, w2 = gr ? vw[2].y : vw[2].x,
-                     w3 = gr ? vw[3].y : vw[3].x;
+        for (int hl = 0; hl < 2; ++hl) {               // low / high half of the word: channels 0-3 / 4-7
+          const uint32_t sel = hl ? 0x7632 : 0x5410;
+          const uint32_t u0 = __byte_perm(w0, w1, sel), u1 = __byte_perm(w2, w3, sel);
 #pragma unroll
-      for (int hl = 0; hl < 2; ++hl) {               // low / high half of the word: channels 0-3 / 4-7
-        const uint32_t sel = hl ? 0x7632 : 0x5410;
-        const uint32_t u0 = __byte_perm(w0, w1, sel), u1 = __byte_perm(w2, w3, sel);
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t a[4] = {kv4::centred(kv4::biased(u0, 8 * j)), kv4::centred(kv4::biased(u0, 8 * j + 4)),
+                                   kv4::centred(kv4::biased(u1, 8 * j)), kv4::centred(kv4::biased(u1, 8 * j + 4))};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t a[4] = {kv4::centred(kv4::biased(u0, 8 * i)), kv4::centred(kv4::biased(u0, 8 * i + 4)),
-                                 kv4::centred(kv4::biased(u1, 8 * i)), kv4::centred(kv4::biased(u1, 8 * i + 4))};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][gr][hl * 2 + i], a, pf[nt][gr][0], pf[nt][gr][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][gr][hl * 2 + j], a, pf[nt][gr][0], pf[nt][gr][1]);
+          }
         }
       }
     }
   }
+  cp_async_wait<0>();
 
-  // Sums over the token lanes, then the warps through shared memory.
+  // Sums over the token lanes, then the warps through the (now idle) ring.
+  __syncthreads();
+  float* sm_o = reinterpret_cast<float*>(smem);                    // [warp][8 NT][128]
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -241,57 +390,85 @@ __global__ void __launch_bounds__(kDecWarps * 32) kv4_decode_kernel(const Params
         cen[nt][1][hd] += __shfl_xor_sync(0xffffffffu, cen[nt][1][hd], x);
       }
       const int head = nt * 8 + 2 * t + hd;
+      if (head < G) {
 #pragma unroll
-      for (int gr = 0; gr < 2; ++gr)
+        for (int gr = 0; gr < 2; ++gr)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<float2*>(&sm_o[warp][head][16 * g + 8 * gr + 2 * i]) =
-              make_float2(o[nt][gr][i][hd] + cen[nt][gr][hd], o[nt][gr][i][2 + hd] + cen[nt][gr][hd]);
-      if (g == 0) {
-        sm_m[warp][head] = m[nt][hd];
-        sm_l[warp][head] = l[nt][hd];
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float2*>(&sm_o[(warp * 8 * NT + head) * kD + 16 * g + 8 * gr + 2 * i]) =
+                make_float2(o[nt][gr][i][hd] + cen[nt][gr][hd], o[nt][gr][i][2 + hd] + cen[nt][gr][hd]);
+        if (g == 0) {
+          sm_m[warp][head] = m[nt][hd];
+          sm_l[warp][head] = l[nt][hd];
+        }
       }
     }
   __syncthreads();
-  for (int idx = threadIdx.x; idx < G * kD; idx += blockDim.x) {
-    const int r = idx / kD, d = idx - r * kD;
-    float M = -CUDART_INF_F;
+  // Four channels a thread. Sums stay unnormalised until the last join; maxima are in unscaled score units.
+  for (int idx = threadIdx.x; idx < G * (kD / 4); idx += blockDim.x) {
+    const int r = idx / (kD / 4), d = (idx % (kD / 4)) * 4;
+    float M = kNoMax;
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sm_m[w][r]);
-    const float base = M == -CUDART_INF_F ? 0.f : M;     // nothing seen, or nothing but NaN: sums decide
-    float L = 0.f, acc = 0.f;
+    for (int w = 0; w < W; ++w) M = fmaxf(M, sm_m[w][r]);
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-      const float sc = exp2f(sm_m[w][r] - base);
-      L += sm_l[w][r] * sc;
-      acc += sm_o[w][r][d] * sc;
+    for (int w = 0; w < W; ++w) {
+      const float f = exp2f((sm_m[w][r] - M) * scale);
+      const float4 v = *reinterpret_cast<const float4*>(&sm_o[(w * 8 * NT + r) * kD + d]);
+      L += sm_l[w][r] * f;
+      acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
     }
-    const float val = L == 0.f ? 0.f : acc / L;
     const size_t row = static_cast<size_t>(b) * p.hq + h * G + r;
     if (p.splits == 1) {
-      p.out[row * kD + d] = __float2bfloat16(val);
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      *reinterpret_cast<uint2*>(p.out + row * kD + d) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    } else if (p.ws_o != nullptr) {
+      *reinterpret_cast<float4*>(p.ws_o + (row * p.splits + split) * kD + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + (row * p.splits + split) * 2) = make_float2(M * scale, L);
     } else {
-      p.ws_o[(row * p.splits + split) * kD + d] = val;
-      if (d == 0) p.ws_lse[row * p.splits + split] = L == 0.f ? -CUDART_INF_F : base + log2f(L);
+      *reinterpret_cast<float4*>(&part_o[r][d]) = acc;
+      if (d == 0) {
+        part_m[r] = M * scale;
+        part_l[r] = L;
+      }
     }
   }
+  if (p.splits == 1 || p.ws_o != nullptr) return;
+  // The cluster's CTAs hold one split each: every CTA joins a share of the (head, channel) outputs.
+  cluster_sync_all();
+  const uint32_t so = smem_u32(part_o), sm = smem_u32(part_m), sl = smem_u32(part_l);
+  for (int idx = split * blockDim.x + threadIdx.x; idx < G * kD; idx += blockDim.x * p.splits) {
+    const int r = idx / kD;
+    float M = kNoMax;
+    for (int c = 0; c < p.splits; ++c) M = fmaxf(M, ld_cluster_f32(map_to_cta(sm + r * 4, c)));
+    float L = 0.f, acc = 0.f;
+    for (int c = 0; c < p.splits; ++c) {
+      const float f = exp2f(ld_cluster_f32(map_to_cta(sm + r * 4, c)) - M);
+      L += ld_cluster_f32(map_to_cta(sl + r * 4, c)) * f;
+      acc += ld_cluster_f32(map_to_cta(so + idx * 4, c)) * f;
+    }
+    p.out[(static_cast<size_t>(b) * p.hq + h * G) * kD + idx] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
+  }
+  cluster_sync_all();                // nobody leaves while its shared memory is being read
 }
 
-// out[seq, head, :] = sum_s w_s * O_s with w_s = 2^(lse_s - max) / sum; a row that no split saw anything of is zero.
-__global__ void kv4_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_lse,
-                                   __nv_bfloat16* __restrict__ out, int splits) {
+// Joins the splits of a launch that has more of them than a cluster: one CTA per (sequence, query head).
+__global__ void __launch_bounds__(kD) kv4_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_ml,
+                                                         __nv_bfloat16* __restrict__ out, int splits) {
   grid_dep_launch();
   grid_dep_wait();
-  const size_t row = blockIdx.x;      // seq * hq + head
+  const size_t row = blockIdx.x;
   const int d = threadIdx.x;
-  float M = -CUDART_INF_F;
-  for (int s = 0; s < splits; ++s) M = fmaxf(M, ws_lse[row * splits + s]);
+  float M = kNoMax;
+  for (int s = 0; s < splits; ++s) M = fmaxf(M, ws_ml[(row * splits + s) * 2]);
   float L = 0.f, acc = 0.f;
+#pragma unroll 4
   for (int s = 0; s < splits; ++s) {
-    const float e = ws_lse[row * splits + s];
-    const float w = e == -CUDART_INF_F ? 0.f : exp2f(e - (M == -CUDART_INF_F ? 0.f : M));   // NaN stays NaN
-    L += w;
-    acc += w * ws_o[(row * splits + s) * kD + d];
+    const float2 ml = *reinterpret_cast<const float2*>(ws_ml + (row * splits + s) * 2);
+    const float f = exp2f(ml.x - M);
+    L += ml.y * f;
+    acc += ws_o[(row * splits + s) * kD + d] * f;
   }
   out[row * kD + d] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
 }
@@ -527,22 +704,42 @@ int fill(Params& p, const void* q, const void* k_cache, const void* v_cache, con
   return 0;
 }
 
+using DecodeKernel = void (*)(Params);
+// Shared memory above 48 KiB is opted into once per device.
+int decode_kernel(bool wide, DecodeKernel* out) {
+  static constexpr DecodeKernel all[2] = {kv4_decode_kernel<1, 4>, kv4_decode_kernel<2, 4>};
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return XV_ERR_LAUNCH;
+  if (!done[dev].load(std::memory_order_acquire)) {
+    for (DecodeKernel k : all)
+      if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(4)) != cudaSuccess)
+        return XV_ERR_LAUNCH;
+    done[dev].store(true, std::memory_order_release);
+  }
+  *out = all[wide];
+  return 0;
+}
+
 inline int launch_ok() { return cudaGetLastError() == cudaSuccess ? 0 : XV_ERR_LAUNCH; }
 
 }  // namespace
 
 extern "C" {
 
-// KV splits so that a small batch still fills the GPU; from launch-shape constants only (never from sequence lengths),
-// so a captured graph keeps its shape.
+// KV splits of a decode launch. From launch-shape constants only (never from sequence lengths), so a captured graph keeps
+// its shape. Up to 8 are one cluster per (sequence, KV head); more go through a workspace and a second kernel.
 int xv_kv4_decode_splits(int num_seqs, int hkv, int num_sms, int max_tokens_per_seq) {
-  const int ctas = max(1, num_seqs * hkv);
-  const int want = (4 * num_sms + ctas - 1) / ctas, by_len = max(1, max_tokens_per_seq / 256);
-  return max(1, min(min(want, by_len), 64));
+  const long long ctas = static_cast<long long>(num_seqs) * hkv;
+  int s = 1;
+  while (s < 8 && ctas * s < 2 * num_sms && max_tokens_per_seq / (2 * s) >= 128) s *= 2;
+  if (s == 8 && ctas * s < num_sms && max_tokens_per_seq >= 8192)
+    s = static_cast<int>(std::min<long long>(3 * num_sms / ctas, max_tokens_per_seq / 256));
+  return s;
 }
 
 long long xv_kv4_decode_workspace_bytes(int num_seqs, int hq, int splits) {
-  return splits <= 1 ? 0 : static_cast<long long>(num_seqs) * hq * splits * (kD + 1) * 4;
+  return splits <= 8 ? 0 : static_cast<long long>(num_seqs) * hq * splits * (kD + 2) * 4;
 }
 
 int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* kv_lens,
@@ -554,15 +751,21 @@ int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const
                     scale, status))
     return rc;
   if (hq / hkv > 16 || hkv > 65535 || num_seqs > 65535 || splits < 1) return XV_ERR_SHAPE;
-  if (xv_kv4_decode_workspace_bytes(num_seqs, hq, splits) > workspace_bytes) return XV_ERR_WORKSPACE;
+  if (static_cast<long long>(hkv) * block_size * kv4::kRow > 0xffffffffLL) return XV_ERR_SHAPE;    // bytes of a page: 32-bit
+  const long long need = xv_kv4_decode_workspace_bytes(num_seqs, hq, splits);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return XV_ERR_WORKSPACE;
+  if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15)) return XV_ERR_ALIGN;
   p.splits = splits;
-  p.ws_o = static_cast<float*>(workspace);
-  p.ws_lse = splits > 1 ? p.ws_o + static_cast<size_t>(num_seqs) * hq * splits * kD : nullptr;
-  const dim3 grid(splits, hkv, num_seqs);
-  launch_pdl(hq / hkv <= 8 ? kv4_decode_kernel<1> : kv4_decode_kernel<2>, grid, dim3(kDecWarps * 32), 0, stream, p);
+  if (need > 0) {
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_ml = p.ws_o + static_cast<size_t>(num_seqs) * hq * splits * kD;
+  }
+  DecodeKernel kernel;
+  if (int rc = decode_kernel(hq / hkv > 8, &kernel)) return rc;
+  launch_pdl_cluster(kernel, dim3(splits, hkv, num_seqs), dim3(4 * 32), decode_smem(4), stream, need > 0 ? 1u : splits, p);
   if (int rc = launch_ok()) return rc;
-  if (splits > 1) {
-    launch_pdl(kv4_combine_kernel, dim3(num_seqs * hq), dim3(kD), 0, stream, p.ws_o, p.ws_lse, p.out, splits);
+  if (need > 0) {
+    launch_pdl(kv4_combine_kernel, dim3(num_seqs * hq), dim3(kD), 0, stream, p.ws_o, p.ws_ml, p.out, splits);
     return launch_ok();
   }
   return 0;

@@ -161,6 +161,7 @@ int xv_kv4_read(const void* k_cache, const void* v_cache, const int* slots, void
                 int d, int block_size, int num_blocks, int* status, cudaStream_t stream);
 // As xv_attn_decode / xv_attn_prefill. Block-table entries outside [0, num_blocks), lengths beyond the table and query
 // ranges beyond total_rows are reported through `status`, never followed.
+// Up to 8 decode splits are joined inside a cluster; more need xv_kv4_decode_workspace_bytes(...) bytes.
 int xv_kv4_decode_splits(int num_seqs, int hkv, int num_sms, int max_tokens_per_seq);
 long long xv_kv4_decode_workspace_bytes(int num_seqs, int hq, int splits);
 int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* kv_lens,

@@ -469,7 +469,7 @@ def _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, 
     L, st, stream = lib(), _state(q), torch._C._cuda_getCurrentRawStream(dev.index)
     if n_d:
         splits = L.xv_kv4_decode_splits(n_d, num_kv_heads, st.num_sms, maxb * bs)
-        need = L.xv_kv4_decode_workspace_bytes(n_d, num_q_heads, splits) if splits > 1 else 0
+        need = L.xv_kv4_decode_workspace_bytes(n_d, num_q_heads, splits) if splits > 8 else 0
         # from torch's allocator, call by call: calls on two streams, or two captured graphs, never share it
         ws = k_cache.new_empty(need) if need else None
         _check(L.xv_kv4_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), tables, lens, out.data_ptr(), n_d,
