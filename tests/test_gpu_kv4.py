@@ -219,6 +219,33 @@ def test_decode_many_splits_and_long_tables():
     _attend([1, 1], [1100, 513], 8, 2, n_decode=2, extra_pages=2000)       # most splits see nothing
 
 
+WIDE = 20000       # pages of block table: the launch bound that makes decode deal its tokens in even shares
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 8), (3, 1), (16, 2), (9, 1)])
+def test_even_shares_groups_and_ragged_lengths(hq, hkv):
+    _attend([1] * 7, [0, 1, 150, 0, 17, 400, 33], hq, hkv, n_decode=7, seed=hq, extra_pages=WIDE)
+
+
+@pytest.mark.parametrize("bs", [48, 128])
+def test_even_shares_page_sizes_and_nan_around_the_sequences(bs):
+    _attend([1] * 5, [bs - 1, 3 * bs, 1, 0, 2 * bs + 5], 8, 2, bs=bs, n_decode=5, poison=True, extra_pages=WIDE)
+
+
+def test_even_shares_one_sequence_many_runs_and_mixed_batch():
+    _attend([1], [1500], 8, 2, n_decode=1, q_scale=3.0, extra_pages=WIDE)
+    _attend([1, 1, 40], [90, 333, 56], 8, 2, n_decode=2, extra_pages=WIDE)
+
+
+def test_even_shares_all_rows_empty():
+    assert not _attend([1] * 3, [0, 0, 0], 4, 2, n_decode=3, extra_pages=WIDE).any()
+
+
+def test_even_shares_more_sequences_than_threads_of_the_scan():
+    lens = [(i * 7) % 23 for i in range(300)]
+    _attend([1] * 300, lens, 2, 2, n_decode=300, extra_pages=600)
+
+
 def test_decode_growing_maxima():
     _attend([1, 1], [400, 700], 8, 1, n_decode=2, q_scale=8.0, seed=4)
 
@@ -312,7 +339,7 @@ def test_refusals():
 
 
 def test_two_streams_and_graph_replay_do_not_share_scratch():
-    """Two captured decode calls with splits, replayed at the same time on two streams, and an eager one between."""
+    """Two captured decode calls with a workspace, replayed at the same time on two streams, and an eager one between."""
     ops = _ops()
     runs = []
     for seed in (1, 2):
@@ -320,7 +347,8 @@ def test_two_streams_and_graph_replay_do_not_share_scratch():
         g = torch.Generator().manual_seed(seed)
         q = torch.randn(1, 8 * D, generator=g).bfloat16().to(DEV)
         i32 = dict(dtype=torch.int32, device=DEV)
-        table = torch.randperm(70, generator=g).to(**i32)[None]
+        table = torch.zeros(1, WIDE, **i32)
+        table[0, :70] = torch.randperm(70, generator=g).to(**i32)
         attn = AttnBatch(torch.tensor([0, 1], **i32), torch.tensor([1100], **i32), table, 1, 1, 1, 1100, 1)
         want = ops.paged_attention(q, k, v, attn, 0.09, 8, 2, D).clone()
         torch.cuda.synchronize()

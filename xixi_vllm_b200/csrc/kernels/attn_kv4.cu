@@ -1,10 +1,10 @@
 // Paged causal GQA attention over a KV cache held in 4 bits (format: common/kv4.cuh), head_dim 128.
 //
 //   kv4_decode_kernel  - one query row per sequence; a cluster of CTAs, one per KV split, owns (sequence, KV head). Each
-//                        of a CTA's 8 warps streams its own 16-token units through a ring of shared-memory slots (five
-//                        16-byte cp.async a lane for K and V; no block-wide barrier in the loop). Tokens
-//                        are the M rows of both products and the group's query heads (up to 8, or 16 as two column
-//                        tiles) the N columns, so one MMA covers 16 x 16 cache values:
+//                        warp streams its own 16-token units through a ring of shared-memory slots (five 16-byte
+//                        cp.async a lane for K and V of a unit; no block-wide barrier in the loop). Tokens are the M rows
+//                        of both products and the group's query heads (up to 8, or 16 as two column tiles) the N
+//                        columns, so one MMA covers 16 x 16 cache values:
 //                          S^T[token, head] = s_g * (n Q^T) + c_g * sum(Q)   per channel group g
 //                          O^T[channel, head] = (n - 8)^T (s_g P) + c_g^T P
 //                        The MMAs see the codes as exact bf16 integers; scales and centres stay in fp32 (the scale of V
@@ -12,6 +12,8 @@
 //                        lanes pair two tokens with PRMT, so codes go from shared memory to MMA operands in registers.
 //                        Warps are merged through shared memory, splits through the cluster's distributed shared
 //                        memory: one launch, no workspace.
+//   kv4_share_kernel   - the same arithmetic for large or ragged batches: all units dealt to the warps in equal runs,
+//   kv4_join_kernel      partial results of pairs that span runs joined by a second kernel.
 //   kv4_prefill_kernel - packed query chunks: 64 query rows of one head per CTA, KV tiles of 64 tokens dequantised to
 //                        bf16 in shared memory.
 
@@ -43,8 +45,6 @@ struct Params {
   const int* cu_q;
   const int* kv_lens;
   __nv_bfloat16* out;
-  float* ws_o;      // [seq, hq, split, 128], when the splits do not fit a cluster
-  float* ws_ml;     // [seq, hq, split, 2]: maximum (log2 units), sum
   int* status;
   int hq, hkv, block_size, max_blocks, num_blocks, splits, seq_begin, total_rows;
   float scale_log2;
@@ -100,167 +100,110 @@ constexpr float kLazy = 8.f;             // log2 units a running maximum may lag
 
 constexpr int decode_smem(int warps) { return warps * kStages * kSlot; }
 
+// Four channels of an output row from unnormalised sums; a row that saw nothing is zero.
+__device__ __forceinline__ void store_out(__nv_bfloat16* dst, const float4& v, float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+}
+
 // D = A B: the first product of an accumulation.
 __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// NT: column tiles of 8 query heads; W: warps.
-template <int NT, int W>
-__global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_kernel(const Params p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float sm_m[W][8 * NT], sm_l[W][8 * NT];
-  __shared__ float part_o[8 * NT][kD], part_m[8 * NT], part_l[8 * NT];     // this CTA's result, read by the cluster
-  grid_dep_launch();
-  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const int G = p.hq / p.hkv;
-  uint8_t* ring = smem + warp * kStages * kSlot;
-  grid_dep_wait();
-  const int kv_len = kv_len_of(p, b, kIdDecode);
-  // Consecutive units per warp, so that a page and a place in it follow from the ones before without a division.
-  const int tiles = (kv_len + 15) / 16;
-  const int per = (tiles + p.splits * W - 1) / (p.splits * W);
-  const int tile0 = min((split * W + warp) * per, tiles);
-  const int n_tiles = min(per, tiles - tile0);
-  const int upp = p.block_size / kv4::kUnit;
+// D += A B. Unlike ptx.cuh's form not volatile: the two units of a slot may be interleaved.
+__device__ __forceinline__ void mma_more(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
-  // Pages are looked up 32 at a time, one batch ahead of use.
-  const int page0 = tile0 / upp, last_page = max(0, (tiles - 1) / upp);
-  auto lookup = [&](int i) { return page_of(p, b, min(page0 + i, last_page), kIdDecode); };
-  int pages = 0, pages_next = 0;
-  if (n_tiles > 0) {
-    pages = lookup(lane);
-    pages_next = lookup(32 + lane);
-  }
-  // A unit in a slot: K's 1152 bytes, then V's. Five copies of 16 bytes a lane: K's codes, V's codes, and both parameter
-  // blocks by half a warp.
-  const uint32_t page_bytes = static_cast<uint32_t>(p.hkv) * upp * kv4::kUnitBytes;
-  const uint8_t* k_src = p.k_cache + static_cast<size_t>(h) * upp * kv4::kUnitBytes + lane * 16;
-  const uint8_t* v_src = p.v_cache + static_cast<size_t>(h) * upp * kv4::kUnitBytes + lane * 16;
-  const uint8_t* par_src = (lane < 8 ? k_src : v_src - 128) + kv4::kParBase;
-  const uint32_t ring_u32 = smem_u32(ring) + lane * 16;
-  const uint32_t par_dst = (lane < 8 ? 0 : kv4::kUnitBytes - 128) + kv4::kParBase;
-  int page_i = 0, place = tile0 - page0 * upp;               // of the next unit to fetch
-  unsigned fetched = 0, slot_in = 0;
-  auto issue = [&]() {                                       // the next kPair units into the next slot
-#pragma unroll
-    for (int u = 0; u < kPair; ++u) {
-      if (fetched < static_cast<unsigned>(n_tiles)) {
-        if (place == upp) {
-          place = 0;
-          if ((++page_i & 31) == 0) {
-            pages = pages_next;
-            pages_next = lookup(page_i + 32 + lane);
-          }
-        }
-        const uint32_t blk = __shfl_sync(0xffffffffu, pages, page_i & 31);
-        const uint64_t at = static_cast<uint64_t>(blk) * page_bytes + static_cast<uint32_t>(place * kv4::kUnitBytes);
-        const uint32_t dst = ring_u32 + slot_in * kSlot + u * kUnitSlot;
-        cp_async16_u32(dst, k_src + at);
-        cp_async16_u32(dst + 512, k_src + at + 512);
-        cp_async16_u32(dst + kv4::kUnitBytes, v_src + at);
-        cp_async16_u32(dst + kv4::kUnitBytes + 512, v_src + at + 512);
-        if (lane < 16) cp_async16_u32(dst + par_dst, par_src + at);
-        ++place;
-        ++fetched;
-      }
-    }
-    cp_async_commit();                                       // one group per call, empty ones included
-    slot_in = slot_in == kStages - 1 ? 0 : slot_in + 1;
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue();
-
-  // Q as the B operand: MMA (word w, half hf) of lane (g, t) multiplies channels 32 t + 8 w + 2 hf + {0, 4, 1, 5}.
-  uint32_t qf[NT][4][2][2];
+// The group's queries as B operands. NT: column tiles of 8 query heads.
+template <int NT>
+struct Query {
+  // MMA (word w, half hf) of lane (g, t) multiplies channels 32 t + 8 w + 2 hf + {0, 4, 1, 5}.
+  uint32_t f[NT][4][2][2];
   // The centres' share of a score, sum over groups of c_g Qs_g - 136 s_g Qs_g with Qs_g the group's sum of Q, is one more
   // MMA: its A operand is the parameter words as stored, its B operand {-136 Qs_g, Qs_g} as three bf16 terms (24 bits).
-  uint32_t qc[NT][2];
-  // A negative scale is Q's sign, so the running maxima need not know it; zero becomes a scale too small to matter.
-  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-  const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
+  uint32_t c[NT][2];
+
+  // `row`: sequence * hq + first query head of the group; `flip`: sign bits to apply to Q.
+  __device__ __forceinline__ void load(const Params& p, size_t row, int G, uint32_t flip, int g, int t) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int head = nt * 8 + g;
-    const uint4* src = reinterpret_cast<const uint4*>(p.q + (static_cast<size_t>(b) * p.hq + h * G + head) * kD + 32 * t);
-    float sum[2] = {0.f, 0.f};
+    for (int nt = 0; nt < NT; ++nt) {
+      const int head = nt * 8 + g;
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (row + head) * kD + 32 * t);
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint4 raw = head < G ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
-      const uint32_t r[4] = {raw.x ^ flip, raw.y ^ flip, raw.z ^ flip, raw.w ^ flip};
+      for (int w = 0; w < 4; ++w) {
+        const uint4 raw = head < G ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
+        const uint32_t r[4] = {raw.x ^ flip, raw.y ^ flip, raw.z ^ flip, raw.w ^ flip};
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        qf[nt][w][hf][0] = __byte_perm(r[hf], r[hf + 2], 0x5410);     // channels 2 hf, 2 hf + 4
-        qf[nt][w][hf][1] = __byte_perm(r[hf], r[hf + 2], 0x7632);     // channels 2 hf + 1, 2 hf + 5
+        for (int hf = 0; hf < 2; ++hf) {
+          f[nt][w][hf][0] = __byte_perm(r[hf], r[hf + 2], 0x5410);     // channels 2 hf, 2 hf + 4
+          f[nt][w][hf][1] = __byte_perm(r[hf], r[hf + 2], 0x7632);     // channels 2 hf + 1, 2 hf + 5
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[w & 1] += __uint_as_float(r[i] << 16) + __uint_as_float(r[i] & 0xffff0000u);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[w & 1] += __uint_as_float(r[i] << 16) + __uint_as_float(r[i] & 0xffff0000u);
+      for (int gr = 0; gr < 2; ++gr) {
+        sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
+        sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
+      }
+      // Lane (g, t) holds K rows 2t, 2t + 1 of B (first register) and 2t + 8, 2t + 9 (second): group t & 1; the first
+      // term for t < 2, the second for t >= 2, the third in the second register for t < 2.
+      const float qs = (t & 1) ? sum[1] : sum[0], bs = -kv4::kBias * qs;
+      const float q1 = __bfloat162float(__float2bfloat16(qs)), b1 = __bfloat162float(__float2bfloat16(bs));
+      const float q2 = __bfloat162float(__float2bfloat16(qs - q1)), b2 = __bfloat162float(__float2bfloat16(bs - b1));
+      c[nt][0] = t < 2 ? pack_bf16(b1, q1) : pack_bf16(b2, q2);
+      c[nt][1] = t < 2 ? pack_bf16(bs - b1 - b2, qs - q1 - q2) : 0u;
     }
-#pragma unroll
-    for (int gr = 0; gr < 2; ++gr) {
-      sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
-      sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
-    }
-    // Lane (g, t) holds K rows 2t, 2t + 1 of B (first register) and 2t + 8, 2t + 9 (second): group t & 1; the first term
-    // for t < 2, the second for t >= 2, the third in the second register for t < 2.
-    const float qs = (t & 1) ? sum[1] : sum[0], bs = -kv4::kBias * qs;
-    const float q1 = __bfloat162float(__float2bfloat16(qs)), b1 = __bfloat162float(__float2bfloat16(bs));
-    const float q2 = __bfloat162float(__float2bfloat16(qs - q1)), b2 = __bfloat162float(__float2bfloat16(bs - b1));
-    qc[nt][0] = t < 2 ? pack_bf16(b1, q1) : pack_bf16(b2, q2);
-    qc[nt][1] = t < 2 ? pack_bf16(bs - b1 - b2, qs - q1 - q2) : 0u;
   }
+};
 
+// Running state of the softmax over the tokens a warp has seen.
+template <int NT>
+struct Softmax {
   float o[NT][2][4][4];            // [group][MMA]: rows g, g + 8 = channels 16 g + 8 group + 2 i + {0, 1}; heads 2t, 2t+1
   float cen[NT][2][2];             // sum of P * centre, this lane's tokens
-  float m[NT][2], l[NT][2];        // running maximum of the unscaled scores, sum of P
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int gr = 0; gr < 2; ++gr) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[nt][gr][i][0] = o[nt][gr][i][1] = o[nt][gr][i][2] = o[nt][gr][i][3] = 0.f;
-      cen[nt][gr][0] = cen[nt][gr][1] = 0.f;
-    }
-    m[nt][0] = m[nt][1] = kNoMax;
-    l[nt][0] = l[nt][1] = 0.f;
-  }
-  const float lag = kLazy / scale;
+  float m[NT][2], l[NT][2];        // running maximum of the unscaled scores (may lag), sum of P of this lane's tokens
 
-  const int tok = token_of_row(g);
-  const uint8_t* const lane_k = ring + tok * 64 + t * 16;
-  const uint8_t* const lane_p = ring + kv4::kParBase + tok * 8;
-  const uint8_t* const lane_v0 = ring + kv4::kUnitBytes + token_of_row(2 * t) * 64 + g * 8;
-  const uint8_t* const lane_v1 = ring + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8;
-  int left = kv_len - tile0 * 16;        // tokens from the slot's first unit on
-  unsigned slot = 0;
-  for (int i = 0; i < n_tiles; i += kPair, left -= 16 * kPair) {
-    cp_async_wait<kStages - 2>();
-    __syncwarp();                        // everyone's part of the slot has landed, and everyone has read the slot filled next
-    issue();
-    const unsigned at = slot * kSlot;
-    slot = slot == kStages - 1 ? 0 : slot + 1;
-    // With an odd number of units the second half of the last slot is an old unit whose tokens are all past the end of
-    // this warp's range.
-    const int mine = min(left, (n_tiles - i) * 16);
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int gr = 0; gr < 2; ++gr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[nt][gr][i][0] = o[nt][gr][i][1] = o[nt][gr][i][2] = o[nt][gr][i][3] = 0.f;
+        cen[nt][gr][0] = cen[nt][gr][1] = 0.f;
+      }
+      m[nt][0] = m[nt][1] = kNoMax;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+  }
+
+  // One slot of kPair units, of which the first `mine` tokens count. lane_k .. lane_v1: this lane's places in the slot.
+  __device__ __forceinline__ void add(const Query<NT>& q, const uint8_t* lane_k, const uint8_t* lane_p, const uint8_t* lane_v0,
+                                      const uint8_t* lane_v1, int mine, int tok, int t, float scale, float lag) {
     float x[kPair][NT][4];               // (row g: heads 2t, 2t + 1), (row g + 8: the same)
 #pragma unroll
     for (int u = 0; u < kPair; ++u) {
-      const uint4 k0 = *reinterpret_cast<const uint4*>(lane_k + at + u * kUnitSlot);
-      const uint4 k1 = *reinterpret_cast<const uint4*>(lane_k + at + u * kUnitSlot + 8 * 64);
-      const uint2 kp0 = *reinterpret_cast<const uint2*>(lane_p + at + u * kUnitSlot);
-      const uint2 kp1 = *reinterpret_cast<const uint2*>(lane_p + at + u * kUnitSlot + 64);
+      const uint4 k0 = *reinterpret_cast<const uint4*>(lane_k + u * kUnitSlot);
+      const uint4 k1 = *reinterpret_cast<const uint4*>(lane_k + u * kUnitSlot + 8 * 64);
+      const uint2 kp0 = *reinterpret_cast<const uint2*>(lane_p + u * kUnitSlot);
+      const uint2 kp1 = *reinterpret_cast<const uint2*>(lane_p + u * kUnitSlot + 64);
       const uint32_t ka[4] = {k0.x, k0.y, k0.z, k0.w}, kb[4] = {k1.x, k1.y, k1.z, k1.w};
       const uint32_t w0 = (t & 1) ? kp0.y : kp0.x, w1 = (t & 1) ? kp1.y : kp1.x;
       const uint32_t ac[4] = {w0, w1, w0, w1};
       float s[NT][2][4], sc[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_first(sc[nt], ac, qc[nt][0], qc[nt][1]);
+      for (int nt = 0; nt < NT; ++nt) mma_first(sc[nt], ac, q.c[nt][0], q.c[nt][1]);
 #pragma unroll
       for (int w = 0; w < 4; ++w)
 #pragma unroll
@@ -269,8 +212,8 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
                                  kv4::biased(kb[w], 8 * hf + 4)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            if (w < 2 && hf == 0) mma_first(s[nt][w], a, qf[nt][w][hf][0], qf[nt][w][hf][1]);
-            else mma_bf16_16816(s[nt][w & 1], a, qf[nt][w][hf][0], qf[nt][w][hf][1]);
+            if (w < 2 && hf == 0) mma_first(s[nt][w], a, q.f[nt][w][hf][0], q.f[nt][w][hf][1]);
+            else mma_more(s[nt][w & 1], a, q.f[nt][w][hf][0], q.f[nt][w][hf][1]);
           }
         }
 #pragma unroll
@@ -325,13 +268,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
     }
 #pragma unroll
     for (int u = 0; u < kPair; ++u) {
-      uint2 vp0 = *reinterpret_cast<const uint2*>(lane_p + at + u * kUnitSlot + kv4::kUnitBytes);
-      uint2 vp1 = *reinterpret_cast<const uint2*>(lane_p + at + u * kUnitSlot + kv4::kUnitBytes + 64);
+      uint2 vp0 = *reinterpret_cast<const uint2*>(lane_p + u * kUnitSlot + kv4::kUnitBytes);
+      uint2 vp1 = *reinterpret_cast<const uint2*>(lane_p + u * kUnitSlot + kv4::kUnitBytes + 64);
       uint2 vw[4];                       // tokens of rows 2t, 2t + 1, then the same 8 further
-      vw[0] = *reinterpret_cast<const uint2*>(lane_v0 + at + u * kUnitSlot);
-      vw[1] = *reinterpret_cast<const uint2*>(lane_v1 + at + u * kUnitSlot);
-      vw[2] = *reinterpret_cast<const uint2*>(lane_v0 + at + u * kUnitSlot + 8 * 64);
-      vw[3] = *reinterpret_cast<const uint2*>(lane_v1 + at + u * kUnitSlot + 8 * 64);
+      vw[0] = *reinterpret_cast<const uint2*>(lane_v0 + u * kUnitSlot);
+      vw[1] = *reinterpret_cast<const uint2*>(lane_v1 + u * kUnitSlot);
+      vw[2] = *reinterpret_cast<const uint2*>(lane_v0 + u * kUnitSlot + 8 * 64);
+      vw[3] = *reinterpret_cast<const uint2*>(lane_v1 + u * kUnitSlot + 8 * 64);
       if (ragged) {                      // P is 0 there, and whatever parameters an earlier owner of the page left (NaN
         if (16 * u + tok >= mine) vp0 = make_uint2(0u, 0u);        // among them) must not reach the sums; codes are
         if (16 * u + tok + 8 >= mine) vp1 = make_uint2(0u, 0u);    // always finite
@@ -368,43 +311,182 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
             const uint32_t a[4] = {kv4::centred(kv4::biased(u0, 8 * j)), kv4::centred(kv4::biased(u0, 8 * j + 4)),
                                    kv4::centred(kv4::biased(u1, 8 * j)), kv4::centred(kv4::biased(u1, 8 * j + 4))};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(o[nt][gr][hl * 2 + j], a, pf[nt][gr][0], pf[nt][gr][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_more(o[nt][gr][hl * 2 + j], a, pf[nt][gr][0], pf[nt][gr][1]);
           }
         }
       }
     }
   }
+
+  // Sums over the lanes of equal t; the centres join the outputs. Then every lane holds, for its two heads, 16 channels.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int hd = 0; hd < 2; ++hd) {
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) {
+          l[nt][hd] += __shfl_xor_sync(0xffffffffu, l[nt][hd], x);
+          cen[nt][0][hd] += __shfl_xor_sync(0xffffffffu, cen[nt][0][hd], x);
+          cen[nt][1][hd] += __shfl_xor_sync(0xffffffffu, cen[nt][1][hd], x);
+        }
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            o[nt][gr][i][hd] += cen[nt][gr][hd];
+            o[nt][gr][i][2 + hd] += cen[nt][gr][hd];
+          }
+      }
+  }
+  // Channels 16 g + 4 j .. + 3 of head (nt, hd) after finish().
+  __device__ __forceinline__ float4 quad(int nt, int hd, int j) const {
+    const float(&a)[4] = o[nt][j >> 1][2 * (j & 1)], (&b)[4] = o[nt][j >> 1][2 * (j & 1) + 1];
+    return hd ? make_float4(a[1], a[3], b[1], b[3]) : make_float4(a[0], a[2], b[0], b[2]);
+  }
+};
+
+// A warp's ring of slots in shared memory and the walk over the units of one (sequence, KV head) that fills it. A unit in
+// a slot: K's 1152 bytes, then V's; five cp.async of 16 bytes a lane (K's codes, V's codes, both parameter blocks by half
+// a warp). Pages are looked up 32 at a time, one batch ahead of use.
+struct Ring {
+  uint32_t dst, slot;
+  int lane;
+  // units still to fetch, and where they are
+  const uint8_t *k_src, *v_src;
+  uint32_t page_bytes;
+  int b, left, place, upp, page0, page_i, last_page, pages, pages_next;
+
+  __device__ __forceinline__ void init(uint8_t* ring, int lane_, int upp_, int hkv) {
+    lane = lane_;
+    upp = upp_;
+    dst = smem_u32(ring) + lane * 16;
+    slot = 0;
+    left = 0;
+    page_bytes = static_cast<uint32_t>(hkv) * upp * kv4::kUnitBytes;
+  }
+  __device__ __forceinline__ int lookup(const Params& p, int i) const {
+    return page_of(p, b, min(page0 + i, last_page), kIdDecode);
+  }
+  // n units from `first` on of the `units` that sequence b has.
+  __device__ __forceinline__ void start(const Params& p, int b_, int h, int first, int n, int units) {
+    b = b_;
+    left = n;
+    page0 = first / upp;
+    place = first - page0 * upp;
+    last_page = max(0, (units - 1) / upp);
+    page_i = 0;
+    const size_t head = static_cast<size_t>(h) * upp * kv4::kUnitBytes + lane * 16;
+    k_src = p.k_cache + head;
+    v_src = p.v_cache + head;
+    if (n > 0) {
+      pages = lookup(p, lane);
+      pages_next = lookup(p, 32 + lane);
+    }
+  }
+  // The next kPair units (or what is left of them) into the next slot; one commit group per call, empty ones included.
+  __device__ __forceinline__ void issue(const Params& p) {
+#pragma unroll
+    for (int u = 0; u < kPair; ++u) {
+      if (left > 0) {
+        if (place == upp) {
+          place = 0;
+          if ((++page_i & 31) == 0) {
+            pages = pages_next;
+            pages_next = lookup(p, page_i + 32 + lane);
+          }
+        }
+        const uint32_t blk = __shfl_sync(0xffffffffu, pages, page_i & 31);
+        const uint64_t at = static_cast<uint64_t>(blk) * page_bytes + static_cast<uint32_t>(place * kv4::kUnitBytes);
+        const uint32_t to = dst + slot * kSlot + u * kUnitSlot;
+        cp_async16_u32(to, k_src + at);
+        cp_async16_u32(to + 512, k_src + at + 512);
+        cp_async16_u32(to + kv4::kUnitBytes, v_src + at);
+        cp_async16_u32(to + kv4::kUnitBytes + 512, v_src + at + 512);
+        if (lane < 16)
+          cp_async16_u32(to + kv4::kParBase + (lane < 8 ? 0 : kv4::kUnitBytes - 128),
+                         (lane < 8 ? k_src : v_src - 128) + at + kv4::kParBase);
+        ++place;
+        --left;
+      }
+    }
+    cp_async_commit();
+    slot = slot == kStages - 1 ? 0 : slot + 1;
+  }
+};
+
+// A negative scale is Q's sign, so the running maxima need not know it; zero becomes a scale too small to matter.
+struct Scale {
+  float scale, lag;
+  uint32_t flip;
+  __device__ __forceinline__ explicit Scale(float s) : scale(fmaxf(fabsf(s), 1e-30f)), lag(kLazy / scale), flip(s < 0.f ? 0x80008000u : 0u) {}
+};
+
+// A cluster of CTAs, one per KV split, per (sequence, KV head). NT: column tiles of 8 query heads; W: warps.
+template <int NT, int W>
+__global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_kernel(const Params p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float sm_m[W][8 * NT], sm_l[W][8 * NT];
+  __shared__ float part_m[8 * NT], part_l[8 * NT];       // this CTA's result, read by the cluster (part_o: in the ring)
+  grid_dep_launch();
+  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int G = p.hq / p.hkv;
+  uint8_t* ring_mem = smem + warp * kStages * kSlot;
+  grid_dep_wait();
+  const int kv_len = kv_len_of(p, b, kIdDecode);
+  const int units = (kv_len + 15) / 16;
+  const int per = (units + p.splits * W - 1) / (p.splits * W);
+  const int first = min((split * W + warp) * per, units);
+  const int n = min(per, units - first);
+  Ring ring;
+  ring.init(ring_mem, lane, p.block_size / kv4::kUnit, p.hkv);
+  ring.start(p, b, h, first, n, units);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) ring.issue(p);
+  const Scale sc(p.scale_log2);
+  Query<NT> q;
+  q.load(p, static_cast<size_t>(b) * p.hq + h * G, G, sc.flip, g, t);
+  Softmax<NT> st;
+  st.clear();
+
+  const int tok = token_of_row(g);
+  const uint8_t* at = ring_mem;
+  int mine = min(kv_len - first * 16, n * 16);           // tokens of this warp still to come
+  for (int i = 0; i < n; i += kPair, mine -= 16 * kPair) {
+    cp_async_wait<kStages - 2>();
+    __syncwarp();                        // everyone's part of the slot has landed, and everyone has read the slot filled next
+    ring.issue(p);
+    st.add(q, at + tok * 64 + t * 16, at + kv4::kParBase + tok * 8, at + kv4::kUnitBytes + token_of_row(2 * t) * 64 + g * 8,
+           at + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8, mine, tok, t, sc.scale, sc.lag);
+    at = at == ring_mem + (kStages - 1) * kSlot ? ring_mem : at + kSlot;
+  }
   cp_async_wait<0>();
 
-  // Sums over the token lanes, then the warps through the (now idle) ring.
+  // The warps meet in the (now idle) ring.
+  st.finish();
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(smem);                    // [warp][8 NT][128]
+  float* part_o = sm_o + W * 8 * NT * kD;                          // [8 NT][128]
+  static_assert((W + 1) * 8 * NT * kD * 4 <= decode_smem(W));
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int hd = 0; hd < 2; ++hd) {
-#pragma unroll
-      for (int x = 4; x <= 16; x <<= 1) {
-        l[nt][hd] += __shfl_xor_sync(0xffffffffu, l[nt][hd], x);
-        cen[nt][0][hd] += __shfl_xor_sync(0xffffffffu, cen[nt][0][hd], x);
-        cen[nt][1][hd] += __shfl_xor_sync(0xffffffffu, cen[nt][1][hd], x);
-      }
       const int head = nt * 8 + 2 * t + hd;
       if (head < G) {
 #pragma unroll
-        for (int gr = 0; gr < 2; ++gr)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<float2*>(&sm_o[(warp * 8 * NT + head) * kD + 16 * g + 8 * gr + 2 * i]) =
-                make_float2(o[nt][gr][i][hd] + cen[nt][gr][hd], o[nt][gr][i][2 + hd] + cen[nt][gr][hd]);
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float4*>(&sm_o[(warp * 8 * NT + head) * kD + 16 * g + 4 * j]) = st.quad(nt, hd, j);
         if (g == 0) {
-          sm_m[warp][head] = m[nt][hd];
-          sm_l[warp][head] = l[nt][hd];
+          sm_m[warp][head] = st.m[nt][hd];
+          sm_l[warp][head] = st.l[nt][hd];
         }
       }
     }
   __syncthreads();
-  // Four channels a thread. Sums stay unnormalised until the last join; maxima are in unscaled score units.
+  // Four channels a thread. Sums stay unnormalised until the last join.
   for (int idx = threadIdx.x; idx < G * (kD / 4); idx += blockDim.x) {
     const int r = idx / (kD / 4), d = (idx % (kD / 4)) * 4;
     float M = kNoMax;
@@ -414,27 +496,22 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float f = exp2f((sm_m[w][r] - M) * scale);
+      const float f = exp2f((sm_m[w][r] - M) * sc.scale);
       const float4 v = *reinterpret_cast<const float4*>(&sm_o[(w * 8 * NT + r) * kD + d]);
       L += sm_l[w][r] * f;
       acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
     }
-    const size_t row = static_cast<size_t>(b) * p.hq + h * G + r;
     if (p.splits == 1) {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      *reinterpret_cast<uint2*>(p.out + row * kD + d) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-    } else if (p.ws_o != nullptr) {
-      *reinterpret_cast<float4*>(p.ws_o + (row * p.splits + split) * kD + d) = acc;
-      if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + (row * p.splits + split) * 2) = make_float2(M * scale, L);
+      store_out(p.out + (static_cast<size_t>(b) * p.hq + h * G + r) * kD + d, acc, L);
     } else {
-      *reinterpret_cast<float4*>(&part_o[r][d]) = acc;
+      *reinterpret_cast<float4*>(part_o + r * kD + d) = acc;
       if (d == 0) {
-        part_m[r] = M * scale;
+        part_m[r] = M;
         part_l[r] = L;
       }
     }
   }
-  if (p.splits == 1 || p.ws_o != nullptr) return;
+  if (p.splits == 1) return;
   // The cluster's CTAs hold one split each: every CTA joins a share of the (head, channel) outputs.
   cluster_sync_all();
   const uint32_t so = smem_u32(part_o), sm = smem_u32(part_m), sl = smem_u32(part_l);
@@ -444,7 +521,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
     for (int c = 0; c < p.splits; ++c) M = fmaxf(M, ld_cluster_f32(map_to_cta(sm + r * 4, c)));
     float L = 0.f, acc = 0.f;
     for (int c = 0; c < p.splits; ++c) {
-      const float f = exp2f(ld_cluster_f32(map_to_cta(sm + r * 4, c)) - M);
+      const float f = exp2f((ld_cluster_f32(map_to_cta(sm + r * 4, c)) - M) * sc.scale);
       L += ld_cluster_f32(map_to_cta(sl + r * 4, c)) * f;
       acc += ld_cluster_f32(map_to_cta(so + idx * 4, c)) * f;
     }
@@ -453,24 +530,223 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
   cluster_sync_all();                // nobody leaves while its shared memory is being read
 }
 
-// Joins the splits of a launch that has more of them than a cluster: one CTA per (sequence, query head).
-__global__ void __launch_bounds__(kD) kv4_combine_kernel(const float* __restrict__ ws_o, const float* __restrict__ ws_ml,
-                                                         __nv_bfloat16* __restrict__ out, int splits) {
+// ---- even shares ----
+// All units of the batch, in the order (sequence, KV head, unit), are dealt to the launch's warps in equal runs, so that
+// ragged lengths leave no tail. A run crosses from one (sequence, head) pair to the next; a pair that lies in one run is
+// finished there, the others leave one partial result per run for kv4_join_kernel. Runs and pairs are numbered in the
+// same order, so the partial of (run w, pair x) has the slot w + x and a pair's slots are consecutive.
+struct Shares {
+  float* o;         // [slot][8 NT][128]
+  float* ml;        // [slot][8 NT][2]: running maximum (unscaled), sum
+  int* begin;       // [seq + 1]: units of one head before the sequence; then the units per run
+};
+constexpr int kShareWarps = 4, kMinRun = 4;
+
+template <int NT>
+__global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_kernel(const Params p, const Shares ws, int num_seqs) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int T = kShareWarps * 32;
+  __shared__ int sums[T + 1];
+  grid_dep_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int G = p.hq / p.hkv;
+  uint8_t* ring_mem = smem + warp * kStages * kSlot;
+  grid_dep_wait();
+  // Every CTA counts the units: a thread a run of sequences, then a scan over the threads.
+  const int chunk = (num_seqs + T - 1) / T;
+  const int c0 = min(static_cast<int>(threadIdx.x) * chunk, num_seqs), c1 = min(c0 + chunk, num_seqs);
+  int mine_units = 0;
+  for (int b = c0; b < c1; ++b) mine_units += (kv_len_of(p, b, kIdDecode) + 15) / 16;
+  int incl = mine_units;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kShareWarps; ++w) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  __syncthreads();
+  sums[threadIdx.x + 1] = before + incl;
+  if (threadIdx.x == 0) sums[0] = 0;
+  const int runs = gridDim.x * kShareWarps;
+  const int all = total * p.hkv;
+  const int per = max((all + runs - 1) / runs, kMinRun);
+  if (blockIdx.x == 0) {                       // for the joining kernel
+    int at = before + incl - mine_units;
+    for (int b = c0; b < c1; ++b) {
+      ws.begin[b] = at;
+      at += (kv_len_of(p, b, kIdDecode) + 15) / 16;
+    }
+    if (threadIdx.x == 0) {
+      ws.begin[num_seqs] = total;
+      ws.begin[num_seqs + 1] = per;
+    }
+  }
+  __syncthreads();
+  const int run = blockIdx.x * kShareWarps + warp;
+  const long long from = static_cast<long long>(run) * per;
+  if (from >= all) return;
+  int todo = min(per, all - static_cast<int>(from));      // units of this run still to be consumed
+
+  // The sequence that holds the first one: the thread chunk by bisection, then one by one.
+  int b, units, kv_len, h, first;
+  {
+    const int u = static_cast<int>(from / p.hkv);          // of one head
+    int lo = 0, hi = T;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (sums[mid] <= u) lo = mid; else hi = mid;
+    }
+    int at = sums[lo];
+    b = lo * chunk;
+    for (;; ++b) {
+      kv_len = kv_len_of(p, b, kIdDecode);
+      units = (kv_len + 15) / 16;
+      if (u < at + units) break;
+      at += units;
+    }
+    const int rest = static_cast<int>(from - static_cast<long long>(at) * p.hkv);
+    h = rest / units;
+    first = rest - h * units;
+  }
+
+  Ring ring;
+  ring.init(ring_mem, lane, p.block_size / kv4::kUnit, p.hkv);
+  const Scale sc(p.scale_log2);
+  const int tok = token_of_row(g);
+  const uint8_t* at = ring_mem;
+  // The fetching side runs kStages - 1 slots ahead and may already be in the next pair.
+  int f_b = b, f_h = h, f_units = units, f_todo = todo;
+  auto fetch_pair = [&](int start) {
+    const int n = min(f_units - start, f_todo);
+    f_todo -= n;
+    ring.start(p, f_b, f_h, start, n, f_units);
+  };
+  auto fetch = [&]() {
+    if (ring.left == 0 && f_todo > 0) {
+      if (++f_h == p.hkv) {
+        f_h = 0;
+        do f_units = (kv_len_of(p, ++f_b, kIdDecode) + 15) / 16;
+        while (f_units == 0);
+      }
+      fetch_pair(0);
+    }
+    ring.issue(p);
+  };
+  fetch_pair(first);
+  ring.issue(p);
+#pragma unroll
+  for (int i = 1; i < kStages - 1; ++i) fetch();
+
+  for (;;) {
+    const int n = min(units - first, todo);
+    Query<NT> q;
+    q.load(p, static_cast<size_t>(b) * p.hq + h * G, G, sc.flip, g, t);
+    Softmax<NT> st;
+    st.clear();
+    int mine = min(kv_len - first * 16, n * 16);
+    for (int i = 0; i < n; i += kPair, mine -= 16 * kPair) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      fetch();
+      st.add(q, at + tok * 64 + t * 16, at + kv4::kParBase + tok * 8, at + kv4::kUnitBytes + token_of_row(2 * t) * 64 + g * 8,
+             at + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8, mine, tok, t, sc.scale, sc.lag);
+      at = at == ring_mem + (kStages - 1) * kSlot ? ring_mem : at + kSlot;
+    }
+    st.finish();
+    const bool whole = n == units;
+    const int pair = b * p.hkv + h;
+    const size_t slot = static_cast<size_t>(run) + pair;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int hd = 0; hd < 2; ++hd) {
+        const int head = nt * 8 + 2 * t + hd;
+        if (head < G) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 v = st.quad(nt, hd, j);
+            if (whole)
+              store_out(p.out + (static_cast<size_t>(pair) * G + head) * kD + 16 * g + 4 * j, v, st.l[nt][hd]);
+            else
+              *reinterpret_cast<float4*>(ws.o + (slot * 8 * NT + head) * kD + 16 * g + 4 * j) = v;
+          }
+          if (!whole && g == 0)
+            *reinterpret_cast<float2*>(ws.ml + (slot * 8 * NT + head) * 2) = make_float2(st.m[nt][hd], st.l[nt][hd]);
+        }
+      }
+    todo -= n;
+    if (todo == 0) break;
+    first = 0;
+    if (++h == p.hkv) {
+      h = 0;
+      do {
+        kv_len = kv_len_of(p, ++b, kIdDecode);
+        units = (kv_len + 15) / 16;
+      } while (units == 0);
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// Joins the partial results of the pairs that several runs share, and clears the rows of empty sequences. A CTA per
+// (pair, query head); its warps take the partials in turn, a lane four channels.
+__global__ void kv4_join_kernel(const Params p, const Shares ws, int num_seqs, int rows) {
   grid_dep_launch();
   grid_dep_wait();
-  const size_t row = blockIdx.x;
-  const int d = threadIdx.x;
-  float M = kNoMax;
-  for (int s = 0; s < splits; ++s) M = fmaxf(M, ws_ml[(row * splits + s) * 2]);
-  float L = 0.f, acc = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(ws_ml + (row * splits + s) * 2);
-    const float f = exp2f(ml.x - M);
-    L += ml.y * f;
-    acc += ws_o[(row * splits + s) * kD + d] * f;
+  __shared__ float4 sm_o[16][32];
+  __shared__ float sm_m[16], sm_l[16];
+  const int G = p.hq / p.hkv;
+  const int pair = blockIdx.x, head = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int b = pair / p.hkv, h = pair - b * p.hkv;
+  const int before = ws.begin[b], units = ws.begin[b + 1] - before, per = ws.begin[num_seqs + 1];
+  __nv_bfloat16* dst = p.out + (static_cast<size_t>(pair) * G + head) * kD + lane * 4;
+  if (units == 0) {
+    if (warp == 0) *reinterpret_cast<uint2*>(dst) = make_uint2(0u, 0u);
+    return;
   }
-  out[row * kD + d] = __float2bfloat16(L == 0.f ? 0.f : acc / L);
+  const long long from = static_cast<long long>(before) * p.hkv + static_cast<long long>(h) * units;
+  const int run0 = static_cast<int>(from / per), run1 = static_cast<int>((from + units - 1) / per);
+  if (run0 == run1) return;                    // written by its run
+  const float scale = Scale(p.scale_log2).scale;
+  float M = kNoMax, L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int r = run0 + warp; r <= run1; r += warps) {
+    const size_t slot = (static_cast<size_t>(r) + pair) * rows + head;
+    const float2 ml = *reinterpret_cast<const float2*>(ws.ml + slot * 2);
+    const float4 v = *reinterpret_cast<const float4*>(ws.o + slot * kD + lane * 4);
+    const float mn = fmaxf(M, ml.x), f0 = exp2f((M - mn) * scale), f1 = exp2f((ml.x - mn) * scale);
+    M = mn;
+    L = L * f0 + ml.y * f1;
+    acc.x = acc.x * f0 + v.x * f1; acc.y = acc.y * f0 + v.y * f1;
+    acc.z = acc.z * f0 + v.z * f1; acc.w = acc.w * f0 + v.w * f1;
+  }
+  sm_o[warp][lane] = acc;
+  if (lane == 0) {
+    sm_m[warp] = M;
+    sm_l[warp] = L;
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  for (int w = 0; w < warps; ++w) M = fmaxf(M, sm_m[w]);
+  L = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int w = 0; w < warps; ++w) {
+    const float f = exp2f((sm_m[w] - M) * scale);
+    const float4 v = sm_o[w][lane];
+    L += sm_l[w] * f;
+    acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+  }
+  store_out(dst, acc, L);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -704,22 +980,22 @@ int fill(Params& p, const void* q, const void* k_cache, const void* v_cache, con
   return 0;
 }
 
-using DecodeKernel = void (*)(Params);
 // Shared memory above 48 KiB is opted into once per device.
-int decode_kernel(bool wide, DecodeKernel* out) {
-  static constexpr DecodeKernel all[2] = {kv4_decode_kernel<1, 4>, kv4_decode_kernel<2, 4>};
+int allow_decode_kernels() {
   static std::atomic<bool> done[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return XV_ERR_LAUNCH;
-  if (!done[dev].load(std::memory_order_acquire)) {
-    for (DecodeKernel k : all)
-      if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(4)) != cudaSuccess)
-        return XV_ERR_LAUNCH;
-    done[dev].store(true, std::memory_order_release);
-  }
-  *out = all[wide];
+  if (done[dev].load(std::memory_order_acquire)) return 0;
+  const auto at = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  if (cudaFuncSetAttribute(kv4_decode_kernel<1, 4>, at, decode_smem(4)) != cudaSuccess ||
+      cudaFuncSetAttribute(kv4_decode_kernel<2, 4>, at, decode_smem(4)) != cudaSuccess ||
+      cudaFuncSetAttribute(kv4_share_kernel<1>, at, decode_smem(kShareWarps)) != cudaSuccess ||
+      cudaFuncSetAttribute(kv4_share_kernel<2>, at, decode_smem(kShareWarps)) != cudaSuccess)
+    return XV_ERR_LAUNCH;
+  done[dev].store(true, std::memory_order_release);
   return 0;
 }
+int share_ctas(int num_sms, int nt) { return num_sms * (nt == 1 ? 3 : 2); }
 
 inline int launch_ok() { return cudaGetLastError() == cudaSuccess ? 0 : XV_ERR_LAUNCH; }
 
@@ -727,48 +1003,59 @@ inline int launch_ok() { return cudaGetLastError() == cudaSuccess ? 0 : XV_ERR_L
 
 extern "C" {
 
-// KV splits of a decode launch. From launch-shape constants only (never from sequence lengths), so a captured graph keeps
-// its shape. Up to 8 are one cluster per (sequence, KV head); more go through a workspace and a second kernel.
+// How a decode launch divides its work, from launch-shape constants only (never from sequence lengths), so that a captured
+// graph keeps its shape: 1, 2, 4 or 8 CTAs (one cluster) per (sequence, KV head), or 0 for even shares.
 int xv_kv4_decode_splits(int num_seqs, int hkv, int num_sms, int max_tokens_per_seq) {
-  const long long ctas = static_cast<long long>(num_seqs) * hkv;
+  const long long pairs = static_cast<long long>(num_seqs) * hkv;
+  if (pairs * max_tokens_per_seq > 2048ll * num_sms) return 0;
   int s = 1;
-  while (s < 8 && ctas * s < 2 * num_sms && max_tokens_per_seq / (2 * s) >= 128) s *= 2;
-  if (s == 8 && ctas * s < num_sms && max_tokens_per_seq >= 8192)
-    s = static_cast<int>(std::min<long long>(3 * num_sms / ctas, max_tokens_per_seq / 256));
+  while (s < 8 && pairs * s < 2 * num_sms && max_tokens_per_seq / (2 * s) >= 128) s *= 2;
   return s;
 }
 
-long long xv_kv4_decode_workspace_bytes(int num_seqs, int hq, int splits) {
-  return splits <= 8 ? 0 : static_cast<long long>(num_seqs) * hq * splits * (kD + 2) * 4;
+long long xv_kv4_decode_workspace_bytes(int num_seqs, int hq, int hkv, int splits, int num_sms) {
+  if (splits > 0) return 0;
+  const int nt = hq / hkv > 8 ? 2 : 1;
+  const long long slots = static_cast<long long>(share_ctas(num_sms, nt)) * kShareWarps + static_cast<long long>(num_seqs) * hkv;
+  return slots * 8 * nt * (kD + 2) * 4 + (static_cast<long long>(num_seqs) + 2) * 4;
 }
 
 int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* kv_lens,
                   void* out, int num_seqs, int hq, int hkv, int d, int block_size, int max_blocks, int num_blocks,
-                  float scale, int splits, void* workspace, long long workspace_bytes, int* status, cudaStream_t stream) {
+                  float scale, int splits, int num_sms, void* workspace, long long workspace_bytes, int* status,
+                  cudaStream_t stream) {
   if (num_seqs <= 0) return 0;
   Params p;
   if (int rc = fill(p, q, k_cache, v_cache, block_tables, kv_lens, out, hq, hkv, d, block_size, max_blocks, num_blocks,
                     scale, status))
     return rc;
-  if (hq / hkv > 16 || hkv > 65535 || num_seqs > 65535 || splits < 1) return XV_ERR_SHAPE;
+  if (hq / hkv > 16 || hkv > 65535 || num_seqs > 65535 || splits < 0 || splits > 8) return XV_ERR_SHAPE;
   if (static_cast<long long>(hkv) * block_size * kv4::kRow > 0xffffffffLL) return XV_ERR_SHAPE;    // bytes of a page: 32-bit
-  const long long need = xv_kv4_decode_workspace_bytes(num_seqs, hq, splits);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return XV_ERR_WORKSPACE;
-  if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15)) return XV_ERR_ALIGN;
+  if (int rc = allow_decode_kernels()) return rc;
   p.splits = splits;
-  if (need > 0) {
-    p.ws_o = static_cast<float*>(workspace);
-    p.ws_ml = p.ws_o + static_cast<size_t>(num_seqs) * hq * splits * kD;
-  }
-  DecodeKernel kernel;
-  if (int rc = decode_kernel(hq / hkv > 8, &kernel)) return rc;
-  launch_pdl_cluster(kernel, dim3(splits, hkv, num_seqs), dim3(4 * 32), decode_smem(4), stream, need > 0 ? 1u : splits, p);
-  if (int rc = launch_ok()) return rc;
-  if (need > 0) {
-    launch_pdl(kv4_combine_kernel, dim3(num_seqs * hq), dim3(kD), 0, stream, p.ws_o, p.ws_ml, p.out, splits);
+  const int nt = hq / hkv > 8 ? 2 : 1;
+  if (splits > 0) {
+    launch_pdl_cluster(nt == 1 ? kv4_decode_kernel<1, 4> : kv4_decode_kernel<2, 4>, dim3(splits, hkv, num_seqs), dim3(4 * 32),
+                       decode_smem(4), stream, splits, p);
     return launch_ok();
   }
-  return 0;
+  const long long units = static_cast<long long>(max_blocks) * (block_size / kv4::kUnit);
+  if (units * num_seqs * hkv > 0x7fffffffLL || static_cast<long long>(num_seqs) * hkv > 0x7fffffffLL) return XV_ERR_SHAPE;
+  if (!workspace || workspace_bytes < xv_kv4_decode_workspace_bytes(num_seqs, hq, hkv, 0, num_sms)) return XV_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return XV_ERR_ALIGN;
+  const int ctas = share_ctas(num_sms, nt);
+  Shares ws;
+  ws.o = static_cast<float*>(workspace);
+  const size_t slots = static_cast<size_t>(ctas) * kShareWarps + static_cast<size_t>(num_seqs) * hkv;
+  ws.ml = ws.o + slots * 8 * nt * kD;
+  ws.begin = reinterpret_cast<int*>(ws.ml + slots * 8 * nt * 2);
+  launch_pdl(nt == 1 ? kv4_share_kernel<1> : kv4_share_kernel<2>, dim3(ctas), dim3(kShareWarps * 32), decode_smem(kShareWarps),
+             stream, p, ws, num_seqs);
+  if (int rc = launch_ok()) return rc;
+  // Few pairs have many partials each: more warps per row.
+  const int threads = num_seqs * hkv <= 64 ? 512 : 64;
+  launch_pdl(kv4_join_kernel, dim3(num_seqs * hkv, hq / hkv), dim3(threads), 0, stream, p, ws, num_seqs, 8 * nt);
+  return launch_ok();
 }
 
 int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_q,

@@ -190,7 +190,7 @@ int xv_qwen3_forward(const XvModelDesc* m, const XvBatchDesc* b, const XvArena* 
   const int splits_attn = n_dec <= 0 ? 1
                           : m->kv4   ? xv_kv4_decode_splits(n_dec, m->hkv, a->num_sms, max_kv)
                                      : decode_splits(n_dec, m->hkv, a->num_sms, max_kv);
-  if (n_dec > 0 && (m->kv4 ? xv_kv4_decode_workspace_bytes(n_dec, m->hq, splits_attn)
+  if (n_dec > 0 && (m->kv4 ? xv_kv4_decode_workspace_bytes(n_dec, m->hq, m->hkv, splits_attn, a->num_sms)
                            : xv_attn_decode_workspace_bytes(n_dec, m->hq, D, splits_attn)) > a->attn_ws_bytes) {
     g_failed_op = 20;
     return XV_ERR_WORKSPACE;
@@ -224,8 +224,8 @@ int xv_qwen3_forward(const XvModelDesc* m, const XvBatchDesc* b, const XvArena* 
     if (m->kv4) {
       if (n_dec > 0)
         XV_TRY(37, xv_kv4_decode(a->q, w.k_cache, w.v_cache, b->block_tables, b->kv_lens, a->attn, n_dec, m->hq, m->hkv, D,
-                                 m->block_size, b->max_blocks, m->num_kv_blocks, m->attn_scale, splits_attn, a->attn_ws,
-                                 a->attn_ws_bytes, a->status, stream));
+                                 m->block_size, b->max_blocks, m->num_kv_blocks, m->attn_scale, splits_attn, a->num_sms,
+                                 a->attn_ws, a->attn_ws_bytes, a->status, stream));
       if (n_pre > 0)
         XV_TRY(38, xv_kv4_prefill(a->q, w.k_cache, w.v_cache, b->block_tables, b->cu_q, b->kv_lens, a->attn, n_dec, n_pre,
                                   b->max_q_len, T, m->hq, m->hkv, D, m->block_size, b->max_blocks, m->num_kv_blocks,

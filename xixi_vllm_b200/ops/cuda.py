@@ -85,10 +85,10 @@ def lib():
                                _i32, _i32, _i32, _vp, _vp]
     L.xv_kv4_read.argtypes = [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp]
     L.xv_kv4_decode_splits.argtypes = [_i32, _i32, _i32, _i32]
-    L.xv_kv4_decode_workspace_bytes.argtypes = [_i32, _i32, _i32]
+    L.xv_kv4_decode_workspace_bytes.argtypes = [_i32] * 5
     L.xv_kv4_decode_workspace_bytes.restype = _i64
-    L.xv_kv4_decode.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp,
-                                _i64, _vp, _vp]
+    L.xv_kv4_decode.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32,
+                                _vp, _i64, _vp, _vp]
     L.xv_kv4_prefill.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                  _i32, _f32, _vp, _vp]
     L.xv_argmax.argtypes = [_vp, _vp, _i32, _i32, _i64, _vp]
@@ -469,11 +469,11 @@ def _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, 
     L, st, stream = lib(), _state(q), torch._C._cuda_getCurrentRawStream(dev.index)
     if n_d:
         splits = L.xv_kv4_decode_splits(n_d, num_kv_heads, st.num_sms, maxb * bs)
-        need = L.xv_kv4_decode_workspace_bytes(n_d, num_q_heads, splits) if splits > 8 else 0
+        need = 0 if splits else L.xv_kv4_decode_workspace_bytes(n_d, num_q_heads, num_kv_heads, 0, st.num_sms)
         # from torch's allocator, call by call: calls on two streams, or two captured graphs, never share it
         ws = k_cache.new_empty(need) if need else None
         _check(L.xv_kv4_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), tables, lens, out.data_ptr(), n_d,
-                               num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale, splits,
+                               num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale, splits, st.num_sms,
                                ws.data_ptr() if need else None, need, st.status.data_ptr(), stream), "kv4_decode")
     if n_p:
         _check(L.xv_kv4_prefill(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), tables,

@@ -158,11 +158,8 @@ class NativeForward:
             self.t["gu"] = buf(T, 2 * d.inter_local)
         st = cuda._state(self.t["h"])
         if d.kv4:
-            # splits shrink as the batch grows, so the largest need is looked for, up to the longest block table
-            tokens = -(-cfg.max_position_embeddings // d.block_size) * d.block_size
-            need = max(L.xv_kv4_decode_workspace_bytes(n, d.hq, L.xv_kv4_decode_splits(n, d.hkv, st.num_sms, tokens))
-                       for n in range(1, max_samples + 1))
-            attn_ws = self.t["attn_ws"] = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+            need = L.xv_kv4_decode_workspace_bytes(max_samples, d.hq, d.hkv, 0, st.num_sms)
+            attn_ws = self.t["attn_ws"] = torch.empty(need, dtype=torch.uint8, device=dev)
         else:
             need = L.xv_attn_decode_workspace_bytes(max_samples, d.hq, d.head_dim, 16)
             if need > st.attn_ws.numel():
