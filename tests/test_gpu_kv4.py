@@ -283,6 +283,62 @@ def test_long_chunks(q_len, kv_len):
     _attend([q_len, 67], [kv_len, 67], 4, 2, seed=q_len)
 
 
+@pytest.mark.parametrize("hq,hkv,bs", [(8, 8, 16), (2, 1, 48), (5, 1, 16), (8, 1, 128), (16, 1, 32), (12, 1, 16)])
+def test_chunks_of_every_group_size(hq, hkv, bs):
+    _attend([70, 1, 33], [70 + 131, 1, 33], hq, hkv, bs=bs, seed=hq)
+
+
+def test_chunk_growing_maxima():
+    _attend([150], [500], 4, 1, q_scale=8.0, seed=9)
+
+
+def test_chunk_values_of_mixed_magnitude():
+    """Tiles of K and V whose magnitudes differ by 2^20 either way: the tile exponents move up and down."""
+    hq, hkv, bs, n = 4, 1, 16, 400
+    nb = n // bs + 2
+    g = torch.Generator().manual_seed(3)
+    ramp = torch.tensor([2.0 ** (20 * ((t // 130) % 3 - 1)) for t in range(nb * bs)])[:, None, None]
+    k, v = (torch.zeros(nb, hkv, bs, kv4.row_bytes(D), dtype=torch.uint8) for _ in range(2))
+    kv4.write_rows(k, torch.arange(nb * bs), torch.randn(nb * bs, hkv, D, generator=g) * ramp.clamp(max=1.0))
+    kv4.write_rows(v, torch.arange(nb * bs), torch.randn(nb * bs, hkv, D, generator=g) * ramp)
+    q = (torch.randn(n, hq * D, generator=g) * 0.5).bfloat16()
+    table = torch.arange(nb, dtype=torch.int32)[None]
+    i32 = dict(dtype=torch.int32, device=DEV)
+    attn = AttnBatch(torch.tensor([0, n], **i32), torch.tensor([n], **i32), table.to(DEV), 1, 0, n, n, n)
+    out = _ops().paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), attn, D ** -0.5, hq, hkv, D)
+    _cuda().check_status()
+    ref, mag, _, qk = kv4_ref.attention(q, k, v, [n], [n], table, D ** -0.5, hq)
+    got = out.double().cpu().numpy().reshape(n, hq, D)
+    # as in _attend: bf16 roundings of K, V, P and the output bound any of the kernels
+    tol = HALF_BF16 * (np.abs(ref) + 2 * mag) * (1 + HALF_BF16) + (np.exp(2 * HALF_BF16 * qk[..., None]) - 1) * mag + 2.0 ** -18 * mag
+    assert ((np.abs(got - ref) - tol) <= 0).all()
+
+
+@pytest.mark.parametrize("q_len", [40, 200])
+def test_chunk_nan_in_the_sequence_reaches_the_rows_that_see_it(q_len):
+    """NaN parameters of K and of V at single positions: rows before them are as if they were not there."""
+    hq, hkv, bs = 4, 1, 16
+    n = q_len + 30
+    nb = n // bs + 2
+    k, v = _random(nb, hkv, bs, 5)
+    hk, hv = k.cpu(), v.cpu()
+    bad_k, bad_v = 30 + q_len // 2, 30 + 3 * q_len // 4
+    kv4.write_rows(hk, torch.tensor([bad_k]), torch.full((1, hkv, D), float("nan")))
+    kv4.write_rows(hv, torch.tensor([bad_v]), torch.full((1, hkv, D), float("nan")))
+    q = torch.randn(q_len, hq * D, generator=torch.Generator().manual_seed(6)).bfloat16().to(DEV)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    table = torch.arange(nb, **i32)[None]
+    attn = AttnBatch(torch.tensor([0, q_len], **i32), torch.tensor([n], **i32), table, 1, 0, q_len, n, q_len)
+    clean = _ops().paged_attention(q, k, v, attn, 0.09, hq, hkv, D)
+    for c, b in ((hk, bad_k), (hv, bad_v)):
+        args = (c.to(DEV), v) if c is hk else (k, c.to(DEV))
+        out = _ops().paged_attention(q, *args, attn, 0.09, hq, hkv, D)
+        first = b - 30                                       # the query row at that position
+        assert torch.equal(out[:first], clean[:first])
+        assert bool(out[first:].isnan().any(-1).all())
+    _cuda().check_status()
+
+
 def test_small_and_large_values():
     _attend([1, 30], [40, 60], 4, 2, n_decode=1, v_scale=2.0 ** -60, q_scale=2.0 ** 60)
     _attend([1, 30], [40, 60], 4, 2, n_decode=1, v_scale=2.0 ** 40, q_scale=2.0 ** -40)

@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 
 #include "../common/kv4.cuh"
 #include "../common/launch.cuh"
@@ -1067,6 +1068,10 @@ int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, cons
   if (int rc = fill(p, q, k_cache, v_cache, block_tables, kv_lens, out, hq, hkv, d, block_size, max_blocks, num_blocks,
                     scale, status))
     return rc;
+  const char* e = std::getenv("XV_KV4_TC");
+  if (hq / hkv <= 16 && max_q_len * (hq / hkv) > (e ? std::atoi(e) : 64))
+    return xv_kv4_prefill_tc(q, k_cache, v_cache, block_tables, cu_q, kv_lens, out, seq_begin, num_seqs, max_q_len, total_rows,
+                             hq, hkv, d, block_size, max_blocks, num_blocks, scale, status, stream);
   if (hq > 65535 || num_seqs > 65535) return XV_ERR_SHAPE;
   p.cu_q = cu_q;
   p.seq_begin = seq_begin;

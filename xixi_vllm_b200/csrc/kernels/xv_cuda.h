@@ -173,6 +173,11 @@ int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, cons
                    const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq,
                    int hkv, int d, int block_size, int max_blocks, int num_blocks, float scale, int* status,
                    cudaStream_t stream);
+// The chunk form on tcgen05 tensor cores (attn_prefill_kv4_sm100.cu); xv_kv4_prefill calls it where it is the faster one.
+int xv_kv4_prefill_tc(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_q,
+                      const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq,
+                      int hkv, int d, int block_size, int max_blocks, int num_blocks, float scale, int* status,
+                      cudaStream_t stream);
 
 // Input ids < 0 are references into the previous step's samples: ids[i] = prev[-ids[i] - 1] (elementwise.cu).
 int xv_resolve_token_refs(int* ids, int n, const long long* prev, int n_prev, cudaStream_t stream);
