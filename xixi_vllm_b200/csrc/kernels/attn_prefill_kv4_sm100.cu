@@ -44,7 +44,7 @@ constexpr int kBM = 128, kBN = 128;               // lanes of a unit, tokens of 
 constexpr int kHalf = kBN * 128;                  // bytes of 64 channels of a tile
 constexpr int kTileBytes = 2 * kHalf;             // 32 KiB
 constexpr int kNK = 3, kNV = 2;                   // ring slots
-constexpr int kBarBytes = 512;
+constexpr int kBarBytes = 512 + 2 * kBM * 4;      // barriers and small arrays; a float per lane
 constexpr int kSmem = (2 + kNK + kNV) * kTileBytes + 1024 + kBarBytes;
 constexpr uint32_t kTmemCols = 512, kTmemUnit = 256, kTmemO = 128;
 constexpr int kId = 12;
@@ -73,6 +73,11 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ uint32_t idesc_f16(int m, int n) {
   return (1u << 4) | static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
@@ -82,9 +87,13 @@ __device__ __forceinline__ void set_regs_up() { asm volatile("setmaxnreg.inc.syn
 template <int N>
 __device__ __forceinline__ void set_regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// Byte offset of 16-byte chunk c (0..15: one word of channels) of row r in a tile.
-__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
-  return static_cast<uint32_t>((c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+// Address of 16-byte chunk c (0..15: one word of channels) of a row: `row_at` is the row's start with its swizzle (row & 7)
+// in the chunk bits.
+__device__ __forceinline__ uint32_t row_start(uint32_t tile, int row) {
+  return tile + static_cast<uint32_t>(row * 128 + ((row & 7) << 4));
+}
+__device__ __forceinline__ uint32_t chunk_at(uint32_t row_at, int c) {
+  return (row_at ^ static_cast<uint32_t>((c & 7) << 4)) + (c >> 3) * kHalf;
 }
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -101,21 +110,26 @@ __device__ __forceinline__ __half2 centred_f16(uint32_t w, bool odd) {
   return __hsub2(*reinterpret_cast<const __half2*>(&r), __floats2half2_rn(1032.f, 1032.f));
 }
 
-// 32 of a row's 64 code bytes as fp16 c + s (n - 8) into chunks 4 c0 .. : words of even index belong to group 0.
-__device__ __forceinline__ void put_words(uint32_t tile, int row, int c0, const uint4& codes, __half2 s0, __half2 o0,
-                                          __half2 s1, __half2 o1) {
+// A group's parameters as fp16 pairs, the tile's power of two taken out.
+struct Pair {
+  __half2 s, c;
+  __device__ __forceinline__ Pair(uint32_t w, float f) : s(__float2half2_rn(kv4::par_s(w) * f)), c(__float2half2_rn(kv4::par_c(w) * f)) {}
+};
+
+// 16 of a row's 64 code bytes as fp16 c + s (n - 8) into chunks c0 .. c0 + 3: words of even index belong to group 0.
+__device__ __forceinline__ void put_words(uint32_t row_at, int c0, const uint4& codes, const Pair& g0, const Pair& g1) {
   const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 s = (i & 1) ? s1 : s0, o = (i & 1) ? o1 : o0;
+    const Pair& g = (i & 1) ? g1 : g0;
     const uint32_t hi = w[i] >> 8;
     uint32_t v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const __half2 x = __hfma2(centred_f16(j < 2 ? w[i] : hi, j & 1), s, o);
+      const __half2 x = __hfma2(centred_f16(j < 2 ? w[i] : hi, j & 1), g.s, g.c);
       v[j] = *reinterpret_cast<const uint32_t*>(&x);
     }
-    st_shared_v4(tile + chunk_at(row, c0 + i), v[0], v[1], v[2], v[3]);
+    st_shared_v4(chunk_at(row_at, c0 + i), v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -166,6 +180,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   uint32_t* red = reinterpret_cast<uint32_t*>(scales + 8);   // [2][12]
   uint32_t* tmem_slot = red + 24;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* row_power = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);      // [2][128]
 
   if (threadIdx.x == 0) {
     for (int u = 0; u < 2; ++u) {
@@ -201,73 +216,85 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     const int row = threadIdx.x & 127;
     const int upp = p.block_size / kv4::kUnit;
     const int* table = p.block_tables + static_cast<size_t>(b) * p.max_blocks;
-    // This thread's row of tile j: offsets of its codes and parameters (a row past the end reads the last token's).
-    auto place = [&](int j, size_t* code, size_t* par) {
-      const int tok = min(j * kBN + row, n_kv - 1);
-      const int page = tok / p.block_size, r = tok - page * p.block_size;
-      int blk = __ldg(table + page);
-      if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) {
-        report_status(p.status, kId, kBadIndex);
-        blk = 0;
+    // This thread's row, tile by tile: page and place in it follow from the tile before. Pages past the last one are
+    // replaced by it; whatever row that reads does not count. A page's number is read two tiles ahead of its bytes' use.
+    const int last_page = (max(n_kv, 1) - 1) / p.block_size;
+    const int page_step = kBN / p.block_size, place_step = kBN % p.block_size;
+    int page = row / p.block_size, place = row - page * p.block_size, place_next = 0, entry = 0;
+    auto look = [&]() { entry = __ldg(table + min(page, last_page)); place_next = place; };
+    auto step = [&]() {
+      page += page_step;
+      place += place_step;
+      if (place >= p.block_size) {
+        place -= p.block_size;
+        ++page;
       }
-      const size_t unit = ((static_cast<size_t>(blk) * p.hkv + hk) * upp + r / kv4::kUnit) * kv4::kUnitBytes;
-      *code = unit + (r % kv4::kUnit) * kv4::kCodeRow;
-      *par = unit + kv4::kParBase + (r % kv4::kUnit) * kv4::kParRow;
     };
-    size_t code = 0, par = 0;
-    uint4 kc[4], vc[4];
-    uint2 kp = make_uint2(0, 0), vp = make_uint2(0, 0), kp_next, vp_next;
-    auto load_codes = [&](uint4 (&c)[4], const uint8_t* cache) {
+    const uint8_t *code = nullptr, *par = nullptr;           // in K's cache; V's is v_off further
+    const ptrdiff_t v_off = p.v_cache - p.k_cache;
+    auto resolve = [&]() {                                   // addresses from the entry that look() read
+      if (static_cast<unsigned>(entry) >= static_cast<unsigned>(p.num_blocks)) {
+        report_status(p.status, kId, kBadIndex);
+        entry = 0;
+      }
+      const size_t unit = ((static_cast<size_t>(entry) * p.hkv + hk) * upp + (place_next >> 4)) * kv4::kUnitBytes;
+      code = p.k_cache + unit + (place_next & 15) * kv4::kCodeRow;
+      par = p.k_cache + unit + kv4::kParBase + (place_next & 15) * kv4::kParRow;
+    };
+    auto load_codes = [&](uint4 (&c)[4], const uint8_t* at) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = __ldg(reinterpret_cast<const uint4*>(cache + code) + i);
+      for (int i = 0; i < 4; ++i) c[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
     };
-    if (n_tiles > 0) {
-      place(0, &code, &par);
-      kp = __ldg(reinterpret_cast<const uint2*>(p.k_cache + par));
-      vp = __ldg(reinterpret_cast<const uint2*>(p.v_cache + par));
-      load_codes(kc, p.k_cache);
-      load_codes(vc, p.v_cache);
-      place(min(1, n_tiles - 1), &code, &par);
-    }
-    int ek = 0, ev = 0;
-    // A wait that runs out is only noted: the four warps leave together, at the barrier of the next tile.
-    bool ok = true;
-    for (int j = 0; j < n_tiles; ++j) {
-      // The next tile's parameters now, its codes as the registers of this tile's become free.
-      kp_next = __ldg(reinterpret_cast<const uint2*>(p.k_cache + par));
-      vp_next = __ldg(reinterpret_cast<const uint2*>(p.v_cache + par));
+    uint4 kc[4], vc[4];
+    uint2 kp, vp, kp_next = make_uint2(0u, 0u), vp_next = make_uint2(0u, 0u);
+    // What counts of tile j's parameters (a V that is not finite makes K not finite instead), and the tile's largest
+    // possible magnitudes, left in `red` for everyone.
+    auto admit = [&](int j, bool ok) {
       if (j * kBN + row >= n_kv) kp = vp = make_uint2(0u, 0u);
-      // exponent bits all ones: not finite
       auto finite = [](uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; };
       if (!finite(vp.x) || !finite(vp.y)) {
         vp = make_uint2(0u, 0u);
         kp = make_uint2(0x7fff7fffu, 0x7fff7fffu);
       }
-      const float ks0 = kv4::par_s(kp.x), kc0 = kv4::par_c(kp.x), ks1 = kv4::par_s(kp.y), kc1 = kv4::par_c(kp.y);
-      const float vs0 = kv4::par_s(vp.x), vc0 = kv4::par_c(vp.x), vs1 = kv4::par_s(vp.y), vc1 = kv4::par_c(vp.y);
-      const bool k_fine = finite(kp.x) && finite(kp.y);
-      const float kb = k_fine ? fmaxf(fabsf(kc0) + 8.f * fabsf(ks0), fabsf(kc1) + 8.f * fabsf(ks1)) : 0.f;
-      const float vb = fmaxf(fabsf(vc0) + 8.f * fabsf(vs0), fabsf(vc1) + 8.f * fabsf(vs1));
-      const uint32_t kw = __reduce_max_sync(0xffffffffu, __float_as_uint(kb));
-      const uint32_t vw = __reduce_max_sync(0xffffffffu, __float_as_uint(vb));
-      uint32_t* slot_red = red + (j & 1) * 12;
-      if (lane == 0) {
-        slot_red[warp & 3] = kw;
-        slot_red[4 + (warp & 3)] = vw;
-        slot_red[8 + (warp & 3)] = ok ? 0u : 1u;
-      }
-      named_barrier(1, 128);
-      if ((slot_red[8] | slot_red[9] | slot_red[10] | slot_red[11]) != 0u) break;
-      const uint32_t kbits = max(max(slot_red[0], slot_red[1]), max(slot_red[2], slot_red[3]));
-      const uint32_t vbits = max(max(slot_red[4], slot_red[5]), max(slot_red[6], slot_red[7]));
-      // Largest magnitude of the stored tile: 8 .. 16 when an exponent is chosen, kept while it stays in 2^-4 .. 2^15.
-      auto choose = [](int e, uint32_t bits) {
-        const int top = static_cast<int>(bits >> 23) - 127;
-        if (bits != 0 && (top - e > 14 || top - e < -4)) e = top - 3;
-        return max(-100, min(100, e));
+      auto bound = [](uint2 w) {
+        return fmaxf(fabsf(kv4::par_c(w.x)) + 8.f * fabsf(kv4::par_s(w.x)), fabsf(kv4::par_c(w.y)) + 8.f * fabsf(kv4::par_s(w.y)));
       };
-      ek = choose(ek, kbits);
-      ev = choose(ev, vbits);
+      const uint32_t kb = __float_as_uint(finite(kp.x) && finite(kp.y) ? bound(kp) : 0.f), vb = __float_as_uint(bound(vp));
+      const uint32_t kw = __reduce_max_sync(0xffffffffu, kb), vw = __reduce_max_sync(0xffffffffu, vb);
+      if (lane == 0) {
+        uint32_t* at = red + (j & 1) * 12 + (warp & 3);
+        at[0] = kw;
+        at[4] = vw;
+        at[8] = ok ? 0u : 1u;
+      }
+    };
+    // Largest magnitude of a stored tile: 2^14 .. 2^15 when an exponent is chosen (smaller values of the tile then keep
+    // fp16's precision down to 2^-29 of it), kept while it stays in 2^7 .. 2^15.
+    auto choose = [](int e, uint32_t bits) {
+      const int top = static_cast<int>(bits >> 23) - 127;
+      if (bits != 0 && (top - e > 14 || top - e < 7)) e = top - 12;
+      return max(-100, min(100, e));
+    };
+    int ek = 0, ev = 0;
+    // A wait that runs out is only noted: the four warps leave together, at the barrier of the next tile.
+    bool ok = true;
+    if (n_tiles > 0) {
+      look();
+      resolve();
+      kp = __ldg(reinterpret_cast<const uint2*>(par));
+      vp = __ldg(reinterpret_cast<const uint2*>(par + v_off));
+      load_codes(kc, code);
+      load_codes(vc, code + v_off);
+      step();
+      look();
+      admit(0, true);
+    }
+    for (int j = 0; j < n_tiles; ++j) {
+      named_barrier(1, 128);
+      const uint32_t* seen = red + (j & 1) * 12;
+      if ((seen[8] | seen[9] | seen[10] | seen[11]) != 0u) break;
+      ek = choose(ek, max(max(seen[0], seen[1]), max(seen[2], seen[3])));
+      ev = choose(ev, max(max(seen[4], seen[5]), max(seen[6], seen[7])));
       if (row == 0) {
         TileScale sc;
         sc.k = pow2(ek);
@@ -276,35 +303,42 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         sc.unused = 0.f;
         scales[j & 7] = sc;
       }
+      const bool more = j + 1 < n_tiles;
+      if (more) {                                            // the next tile's parameters now, its codes as registers become free
+        resolve();
+        kp_next = __ldg(reinterpret_cast<const uint2*>(par));
+        vp_next = __ldg(reinterpret_cast<const uint2*>(par + v_off));
+        step();
+        look();
+      }
       const int ks = j % kNK, vs = j % kNV;
-      ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[ks], ((j / kNK) & 1) ^ 1) && *abort_flag == 0);
+      const uint2 vp_now = vp;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&k_empty[ks], ((j / kNK) & 1) ^ 1) && *abort_flag == 0);
       if (ok) {
         const float f = pow2(-ek);
-        const __half2 s0 = __float2half2_rn(ks0 * f), o0 = __float2half2_rn(kc0 * f), s1 = __float2half2_rn(ks1 * f),
-                      o1 = __float2half2_rn(kc1 * f);
-        const uint32_t tile = smem_u32(k_ring) + ks * kTileBytes;
+        const Pair g0(kp.x, f), g1(kp.y, f);
+        const uint32_t at = row_start(smem_u32(k_ring) + ks * kTileBytes, row);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) put_words(tile, row, 4 * i, kc[i], s0, o0, s1, o1);
+        for (int i = 0; i < 4; ++i) put_words(at, 4 * i, kc[i], g0, g1);
         fence_proxy_async_smem();
         mbar_arrive(&k_full[ks]);
       }
-      if (j + 1 < n_tiles) load_codes(kc, p.k_cache);
+      if (more) load_codes(kc, code);
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&v_empty[vs], ((j / kNV) & 1) ^ 1) && *abort_flag == 0);
       if (ok) {
         const float f = pow2(-ev);
-        const __half2 s0 = __float2half2_rn(vs0 * f), o0 = __float2half2_rn(vc0 * f), s1 = __float2half2_rn(vs1 * f),
-                      o1 = __float2half2_rn(vc1 * f);
-        const uint32_t tile = smem_u32(v_ring) + vs * kTileBytes;
+        const Pair g0(vp_now.x, f), g1(vp_now.y, f);
+        const uint32_t at = row_start(smem_u32(v_ring) + vs * kTileBytes, row);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) put_words(tile, row, 4 * i, vc[i], s0, o0, s1, o1);
+        for (int i = 0; i < 4; ++i) put_words(at, 4 * i, vc[i], g0, g1);
         fence_proxy_async_smem();
         mbar_arrive(&v_full[vs]);
       }
-      if (j + 1 < n_tiles) {
-        load_codes(vc, p.v_cache);
+      if (more) {
+        load_codes(vc, code + v_off);
         kp = kp_next;
         vp = vp_next;
-        place(min(j + 2, n_tiles - 1), &code, &par);
+        admit(j + 1, ok);
       }
     }
     if (!ok && lane == 0) {
@@ -312,45 +346,61 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       *abort_flag = 1;
     }
   } else if (wg == 3) {
-    // ---------------- MMA issuers: one thread per unit ----------------
+    // ---------------- MMA issuers: one warp per unit, one elected lane issues ----------------
+    // The whole warp walks the loop, so that descriptors stay in uniform registers: a lone lane took about 120 cycles an
+    // MMA, twice what the MMA itself takes.
     set_regs_down<48>();
-    const int u = warp - 12;
-    if (u < 2 && lane == 0 && n_tiles > 0) {
+    const int u = __shfl_sync(0xffffffffu, warp, 0) - 12;
+    if (u < 2 && n_tiles > 0) {
       const uint32_t idesc_s = idesc_f16(kBM, kBN), idesc_o = idesc_f16(kBM, kD) | (1u << 16);
-      const uint32_t q_addr = smem_u32(q_s) + u * kTileBytes;
-      const uint32_t k_addr0 = smem_u32(k_ring), v_addr0 = smem_u32(v_ring);
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s) + u * kTileBytes);
+      const uint64_t k_desc0 = umma_desc_sw128(smem_u32(k_ring)), v_desc0 = umma_desc_sw128_mn(smem_u32(v_ring), kHalf, 1024);
       const uint32_t s_tmem = tmem_base + u * kTmemUnit, o_tmem = s_tmem + kTmemO;
       bool ok = mbar_wait(&q_full[u], 0);
       int reason = kWaitFullTimeout;
-      auto issue_s = [&](int j) -> bool {
-        const int slot = j % kNK;
-        if (!mbar_wait(&k_full[slot], (j / kNK) & 1)) return false;
+      int ks = 0, vs = 0;                                     // ring slots and their phases
+      uint32_t kph = 0, vph = 0;
+      auto issue_s = [&]() -> bool {
+        if (!mbar_wait(&k_full[ks], kph)) return false;
         tc_fence_after_sync();
-        const uint32_t k_addr = k_addr0 + slot * kTileBytes;
+        if (elect_one()) {
+          const uint64_t k_desc = k_desc0 + static_cast<uint64_t>(ks * (kTileBytes >> 4));
 #pragma unroll
-        for (int ks = 0; ks < kD / 16; ++ks)
-          umma_bf16(s_tmem, umma_desc_sw128(q_addr + (ks >> 2) * kHalf + (ks & 3) * 32),
-                    umma_desc_sw128(k_addr + (ks >> 2) * kHalf + (ks & 3) * 32), idesc_s, ks > 0);
-        umma_commit(&s_full[u]);
-        umma_commit(&k_empty[slot]);
+          for (int i = 0; i < kD / 16; ++i) {
+            const uint64_t off = ((i >> 2) * kHalf + (i & 3) * 32) >> 4;
+            umma_bf16(s_tmem, q_desc + off, k_desc + off, idesc_s, i > 0);
+          }
+          umma_commit(&s_full[u]);
+          umma_commit(&k_empty[ks]);
+        }
+        __syncwarp();
+        if (++ks == kNK) {
+          ks = 0;
+          kph ^= 1;
+        }
         return true;
       };
-      if (ok) ok = issue_s(0);
+      ok = ok && issue_s();
       for (int j = 0; ok && j < n_tiles; ++j) {
         if (!mbar_wait(&p_ready[u], j & 1)) { ok = false; reason = kWaitAccumTimeout; break; }
-        const int slot = j % kNV;
-        if (!mbar_wait(&v_full[slot], (j / kNV) & 1)) { ok = false; break; }
+        if (!mbar_wait(&v_full[vs], vph)) { ok = false; break; }
         tc_fence_after_sync();
-        const uint32_t v_addr = v_addr0 + slot * kTileBytes;
+        if (elect_one()) {
+          const uint64_t v_desc = v_desc0 + static_cast<uint64_t>(vs * (kTileBytes >> 4));
 #pragma unroll
-        for (int ks = 0; ks < kBN / 16; ++ks)
-          umma_bf16_a_tmem(o_tmem, s_tmem + ks * 8, umma_desc_sw128_mn(v_addr + ks * 2048, kHalf, 1024), idesc_o,
-                           (j > 0 || ks > 0) ? 1u : 0u);
-        umma_commit(&o_done[u]);
-        umma_commit(&v_empty[slot]);
-        if (j + 1 < n_tiles && !issue_s(j + 1)) ok = false;
+          for (int i = 0; i < kBN / 16; ++i)
+            umma_bf16_a_tmem(o_tmem, s_tmem + i * 8, v_desc + i * (2048 >> 4), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
+          umma_commit(&o_done[u]);
+          umma_commit(&v_empty[vs]);
+        }
+        __syncwarp();
+        if (++vs == kNV) {
+          vs = 0;
+          vph ^= 1;
+        }
+        if (j + 1 < n_tiles && !issue_s()) ok = false;
       }
-      if (!ok || *abort_flag) {
+      if (lane == 0 && (!ok || *abort_flag)) {
         if (!ok) report_status(p.status, kId, reason);
         *abort_flag = 1;
       }
@@ -359,43 +409,50 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     // ---------------- softmax and output: thread r of unit u is query row r / G, head r % G ----------------
     set_regs_up<184>();
     const int u = wg, r = threadIdx.x & 127;
-    const int qr = r / G, hd = r - qr * G;
-    const int row = row0 + u * rpu + qr;
-    const bool live = qr < rpu && row < q_len;
+    const int row = row0 + u * rpu + r / G;
     const int pos = pos0 + min(row, q_len - 1);              // lanes without a row follow the last one
-    // Q: a power of two per row keeps it in fp16's range; a negative scale is its sign.
-    float row_scale;
+    // Q: a power of two per row keeps it in fp16's range; a negative scale is its sign. Sixteen lanes a row, two rows at a
+    // time, so that the reads are whole lines; the row's power goes to its own lane through shared memory.
     {
-      const uint4* src = reinterpret_cast<const uint4*>(
-          p.q + (static_cast<size_t>(q_begin + (live ? row : row0)) * p.hq + hk * G + (live ? hd : 0)) * kD);
-      uint4 v[16];
-      uint32_t top = 0;
+      const int c = lane & 15;
+      uint4 v[16];                                           // all reads in flight at once
+      {
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        v[c] = __ldg(src + c);
-        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-      }
-      const int e = max(-100, min(100, static_cast<int>(top >> 7) - 127));
-      const float f = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
-      row_scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * pow2(e);
-      const uint32_t tile = smem_u32(q_s) + u * kTileBytes;
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};   // channels 0 1, 2 3, 4 5, 6 7 of the word
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[2 * i] = __uint_as_float(w[i] << 16) * f;
-          x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * f;
+        for (int i = 0; i < 16; ++i) {
+          const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4), rr = qr_ / G, hh = qr_ - rr * G;
+          const int qrow = row0 + u * rpu + rr;
+          const bool there = rr < rpu && qrow < q_len;
+          v[i] = there ? __ldg(reinterpret_cast<const uint4*>(
+                                   p.q + (static_cast<size_t>(q_begin + qrow) * p.hq + hk * G + hh) * kD) + c)
+                       : make_uint4(0u, 0u, 0u, 0u);
         }
-        st_shared_v4(tile + chunk_at(r, c), pack_f16(x[0], x[4]), pack_f16(x[1], x[5]), pack_f16(x[2], x[6]),
-                     pack_f16(x[3], x[7]));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4);
+          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};       // channels 0 1, 2 3, 4 5, 6 7 of the word
+          uint32_t top = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+#pragma unroll
+          for (int k = 1; k < 16; k <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
+          const int e = max(-100, min(100, static_cast<int>(top >> 7) - 127));
+          const float f = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
+          float x[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            x[2 * k] = __uint_as_float(w[k] << 16) * f;
+            x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u) * f;
+          }
+          st_shared_v4(chunk_at(row_start(smem_u32(q_s) + u * kTileBytes, qr_), c), pack_f16(x[0], x[4]), pack_f16(x[1], x[5]),
+                       pack_f16(x[2], x[6]), pack_f16(x[3], x[7]));
+          if (c == 0) row_power[u * kBM + qr_] = pow2(e);
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(&q_full[u]);
+      __syncwarp();                                          // a warp's lanes read their own rows' powers only
     }
+    const float row_scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * row_power[u * kBM + r];
     const uint32_t taddr = tmem_base + u * kTmemUnit + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     float m = kNoMax, l = 0.f, vf = 1.f;
     bool ok = true;
@@ -403,31 +460,31 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[u], j & 1) && *abort_flag == 0);
       if (!ok) break;
       tc_fence_after_sync();
-      uint32_t sr[8][16];                                    // the score row: 128 fp32
-#pragma unroll
-      for (int c = 0; c < 8; ++c) tmem_ld16(taddr + c * 16, sr[c]);
+      uint32_t sr[4][32];                                    // the score row: 128 fp32
       const TileScale ts = scales[j & 7];
-      tmem_ld_wait();
       const int k0 = j * kBN;
-      if (k0 + kBN - 1 > pos) {
+      const bool diagonal = k0 + kBN - 1 > pos;
+      float mx[4];
+      tmem_ld32(taddr, sr[0]);
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
+      for (int c = 0; c < 4; ++c) {                          // the maximum of one quarter while the next is on its way
+        tmem_ld_wait();
+        tmem_ld_fence_regs(sr[c]);
+        if (c < 3) tmem_ld32(taddr + (c + 1) * 32, sr[c + 1]);
+        if (diagonal) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (k0 + c * 16 + i > pos) sr[c][i] = 0xff800000u;       // -inf
-      }
-      float mx[8];
+          for (int i = 0; i < 32; ++i)
+            if (k0 + c * 32 + i > pos) sr[c][i] = 0xff800000u;       // -inf
+        }
+        float a[10];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const float a0 = fmax3(__uint_as_float(sr[c][0]), __uint_as_float(sr[c][1]), __uint_as_float(sr[c][2]));
-        const float a1 = fmax3(__uint_as_float(sr[c][3]), __uint_as_float(sr[c][4]), __uint_as_float(sr[c][5]));
-        const float a2 = fmax3(__uint_as_float(sr[c][6]), __uint_as_float(sr[c][7]), __uint_as_float(sr[c][8]));
-        const float a3 = fmax3(__uint_as_float(sr[c][9]), __uint_as_float(sr[c][10]), __uint_as_float(sr[c][11]));
-        const float a4 = fmax3(__uint_as_float(sr[c][12]), __uint_as_float(sr[c][13]), __uint_as_float(sr[c][14]));
-        mx[c] = fmax3(fmax3(a0, a1, a2), fmax3(a3, a4, __uint_as_float(sr[c][15])), -INFINITY);
+        for (int i = 0; i < 10; ++i)
+          a[i] = fmax3(__uint_as_float(sr[c][3 * i]), __uint_as_float(sr[c][3 * i + 1]), __uint_as_float(sr[c][3 * i + 2]));
+        mx[c] = fmax3(fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]), fmax3(a[6], a[7], a[8])),
+                      fmax3(a[9], __uint_as_float(sr[c][30]), __uint_as_float(sr[c][31])), -INFINITY);
       }
       const float scale = row_scale * ts.k;
-      const float mt = fmaxf(fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * scale, kNoMax);
+      const float mt = fmaxf(fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale, kNoMax);
       if (j == 0) {
         m = mt;
         vf = ts.v;
@@ -467,24 +524,25 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         if (!ok) break;
       }
       const uint64_t scale2 = pack_f32x2(scale, scale), negm2 = pack_f32x2(-m, -m);
-      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+      uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
-      for (int c = 0; c < 8; c += 2) {
+      for (int c = 0; c < 4; ++c) {
         uint32_t packed[16];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float x0, x1;
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sr[c + h][i]), __uint_as_float(sr[c + h][i + 1])), scale2, negm2),
-                         x0, x1);
-            const float p0 = exp2f(x0), p1 = exp2f(x1);
-            sums[(i >> 1) & 3] += p0 + p1;
-            packed[h * 8 + (i >> 1)] = pack_f16(p0, p1);
-          }
-        tmem_st16(taddr + (c >> 1) * 16, packed);
+        for (int i = 0; i < 32; i += 2) {
+          float x0, x1;
+          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1])), scale2, negm2), x0, x1);
+          const float p0 = exp2f(x0), p1 = exp2f(x1);
+          sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(p0, p1));
+          packed[i >> 1] = pack_f16(p0, p1);
+        }
+        tmem_st16(taddr + c * 16, packed);
       }
-      l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      {
+        float a, c;
+        unpack_f32x2(add_f32x2(sums[0], sums[1]), a, c);
+        l += a + c;
+      }
       mbar_arrive(&xu_done[u]);
       tmem_st_wait();
       tc_fence_before_sync();
@@ -494,8 +552,9 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     if (ok) {
       tc_fence_after_sync();
       const float inv = l == 0.f ? 0.f : vf / l;
-      __nv_bfloat16* dst = p.out + (static_cast<size_t>(q_begin + (live ? row : 0)) * p.hq + hk * G + hd) * kD;
-#pragma unroll 1
+      // Rows leave through the unit's Q tile (all its MMAs are over), so that the writes are whole lines.
+      const uint32_t at = row_start(smem_u32(q_s) + u * kTileBytes, r);
+#pragma unroll 2
       for (int ch = 0; ch < kD / 16; ++ch) {
         uint32_t o[16];
         if (n_tiles > 0) {
@@ -505,14 +564,22 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = 0u;
         }
-        if (live) {
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {                      // words of channels 0 4 1 5 2 6 3 7
-            auto at = [&](int i) { return l == 0.f ? 0.f : __uint_as_float(o[8 * w + i]) * inv; };
-            *reinterpret_cast<uint4*>(dst + ch * 16 + 8 * w) = make_uint4(
-                pack_bf16(at(0), at(2)), pack_bf16(at(4), at(6)), pack_bf16(at(1), at(3)), pack_bf16(at(5), at(7)));
-          }
+        for (int w = 0; w < 2; ++w) {                        // words of channels 0 4 1 5 2 6 3 7
+          auto x = [&](int i) { return l == 0.f ? 0.f : __uint_as_float(o[8 * w + i]) * inv; };
+          st_shared_v4(chunk_at(at, 2 * ch + w), pack_bf16(x(0), x(2)), pack_bf16(x(4), x(6)), pack_bf16(x(1), x(3)),
+                       pack_bf16(x(5), x(7)));
         }
+      }
+      __syncwarp();
+      const int c = lane & 15;
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) {
+        const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4), rr = qr_ / G, hh = qr_ - rr * G;
+        const int qrow = row0 + u * rpu + rr;
+        if (rr < rpu && qrow < q_len)
+          *(reinterpret_cast<uint4*>(p.out + (static_cast<size_t>(q_begin + qrow) * p.hq + hk * G + hh) * kD) + c) =
+              *reinterpret_cast<const uint4*>(q_s + u * kTileBytes + (chunk_at(row_start(0u, qr_), c)));
       }
     } else if (lane == 0) {
       report_status(p.status, kId, kWaitAccumTimeout);
