@@ -190,8 +190,11 @@ def _attend(q_lens, kv_lens, hq, hkv, bs=16, n_decode=0, seed=0, poison=False, q
     # Decode rows: the output and P s_g are each rounded to bf16 once; scores are fp32 sums of at most 2 * 64 products
     # no larger than 17 times those of q and k (codes biased by 136), so 2^-24 * 17 * 8 bounds their relative error.
     tol = HALF_BF16 * (np.abs(ref) + swing) + 2 * (2.0 ** -24 * 17 * 8 * qk + 2.0 ** -20) * mag
-    # Chunks: K, V and P are rounded to bf16 (K: the score moves by 2^-8 of sum |q| |k|, a probability by twice that).
-    chunk = HALF_BF16 * (np.abs(ref) + 2 * mag) * (1 + HALF_BF16) + (np.exp(2 * HALF_BF16 * qk) - 1) * mag + 2.0 ** -18 * mag
+    # Chunks: K, V and P are rounded to fp16 (a value c + s (n - 8) after its s and c: three roundings of 2^-11 of magnitudes
+    # no larger than |x| + 2 |s (n - 8)|; a score then moves by 2^-11 of sum |q| |k|, a probability by twice that) and the
+    # output to bf16. `mag` stands for sum p |v| and is at least a third of sum p (|v| + 2 |s (n - 8)|) for these caches' rows
+    # by a margin of two: 2^-9 is allowed.
+    chunk = HALF_BF16 * np.abs(ref) + 2.0 ** -9 * (mag + swing) + (np.exp(2.0 ** -9 * qk) - 1) * mag + 2.0 ** -18 * mag
     tol[n_decode:] = chunk[n_decode:]
     worst = (np.abs(got - ref) - tol).max()
     assert worst <= 0, worst
@@ -288,6 +291,15 @@ def test_chunks_of_every_group_size(hq, hkv, bs):
     _attend([70, 1, 33], [70 + 131, 1, 33], hq, hkv, bs=bs, seed=hq)
 
 
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (5, 1), (16, 2)])
+def test_short_chunks_behind_long_prefixes_split_the_range(hq, hkv):
+    _attend([1, 9, 40], [1400, 1209, 40], hq, hkv, seed=hq, extra_pages=300)
+
+
+def test_split_chunks_with_nan_around_and_bad_pages():
+    _attend([30, 2], [700, 130], 4, 2, poison=True, extra_pages=300)
+
+
 def test_chunk_growing_maxima():
     _attend([150], [500], 4, 1, q_scale=8.0, seed=9)
 
@@ -307,10 +319,9 @@ def test_chunk_values_of_mixed_magnitude():
     attn = AttnBatch(torch.tensor([0, n], **i32), torch.tensor([n], **i32), table.to(DEV), 1, 0, n, n, n)
     out = _ops().paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), attn, D ** -0.5, hq, hkv, D)
     _cuda().check_status()
-    ref, mag, _, qk = kv4_ref.attention(q, k, v, [n], [n], table, D ** -0.5, hq)
+    ref, mag, swing, qk = kv4_ref.attention(q, k, v, [n], [n], table, D ** -0.5, hq)
     got = out.double().cpu().numpy().reshape(n, hq, D)
-    # as in _attend: bf16 roundings of K, V, P and the output bound any of the kernels
-    tol = HALF_BF16 * (np.abs(ref) + 2 * mag) * (1 + HALF_BF16) + (np.exp(2 * HALF_BF16 * qk[..., None]) - 1) * mag + 2.0 ** -18 * mag
+    tol = HALF_BF16 * np.abs(ref) + 2.0 ** -9 * (mag + swing) + (np.exp(2.0 ** -9 * qk[..., None]) - 1) * mag + 2.0 ** -18 * mag
     assert ((np.abs(got - ref) - tol) <= 0).all()
 
 

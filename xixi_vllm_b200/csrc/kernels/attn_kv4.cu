@@ -1,4 +1,4 @@
-// Paged causal GQA attention over a KV cache held in 4 bits (format: common/kv4.cuh), head_dim 128.
+// Paged GQA attention of single query rows over a KV cache held in 4 bits (format: common/kv4.cuh), head_dim 128.
 //
 //   kv4_decode_kernel  - one query row per sequence; a cluster of CTAs, one per KV split, owns (sequence, KV head). Each
 //                        warp streams its own 16-token units through a ring of shared-memory slots (five 16-byte
@@ -14,8 +14,7 @@
 //                        memory: one launch, no workspace.
 //   kv4_share_kernel   - the same arithmetic for large or ragged batches: all units dealt to the warps in equal runs,
 //   kv4_join_kernel      partial results of pairs that span runs joined by a second kernel.
-//   kv4_prefill_kernel - packed query chunks: 64 query rows of one head per CTA, KV tiles of 64 tokens dequantised to
-//                        bf16 in shared memory.
+// Prompt chunks: attn_prefill_kv4_sm100.cu.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -23,7 +22,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 
 #include "../common/kv4.cuh"
 #include "../common/launch.cuh"
@@ -35,7 +33,7 @@ namespace {
 using namespace xv;
 
 constexpr int kD = kv4::kD;
-constexpr int kIdDecode = 10, kIdPrefill = 11;
+constexpr int kIdDecode = 10;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Params {
@@ -43,30 +41,29 @@ struct Params {
   const uint8_t* k_cache;
   const uint8_t* v_cache;
   const int* block_tables;
-  const int* cu_q;
   const int* kv_lens;
   __nv_bfloat16* out;
   int* status;
-  int hq, hkv, block_size, max_blocks, num_blocks, splits, seq_begin, total_rows;
+  int hq, hkv, block_size, max_blocks, num_blocks, splits;
   float scale_log2;
 };
 
 // Page of a block-table entry; an entry outside the cache is recorded and replaced by page 0.
-__device__ __forceinline__ int page_of(const Params& p, int b, int entry, int id) {
+__device__ __forceinline__ int page_of(const Params& p, int b, int entry) {
   int blk = __ldg(p.block_tables + static_cast<size_t>(b) * p.max_blocks + entry);
   if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) {
-    report_status(p.status, id, kBadIndex);
+    report_status(p.status, kIdDecode, kBadIndex);
     blk = 0;
   }
   return blk;
 }
 
 // Cached tokens of a sequence, never more than its block table can name.
-__device__ __forceinline__ int kv_len_of(const Params& p, int b, int id) {
+__device__ __forceinline__ int kv_len_of(const Params& p, int b) {
   const int n = p.kv_lens[b];
   const long long most = static_cast<long long>(p.max_blocks) * p.block_size;
   if (n > most) {
-    if (threadIdx.x == 0) report_status(p.status, id, kBadIndex);
+    if (threadIdx.x == 0) report_status(p.status, kIdDecode, kBadIndex);
     return static_cast<int>(most);
   }
   return n < 0 ? 0 : n;
@@ -367,7 +364,7 @@ struct Ring {
     page_bytes = static_cast<uint32_t>(hkv) * upp * kv4::kUnitBytes;
   }
   __device__ __forceinline__ int lookup(const Params& p, int i) const {
-    return page_of(p, b, min(page0 + i, last_page), kIdDecode);
+    return page_of(p, b, min(page0 + i, last_page));
   }
   // n units from `first` on of the `units` that sequence b has.
   __device__ __forceinline__ void start(const Params& p, int b_, int h, int first, int n, int units) {
@@ -436,7 +433,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
   const int G = p.hq / p.hkv;
   uint8_t* ring_mem = smem + warp * kStages * kSlot;
   grid_dep_wait();
-  const int kv_len = kv_len_of(p, b, kIdDecode);
+  const int kv_len = kv_len_of(p, b);
   const int units = (kv_len + 15) / 16;
   const int per = (units + p.splits * W - 1) / (p.splits * W);
   const int first = min((split * W + warp) * per, units);
@@ -558,7 +555,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
   const int chunk = (num_seqs + T - 1) / T;
   const int c0 = min(static_cast<int>(threadIdx.x) * chunk, num_seqs), c1 = min(c0 + chunk, num_seqs);
   int mine_units = 0;
-  for (int b = c0; b < c1; ++b) mine_units += (kv_len_of(p, b, kIdDecode) + 15) / 16;
+  for (int b = c0; b < c1; ++b) mine_units += (kv_len_of(p, b) + 15) / 16;
   int incl = mine_units;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -583,7 +580,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
     int at = before + incl - mine_units;
     for (int b = c0; b < c1; ++b) {
       ws.begin[b] = at;
-      at += (kv_len_of(p, b, kIdDecode) + 15) / 16;
+      at += (kv_len_of(p, b) + 15) / 16;
     }
     if (threadIdx.x == 0) {
       ws.begin[num_seqs] = total;
@@ -608,7 +605,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
     int at = sums[lo];
     b = lo * chunk;
     for (;; ++b) {
-      kv_len = kv_len_of(p, b, kIdDecode);
+      kv_len = kv_len_of(p, b);
       units = (kv_len + 15) / 16;
       if (u < at + units) break;
       at += units;
@@ -634,7 +631,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
     if (ring.left == 0 && f_todo > 0) {
       if (++f_h == p.hkv) {
         f_h = 0;
-        do f_units = (kv_len_of(p, ++f_b, kIdDecode) + 15) / 16;
+        do f_units = (kv_len_of(p, ++f_b) + 15) / 16;
         while (f_units == 0);
       }
       fetch_pair(0);
@@ -689,7 +686,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
     if (++h == p.hkv) {
       h = 0;
       do {
-        kv_len = kv_len_of(p, ++b, kIdDecode);
+        kv_len = kv_len_of(p, ++b);
         units = (kv_len + 15) / 16;
       } while (units == 0);
     }
@@ -750,216 +747,6 @@ __global__ void kv4_join_kernel(const Params p, const Shares ws, int num_seqs, i
   store_out(dst, acc, L);
 }
 
-// ------------------------------------------------------------------------------------------
-// Prompt chunks
-// ------------------------------------------------------------------------------------------
-constexpr int kPfM = 64, kPfN = 64, kPfWarps = 4, kRowBytes = kD * 2;
-constexpr int kPfTile = kPfN * kRowBytes;                       // 16 KiB
-constexpr int kPfSmem = kPfM * kRowBytes + 2 * kPfTile;         // Q, K, V: 48 KiB
-
-// Byte offset of 16-byte chunk c of row r inside a swizzled tile with 256-byte rows.
-__device__ __forceinline__ uint32_t swz(int r, int c) { return static_cast<uint32_t>(r * kRowBytes + ((c ^ (r & 7)) << 4)); }
-
-// Eight channels of one word as bf16: c + s * (n - 8), rounded once.
-__device__ __forceinline__ uint4 dequant8(uint32_t w, uint32_t par) {
-  const uint32_t s2 = __byte_perm(par, par, 0x1010), c2 = __byte_perm(par, par, 0x3232);
-  const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&s2), c = *reinterpret_cast<const __nv_bfloat162*>(&c2);
-  uint32_t v[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {                                  // channels j and j + 4
-    const uint32_t n = kv4::centred(kv4::biased(w, 4 * j));
-    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&n), s, c);
-    v[j] = *reinterpret_cast<const uint32_t*>(&r);
-  }
-  return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
-                    __byte_perm(v[2], v[3], 0x7632));
-}
-
-__global__ void __launch_bounds__(kPfWarps * 32) kv4_prefill_kernel(const Params p) {
-  grid_dep_launch();
-  grid_dep_wait();
-  extern __shared__ __align__(128) uint8_t smem[];
-  const int head = blockIdx.y, b = p.seq_begin + blockIdx.z;
-  const int q_begin = p.cu_q[b];
-  int q_len = p.cu_q[b + 1] - q_begin;
-  const int row0 = blockIdx.x * kPfM;
-  if (q_begin < 0 || q_len < 0 || q_len > p.total_rows - q_begin) {
-    if (threadIdx.x == 0) report_status(p.status, kIdPrefill, kBadIndex);
-    return;
-  }
-  if (row0 >= q_len) return;
-  const int kv_len = kv_len_of(p, b, kIdPrefill);
-  const int pos0 = kv_len - q_len;                    // absolute position of query row 0 (negative rows see nothing)
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const int hk = head / (p.hq / p.hkv);
-  const int rows_here = min(kPfM, q_len - row0);
-  const int n_kv = max(0, min(kv_len, pos0 + row0 + rows_here));
-  const int n_tiles = (n_kv + kPfN - 1) / kPfN;
-  const int units_per_page = p.block_size / kv4::kUnit;
-
-  uint8_t* sq = smem;
-  uint8_t* sk = smem + kPfM * kRowBytes;
-  uint8_t* sv = sk + kPfTile;
-  {
-    const size_t ld = static_cast<size_t>(p.hq) * kD;
-    const __nv_bfloat16* qb = p.q + (static_cast<size_t>(q_begin) + row0) * ld + static_cast<size_t>(head) * kD;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = threadIdx.x + 128 * j, r = c >> 4, ch = c & 15;
-      const bool ok = r < rows_here;
-      cp_async16_zfill(sq + swz(r, ch), qb + (ok ? static_cast<size_t>(r) * ld + ch * 8 : 0), ok);
-    }
-    cp_async_commit();
-  }
-  // Thread i of a tile: codes of row i / 2, 32 of its 64 bytes, of K and of V.
-  const int lr = threadIdx.x >> 1, lh = threadIdx.x & 1;
-  uint4 kc[2], vc[2];
-  uint2 kp, vp;
-  auto fetch = [&](int j) {
-    const int tok = j * kPfN + lr;
-    kp = vp = make_uint2(0u, 0u);
-    kc[0] = kc[1] = vc[0] = vc[1] = make_uint4(0u, 0u, 0u, 0u);
-    if (tok < n_kv) {
-      const int blk = page_of(p, b, tok / p.block_size, kIdPrefill);
-      const int r = tok % p.block_size;
-      const size_t unit = (static_cast<size_t>(blk) * p.hkv + hk) * units_per_page * kv4::kUnitBytes +
-                          static_cast<size_t>(r / kv4::kUnit) * kv4::kUnitBytes;
-      const size_t co = unit + (r % kv4::kUnit) * kv4::kCodeRow + lh * 32;
-      const size_t po = unit + kv4::kParBase + (r % kv4::kUnit) * kv4::kParRow;
-      kc[0] = __ldg(reinterpret_cast<const uint4*>(p.k_cache + co));
-      kc[1] = __ldg(reinterpret_cast<const uint4*>(p.k_cache + co + 16));
-      vc[0] = __ldg(reinterpret_cast<const uint4*>(p.v_cache + co));
-      vc[1] = __ldg(reinterpret_cast<const uint4*>(p.v_cache + co + 16));
-      kp = __ldg(reinterpret_cast<const uint2*>(p.k_cache + po));
-      vp = __ldg(reinterpret_cast<const uint2*>(p.v_cache + po));
-    }
-  };
-  auto put = [&](uint8_t* tile, const uint4 (&c)[2], uint2 par) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        *reinterpret_cast<uint4*>(tile + swz(lr, lh * 8 + i * 4 + k)) = dequant8(w[k], (k & 1) ? par.y : par.x);
-    }
-  };
-  fetch(0);
-
-  float o[16][4];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f;
-  uint32_t qf[8][4];
-  const int my_pos0 = pos0 + row0 + warp * 16 + g;     // position of row g; row g + 8 is + 8
-  cp_async_wait<0>();
-  __syncthreads();
-  {
-    const int mi = lane >> 3;
-    const int r = warp * 16 + ((mi & 1) << 3) + (lane & 7);
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) ldmatrix_x4(qf[kk], smem_u32(sq) + swz(r, 2 * kk + (mi >> 1)));
-  }
-
-  for (int j = 0; j < n_tiles; ++j) {
-    put(sk, kc, kp);
-    put(sv, vc, vp);
-    if (j + 1 < n_tiles) fetch(j + 1);
-    __syncthreads();
-    const uint32_t kb = smem_u32(sk), vb = smem_u32(sv);
-    const int tile_k0 = j * kPfN;
-    if (tile_k0 <= my_pos0 - g + 15) {                 // warp-uniform: some row of the warp sees this tile
-      float s[8][4];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-      {
-        const int mi = lane >> 3;
-        const int r = ((mi >> 1) << 3) + (lane & 7);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-          for (int jp = 0; jp < 4; ++jp) {
-            uint32_t kf[4];
-            ldmatrix_x4(kf, kb + swz(jp * 16 + r, 2 * kk + (mi & 1)));
-            mma_bf16_16816(s[2 * jp], qf[kk], kf[0], kf[1]);
-            mma_bf16_16816(s[2 * jp + 1], qf[kk], kf[2], kf[3]);
-          }
-      }
-      float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F;
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = tile_k0 + nt * 8 + 2 * t + e;
-          const bool in = key < n_kv;
-          s[nt][e] = (in && key <= my_pos0) ? s[nt][e] * p.scale_log2 : -CUDART_INF_F;
-          s[nt][2 + e] = (in && key <= my_pos0 + 8) ? s[nt][2 + e] * p.scale_log2 : -CUDART_INF_F;
-          mx0 = fmaxf(mx0, s[nt][e]);
-          mx1 = fmaxf(mx1, s[nt][2 + e]);
-        }
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-      const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
-      const float base0 = mn0 == -CUDART_INF_F ? 0.f : mn0, base1 = mn1 == -CUDART_INF_F ? 0.f : mn1;
-      const float cr0 = exp2f(m0 - base0), cr1 = exp2f(m1 - base1);
-      m0 = mn0;
-      m1 = mn1;
-      float ps0 = 0.f, ps1 = 0.f;
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        s[nt][0] = exp2f(s[nt][0] - base0);
-        s[nt][1] = exp2f(s[nt][1] - base0);
-        s[nt][2] = exp2f(s[nt][2] - base1);
-        s[nt][3] = exp2f(s[nt][3] - base1);
-        ps0 += s[nt][0] + s[nt][1];
-        ps1 += s[nt][2] + s[nt][3];
-      }
-      l0 = l0 * cr0 + ps0;
-      l1 = l1 * cr1 + ps1;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        o[i][0] *= cr0; o[i][1] *= cr0; o[i][2] *= cr1; o[i][3] *= cr1;
-      }
-      {
-        const int mi = lane >> 3;
-        const int r = ((mi & 1) << 3) + (lane & 7);
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const uint32_t pf[4] = {pack_bf16(s[2 * ks][0], s[2 * ks][1]), pack_bf16(s[2 * ks][2], s[2 * ks][3]),
-                                  pack_bf16(s[2 * ks + 1][0], s[2 * ks + 1][1]), pack_bf16(s[2 * ks + 1][2], s[2 * ks + 1][3])};
-#pragma unroll
-          for (int jd = 0; jd < 8; ++jd) {
-            uint32_t vf[4];
-            ldmatrix_x4_trans(vf, vb + swz(ks * 16 + r, 2 * jd + (mi >> 1)));
-            mma_bf16_16816(o[2 * jd], pf, vf[0], vf[1]);
-            mma_bf16_16816(o[2 * jd + 1], pf, vf[2], vf[3]);
-          }
-        }
-      }
-    }
-    __syncthreads();    // everyone is done with the tile before the next one overwrites it
-  }
-
-  l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-  l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-  l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-  l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-  const float inv0 = l0 == 0.f ? 0.f : 1.f / l0, inv1 = l1 == 0.f ? 0.f : 1.f / l1;
-  const int r0 = row0 + warp * 16 + g, r1 = r0 + 8;
-  const size_t ld = static_cast<size_t>(p.hq) * kD;
-  __nv_bfloat16* ob = p.out + static_cast<size_t>(q_begin) * ld + static_cast<size_t>(head) * kD;
-#pragma unroll
-  for (int nt = 0; nt < 16; ++nt) {
-    const int d0 = nt * 8 + 2 * t;
-    if (r0 < q_len)
-      *reinterpret_cast<uint32_t*>(ob + static_cast<size_t>(r0) * ld + d0) = pack_bf16(o[nt][0] * inv0, o[nt][1] * inv0);
-    if (r1 < q_len)
-      *reinterpret_cast<uint32_t*>(ob + static_cast<size_t>(r1) * ld + d0) = pack_bf16(o[nt][2] * inv1, o[nt][3] * inv1);
-  }
-}
-
 int fill(Params& p, const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* kv_lens,
          void* out, int hq, int hkv, int d, int block_size, int max_blocks, int num_blocks, float scale, int* status) {
   if (d != kD) return XV_ERR_UNSUPPORTED;
@@ -1008,7 +795,7 @@ extern "C" {
 // graph keeps its shape: 1, 2, 4 or 8 CTAs (one cluster) per (sequence, KV head), or 0 for even shares.
 int xv_kv4_decode_splits(int num_seqs, int hkv, int num_sms, int max_tokens_per_seq) {
   const long long pairs = static_cast<long long>(num_seqs) * hkv;
-  if (pairs * max_tokens_per_seq > 2048ll * num_sms) return 0;
+  if (pairs * max_tokens_per_seq > 4096ll * num_sms) return 0;
   int s = 1;
   while (s < 8 && pairs * s < 2 * num_sms && max_tokens_per_seq / (2 * s) >= 128) s *= 2;
   return s;
@@ -1056,27 +843,6 @@ int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const
   // Few pairs have many partials each: more warps per row.
   const int threads = num_seqs * hkv <= 64 ? 512 : 64;
   launch_pdl(kv4_join_kernel, dim3(num_seqs * hkv, hq / hkv), dim3(threads), 0, stream, p, ws, num_seqs, 8 * nt);
-  return launch_ok();
-}
-
-int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_q,
-                   const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq,
-                   int hkv, int d, int block_size, int max_blocks, int num_blocks, float scale, int* status,
-                   cudaStream_t stream) {
-  if (num_seqs <= 0 || max_q_len <= 0) return 0;
-  Params p;
-  if (int rc = fill(p, q, k_cache, v_cache, block_tables, kv_lens, out, hq, hkv, d, block_size, max_blocks, num_blocks,
-                    scale, status))
-    return rc;
-  const char* e = std::getenv("XV_KV4_TC");
-  if (hq / hkv <= 16 && max_q_len * (hq / hkv) > (e ? std::atoi(e) : 64))
-    return xv_kv4_prefill_tc(q, k_cache, v_cache, block_tables, cu_q, kv_lens, out, seq_begin, num_seqs, max_q_len, total_rows,
-                             hq, hkv, d, block_size, max_blocks, num_blocks, scale, status, stream);
-  if (hq > 65535 || num_seqs > 65535) return XV_ERR_SHAPE;
-  p.cu_q = cu_q;
-  p.seq_begin = seq_begin;
-  p.total_rows = total_rows;
-  launch_pdl(kv4_prefill_kernel, dim3((max_q_len + kPfM - 1) / kPfM, hq, num_seqs), dim3(kPfWarps * 32), kPfSmem, stream, p);
   return launch_ok();
 }
 

@@ -27,6 +27,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 
@@ -61,7 +62,9 @@ struct Params {
   const int* kv_lens;
   __nv_bfloat16* out;
   int* status;
-  int seq_begin, hq, hkv, block_size, max_blocks, num_blocks, total_rows;
+  float* ws_o;                                    // [CTA][split][256 lanes][128] unnormalised outputs, when splits > 1
+  float* ws_ml;                                   // [CTA][split][256 lanes][2]: maximum (log2 units), sum
+  int seq_begin, hq, hkv, block_size, max_blocks, num_blocks, total_rows, splits;
   float scale_log2;
 };
 
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   grid_dep_launch();
   grid_dep_wait();
-  const int b = p.seq_begin + blockIdx.z, hk = blockIdx.y;
+  const int b = p.seq_begin + blockIdx.z / p.splits, split = blockIdx.z % p.splits, hk = blockIdx.y;
   const int q_begin = p.cu_q[b];
   const int q_len = p.cu_q[b + 1] - q_begin;
   if (q_begin < 0 || q_len < 0 || q_len > p.total_rows - q_begin) {
@@ -157,7 +160,9 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   const int pos0 = kv_len - q_len;                           // position of query row 0; rows before position 0 see nothing
   const int rows_here = min(2 * rpu, q_len - row0);
   const int n_kv = max(0, min(kv_len, pos0 + row0 + rows_here));
-  const int n_tiles = (n_kv + kBN - 1) / kBN;
+  // This CTA's run of tiles.
+  const int all_tiles = (n_kv + kBN - 1) / kBN, per_split = (all_tiles + p.splits - 1) / p.splits;
+  const int tile0 = min(split * per_split, all_tiles), n_tiles = min(per_split, all_tiles - tile0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wg = warp >> 2;
 
@@ -220,7 +225,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     // replaced by it; whatever row that reads does not count. A page's number is read two tiles ahead of its bytes' use.
     const int last_page = (max(n_kv, 1) - 1) / p.block_size;
     const int page_step = kBN / p.block_size, place_step = kBN % p.block_size;
-    int page = row / p.block_size, place = row - page * p.block_size, place_next = 0, entry = 0;
+    int page = (tile0 * kBN + row) / p.block_size, place = tile0 * kBN + row - page * p.block_size, place_next = 0, entry = 0;
     auto look = [&]() { entry = __ldg(table + min(page, last_page)); place_next = place; };
     auto step = [&]() {
       page += page_step;
@@ -250,7 +255,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     // What counts of tile j's parameters (a V that is not finite makes K not finite instead), and the tile's largest
     // possible magnitudes, left in `red` for everyone.
     auto admit = [&](int j, bool ok) {
-      if (j * kBN + row >= n_kv) kp = vp = make_uint2(0u, 0u);
+      if ((tile0 + j) * kBN + row >= n_kv) kp = vp = make_uint2(0u, 0u);
       auto finite = [](uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; };
       if (!finite(vp.x) || !finite(vp.y)) {
         vp = make_uint2(0u, 0u);
@@ -462,7 +467,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       tc_fence_after_sync();
       uint32_t sr[4][32];                                    // the score row: 128 fp32
       const TileScale ts = scales[j & 7];
-      const int k0 = j * kBN;
+      const int k0 = (tile0 + j) * kBN;
       const bool diagonal = k0 + kBN - 1 > pos;
       float mx[4];
       tmem_ld32(taddr, sr[0]);
@@ -549,7 +554,25 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       mbar_arrive(&p_ready[u]);
     }
     if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[u], (n_tiles - 1) & 1) && *abort_flag == 0);
-    if (ok) {
+    if (ok && p.splits > 1) {
+      tc_fence_after_sync();
+      const size_t slot = (((static_cast<size_t>(blockIdx.z / p.splits) * gridDim.y + hk) * gridDim.x + blockIdx.x) * p.splits + split) *
+                              (2 * kBM) + u * kBM + r;
+      *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(m, l);
+      for (int ch = 0; ch < kD / 16 && n_tiles > 0; ++ch) {  // a split without tiles leaves no output, only m = kNoMax, l = 0
+        uint32_t o[16];
+        tmem_ld16(taddr + kTmemO + ch * 16, o);
+        tmem_ld_wait();
+        tmem_ld_fence_regs(o);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {                        // words of channels 0 4 1 5 2 6 3 7
+          auto x = [&](int i) { return __uint_as_float(o[8 * w + i]) * vf; };
+          float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * kD + ch * 16 + 8 * w);
+          dst[0] = make_float4(x(0), x(2), x(4), x(6));
+          dst[1] = make_float4(x(1), x(3), x(5), x(7));
+        }
+      }
+    } else if (ok) {
       tc_fence_after_sync();
       const float inv = l == 0.f ? 0.f : vf / l;
       // Rows leave through the unit's Q tile (all its MMAs are over), so that the writes are whole lines.
@@ -595,19 +618,74 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   }
 }
 
+// Joins the splits: a warp a lane (query row, head) of the launch above, four channels a thread.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(kJoinWarps * 32) kv4_prefill_join_kernel(const Params p, int blocks) {
+  grid_dep_launch();
+  grid_dep_wait();
+  const int b = p.seq_begin + blockIdx.z, hk = blockIdx.y;
+  const int q_begin = p.cu_q[b], q_len = p.cu_q[b + 1] - q_begin;
+  if (q_begin < 0 || q_len < 0 || q_len > p.total_rows - q_begin) return;
+  const int G = p.hq / p.hkv, rpu = kBM / G;
+  const int i = blockIdx.x * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int block = i / (2 * kBM), u = (i / kBM) & 1, r = i % kBM;
+  const int row = (blocks - 1 - block) * 2 * rpu + u * rpu + r / G;
+  if (r >= rpu * G || row >= q_len) return;
+  const size_t slot = ((static_cast<size_t>(blockIdx.z) * gridDim.y + hk) * blocks + block) * p.splits * (2 * kBM) + i % (2 * kBM);
+  float M = kNoMax;
+  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.ws_ml[(slot + s * (2 * kBM)) * 2]);
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const size_t at = slot + s * (2 * kBM);
+    const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + at * 2);
+    if (ml.x == kNoMax && ml.y == 0.f) continue;             // saw nothing, and may have written nothing
+    const float f = exp2f(ml.x - M);
+    const float4 v = *reinterpret_cast<const float4*>(p.ws_o + at * kD + lane * 4);
+    L += ml.y * f;
+    acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(q_begin + row) * p.hq + hk * G + r % G) * kD + lane * 4) =
+      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+}
+
+int blocks_of(int max_q_len, int hq, int hkv) {
+  const int rows = 2 * (kBM / (hq / hkv));
+  return (max_q_len + rows - 1) / rows;
+}
+
 }  // namespace
 
 extern "C" {
 
-int xv_kv4_prefill_tc(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_q,
-                      const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq,
-                      int hkv, int d, int block_size, int max_blocks, int num_blocks, float scale, int* status,
-                      cudaStream_t stream) {
+// Splits of the KV range, from launch-shape constants: only where the CTAs would leave most SMs idle, at least four tiles
+// each.
+int xv_kv4_prefill_splits(int num_seqs, int max_q_len, int hq, int hkv, int max_tokens_per_seq, int num_sms) {
+  if (num_seqs <= 0 || max_q_len <= 0 || hkv <= 0 || hq < hkv || hq / hkv > 16) return 1;
+  const long long ctas = static_cast<long long>(num_seqs) * hkv * blocks_of(max_q_len, hq, hkv);
+  const long long by_sms = num_sms / ctas, by_len = max_tokens_per_seq / (4 * kBN);
+  return static_cast<int>(std::max(1ll, std::min({by_sms, by_len, 16ll})));
+}
+
+long long xv_kv4_prefill_workspace_bytes(int num_seqs, int max_q_len, int hq, int hkv, int splits) {
+  if (splits <= 1 || hkv <= 0 || hq < hkv || hq / hkv > 16) return 0;
+  return static_cast<long long>(num_seqs) * hkv * blocks_of(max_q_len, hq, hkv) * splits * (2 * kBM) * (kD + 2) * 4;
+}
+
+int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_q,
+                   const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq, int hkv,
+                   int d, int block_size, int max_blocks, int num_blocks, float scale, int splits, void* workspace,
+                   long long workspace_bytes, int* status, cudaStream_t stream) {
   if (num_seqs <= 0 || max_q_len <= 0) return 0;
   if (d != kD) return XV_ERR_UNSUPPORTED;
   if (hkv <= 0 || hq <= 0 || hq % hkv || hq / hkv > 16 || block_size <= 0 || block_size % kv4::kUnit || max_blocks <= 0 ||
-      num_blocks <= 0 || hkv > 65535 || num_seqs > 65535)
+      num_blocks <= 0 || hkv > 65535 || splits < 1 || static_cast<long long>(num_seqs) * splits > 65535)
     return XV_ERR_SHAPE;
+  if (splits > 1 && (!workspace || workspace_bytes < xv_kv4_prefill_workspace_bytes(num_seqs, max_q_len, hq, hkv, splits)))
+    return XV_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return XV_ERR_ALIGN;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
        reinterpret_cast<uintptr_t>(out)) & 15)
     return XV_ERR_ALIGN;
@@ -631,9 +709,18 @@ int xv_kv4_prefill_tc(const void* q, const void* k_cache, const void* v_cache, c
   p.seq_begin = seq_begin; p.hq = hq; p.hkv = hkv; p.block_size = block_size; p.max_blocks = max_blocks;
   p.num_blocks = num_blocks; p.total_rows = total_rows;
   p.scale_log2 = scale * kLog2e;
-  const int rows = 2 * (kBM / (hq / hkv));
-  launch_pdl(kv4_prefill_tc_kernel, dim3((max_q_len + rows - 1) / rows, hkv, num_seqs), dim3(512), kSmem, stream, p);
-  return cudaGetLastError() == cudaSuccess ? 0 : XV_ERR_LAUNCH;
+  const int blocks = blocks_of(max_q_len, hq, hkv);
+  p.splits = splits;
+  p.ws_o = static_cast<float*>(workspace);
+  p.ws_ml = splits > 1 ? p.ws_o + static_cast<size_t>(num_seqs) * hkv * blocks * splits * (2 * kBM) * kD : nullptr;
+  launch_pdl(kv4_prefill_tc_kernel, dim3(blocks, hkv, num_seqs * splits), dim3(512), kSmem, stream, p);
+  if (cudaGetLastError() != cudaSuccess) return XV_ERR_LAUNCH;
+  if (splits > 1) {
+    launch_pdl(kv4_prefill_join_kernel, dim3(blocks * (2 * kBM / kJoinWarps), hkv, num_seqs), dim3(kJoinWarps * 32), 0, stream, p,
+               blocks);
+    if (cudaGetLastError() != cudaSuccess) return XV_ERR_LAUNCH;
+  }
+  return 0;
 }
 
 }  // extern "C"

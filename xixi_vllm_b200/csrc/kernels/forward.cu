@@ -196,6 +196,8 @@ int xv_qwen3_forward(const XvModelDesc* m, const XvBatchDesc* b, const XvArena* 
     return XV_ERR_WORKSPACE;
   }
 
+  const int splits_pre = m->kv4 && n_pre > 0 ? xv_kv4_prefill_splits(n_pre, b->max_q_len, m->hq, m->hkv, max_kv, a->num_sms) : 1;
+
   // Short chunks do not fill a 128-row tile; they stay on the 64-row warp-MMA kernel.
   const bool prefill_tc = m->prefill_tc && m->num_kv_blocks > 0 && b->max_q_len > 64 &&
                           xv_attn_prefill_tc_supported(D, m->block_size);
@@ -229,7 +231,7 @@ int xv_qwen3_forward(const XvModelDesc* m, const XvBatchDesc* b, const XvArena* 
       if (n_pre > 0)
         XV_TRY(38, xv_kv4_prefill(a->q, w.k_cache, w.v_cache, b->block_tables, b->cu_q, b->kv_lens, a->attn, n_dec, n_pre,
                                   b->max_q_len, T, m->hq, m->hkv, D, m->block_size, b->max_blocks, m->num_kv_blocks,
-                                  m->attn_scale, a->status, stream));
+                                  m->attn_scale, splits_pre, a->attn_ws, a->attn_ws_bytes, a->status, stream));
     } else {
       if (n_dec > 0)
         XV_TRY(33, xv_attn_decode(a->q, w.k_cache, w.v_cache, b->block_tables, b->kv_lens, a->attn, n_dec, m->hq, m->hkv,

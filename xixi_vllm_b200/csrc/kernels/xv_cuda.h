@@ -169,15 +169,14 @@ int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const
                   void* out, int num_seqs, int hq, int hkv, int d, int block_size, int max_blocks, int num_blocks,
                   float scale, int splits, int num_sms, void* workspace, long long workspace_bytes, int* status,
                   cudaStream_t stream);
+// Chunks on tcgen05 tensor cores (attn_prefill_kv4_sm100.cu). splits > 1 cuts the KV range for launches that would leave
+// most SMs idle; the workspace holds their partial results.
+int xv_kv4_prefill_splits(int num_seqs, int max_q_len, int hq, int hkv, int max_tokens_per_seq, int num_sms);
+long long xv_kv4_prefill_workspace_bytes(int num_seqs, int max_q_len, int hq, int hkv, int splits);
 int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_q,
-                   const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq,
-                   int hkv, int d, int block_size, int max_blocks, int num_blocks, float scale, int* status,
-                   cudaStream_t stream);
-// The chunk form on tcgen05 tensor cores (attn_prefill_kv4_sm100.cu); xv_kv4_prefill calls it where it is the faster one.
-int xv_kv4_prefill_tc(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_q,
-                      const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq,
-                      int hkv, int d, int block_size, int max_blocks, int num_blocks, float scale, int* status,
-                      cudaStream_t stream);
+                   const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq, int hkv,
+                   int d, int block_size, int max_blocks, int num_blocks, float scale, int splits, void* workspace,
+                   long long workspace_bytes, int* status, cudaStream_t stream);
 
 // Input ids < 0 are references into the previous step's samples: ids[i] = prev[-ids[i] - 1] (elementwise.cu).
 int xv_resolve_token_refs(int* ids, int n, const long long* prev, int n_prev, cudaStream_t stream);

@@ -89,8 +89,11 @@ def lib():
     L.xv_kv4_decode_workspace_bytes.restype = _i64
     L.xv_kv4_decode.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32,
                                 _vp, _i64, _vp, _vp]
+    L.xv_kv4_prefill_splits.argtypes = [_i32] * 6
+    L.xv_kv4_prefill_workspace_bytes.argtypes = [_i32] * 5
+    L.xv_kv4_prefill_workspace_bytes.restype = _i64
     L.xv_kv4_prefill.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
-                                 _i32, _f32, _vp, _vp]
+                                 _i32, _f32, _i32, _vp, _i64, _vp, _vp]
     L.xv_argmax.argtypes = [_vp, _vp, _i32, _i32, _i64, _vp]
     L.xv_sample.argtypes = [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp]
     L.xv_tp_reduce_norm.argtypes = [_vp, _vp, _vp, _vp, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _f32,
@@ -476,10 +479,14 @@ def _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, 
                                num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale, splits, st.num_sms,
                                ws.data_ptr() if need else None, need, st.status.data_ptr(), stream), "kv4_decode")
     if n_p:
+        mq = attn.max_q_len
+        splits = L.xv_kv4_prefill_splits(n_p, mq, num_q_heads, num_kv_heads, maxb * bs, st.num_sms)
+        need = L.xv_kv4_prefill_workspace_bytes(n_p, mq, num_q_heads, num_kv_heads, splits) if splits > 1 else 0
+        ws = k_cache.new_empty(need) if need else None
         _check(L.xv_kv4_prefill(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), tables,
-                                _vector(attn.cu_q, B + 1, torch.int32, dev, "cu_q"), lens, out.data_ptr(), n_d, n_p,
-                                attn.max_q_len, T, num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale,
-                                st.status.data_ptr(), stream), "kv4_prefill")
+                                _vector(attn.cu_q, B + 1, torch.int32, dev, "cu_q"), lens, out.data_ptr(), n_d, n_p, mq, T,
+                                num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale, splits,
+                                ws.data_ptr() if need else None, need, st.status.data_ptr(), stream), "kv4_prefill")
     return out
 
 

@@ -158,7 +158,9 @@ class NativeForward:
             self.t["gu"] = buf(T, 2 * d.inter_local)
         st = cuda._state(self.t["h"])
         if d.kv4:
-            need = L.xv_kv4_decode_workspace_bytes(max_samples, d.hq, d.hkv, 0, st.num_sms)
+            # split chunk launches have at most as many CTAs as there are SMs
+            need = max(L.xv_kv4_decode_workspace_bytes(max_samples, d.hq, d.hkv, 0, st.num_sms),
+                       st.num_sms * L.xv_kv4_prefill_workspace_bytes(1, 1, 1, 1, 2) // 2)
             attn_ws = self.t["attn_ws"] = torch.empty(need, dtype=torch.uint8, device=dev)
         else:
             need = L.xv_attn_decode_workspace_bytes(max_samples, d.hq, d.head_dim, 16)
