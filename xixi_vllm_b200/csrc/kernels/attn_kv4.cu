@@ -792,13 +792,15 @@ inline int launch_ok() { return cudaGetLastError() == cudaSuccess ? 0 : XV_ERR_L
 extern "C" {
 
 // How a decode launch divides its work, from launch-shape constants only (never from sequence lengths), so that a captured
-// graph keeps its shape: 1, 2, 4 or 8 CTAs (one cluster) per (sequence, KV head), or 0 for even shares.
+// graph keeps its shape: 1, 2, 4 or 8 CTAs (one cluster) per (sequence, KV head) as long as they are one wave of three an
+// SM, or 0 for even shares where a CTA could get more than 2048 tokens. Device times, clusters of 1 / 2 / 4 / 8 against
+// shares: 256 pairs of up to 1280 tokens 13.0 / 14.7 / 18.3 / 32.2 against 15.8 us; 72 pairs of up to 3001 19.9 / 14.0 /
+// 11.6 / 14.0 against 18.9; 8 pairs of 2000 14.4 / 10.5 / 6.9 / 5.7 against 9.2, of 40960 246 / 128 / 66 / 36 against 22.5.
 int xv_kv4_decode_splits(int num_seqs, int hkv, int num_sms, int max_tokens_per_seq) {
   const long long pairs = static_cast<long long>(num_seqs) * hkv;
-  if (pairs * max_tokens_per_seq > 4096ll * num_sms) return 0;
   int s = 1;
-  while (s < 8 && pairs * s < 2 * num_sms && max_tokens_per_seq / (2 * s) >= 128) s *= 2;
-  return s;
+  while (s < 8 && pairs * 2 * s <= 3 * num_sms && max_tokens_per_seq / (2 * s) >= 128) s *= 2;
+  return max_tokens_per_seq / s > 2048 ? 0 : s;
 }
 
 long long xv_kv4_decode_workspace_bytes(int num_seqs, int hq, int hkv, int splits, int num_sms) {

@@ -4,6 +4,8 @@
 
 Produces ``xixi_vllm_b200/ops/_xv_cuda.so``; the source list is every ``.cu`` under
 ``csrc/kernels``. The shared object carries only sm_100a code: there is no fallback arch.
+``build_torch`` produces ``_xv_torch.so`` with g++: the Python calls of the 4-bit cache operators
+(``csrc/host/kv4_torch.cpp``), compiled against the installed torch.
 """
 
 from __future__ import annotations
@@ -20,6 +22,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(_HERE), "csrc")
 LIB = os.path.join(_HERE, "_xv_cuda.so")
 OBJ_DIR = os.path.join(_HERE, "_build")
+TORCH_SRC = os.path.join(CSRC, "host", "kv4_torch.cpp")
+TORCH_LIB = os.path.join(_HERE, "_xv_torch.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -80,9 +84,32 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
+def build_torch(force: bool = False) -> str:
+    """Compile the Python extension in-tree with g++ (half a minute: torch's headers)."""
+    header = os.path.join(CSRC, "kernels", "xv_cuda.h")
+    if not force and os.path.isfile(TORCH_LIB) and os.path.getmtime(TORCH_LIB) >= max(map(os.path.getmtime, (TORCH_SRC, header))):
+        return TORCH_LIB
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path())))
+    tmp = TORCH_LIB + f".tmp{os.getpid()}"
+    subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+                    "-isystem", os.path.join(root, "include"),
+                    "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                    "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
+                    "-I", os.path.join(CSRC, "kernels"), "-o", tmp, TORCH_SRC,
+                    "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], check=True)
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
+
+
 if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("--force", action="store_true")
     ap.add_argument("--verbose", action="store_true")
     a = ap.parse_args()
     print(build(a.force, a.verbose))
+    print(build_torch(a.force))

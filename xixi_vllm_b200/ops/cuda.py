@@ -17,7 +17,6 @@ import os
 import torch
 
 from . import build as _build
-from . import kv4 as _kv4
 
 __all__ = [
     "lib", "rmsnorm", "add_rmsnorm", "linear", "silu_mul", "embedding", "gather_rows",
@@ -81,19 +80,12 @@ def lib():
                                      _i32, _i32, _i32, _f32, _vp, _vp]
     L.xv_attn_prefill_tc_profile.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                              _i32, _i32, _i32, _f32, _vp, _vp, _vp]
-    L.xv_kv4_write.argtypes = [_vp, _vp, _i32, _i64, _vp, _vp, _f32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32,
-                               _i32, _i32, _i32, _vp, _vp]
-    L.xv_kv4_read.argtypes = [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp]
     L.xv_kv4_decode_splits.argtypes = [_i32, _i32, _i32, _i32]
     L.xv_kv4_decode_workspace_bytes.argtypes = [_i32] * 5
     L.xv_kv4_decode_workspace_bytes.restype = _i64
-    L.xv_kv4_decode.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32,
-                                _vp, _i64, _vp, _vp]
     L.xv_kv4_prefill_splits.argtypes = [_i32] * 6
     L.xv_kv4_prefill_workspace_bytes.argtypes = [_i32] * 5
     L.xv_kv4_prefill_workspace_bytes.restype = _i64
-    L.xv_kv4_prefill.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
-                                 _i32, _f32, _i32, _vp, _i64, _vp, _vp]
     L.xv_argmax.argtypes = [_vp, _vp, _i32, _i32, _i64, _vp]
     L.xv_sample.argtypes = [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp]
     L.xv_tp_reduce_norm.argtypes = [_vp, _vp, _vp, _vp, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _f32,
@@ -348,7 +340,7 @@ def resolve_token_refs(ids, prev) -> None:
 
 def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads,
                        num_kv_heads, head_dim, prefill_begin: int = 0):
-    if _kv4.is_kv4(k_cache):
+    if k_cache.dtype is torch.uint8:
         return _kv4_write(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads, num_kv_heads,
                           head_dim)
     if isinstance(qkv, SplitKPartial):
@@ -373,121 +365,54 @@ def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v
     return q
 
 
-def _vector(t, n: int, dtype, device, what: str) -> int:
-    """Address of ``t``, which must hold at least ``n`` contiguous elements of ``dtype`` on ``device``."""
-    if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < n:
-        raise ValueError(f"{what}: needs {n} contiguous {dtype} values on {device}, got {tuple(t.shape)} {t.dtype} on "
-                         f"{t.device}")
-    return t.data_ptr()
+_calls = None
 
 
-def _kv4_caches(k_cache, v_cache, head_dim: int, num_kv_heads: int | None = None) -> None:
-    _kv4.check_caches(k_cache, v_cache, head_dim, num_kv_heads)
-    if head_dim != 128:
-        raise ValueError(f"4-bit caches on the GPU need head_dim 128, got {head_dim}")
+def _kv4_calls():
+    """The Python extension that launches the 4-bit cache kernels (``csrc/host/kv4_torch.cpp``)."""
+    global _calls
+    if _calls is None:
+        import importlib.util
 
-
-def _elsewhere(dev: torch.device) -> bool:
-    """Whether ``dev`` is not the current device: the caller then enters it (1.4 us that the usual call does not pay)."""
-    return dev.index != torch.cuda.current_device()
+        path = _build.build_torch()
+        spec = importlib.util.spec_from_file_location("_xv_torch", path)
+        calls = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(calls)
+        L = lib()
+        calls.bind(*(ctypes.cast(getattr(L, name), _vp).value for name in (
+            "xv_kv4_write", "xv_kv4_read", "xv_kv4_decode_splits", "xv_kv4_decode_workspace_bytes", "xv_kv4_decode",
+            "xv_kv4_prefill_splits", "xv_kv4_prefill_workspace_bytes", "xv_kv4_prefill")))
+        _calls = calls
+    return _calls
 
 
 def _kv4_write(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads, num_kv_heads, head_dim):
-    _kv4_caches(k_cache, v_cache, head_dim, num_kv_heads)
-    dev = k_cache.device
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return _kv4_write(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads, num_kv_heads,
-                              head_dim)
-    part = isinstance(qkv, SplitKPartial)
-    T, cols = qkv.shape if len(qkv.shape) == 2 else (0, -1)
-    if cols != (num_q_heads + 2 * num_kv_heads) * head_dim or qkv.device != dev:
-        raise ValueError(f"qk_norm_rope_cache: qkv must be [T, {(num_q_heads + 2 * num_kv_heads) * head_dim}] on {dev}, got "
-                         f"{tuple(qkv.shape)} on {qkv.device}")
-    if not part:
-        _bf16(qkv)
-        if not qkv.is_contiguous():
-            raise ValueError("qk_norm_rope_cache needs contiguous qkv and cache tensors")
-    _bf16(q_w, k_w)
-    rows = cos_sin.numel() // head_dim
-    args = (None if part else qkv.data_ptr(), qkv.ws.data_ptr() if part else None, qkv.splits if part else 0,
-            qkv.stride_elems if part else 0, _vector(q_w, head_dim, torch.bfloat16, dev, "q_w"),
-            _vector(k_w, head_dim, torch.bfloat16, dev, "k_w"), eps,
-            _vector(cos_sin, head_dim, torch.float32, dev, "cos_sin"), rows,
-            _vector(positions, T, torch.int32, dev, "positions"), _vector(slots, T, torch.int32, dev, "slots"))
-    q = q_w.new_empty((T, num_q_heads * head_dim))
-    if T:
-        nb, _, bs, _ = k_cache.shape
-        _check(lib().xv_kv4_write(*args, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), T, num_q_heads, num_kv_heads,
-                                  head_dim, bs, nb, _state(k_cache).status.data_ptr(),
-                                  torch._C._cuda_getCurrentRawStream(dev.index)), "kv4_write")
-    return q
+    global launch_count
+    launch_count += 1
+    calls, status = _calls or _kv4_calls(), _state(k_cache).status
+    if isinstance(qkv, SplitKPartial):
+        T, cols = qkv.shape
+        if cols != (num_q_heads + 2 * num_kv_heads) * head_dim:
+            raise ValueError(f"qk_norm_rope_cache: {cols} columns for {num_q_heads} query and {num_kv_heads} KV heads")
+        return calls.write(None, qkv.ws, qkv.splits, T, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache,
+                           num_q_heads, num_kv_heads, head_dim, status)
+    return calls.write(qkv, None, 0, 0, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads,
+                       num_kv_heads, head_dim, status)
 
 
 def read_cache(k_cache, v_cache, slots, head_dim):
     """bf16 rows of a 4-bit cache (see ``dispatch.read_cache``). A slot beyond the cache gives zeros and status 5."""
-    _kv4_caches(k_cache, v_cache, head_dim)
-    dev = k_cache.device
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return read_cache(k_cache, v_cache, slots, head_dim)
-    T = slots.numel()
-    nb, hkv, bs, _ = k_cache.shape
-    at = _vector(slots, T, torch.int32, dev, "slots")
-    k = k_cache.new_empty((T, hkv, head_dim), dtype=torch.bfloat16)
-    v = torch.empty_like(k)
-    if T:
-        _check(lib().xv_kv4_read(k_cache.data_ptr(), v_cache.data_ptr(), at, k.data_ptr(), v.data_ptr(), T, hkv, head_dim,
-                                 bs, nb, _state(k_cache).status.data_ptr(),
-                                 torch._C._cuda_getCurrentRawStream(dev.index)), "kv4_read")
-    return k, v
+    global launch_count
+    launch_count += 1
+    return (_calls or _kv4_calls()).read(k_cache, v_cache, slots, head_dim, _state(k_cache).status)
 
 
 def _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
-    _kv4_caches(k_cache, v_cache, head_dim, num_kv_heads)
-    dev = k_cache.device
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim)
-    _bf16(q)
-    bt, B, n_d = attn.block_tables, attn.num_seqs, attn.num_decode
-    n_p = B - n_d
-    if q.dim() != 2 or q.shape[1] != num_q_heads * head_dim or not q.is_contiguous() or q.device != dev:
-        raise ValueError(f"paged_attention: q must be a contiguous [T, {num_q_heads * head_dim}] tensor on {dev}")
-    if num_q_heads % num_kv_heads or num_q_heads > 16 * num_kv_heads:
-        raise ValueError(f"paged_attention: {num_q_heads} query heads over {num_kv_heads} KV heads (at most 16 to one)")
-    T = q.shape[0]
-    if n_d < 0 or n_p < 0 or n_d > T or bt.dim() != 2 or bt.shape[0] < B:
-        raise ValueError(f"paged_attention: {n_d} decode rows and {n_p} chunks for {T} query rows and a block table of "
-                         f"{tuple(bt.shape)}")
-    if B > 65535:
-        raise ValueError("paged_attention: at most 65535 sequences")
-    maxb = bt.shape[1]
-    tables = _vector(bt, B * maxb, torch.int32, dev, "block_tables")
-    lens = _vector(attn.kv_lens, B, torch.int32, dev, "kv_lens")
-    nb, _, bs, _ = k_cache.shape
-    out = torch.empty_like(q)
-    if maxb == 0 or nb == 0:        # nothing is cached: every row is empty
-        return out.zero_()
-    L, st, stream = lib(), _state(q), torch._C._cuda_getCurrentRawStream(dev.index)
-    if n_d:
-        splits = L.xv_kv4_decode_splits(n_d, num_kv_heads, st.num_sms, maxb * bs)
-        need = 0 if splits else L.xv_kv4_decode_workspace_bytes(n_d, num_q_heads, num_kv_heads, 0, st.num_sms)
-        # from torch's allocator, call by call: calls on two streams, or two captured graphs, never share it
-        ws = k_cache.new_empty(need) if need else None
-        _check(L.xv_kv4_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), tables, lens, out.data_ptr(), n_d,
-                               num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale, splits, st.num_sms,
-                               ws.data_ptr() if need else None, need, st.status.data_ptr(), stream), "kv4_decode")
-    if n_p:
-        mq = attn.max_q_len
-        splits = L.xv_kv4_prefill_splits(n_p, mq, num_q_heads, num_kv_heads, maxb * bs, st.num_sms)
-        need = L.xv_kv4_prefill_workspace_bytes(n_p, mq, num_q_heads, num_kv_heads, splits) if splits > 1 else 0
-        ws = k_cache.new_empty(need) if need else None
-        _check(L.xv_kv4_prefill(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), tables,
-                                _vector(attn.cu_q, B + 1, torch.int32, dev, "cu_q"), lens, out.data_ptr(), n_d, n_p, mq, T,
-                                num_q_heads, num_kv_heads, head_dim, bs, maxb, nb, scale, splits,
-                                ws.data_ptr() if need else None, need, st.status.data_ptr(), stream), "kv4_prefill")
-    return out
+    global launch_count
+    st, n, n_d = _state(k_cache), attn.num_seqs, attn.num_decode
+    launch_count += (n_d > 0) + (n > n_d)
+    return (_calls or _kv4_calls()).attention(q, k_cache, v_cache, attn.cu_q, attn.kv_lens, attn.block_tables, n, n_d,
+                                              attn.max_q_len, scale, num_q_heads, num_kv_heads, head_dim, st.num_sms, st.status)
 
 
 def decode_splits(num_seqs: int, num_kv_heads: int, num_sms: int, max_blocks_tokens: int) -> int:
@@ -518,7 +443,7 @@ def prefill_pair_heads(on: bool) -> None:
 
 def paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
     """Decode rows (the first ``attn.num_decode`` sequences) and prefill chunks of one packed batch."""
-    if _kv4.is_kv4(k_cache):
+    if k_cache.dtype is torch.uint8:
         return _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim)
     _bf16(q, k_cache, v_cache)
     st = _state(q)

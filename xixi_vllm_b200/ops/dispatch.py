@@ -18,10 +18,16 @@ __all__ = [
 build_cos_sin_cache = cpu_ref.build_cos_sin_cache
 
 
-def _cuda():
-    from . import cuda
+_cuda_ops = None
 
-    return cuda
+
+def _cuda():
+    global _cuda_ops
+    if _cuda_ops is None:
+        from . import cuda
+
+        _cuda_ops = cuda
+    return _cuda_ops
 
 
 def rmsnorm(x, w, eps):
@@ -79,9 +85,9 @@ def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v
 def read_cache(k_cache, v_cache, slots, head_dim):
     """What a 4-bit cache holds at ``slots [T]`` (int32, as ``qk_norm_rope_cache`` takes them): bf16 ``k, v`` of shape
     ``[T, kv_heads, head_dim]``. Rows whose slot is negative are zero. A slot may be named any number of times."""
-    kv4.check_caches(k_cache, v_cache, head_dim)
     if k_cache.is_cuda:
         return _cuda().read_cache(k_cache, v_cache, slots, head_dim)
+    kv4.check_caches(k_cache, v_cache, head_dim)
     return cpu_ref.read_cache(k_cache, v_cache, slots)
 
 
