@@ -1,15 +1,20 @@
 // Writing and reading a KV cache held in 4 bits (format: common/kv4.cuh).
 //
 //   kv4_write_kernel - per-head RMSNorm of q and k, NeoX RoPE, q written in bf16, k and v rounded to bf16 (what a bf16
-//                      cache would hold) and quantised into their slots. One warp per (token, head).
-//   kv4_read_kernel  - the bf16 values of a list of slots.
+//                      cache would hold) and quantised into their slots. Half a warp per head, two heads of one kind at
+//                      a time; a lane holds four channels and their four rotary partners.
+//   kv4_read_kernel  - the bf16 values of a list of slots. A warp per token.
+//
+// Both are bound by memory: the writer moves (hq + 2 hkv) 256 + hq 256 + hkv 144 bytes a token, the reader hkv 2 (72 + 256).
 //
 // Quantising is a choice between 16 levels, so K is normalised and rotated in 64 bits from the fp32 row: a value next
-// to a border between two levels then falls the same way wherever the row is computed (sixteen products a lane, for the
-// K heads only).
+// to a border between two levels then falls the same way wherever the row is computed (five double operations a channel,
+// for the K heads only).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "../common/kv4.cuh"
 #include "../common/launch.cuh"
@@ -24,161 +29,268 @@ constexpr int kIdWrite = 8, kIdRead = 9;       // kernel ids in the status word
 
 __device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(__float2bfloat16(x)); }
 
-__device__ __forceinline__ double warp_sum_d(double v) {
+__device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// Sum over the 16 lanes of half a warp.
+template <typename T>
+__device__ __forceinline__ T half_sum(T v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = 1; o <= 8; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// Stores one row: lane l holds channels 2l, 2l+1 (lo) and 64 + 2l, 64 + 2l + 1 (hi), all four in group (l >> 2) & 1.
-// ops/kv4.py fixes the arithmetic; the explicit _rn forms keep it under the library's fast-math flags.
-__device__ __forceinline__ void store_row(uint8_t* unit, int r, int lane, float lo0, float lo1, float hi0, float hi1) {
-  float mx = fmaxf(fmaxf(lo0, lo1), fmaxf(hi0, hi1)), mn = fminf(fminf(lo0, lo1), fminf(hi0, hi1));
-  const bool fine = fabsf(lo0) <= 3.3895314e38f && fabsf(lo1) <= 3.3895314e38f && fabsf(hi0) <= 3.3895314e38f &&
-                    fabsf(hi1) <= 3.3895314e38f;              // the largest bf16; false for NaN
+// Half a warp holds a head's row: lane c (0..15) channels 4c .. 4c + 3 in x[0..3] and 64 + 4c .. in x[4..7], so that rotary
+// partners meet in a lane and all eight channels are of group (c >> 1) & 1.
+//
+// Stores one row of bf16 values. ops/kv4.py fixes the arithmetic; the explicit _rn forms keep it under the library's
+// fast-math flags. A code is the quotient (x - centre) / step rounded to even: from the product with 1 / step, corrected
+// by its exact remainder (ties are common: both are bf16).
+__device__ __forceinline__ void store_row(uint8_t* unit, int r, int c, unsigned half_mask, const float (&x)[8], bool there) {
+  float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+  float mn = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
+  // NaN or infinite anywhere: x - x is not 0
+  const float odd = ((x[0] - x[0]) + (x[1] - x[1])) + ((x[2] - x[2]) + (x[3] - x[3])) + ((x[4] - x[4]) + (x[5] - x[5])) +
+                    ((x[6] - x[6]) + (x[7] - x[7]));
 #pragma unroll
-  for (int o = 1; o <= 16; o <<= 1) {
-    if (o == 4) continue;                                     // lane bit 2 is the group
+  for (int o = 1; o <= 8; o <<= 1) {
+    if (o == 2) continue;                                     // lane bit 1 is the group
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
   }
-  const uint32_t not_fine = __ballot_sync(0xffffffffu, !fine);
-  const bool bad = (not_fine & ((lane & 4) ? 0xf0f0f0f0u : 0x0f0f0f0fu)) != 0;
+  const uint32_t not_fine = __ballot_sync(0xffffffffu, !(odd == 0.f));
+  const bool bad = (not_fine & half_mask & ((c & 2) ? 0xccccccccu : 0x33333333u)) != 0;
   float s = round_bf16(__fdiv_rn(__fsub_rn(0.5f * mx, 0.5f * mn), 7.5f));
   if (s < 1.17549435e-38f) s = 0.f;
-  const float c = round_bf16(__fadd_rn(__fadd_rn(0.5f * mx, 0.5f * mn), 0.5f * s));
-  auto code = [&](float x) -> uint32_t {
-    if (bad || s == 0.f) return 8u;
-    const float n = rintf(__fdiv_rn(__fsub_rn(x, c), s)) + 8.f;
-    return static_cast<uint32_t>(fminf(fmaxf(n, 0.f), 15.f));
-  };
-  uint8_t* codes = unit + r * kv4::kCodeRow;
-  codes[lane] = static_cast<uint8_t>(code(lo0) | code(lo1) << 4);
-  codes[32 + lane] = static_cast<uint8_t>(code(hi0) | code(hi1) << 4);
-  if ((lane & 27) == 0) {                                     // lanes 0 and 4: one parameter word per group
-    uint32_t w = 0x7fff7fffu;
-    if (!bad) w = pack_bf16(s, c);
-    *reinterpret_cast<uint32_t*>(unit + kv4::kParBase + r * kv4::kParRow + lane) = w;
+  const float cen = round_bf16(__fadd_rn(__fadd_rn(0.5f * mx, 0.5f * mn), 0.5f * s));
+  const float r_s = s > 0.f ? __frcp_rn(s) : 0.f;
+  constexpr float kRound = 12582912.f;                        // 1.5 2^23: adding it leaves an integer in the low bits
+  uint32_t code[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = __fsub_rn(x[i], cen);
+    float m = __fadd_rn(fminf(fmaxf(a * r_s, -8.f), 7.f), kRound);
+    const float n = __fsub_rn(m, kRound);
+    const float d = __fmaf_rn(-n, s, a);                      // exact: how far the quotient is from n, in steps of s
+    const float over = __fmaf_rn(2.f, fabsf(d), -s);          // > 0: n is not the nearest; 0: a tie
+    const bool move = over > 0.f || (over == 0.f && (__float_as_uint(m) & 1u));
+    if (move) m = __fadd_rn(m, d < 0.f ? -1.f : 1.f);
+    m = fminf(fmaxf(m, kRound - 8.f), kRound + 7.f);
+    code[i >> 2] |= ((__float_as_uint(m) + 8u) & 15u) << (4 * (i & 3));
+  }
+  if (bad || s == 0.f) code[0] = code[1] = 0x8888u;
+  if (there) {
+    uint8_t* row = unit + r * kv4::kCodeRow + c * 2;
+    *reinterpret_cast<uint16_t*>(row) = static_cast<uint16_t>(code[0]);
+    *reinterpret_cast<uint16_t*>(row + 32) = static_cast<uint16_t>(code[1]);
+    if ((c & 13) == 0)                                        // lanes 0 and 2: one parameter word per group
+      *reinterpret_cast<uint32_t*>(unit + kv4::kParBase + r * kv4::kParRow + c * 2) = bad ? 0x7fff7fffu : pack_bf16(s, cen);
   }
 }
 
-__global__ void __launch_bounds__(256)
-kv4_write_kernel(const __nv_bfloat16* __restrict__ qkv, const float* __restrict__ partials, int splits,
-                 long long split_stride, const __nv_bfloat16* __restrict__ q_w, const __nv_bfloat16* __restrict__ k_w,
-                 float eps, const float* __restrict__ cos_sin, int max_pos, const int* __restrict__ positions,
-                 const int* __restrict__ slots, __nv_bfloat16* __restrict__ q_out, uint8_t* __restrict__ k_cache,
-                 uint8_t* __restrict__ v_cache, int tokens, int hq, int hkv, int block_size, int num_slots, int* status) {
+// What a launch writes and where.
+struct WriteParams {
+  const __nv_bfloat16* qkv;
+  const float* planes;
+  const __nv_bfloat16* q_w;
+  const __nv_bfloat16* k_w;
+  const float* cos_sin;
+  const int* positions;
+  const int* slots;
+  __nv_bfloat16* q_out;
+  uint8_t* k_cache;
+  uint8_t* v_cache;
+  int* status;
+  long long split_stride;
+  float eps;
+  int splits, max_pos, tokens, hq, hkv, block_size, num_slots;
+  int per_warp;                      // pairs of heads a warp takes
+  int q_tasks, tasks;                // warps per token: for Q, and in all
+};
+
+template <bool PLANES>
+__global__ void __launch_bounds__(256, 3) kv4_write_kernel(const WriteParams p) {
   grid_dep_launch();
   grid_dep_wait();
   constexpr int D = kv4::kD, HALF = D / 2;
-  const int heads = hq + 2 * hkv;
-  const long long gw = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (gw >= static_cast<long long>(tokens) * heads) return;
-  const int t = static_cast<int>(gw / heads);
-  const int h = static_cast<int>(gw - static_cast<long long>(t) * heads);
-  int slot = -1;
-  if (h >= hq) {
-    slot = slots[t];
-    if (slot >= num_slots) {
-      if (lane == 0) report_status(status, kIdWrite, kBadIndex);
-      slot = -1;
-    }
-    if (slot < 0) return;                                     // warp-uniform
-  }
-  const size_t off = static_cast<size_t>(t) * heads * D + static_cast<size_t>(h) * D;
+  const int warp = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int t = warp / p.tasks, task = warp - t * p.tasks;
+  if (t >= p.tokens) return;
+  const int lane = threadIdx.x & 31, c = lane & 15, half = lane >> 4;
+  const size_t row0 = static_cast<size_t>(t) * (p.hq + 2 * p.hkv) * D + 4 * c;
 
-  float lo0, lo1, hi0, hi1;
-  if (partials != nullptr) {
-    lo0 = lo1 = hi0 = hi1 = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      const float2 a = *reinterpret_cast<const float2*>(partials + s * split_stride + off + lane * 2);
-      const float2 b = *reinterpret_cast<const float2*>(partials + s * split_stride + off + HALF + lane * 2);
-      lo0 += a.x; lo1 += a.y; hi0 += b.x; hi1 += b.y;
+  // x[0..3] and x[4..7] of head h
+  auto load = [&](int h, uint2& a, uint2& b) {
+    const size_t off = row0 + static_cast<size_t>(h) * D;
+    if constexpr (PLANES) {
+      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+      for (int s = 0; s < p.splits; ++s) {
+        const float4 e = *reinterpret_cast<const float4*>(p.planes + s * p.split_stride + off);
+        const float4 f = *reinterpret_cast<const float4*>(p.planes + s * p.split_stride + off + HALF);
+        u.x += e.x; u.y += e.y; u.z += e.z; u.w += e.w;
+        v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
+      }
+      a = make_uint2(pack_bf16(u.x, u.y), pack_bf16(u.z, u.w));      // as the bf16 GEMM output would have been
+      b = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    } else {
+      a = __ldg(reinterpret_cast<const uint2*>(p.qkv + off));
+      b = __ldg(reinterpret_cast<const uint2*>(p.qkv + off + HALF));
     }
-    // same rounding point as the bf16 GEMM output would have had
-    lo0 = round_bf16(lo0); lo1 = round_bf16(lo1); hi0 = round_bf16(hi0); hi1 = round_bf16(hi1);
-  } else {
-    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(qkv + off + lane * 2));
-    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(qkv + off + HALF + lane * 2));
-    lo0 = a.x; lo1 = a.y; hi0 = b.x; hi1 = b.y;
-  }
-  if (h >= hq + hkv) {
-    store_row(v_cache + kv4::unit_offset(slot / block_size, h - hq - hkv, hkv, block_size, slot % block_size),
-              slot % block_size % kv4::kUnit, lane, lo0, lo1, hi0, hi1);
+  };
+  auto unpack = [](const uint2& a, const uint2& b, float (&x)[8]) {
+    x[0] = lo_f(a.x); x[1] = hi_f(a.x); x[2] = lo_f(a.y); x[3] = hi_f(a.y);
+    x[4] = lo_f(b.x); x[5] = hi_f(b.x); x[6] = lo_f(b.y); x[7] = hi_f(b.y);
+  };
+  // The lane's four rotary pairs: cos, sin, and the two norm weights.
+  float cs[4], sn[4], w[8];
+  auto rotary = [&](const __nv_bfloat16* nw) {
+    int pos = p.positions[t];
+    if (pos < 0 || pos >= p.max_pos) {
+      if (lane == 0) report_status(p.status, kIdWrite, kBadIndex);
+      pos = 0;
+    }
+    const float* at = p.cos_sin + static_cast<size_t>(pos) * D + 4 * c;
+    const float4 a = __ldg(reinterpret_cast<const float4*>(at)), b = __ldg(reinterpret_cast<const float4*>(at + HALF));
+    cs[0] = a.x; cs[1] = a.y; cs[2] = a.z; cs[3] = a.w;
+    sn[0] = b.x; sn[1] = b.y; sn[2] = b.z; sn[3] = b.w;
+    unpack(__ldg(reinterpret_cast<const uint2*>(nw + 4 * c)), __ldg(reinterpret_cast<const uint2*>(nw + HALF + 4 * c)), w);
+  };
+
+  if (task < p.q_tasks) {
+    // ---- Q: heads 2 i + half; a missing second head repeats the first and stores nothing ----
+    const int first = task * p.per_warp, last = min(first + p.per_warp, (p.hq + 1) / 2);
+    uint2 a, b, a_next = make_uint2(0u, 0u), b_next = a_next;
+    load(min(2 * first + half, p.hq - 1), a, b);
+    rotary(p.q_w);
+    float p1[4], p2[4], p3[4], p4[4];                         // w1 cos, w2 sin, w2 cos, w1 sin
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p1[i] = w[i] * cs[i];
+      p2[i] = w[4 + i] * sn[i];
+      p3[i] = w[4 + i] * cs[i];
+      p4[i] = w[i] * sn[i];
+    }
+    for (int i = first; i < last; ++i) {
+      const int h = 2 * i + half;
+      if (i + 1 < last) load(min(h + 2, p.hq - 1), a_next, b_next);
+      float x[8];
+      unpack(a, b, x);
+      float ss = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ss += x[k] * x[k];
+      const float inv = rsqrtf(half_sum(ss) / static_cast<float>(D) + p.eps);
+      float o[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[k] = (x[k] * p1[k] - x[4 + k] * p2[k]) * inv;
+        o[4 + k] = (x[4 + k] * p3[k] + x[k] * p4[k]) * inv;
+      }
+      if (h < p.hq) {
+        __nv_bfloat16* dst = p.q_out + (static_cast<size_t>(t) * p.hq + h) * D + 4 * c;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+        *reinterpret_cast<uint2*>(dst + HALF) = make_uint2(pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
+      }
+      a = a_next;
+      b = b_next;
+    }
     return;
   }
-  int pos = positions[t];
-  if (pos < 0 || pos >= max_pos) {
-    if (lane == 0) report_status(status, kIdWrite, kBadIndex);
-    pos = 0;
+
+  // ---- K and V ----
+  const int slot = p.slots[t];
+  if (slot >= p.num_slots && lane == 0) report_status(p.status, kIdWrite, kBadIndex);
+  if (slot < 0 || slot >= p.num_slots) return;
+  const int kv_pairs = (p.hkv + 1) / 2;
+  const int first = (task - p.q_tasks) * p.per_warp, last = min(first + p.per_warp, 2 * kv_pairs);
+  const int place = slot % p.block_size;
+  const size_t unit0 = kv4::unit_offset(slot / p.block_size, 0, p.hkv, p.block_size, place);
+  const size_t head_bytes = static_cast<size_t>(p.block_size / kv4::kUnit) * kv4::kUnitBytes;
+  const unsigned half_mask = half ? 0xffff0000u : 0x0000ffffu;
+  if (first < kv_pairs) rotary(p.k_w);
+  auto head_of = [&](int pair) { return min(2 * (pair < kv_pairs ? pair : pair - kv_pairs) + half, p.hkv - 1); };
+  auto source = [&](int pair) { return p.hq + (pair < kv_pairs ? 0 : p.hkv) + head_of(pair); };
+  uint2 a, b, a_next = make_uint2(0u, 0u), b_next = a_next;
+  load(source(first), a, b);
+  for (int pair = first; pair < last; ++pair) {
+    if (pair + 1 < last) load(source(pair + 1), a_next, b_next);
+    const bool is_k = pair < kv_pairs;
+    const int h = head_of(pair);
+    const bool there = 2 * (is_k ? pair : pair - kv_pairs) + half < p.hkv;
+    float x[8];
+    unpack(a, b, x);
+    if (is_k) {
+      double ss = 0.0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ss += static_cast<double>(x[k]) * x[k];
+      const double ms = half_sum(ss) * (1.0 / D) + static_cast<double>(p.eps);
+      double inv = rsqrtf(static_cast<float>(ms));            // one Newton step doubles its 22 bits
+      inv = inv + 0.5 * inv * (1.0 - ms * inv * inv);
+      float k8[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {                           // value times weight is exact in fp32: 8 + 8 bits
+        const double u = x[k] * w[k], v = x[4 + k] * w[4 + k], cd = cs[k], sd = sn[k];
+        k8[k] = round_bf16(static_cast<float>((u * cd - v * sd) * inv));
+        k8[4 + k] = round_bf16(static_cast<float>((v * cd + u * sd) * inv));
+      }
+      store_row(p.k_cache + unit0 + h * head_bytes, place % kv4::kUnit, c, half_mask, k8, there);
+    } else {
+      store_row(p.v_cache + unit0 + h * head_bytes, place % kv4::kUnit, c, half_mask, x, there);
+    }
+    a = a_next;
+    b = b_next;
   }
-  const float2 cs = *reinterpret_cast<const float2*>(cos_sin + static_cast<size_t>(pos) * D + lane * 2);
-  const float2 sn = *reinterpret_cast<const float2*>(cos_sin + static_cast<size_t>(pos) * D + HALF + lane * 2);
-  const __nv_bfloat16* w = h < hq ? q_w : k_w;
-  const float2 wl = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(w + lane * 2));
-  const float2 wh = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(w + HALF + lane * 2));
-  if (h < hq) {
-    const float ss = warp_sum(lo0 * lo0 + lo1 * lo1 + hi0 * hi0 + hi1 * hi1);
-    const float inv = rsqrtf(ss / static_cast<float>(D) + eps);
-    const float a0 = lo0 * inv * wl.x, a1 = lo1 * inv * wl.y, b0 = hi0 * inv * wh.x, b1 = hi1 * inv * wh.y;
-    __nv_bfloat16* dst = q_out + static_cast<size_t>(t) * hq * D + static_cast<size_t>(h) * D;
-    *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack_bf16(a0 * cs.x - b0 * sn.x, a1 * cs.y - b1 * sn.y);
-    *reinterpret_cast<uint32_t*>(dst + HALF + lane * 2) = pack_bf16(b0 * cs.x + a0 * sn.x, b1 * cs.y + a1 * sn.y);
-    return;
-  }
-  const double l0 = lo0, l1 = lo1, h0 = hi0, h1 = hi1;
-  const double ms = warp_sum_d(l0 * l0 + l1 * l1 + h0 * h0 + h1 * h1) * (1.0 / D) + static_cast<double>(eps);
-  double inv = rsqrtf(static_cast<float>(ms));                // one Newton step doubles its 22 bits
-  inv = inv + 0.5 * inv * (1.0 - ms * inv * inv);
-  const double a0 = l0 * inv * wl.x, a1 = l1 * inv * wl.y, b0 = h0 * inv * wh.x, b1 = h1 * inv * wh.y;
-  store_row(k_cache + kv4::unit_offset(slot / block_size, h - hq, hkv, block_size, slot % block_size),
-            slot % block_size % kv4::kUnit, lane, round_bf16(static_cast<float>(a0 * cs.x - b0 * sn.x)),
-            round_bf16(static_cast<float>(a1 * cs.y - b1 * sn.y)), round_bf16(static_cast<float>(b0 * cs.x + a0 * sn.x)),
-            round_bf16(static_cast<float>(b1 * cs.y + a1 * sn.y)));
 }
 
-// Sixteen lanes per (token, head): lane i turns word i (8 channels) of K and of V into 16 bytes of bf16.
+// Eight channels of one word as bf16: c + s (n - 8), rounded once.
+__device__ __forceinline__ uint4 dequant8(uint32_t w, uint32_t par) {
+  const uint32_t s2 = __byte_perm(par, par, 0x1010), c2 = __byte_perm(par, par, 0x3232);
+  const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&s2), c = *reinterpret_cast<const __nv_bfloat162*>(&c2);
+  uint32_t v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {                               // channels j and j + 4
+    const uint32_t n = kv4::centred(kv4::biased(w, 4 * j));
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&n), s, c);
+    v[j] = *reinterpret_cast<const uint32_t*>(&r);
+  }
+  return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                    __byte_perm(v[2], v[3], 0x7632));
+}
+
+// A warp per token: one half reads K's heads, the other V's; lane c turns word c (8 channels) into 16 bytes of bf16.
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int* __restrict__ slots,
-                __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, long long rows, int hkv,
-                int block_size, int num_slots, int* status) {
+                __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int tokens, int hkv, int block_size,
+                int num_slots, int* status) {
   grid_dep_launch();
   grid_dep_wait();
-  const long long idx = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const long long row = idx >> 4;
-  const int i = static_cast<int>(idx & 15);
-  if (row >= rows) return;
-  const int t = static_cast<int>(row / hkv), h = static_cast<int>(row - static_cast<long long>(t) * hkv);
-  int slot = slots[t];
-  if (slot >= num_slots) {
-    if (i == 0) report_status(status, kIdRead, kBadIndex);
-    slot = -1;
-  }
-  const size_t dst = static_cast<size_t>(row) * kv4::kD + i * 8;
-  if (slot < 0) {
-    *reinterpret_cast<uint4*>(k_out + dst) = make_uint4(0, 0, 0, 0);
-    *reinterpret_cast<uint4*>(v_out + dst) = make_uint4(0, 0, 0, 0);
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  const int lane = threadIdx.x & 31, c = lane & 15;
+  const int slot = slots[t];
+  uint4* dst = reinterpret_cast<uint4*>((lane < 16 ? k_out : v_out) + static_cast<size_t>(t) * hkv * kv4::kD) + c;
+  if (slot < 0 || slot >= num_slots) {
+    if (slot >= 0 && lane == 0) report_status(status, kIdRead, kBadIndex);
+    for (int h = 0; h < hkv; ++h) dst[h * 16] = make_uint4(0u, 0u, 0u, 0u);
     return;
   }
-  const int r = slot % block_size;
-  const size_t unit = kv4::unit_offset(slot / block_size, h, hkv, block_size, r);
-  const size_t co = unit + (r % kv4::kUnit) * kv4::kCodeRow + i * 4;
-  const size_t po = unit + kv4::kParBase + (r % kv4::kUnit) * kv4::kParRow + (i & 1) * 4;
+  const int place = slot % block_size;
+  const uint8_t* unit = (lane < 16 ? k_cache : v_cache) + kv4::unit_offset(slot / block_size, 0, hkv, block_size, place);
+  const uint8_t* code = unit + (place % kv4::kUnit) * kv4::kCodeRow + c * 4;
+  const uint8_t* par = unit + kv4::kParBase + (place % kv4::kUnit) * kv4::kParRow + (c & 1) * 4;
+  const size_t head_bytes = static_cast<size_t>(block_size / kv4::kUnit) * kv4::kUnitBytes;
+  int h = 0;
+  for (; h + 4 <= hkv; h += 4) {                              // four rows' reads in flight
+    uint32_t w[4], q[4];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const uint8_t* cache = kv ? v_cache : k_cache;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(cache + co), p = *reinterpret_cast<const uint32_t*>(cache + po);
-    const float s = kv4::par_s(p), c = kv4::par_c(p);
-    uint32_t o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float n0 = static_cast<float>(static_cast<int>((w >> (8 * j)) & 15u) - 8);
-      const float n1 = static_cast<float>(static_cast<int>((w >> (8 * j + 4)) & 15u) - 8);
-      o[j] = pack_bf16(fmaf(s, n0, c), fmaf(s, n1, c));
+    for (int i = 0; i < 4; ++i) {
+      w[i] = __ldg(reinterpret_cast<const uint32_t*>(code + (h + i) * head_bytes));
+      q[i] = __ldg(reinterpret_cast<const uint32_t*>(par + (h + i) * head_bytes));
     }
-    *reinterpret_cast<uint4*>((kv ? v_out : k_out) + dst) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[(h + i) * 16] = dequant8(w[i], q[i]);
   }
+  for (; h < hkv; ++h)
+    dst[h * 16] = dequant8(__ldg(reinterpret_cast<const uint32_t*>(code + h * head_bytes)),
+                           __ldg(reinterpret_cast<const uint32_t*>(par + h * head_bytes)));
 }
 
 inline int launch_ok() { return cudaGetLastError() == cudaSuccess ? 0 : XV_ERR_LAUNCH; }
@@ -202,16 +314,34 @@ int xv_kv4_write(const void* qkv, const float* partials, int splits, long long s
   if (tokens <= 0) return 0;
   if (int rc = check_cache(hkv, d, block_size, num_blocks)) return rc;
   if (hq < 0 || max_pos <= 0 || (!qkv && !partials)) return XV_ERR_SHAPE;
-  if (misaligned(qkv, 16) || misaligned(partials, 16) || misaligned(q_w, 4) || misaligned(k_w, 4) ||
-      misaligned(cos_sin, 8) || misaligned(q_out, 16) || misaligned(k_cache, 16) || misaligned(v_cache, 16))
+  if (misaligned(qkv, 16) || misaligned(partials, 16) || misaligned(q_w, 16) || misaligned(k_w, 16) ||
+      misaligned(cos_sin, 16) || misaligned(q_out, 16) || misaligned(k_cache, 16) || misaligned(v_cache, 16))
     return XV_ERR_ALIGN;
-  const long long blocks = (static_cast<long long>(tokens) * (hq + 2 * hkv) + 7) / 8;
-  if (blocks > 0x7fffffffLL) return XV_ERR_SHAPE;
-  launch_pdl(kv4_write_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
-             static_cast<const __nv_bfloat16*>(qkv), partials, splits, split_stride, static_cast<const __nv_bfloat16*>(q_w),
-             static_cast<const __nv_bfloat16*>(k_w), eps, cos_sin, max_pos, positions, slots,
-             static_cast<__nv_bfloat16*>(q_out), static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), tokens, hq,
-             hkv, block_size, num_blocks * block_size, status);
+  // Pairs of heads per warp: one while that leaves a warp slot for each (short steps are latency), up to eight where it
+  // saves making the token's rotary factors again.
+  const int q_pairs = (hq + 1) / 2, kv_pairs = 2 * ((hkv + 1) / 2);
+  WriteParams p;
+  p.per_warp = static_cast<int>(std::max(1ll, std::min(8ll, static_cast<long long>(tokens) * (q_pairs + kv_pairs) / (148 * 48))));
+  p.q_tasks = (q_pairs + p.per_warp - 1) / p.per_warp;
+  p.tasks = p.q_tasks + (kv_pairs + p.per_warp - 1) / p.per_warp;
+  const long long blocks = (static_cast<long long>(tokens) * p.tasks + 7) / 8;
+  if (blocks > 0x0fffffffLL) return XV_ERR_SHAPE;
+  p.qkv = static_cast<const __nv_bfloat16*>(qkv);
+  p.planes = partials;
+  p.q_w = static_cast<const __nv_bfloat16*>(q_w);
+  p.k_w = static_cast<const __nv_bfloat16*>(k_w);
+  p.cos_sin = cos_sin;
+  p.positions = positions;
+  p.slots = slots;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.k_cache = static_cast<uint8_t*>(k_cache);
+  p.v_cache = static_cast<uint8_t*>(v_cache);
+  p.status = status;
+  p.split_stride = split_stride;
+  p.eps = eps;
+  p.splits = splits; p.max_pos = max_pos; p.tokens = tokens; p.hq = hq; p.hkv = hkv; p.block_size = block_size;
+  p.num_slots = num_blocks * block_size;
+  launch_pdl(partials ? kv4_write_kernel<true> : kv4_write_kernel<false>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
   return launch_ok();
 }
 
@@ -221,11 +351,9 @@ int xv_kv4_read(const void* k_cache, const void* v_cache, const int* slots, void
   if (int rc = check_cache(hkv, d, block_size, num_blocks)) return rc;
   if (misaligned(k_cache, 16) || misaligned(v_cache, 16) || misaligned(k_out, 16) || misaligned(v_out, 16))
     return XV_ERR_ALIGN;
-  const long long rows = static_cast<long long>(tokens) * hkv, blocks = (rows + 15) / 16;
-  if (blocks > 0x7fffffffLL) return XV_ERR_SHAPE;
-  launch_pdl(kv4_read_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
+  launch_pdl(kv4_read_kernel, dim3((static_cast<unsigned>(tokens) + 7) / 8), dim3(256), 0, stream,
              static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), slots,
-             static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), rows, hkv, block_size,
+             static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out), tokens, hkv, block_size,
              num_blocks * block_size, status);
   return launch_ok();
 }
