@@ -39,18 +39,25 @@ __device__ __forceinline__ T half_sum(T v) {
   return v;
 }
 
+// a / b rounded correctly, from the correctly rounded 1 / b: one step of the remainder on the product (P. Markstein,
+// IBM J. Res. Dev. 34, 1990). Below 2^-102 the remainder underflows and the last bit may be off.
+__device__ __forceinline__ float quotient(float a, float b, float r_b) {
+  const float q = __fmul_rn(a, r_b);
+  return __fmaf_rn(__fmaf_rn(-q, b, a), r_b, q);
+}
+
 // Half a warp holds a head's row: lane c (0..15) channels 4c .. 4c + 3 in x[0..3] and 64 + 4c .. in x[4..7], so that rotary
 // partners meet in a lane and all eight channels are of group (c >> 1) & 1.
 //
 // Stores one row of bf16 values. ops/kv4.py fixes the arithmetic; the explicit _rn forms keep it under the library's
-// fast-math flags. A code is the quotient (x - centre) / step rounded to even: from the product with 1 / step, corrected
-// by its exact remainder (ties are common: both are bf16).
+// fast-math flags. A code is the quotient (x - centre) / step rounded to even, and ties are common (both are bf16), so
+// the quotient has to be the correctly rounded one.
 __device__ __forceinline__ void store_row(uint8_t* unit, int r, int c, unsigned half_mask, const float (&x)[8], bool there) {
   float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
   float mn = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
-  // NaN or infinite anywhere: x - x is not 0
-  const float odd = ((x[0] - x[0]) + (x[1] - x[1])) + ((x[2] - x[2]) + (x[3] - x[3])) + ((x[4] - x[4]) + (x[5] - x[5])) +
-                    ((x[6] - x[6]) + (x[7] - x[7]));
+  float odd = 0.f;                                            // NaN if any value is NaN or infinite
+#pragma unroll
+  for (int i = 0; i < 8; ++i) odd = __fmaf_rn(x[i], 0.f, odd);
 #pragma unroll
   for (int o = 1; o <= 8; o <<= 1) {
     if (o == 2) continue;                                     // lane bit 1 is the group
@@ -59,24 +66,24 @@ __device__ __forceinline__ void store_row(uint8_t* unit, int r, int c, unsigned 
   }
   const uint32_t not_fine = __ballot_sync(0xffffffffu, !(odd == 0.f));
   const bool bad = (not_fine & half_mask & ((c & 2) ? 0xccccccccu : 0x33333333u)) != 0;
-  float s = round_bf16(__fdiv_rn(__fsub_rn(0.5f * mx, 0.5f * mn), 7.5f));
+  float s = round_bf16(quotient(__fsub_rn(0.5f * mx, 0.5f * mn), 7.5f, 1.f / 7.5f));
   if (s < 1.17549435e-38f) s = 0.f;
   const float cen = round_bf16(__fadd_rn(__fadd_rn(0.5f * mx, 0.5f * mn), 0.5f * s));
-  const float r_s = s > 0.f ? __frcp_rn(s) : 0.f;
-  constexpr float kRound = 12582912.f;                        // 1.5 2^23: adding it leaves an integer in the low bits
+  // 1 / s is rounded correctly too: the step leaves an error of 2^-42, and no reciprocal of an 8-bit s is within 2^-33 of a tie.
+  const float r0 = __fdividef(1.f, s);
+  const float r_s = s > 0.f ? __fmaf_rn(__fmaf_rn(-s, r0, 1.f), r0, r0) : 0.f;
+  // 1.5 2^23 + 8: adding it rounds to an integer, even on ties, and leaves code = integer + 8 in the low bits.
+  constexpr float kRound = 12582920.f;
+  constexpr uint32_t kBits = 0x4B400000u;                     // of 1.5 2^23
   uint32_t code[2] = {0u, 0u};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = __fsub_rn(x[i], cen);
-    float m = __fadd_rn(fminf(fmaxf(a * r_s, -8.f), 7.f), kRound);
-    const float n = __fsub_rn(m, kRound);
-    const float d = __fmaf_rn(-n, s, a);                      // exact: how far the quotient is from n, in steps of s
-    const float over = __fmaf_rn(2.f, fabsf(d), -s);          // > 0: n is not the nearest; 0: a tie
-    const bool move = over > 0.f || (over == 0.f && (__float_as_uint(m) & 1u));
-    if (move) m = __fadd_rn(m, d < 0.f ? -1.f : 1.f);
-    m = fminf(fmaxf(m, kRound - 8.f), kRound + 7.f);
-    code[i >> 2] |= ((__float_as_uint(m) + 8u) & 15u) << (4 * (i & 3));
+  for (int i = 7; i >= 0; --i) {
+    const float t = quotient(__fsub_rn(x[i], cen), s, r_s);
+    const float m = __fadd_rn(fminf(fmaxf(t, -8.f), 7.f), kRound);
+    code[i >> 2] = code[i >> 2] * 16u + __float_as_uint(m);   // the constant part of four of them comes off at the end
   }
+  code[0] -= kBits * 0x1111u;
+  code[1] -= kBits * 0x1111u;
   if (bad || s == 0.f) code[0] = code[1] = 0x8888u;
   if (there) {
     uint8_t* row = unit + r * kv4::kCodeRow + c * 2;
@@ -86,6 +93,11 @@ __device__ __forceinline__ void store_row(uint8_t* unit, int r, int c, unsigned 
       *reinterpret_cast<uint32_t*>(unit + kv4::kParBase + r * kv4::kParRow + c * 2) = bad ? 0x7fff7fffu : pack_bf16(s, cen);
   }
 }
+
+// Warps of a block of the writer. K's warps take longer than Q's, and a block holds its place until its last one ends:
+// 8192 rows (32 + 2 x 8 heads), written and read back, take 62.7 us with eight warps to a block, 59.6 with two and 57.5
+// with one. 64 registers, for 32 warps an SM, are the best too (28: 59.6 us, 24: 63.4; 40 spill: 76).
+constexpr int kWriteWarps = 1;
 
 // What a launch writes and where.
 struct WriteParams {
@@ -108,11 +120,11 @@ struct WriteParams {
 };
 
 template <bool PLANES>
-__global__ void __launch_bounds__(256, 3) kv4_write_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_kernel(const WriteParams p) {
   grid_dep_launch();
   grid_dep_wait();
   constexpr int D = kv4::kD, HALF = D / 2;
-  const int warp = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int warp = blockIdx.x * kWriteWarps + (threadIdx.x >> 5);
   const int t = warp / p.tasks, task = warp - t * p.tasks;
   if (t >= p.tokens) return;
   const int lane = threadIdx.x & 31, c = lane & 15, half = lane >> 4;
@@ -324,7 +336,7 @@ int xv_kv4_write(const void* qkv, const float* partials, int splits, long long s
   p.per_warp = static_cast<int>(std::max(1ll, std::min(8ll, static_cast<long long>(tokens) * (q_pairs + kv_pairs) / (148 * 48))));
   p.q_tasks = (q_pairs + p.per_warp - 1) / p.per_warp;
   p.tasks = p.q_tasks + (kv_pairs + p.per_warp - 1) / p.per_warp;
-  const long long blocks = (static_cast<long long>(tokens) * p.tasks + 7) / 8;
+  const long long blocks = (static_cast<long long>(tokens) * p.tasks + kWriteWarps - 1) / kWriteWarps;
   if (blocks > 0x0fffffffLL) return XV_ERR_SHAPE;
   p.qkv = static_cast<const __nv_bfloat16*>(qkv);
   p.planes = partials;
@@ -341,7 +353,7 @@ int xv_kv4_write(const void* qkv, const float* partials, int splits, long long s
   p.eps = eps;
   p.splits = splits; p.max_pos = max_pos; p.tokens = tokens; p.hq = hq; p.hkv = hkv; p.block_size = block_size;
   p.num_slots = num_blocks * block_size;
-  launch_pdl(partials ? kv4_write_kernel<true> : kv4_write_kernel<false>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
+  launch_pdl(partials ? kv4_write_kernel<true> : kv4_write_kernel<false>, dim3(static_cast<unsigned>(blocks)), dim3(kWriteWarps * 32), 0, stream, p);
   return launch_ok();
 }
 
