@@ -187,13 +187,12 @@ def _attend(q_lens, kv_lens, hq, hkv, bs=16, n_decode=0, seed=0, poison=False, q
     ref, mag, swing, qk = kv4_ref.attention(q, k, v, q_lens, kv_lens, table, scale, hq)
     got = out.double().cpu().numpy().reshape(T, hq, D)
     qk = qk[..., None]
-    # Decode rows: the output and P s_g are each rounded to bf16 once; scores are fp32 sums of at most 2 * 64 products
-    # no larger than 17 times those of q and k (codes biased by 136), so 2^-24 * 17 * 8 bounds their relative error.
+    # Decode rows: the output is rounded to bf16 and P s_g to fp16 once (held to bf16's bound here); scores are fp32 sums
+    # of at most 2 * 64 products no larger than 17 times those of q and k, so 2^-24 * 17 * 8 bounds their relative error.
     tol = HALF_BF16 * (np.abs(ref) + swing) + 2 * (2.0 ** -24 * 17 * 8 * qk + 2.0 ** -20) * mag
-    # Chunks: K, V and P are rounded to fp16 (a value c + s (n - 8) after its s and c: three roundings of 2^-11 of magnitudes
-    # no larger than |x| + 2 |s (n - 8)|; a score then moves by 2^-11 of sum |q| |k|, a probability by twice that) and the
-    # output to bf16. `mag` stands for sum p |v| and is at least a third of sum p (|v| + 2 |s (n - 8)|) for these caches' rows
-    # by a margin of two: 2^-9 is allowed.
+    # Chunks: K, V and P are each rounded to fp16 once, c + s (n - 8) from an exact n - 8, with s and c exact (8 bits): a
+    # score moves by at most 2^-11 of sum |q| |k|, a probability by twice that, V and P by 2^-11 of p |v| each. The output is
+    # rounded to bf16.
     chunk = HALF_BF16 * np.abs(ref) + 2.0 ** -9 * (mag + swing) + (np.exp(2.0 ** -9 * qk) - 1) * mag + 2.0 ** -18 * mag
     tol[n_decode:] = chunk[n_decode:]
     worst = (np.abs(got - ref) - tol).max()

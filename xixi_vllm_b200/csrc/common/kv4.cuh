@@ -4,8 +4,8 @@
 // low nibble of byte i), then 16 rows of parameters (bf16 s0, c0, s1, c1). Eight channels are one 32-bit word; even
 // words form group 0, odd words group 1; a channel stands for c_g + s_g * (code - 8).
 //
-// Integers on the tensor pipe: (word >> 4j) & 0x000f000f | 0x43004300 is the bf16 pair {128 + n_j, 128 + n_(j+4)}
-// (bf16 holds the integers up to 256 exactly), one LOP3 per two channels and no table. Minus 136 it is n - 8, exact.
+// Values from codes: (word >> 4j) & 0x000f000f | 0x43004300 is the bf16 pair {128 + n_j, 128 + n_(j+4)} (bf16 holds the
+// integers up to 256 exactly), one LOP3 per two channels and no table. Minus 136 it is n - 8, exact.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -22,7 +22,6 @@ constexpr int kRow = kCodeRow + kParRow;
 constexpr int kParBase = kUnit * kCodeRow;                 // offset of a unit's parameters
 constexpr int kUnitBytes = kUnit * kRow;                   // 1152
 constexpr uint32_t kMagic = 0x43004300u;                   // bf16 {128, 128}
-constexpr float kBias = 136.f;                             // 128 + 8
 
 // Byte offset of the unit that holds token `r` of page `blk` for KV head `h`.
 __device__ __forceinline__ size_t unit_offset(int blk, int h, int hkv, int block_size, int r) {
@@ -30,7 +29,7 @@ __device__ __forceinline__ size_t unit_offset(int blk, int h, int hkv, int block
 }
 
 // bf16 pair {128 + nibble j of the low half, 128 + the same of the high half}, shift = 4j. The and-or is spelled as the
-// one LOP3 it is: from C operators the compiler makes two (496 -> 424 instructions a unit in the decode kernel).
+// one LOP3 it is: from C operators the compiler makes two.
 __device__ __forceinline__ uint32_t biased(uint32_t w, int shift) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w >> shift), "r"(0x000f000fu), "r"(kMagic));

@@ -5,18 +5,20 @@
 //                        cp.async a lane for K and V of a unit; no block-wide barrier in the loop). Tokens are the M rows
 //                        of both products and the group's query heads (up to 8, or 16 as two column tiles) the N
 //                        columns, so one MMA covers 16 x 16 cache values:
-//                          S^T[token, head] = s_g * (n Q^T) + c_g * sum(Q)   per channel group g
-//                          O^T[channel, head] = (n - 8)^T (s_g P) + c_g^T P
-//                        The MMAs see the codes as exact bf16 integers; scales and centres stay in fp32 (the scale of V
-//                        is folded into P before its one rounding to bf16). K's lanes own 16-byte pieces of a row, V's
-//                        lanes pair two tokens with PRMT, so codes go from shared memory to MMA operands in registers.
-//                        Warps are merged through shared memory, splits through the cluster's distributed shared
-//                        memory: one launch, no workspace.
+//                          S^T[token, head] = s_g * (n Q^T) + (c_g - 8 s_g) * sum(Q)   per channel group g
+//                          O^T[channel, head] = n^T (s_g P) - 8 sum(s_g P) + c_g^T P
+//                        The MMAs are fp16 and see the codes exactly, as the subnormals n 2^-24 and n 2^-20 that the
+//                        nibbles are where they stand, so a code costs an AND (and every second byte of K a shift).
+//                        Scales and centres stay in fp32; the scale of V is folded into P before its one rounding to
+//                        fp16. K's lanes own 16-byte pieces of a row, V's lanes pair two tokens with PRMT, so codes
+//                        go from shared memory to MMA operands in registers. Warps are merged through shared memory,
+//                        splits through the cluster's distributed shared memory: one launch, no workspace.
 //   kv4_share_kernel   - the same arithmetic for large or ragged batches: all units dealt to the warps in equal runs,
 //   kv4_join_kernel      partial results of pairs that span runs joined by a second kernel.
 // Prompt chunks: attn_prefill_kv4_sm100.cu.
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
@@ -45,6 +47,7 @@ struct Params {
   __nv_bfloat16* out;
   int* status;
   int hq, hkv, block_size, max_blocks, num_blocks, splits;
+  int max_tokens;                        // that a block table can name; 32-bit sums of a unit more must not wrap
   float scale_log2;
 };
 
@@ -61,10 +64,9 @@ __device__ __forceinline__ int page_of(const Params& p, int b, int entry) {
 // Cached tokens of a sequence, never more than its block table can name.
 __device__ __forceinline__ int kv_len_of(const Params& p, int b) {
   const int n = p.kv_lens[b];
-  const long long most = static_cast<long long>(p.max_blocks) * p.block_size;
-  if (n > most) {
-    if (threadIdx.x == 0) report_status(p.status, kIdDecode, kBadIndex);
-    return static_cast<int>(most);
+  if (n > p.max_tokens) {
+    report_status(p.status, kIdDecode, kBadIndex);
+    return p.max_tokens;
   }
   return n < 0 ? 0 : n;
 }
@@ -95,6 +97,8 @@ constexpr int kUnitSlot = 2 * kv4::kUnitBytes;
 constexpr int kSlot = kPair * kUnitSlot;
 constexpr float kNoMax = -3.0e38f;       // finite, so that "nothing seen yet" needs no case of its own
 constexpr float kLazy = 8.f;             // log2 units a running maximum may lag behind
+constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;      // nibbles as fp16: n 2^-24, n 2^-20 (subnormals)
+constexpr uint32_t kMinus8 = 0x80088008u;                        // fp16 -8 2^-24
 
 constexpr int decode_smem(int warps) { return warps * kStages * kSlot; }
 
@@ -104,8 +108,8 @@ __device__ __forceinline__ void store_out(__nv_bfloat16* dst, const float4& v, f
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
 }
 
-// D = A B: the first product of an accumulation.
-__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// D = A B on bf16: the centres' share of a score.
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%10, %10, %10, %10};"
@@ -113,41 +117,84 @@ __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// D += A B. Unlike ptx.cuh's form not volatile: the two units of a slot may be interleaved.
+// D = A B on fp16, and D += A B. Unlike ptx.cuh's forms not volatile: the two units of a slot may be interleaved.
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_more(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }       // e in -126 .. 127
+
 // The group's queries as B operands. NT: column tiles of 8 query heads.
 template <int NT>
 struct Query {
-  // MMA (word w, half hf) of lane (g, t) multiplies channels 32 t + 8 w + 2 hf + {0, 4, 1, 5}.
+  // MMA (word w, half hf) of lane (g, t) multiplies channels 32 t + 8 w + 2 hf + {0, 4, 1, 5}. Q is held in fp16, scaled by
+  // a power of two that takes the group's largest value to 2^14 .. 2^15 (exact down to 2^-28 of it); the odd channels meet
+  // codes that are 16 times too large and carry another 1 / 16.
   uint32_t f[NT][4][2][2];
-  // The centres' share of a score, sum over groups of c_g Qs_g - 136 s_g Qs_g with Qs_g the group's sum of Q, is one more
-  // MMA: its A operand is the parameter words as stored, its B operand {-136 Qs_g, Qs_g} as three bf16 terms (24 bits).
+  // The centres' share of a score, sum over groups of c_g Qs_g - 8 s_g Qs_g with Qs_g the group's sum of Q, is one more
+  // MMA: its A operand is the parameter words as stored, its B operand {-8 Qs_g, Qs_g} as three bf16 terms (24 bits).
   uint32_t c[NT][2];
+  float unit;                          // a score over what the MMAs make of it
 
-  // `row`: sequence * hq + first query head of the group; `flip`: sign bits to apply to Q.
-  __device__ __forceinline__ void load(const Params& p, size_t row, int G, uint32_t flip, int g, int t) {
+  // `row`: sequence * hq + first query head of the group; `sign`: applied to Q.
+  __device__ __forceinline__ void load(const Params& p, size_t row, int G, float sign, int g, int t) {
+    uint32_t raw[NT][16], top = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int head = nt * 8 + g;
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (row + head) * kD + 32 * t);
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (row + nt * 8 + g) * kD + 32 * t);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint4 r = nt * 8 + g < G ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
+        raw[nt][4 * w] = r.x; raw[nt][4 * w + 1] = r.y; raw[nt][4 * w + 2] = r.z; raw[nt][4 * w + 3] = r.w;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = __vmaxu2(top, raw[nt][i] & 0x7fff7fffu);
+    }
+    uint32_t most = max(top >> 16, top & 0xffffu);
+    if (__any_sync(0xffffffffu, most >= 0x7f80u)) {        // infinities and NaN do not choose the scale of the other heads
+      most = 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t lo = raw[nt][i] & 0x7fffu, hi = (raw[nt][i] >> 16) & 0x7fffu;
+          most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+        }
+    }
+    const int e = max(static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14, -80);
+    unit = power_of_two(e) * 16777216.f;                   // the codes are n 2^-24
+    const float even = power_of_two(-e) * sign, odd = even * 0.0625f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const uint4 raw = head < G ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
-        const uint32_t r[4] = {raw.x ^ flip, raw.y ^ flip, raw.z ^ flip, raw.w ^ flip};
+        float x[8];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          f[nt][w][hf][0] = __byte_perm(r[hf], r[hf + 2], 0x5410);     // channels 2 hf, 2 hf + 4
-          f[nt][w][hf][1] = __byte_perm(r[hf], r[hf + 2], 0x7632);     // channels 2 hf + 1, 2 hf + 5
+        for (int i = 0; i < 4; ++i) {
+          x[2 * i] = __uint_as_float(raw[nt][4 * w + i] << 16);
+          x[2 * i + 1] = __uint_as_float(raw[nt][4 * w + i] & 0xffff0000u);
+          sum[w & 1] += x[2 * i] + x[2 * i + 1];
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[w & 1] += __uint_as_float(r[i] << 16) + __uint_as_float(r[i] & 0xffff0000u);
+        for (int hf = 0; hf < 2; ++hf) {
+          f[nt][w][hf][0] = pack_f16(x[2 * hf] * even, x[2 * hf + 4] * even);
+          f[nt][w][hf][1] = pack_f16(x[2 * hf + 1] * odd, x[2 * hf + 5] * odd);
+        }
       }
 #pragma unroll
       for (int gr = 0; gr < 2; ++gr) {
@@ -156,7 +203,7 @@ struct Query {
       }
       // Lane (g, t) holds K rows 2t, 2t + 1 of B (first register) and 2t + 8, 2t + 9 (second): group t & 1; the first
       // term for t < 2, the second for t >= 2, the third in the second register for t < 2.
-      const float qs = (t & 1) ? sum[1] : sum[0], bs = -kv4::kBias * qs;
+      const float qs = ((t & 1) ? sum[1] : sum[0]) * even * 5.9604644775390625e-08f, bs = -8.f * qs;      // 2^-24
       const float q1 = __bfloat162float(__float2bfloat16(qs)), b1 = __bfloat162float(__float2bfloat16(bs));
       const float q2 = __bfloat162float(__float2bfloat16(qs - q1)), b2 = __bfloat162float(__float2bfloat16(bs - b1));
       c[nt][0] = t < 2 ? pack_bf16(b1, q1) : pack_bf16(b2, q2);
@@ -170,9 +217,13 @@ template <int NT>
 struct Softmax {
   float o[NT][2][4][4];            // [group][MMA]: rows g, g + 8 = channels 16 g + 8 group + 2 i + {0, 1}; heads 2t, 2t+1
   float cen[NT][2][2];             // sum of P * centre, this lane's tokens
+  float off[NT][4];                // sum of -8 P * s, rounded as it is in o: group 0 (heads 2t, 2t + 1), group 1
   float m[NT][2], l[NT][2];        // running maximum of the unscaled scores (may lag), sum of P of this lane's tokens
+  float vs, v_most;                // power of two that V's scales are multiplied by; the largest scale that it allows
 
   __device__ __forceinline__ void clear() {
+    vs = 1.f;
+    v_most = 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -181,6 +232,7 @@ struct Softmax {
         for (int i = 0; i < 4; ++i) o[nt][gr][i][0] = o[nt][gr][i][1] = o[nt][gr][i][2] = o[nt][gr][i][3] = 0.f;
         cen[nt][gr][0] = cen[nt][gr][1] = 0.f;
       }
+      off[nt][0] = off[nt][1] = off[nt][2] = off[nt][3] = 0.f;
       m[nt][0] = m[nt][1] = kNoMax;
       l[nt][0] = l[nt][1] = 0.f;
     }
@@ -197,17 +249,18 @@ struct Softmax {
       const uint2 kp0 = *reinterpret_cast<const uint2*>(lane_p + u * kUnitSlot);
       const uint2 kp1 = *reinterpret_cast<const uint2*>(lane_p + u * kUnitSlot + 64);
       const uint32_t ka[4] = {k0.x, k0.y, k0.z, k0.w}, kb[4] = {k1.x, k1.y, k1.z, k1.w};
-      const uint32_t w0 = (t & 1) ? kp0.y : kp0.x, w1 = (t & 1) ? kp1.y : kp1.x;
+      const uint32_t w0 = *reinterpret_cast<const uint32_t*>(lane_p + u * kUnitSlot + (t & 1) * 4);
+      const uint32_t w1 = *reinterpret_cast<const uint32_t*>(lane_p + u * kUnitSlot + (t & 1) * 4 + 64);
       const uint32_t ac[4] = {w0, w1, w0, w1};
       float s[NT][2][4], sc[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_first(sc[nt], ac, q.c[nt][0], q.c[nt][1]);
+      for (int nt = 0; nt < NT; ++nt) mma_bf16(sc[nt], ac, q.c[nt][0], q.c[nt][1]);
 #pragma unroll
       for (int w = 0; w < 4; ++w)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          const uint32_t a[4] = {kv4::biased(ka[w], 8 * hf), kv4::biased(kb[w], 8 * hf), kv4::biased(ka[w], 8 * hf + 4),
-                                 kv4::biased(kb[w], 8 * hf + 4)};
+          const uint32_t wa = ka[w] >> (8 * hf), wb = kb[w] >> (8 * hf);
+          const uint32_t a[4] = {wa & kLow, wb & kLow, wa & kHigh, wb & kHigh};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             if (w < 2 && hf == 0) mma_first(s[nt][w], a, q.f[nt][w][hf][0], q.f[nt][w][hf][1]);
@@ -232,7 +285,20 @@ struct Softmax {
           if (16 * u + tok + 8 >= mine) x[u][nt][2] = x[u][nt][3] = -CUDART_INF_F;
         }
     }
-    bool grow = false;
+    uint2 vp[kPair][2];                  // V's parameters of this lane's tokens
+    float s_most = 0.f;
+#pragma unroll
+    for (int u = 0; u < kPair; ++u) {
+      vp[u][0] = *reinterpret_cast<const uint2*>(lane_p + u * kUnitSlot + kv4::kUnitBytes);
+      vp[u][1] = *reinterpret_cast<const uint2*>(lane_p + u * kUnitSlot + kv4::kUnitBytes + 64);
+      if (ragged) {                      // P is 0 there, and whatever parameters an earlier owner of the page left (NaN
+        if (16 * u + tok >= mine) vp[u][0] = make_uint2(0u, 0u);     // among them) must not reach the sums; codes are
+        if (16 * u + tok + 8 >= mine) vp[u][1] = make_uint2(0u, 0u); // always finite
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) s_most = fmaxf(s_most, fmaxf(fabsf(kv4::par_s(vp[u][r].x)), fabsf(kv4::par_s(vp[u][r].y))));
+    }
+    bool grow = s_most > v_most;
     float mx[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -242,6 +308,17 @@ struct Softmax {
         grow |= mx[nt][hd] > m[nt][hd] + lag;
       }
     if (__any_sync(0xffffffffu, grow)) {
+      float back = 1.f;                  // of the sums of P * s
+      s_most = fmaxf(s_most, __shfl_xor_sync(0xffffffffu, s_most, 4));
+      s_most = fmaxf(s_most, __shfl_xor_sync(0xffffffffu, s_most, 8));
+      s_most = fmaxf(s_most, __shfl_xor_sync(0xffffffffu, s_most, 16));
+      if (s_most > v_most) {
+        const int e = min(max((__float_as_int(s_most) >> 23) - 127 - 2, -120), 119);
+        const float now = power_of_two(-e);
+        back = now / vs;
+        vs = now;
+        v_most = power_of_two(e + 7);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -256,28 +333,31 @@ struct Softmax {
 #pragma unroll
           for (int gr = 0; gr < 2; ++gr) {
             cen[nt][gr][hd] *= cr;
+            off[nt][2 * gr + hd] *= cr * back;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              o[nt][gr][j][hd] *= cr;
-              o[nt][gr][j][2 + hd] *= cr;
+              o[nt][gr][j][hd] *= cr * back;
+              o[nt][gr][j][2 + hd] *= cr * back;
             }
           }
         }
     }
 #pragma unroll
     for (int u = 0; u < kPair; ++u) {
-      uint2 vp0 = *reinterpret_cast<const uint2*>(lane_p + u * kUnitSlot + kv4::kUnitBytes);
-      uint2 vp1 = *reinterpret_cast<const uint2*>(lane_p + u * kUnitSlot + kv4::kUnitBytes + 64);
       uint2 vw[4];                       // tokens of rows 2t, 2t + 1, then the same 8 further
       vw[0] = *reinterpret_cast<const uint2*>(lane_v0 + u * kUnitSlot);
       vw[1] = *reinterpret_cast<const uint2*>(lane_v1 + u * kUnitSlot);
       vw[2] = *reinterpret_cast<const uint2*>(lane_v0 + u * kUnitSlot + 8 * 64);
       vw[3] = *reinterpret_cast<const uint2*>(lane_v1 + u * kUnitSlot + 8 * 64);
-      if (ragged) {                      // P is 0 there, and whatever parameters an earlier owner of the page left (NaN
-        if (16 * u + tok >= mine) vp0 = make_uint2(0u, 0u);        // among them) must not reach the sums; codes are
-        if (16 * u + tok + 8 >= mine) vp1 = make_uint2(0u, 0u);    // always finite
-      }
-      const uint32_t vpar[2][2] = {{vp0.x, vp1.x}, {vp0.y, vp1.y}};
+      float vsc[2][2], vce[2][2];        // [group][token g, g + 8]: s (scaled) and c
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr) {
+          const uint32_t w = gr ? vp[u][r].y : vp[u][r].x;
+          vsc[gr][r] = kv4::par_s(w) * vs;
+          vce[gr][r] = kv4::par_c(w);
+        }
       uint32_t pf[NT][2][2];             // P * s_g as the B operand of the second product
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -288,36 +368,33 @@ struct Softmax {
         l[nt][1] += pr[1] + pr[3];
 #pragma unroll
         for (int gr = 0; gr < 2; ++gr) {
-          const float s0 = kv4::par_s(vpar[gr][0]), s1 = kv4::par_s(vpar[gr][1]);
-          pf[nt][gr][0] = movmatrix_trans(pack_bf16(pr[0] * s0, pr[1] * s0));
-          pf[nt][gr][1] = movmatrix_trans(pack_bf16(pr[2] * s1, pr[3] * s1));
-          const float c0 = kv4::par_c(vpar[gr][0]), c1 = kv4::par_c(vpar[gr][1]);
-          cen[nt][gr][0] += pr[0] * c0 + pr[2] * c1;
-          cen[nt][gr][1] += pr[1] * c0 + pr[3] * c1;
+          pf[nt][gr][0] = movmatrix_trans(pack_f16(pr[0] * vsc[gr][0], pr[1] * vsc[gr][0]));
+          pf[nt][gr][1] = movmatrix_trans(pack_f16(pr[2] * vsc[gr][1], pr[3] * vsc[gr][1]));
+          cen[nt][gr][0] = fmaf(pr[0], vce[gr][0], fmaf(pr[2], vce[gr][1], cen[nt][gr][0]));
+          cen[nt][gr][1] = fmaf(pr[1], vce[gr][0], fmaf(pr[3], vce[gr][1], cen[nt][gr][1]));
         }
       }
 #pragma unroll
       for (int gr = 0; gr < 2; ++gr) {
         const uint32_t w0 = gr ? vw[0].y : vw[0].x, w1 = gr ? vw[1].y : vw[1].x, w2 = gr ? vw[2].y : vw[2].x,
                        w3 = gr ? vw[3].y : vw[3].x;
+        const uint32_t a8[4] = {gr ? 0u : kMinus8, gr ? kMinus8 : 0u, gr ? 0u : kMinus8, gr ? kMinus8 : 0u};
 #pragma unroll
-        for (int hl = 0; hl < 2; ++hl) {               // low / high half of the word: channels 0-3 / 4-7
-          const uint32_t sel = hl ? 0x7632 : 0x5410;
-          const uint32_t u0 = __byte_perm(w0, w1, sel), u1 = __byte_perm(w2, w3, sel);
+        for (int nt = 0; nt < NT; ++nt) mma_more(off[nt], a8, pf[nt][gr][0], pf[nt][gr][1]);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t a[4] = {kv4::centred(kv4::biased(u0, 8 * j)), kv4::centred(kv4::biased(u0, 8 * j + 4)),
-                                   kv4::centred(kv4::biased(u1, 8 * j)), kv4::centred(kv4::biased(u1, 8 * j + 4))};
+        for (int i = 0; i < 4; ++i) {                  // byte of the word: channels 2 i, 2 i + 1
+          const uint32_t u0 = __byte_perm(w0, w1, 0x4400 + 0x1111 * i), u1 = __byte_perm(w2, w3, 0x4400 + 0x1111 * i);
+          const uint32_t a[4] = {u0 & kLow, u0 & kHigh, u1 & kLow, u1 & kHigh};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_more(o[nt][gr][hl * 2 + j], a, pf[nt][gr][0], pf[nt][gr][1]);
-          }
+          for (int nt = 0; nt < NT; ++nt) mma_more(o[nt][gr][i], a, pf[nt][gr][0], pf[nt][gr][1]);
         }
       }
     }
   }
 
   // Sums over the lanes of equal t; the centres join the outputs. Then every lane holds, for its two heads, 16 channels.
-  __device__ __forceinline__ void finish() {
+  __device__ __forceinline__ void finish(float unit) {
+    const float back = 1.f / vs;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -332,9 +409,12 @@ struct Softmax {
         for (int gr = 0; gr < 2; ++gr)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            o[nt][gr][i][hd] += cen[nt][gr][hd];
-            o[nt][gr][i][2 + hd] += cen[nt][gr][hd];
+            const float even = (o[nt][gr][i][hd] + off[nt][2 * gr + hd]) * 16777216.f;                 // codes n 2^-24
+            const float odd = fmaf(o[nt][gr][i][2 + hd], 0.0625f, off[nt][2 * gr + hd]) * 16777216.f;  // n 2^-20
+            o[nt][gr][i][hd] = fmaf(even, back, cen[nt][gr][hd]);
+            o[nt][gr][i][2 + hd] = fmaf(odd, back, cen[nt][gr][hd]);
           }
+        m[nt][hd] = m[nt][hd] == kNoMax ? kNoMax : m[nt][hd] * unit;
       }
   }
   // Channels 16 g + 4 j .. + 3 of head (nt, hd) after finish().
@@ -348,10 +428,10 @@ struct Softmax {
 // a slot: K's 1152 bytes, then V's; five cp.async of 16 bytes a lane (K's codes, V's codes, both parameter blocks by half
 // a warp). Pages are looked up 32 at a time, one batch ahead of use.
 struct Ring {
-  uint32_t dst, slot;
+  uint32_t dst, slot, p_to;
   int lane;
   // units still to fetch, and where they are
-  const uint8_t *k_src, *v_src;
+  const uint8_t *k_src, *v_src, *p_src;      // this lane's 16 bytes of K's codes, V's codes and the parameters in page 0
   uint32_t page_bytes;
   int b, left, place, upp, page0, page_i, last_page, pages, pages_next;
 
@@ -359,6 +439,7 @@ struct Ring {
     lane = lane_;
     upp = upp_;
     dst = smem_u32(ring) + lane * 16;
+    p_to = kv4::kParBase + (lane < 8 ? 0 : kv4::kUnitBytes - 128);
     slot = 0;
     left = 0;
     page_bytes = static_cast<uint32_t>(hkv) * upp * kv4::kUnitBytes;
@@ -377,6 +458,7 @@ struct Ring {
     const size_t head = static_cast<size_t>(h) * upp * kv4::kUnitBytes + lane * 16;
     k_src = p.k_cache + head;
     v_src = p.v_cache + head;
+    p_src = (lane < 8 ? k_src : v_src - 128) + kv4::kParBase;
     if (n > 0) {
       pages = lookup(p, lane);
       pages_next = lookup(p, 32 + lane);
@@ -402,8 +484,7 @@ struct Ring {
         cp_async16_u32(to + kv4::kUnitBytes, v_src + at);
         cp_async16_u32(to + kv4::kUnitBytes + 512, v_src + at + 512);
         if (lane < 16)
-          cp_async16_u32(to + kv4::kParBase + (lane < 8 ? 0 : kv4::kUnitBytes - 128),
-                         (lane < 8 ? k_src : v_src - 128) + at + kv4::kParBase);
+          cp_async16_u32(to + p_to, p_src + at);
         ++place;
         --left;
       }
@@ -415,9 +496,10 @@ struct Ring {
 
 // A negative scale is Q's sign, so the running maxima need not know it; zero becomes a scale too small to matter.
 struct Scale {
-  float scale, lag;
-  uint32_t flip;
-  __device__ __forceinline__ explicit Scale(float s) : scale(fmaxf(fabsf(s), 1e-30f)), lag(kLazy / scale), flip(s < 0.f ? 0x80008000u : 0u) {}
+  float scale, sign;
+  __device__ __forceinline__ explicit Scale(float s) : scale(fmaxf(fabsf(s), 1e-30f)), sign(s < 0.f ? -1.f : 1.f) {}
+  // For scores in units of Query::unit.
+  __device__ __forceinline__ float of(float unit) const { return fmaxf(scale * unit, 1e-36f); }
 };
 
 // A cluster of CTAs, one per KV split, per (sequence, KV head). NT: column tiles of 8 query heads; W: warps.
@@ -445,7 +527,8 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
   for (int i = 0; i < kStages - 1; ++i) ring.issue(p);
   const Scale sc(p.scale_log2);
   Query<NT> q;
-  q.load(p, static_cast<size_t>(b) * p.hq + h * G, G, sc.flip, g, t);
+  q.load(p, static_cast<size_t>(b) * p.hq + h * G, G, sc.sign, g, t);
+  const float scale = sc.of(q.unit), lag = kLazy / scale;
   Softmax<NT> st;
   st.clear();
 
@@ -457,13 +540,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
     __syncwarp();                        // everyone's part of the slot has landed, and everyone has read the slot filled next
     ring.issue(p);
     st.add(q, at + tok * 64 + t * 16, at + kv4::kParBase + tok * 8, at + kv4::kUnitBytes + token_of_row(2 * t) * 64 + g * 8,
-           at + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8, mine, tok, t, sc.scale, sc.lag);
+           at + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8, mine, tok, t, scale, lag);
     at = at == ring_mem + (kStages - 1) * kSlot ? ring_mem : at + kSlot;
   }
   cp_async_wait<0>();
 
   // The warps meet in the (now idle) ring.
-  st.finish();
+  st.finish(q.unit);
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(smem);                    // [warp][8 NT][128]
   float* part_o = sm_o + W * 8 * NT * kD;                          // [8 NT][128]
@@ -646,7 +729,8 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
   for (;;) {
     const int n = min(units - first, todo);
     Query<NT> q;
-    q.load(p, static_cast<size_t>(b) * p.hq + h * G, G, sc.flip, g, t);
+    q.load(p, static_cast<size_t>(b) * p.hq + h * G, G, sc.sign, g, t);
+    const float scale = sc.of(q.unit), lag = kLazy / scale;
     Softmax<NT> st;
     st.clear();
     int mine = min(kv_len - first * 16, n * 16);
@@ -655,10 +739,10 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
       __syncwarp();
       fetch();
       st.add(q, at + tok * 64 + t * 16, at + kv4::kParBase + tok * 8, at + kv4::kUnitBytes + token_of_row(2 * t) * 64 + g * 8,
-             at + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8, mine, tok, t, sc.scale, sc.lag);
+             at + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8, mine, tok, t, scale, lag);
       at = at == ring_mem + (kStages - 1) * kSlot ? ring_mem : at + kSlot;
     }
-    st.finish();
+    st.finish(q.unit);
     const bool whole = n == units;
     const int pair = b * p.hkv + h;
     const size_t slot = static_cast<size_t>(run) + pair;
@@ -694,19 +778,23 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
   cp_async_wait<0>();
 }
 
-// Joins the partial results of the pairs that several runs share, and clears the rows of empty sequences. A CTA per
-// (pair, query head); its warps take the partials in turn, a lane four channels.
-__global__ void kv4_join_kernel(const Params p, const Shares ws, int num_seqs, int rows) {
+// Joins the partial results of the pairs that several runs share, and clears the rows of empty sequences. R warps per
+// (pair, query head) take the partials in turn, BATCH at a time (the kernel is a chain of L2 round trips); a lane holds
+// four channels. A row's warps are one CTA; with one warp a row, four rows are.
+template <int R, int BATCH>
+__global__ void __launch_bounds__(R == 1 ? 128 : R * 32) kv4_join_kernel(const Params p, const Shares ws, int num_seqs, int rows) {
   grid_dep_launch();
   grid_dep_wait();
-  __shared__ float4 sm_o[16][32];
-  __shared__ float sm_m[16], sm_l[16];
+  __shared__ float4 sm_o[R][32];
+  __shared__ float sm_m[R], sm_l[R];
   const int G = p.hq / p.hkv;
-  const int pair = blockIdx.x, head = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int warp = R == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = R == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;      // sequence * hq + query head
+  if (row >= num_seqs * p.hq) return;
+  const int pair = row / G, head = row - pair * G;
   const int b = pair / p.hkv, h = pair - b * p.hkv;
   const int before = ws.begin[b], units = ws.begin[b + 1] - before, per = ws.begin[num_seqs + 1];
-  __nv_bfloat16* dst = p.out + (static_cast<size_t>(pair) * G + head) * kD + lane * 4;
+  __nv_bfloat16* dst = p.out + static_cast<size_t>(row) * kD + lane * 4;
   if (units == 0) {
     if (warp == 0) *reinterpret_cast<uint2*>(dst) = make_uint2(0u, 0u);
     return;
@@ -717,32 +805,50 @@ __global__ void kv4_join_kernel(const Params p, const Shares ws, int num_seqs, i
   const float scale = Scale(p.scale_log2).scale;
   float M = kNoMax, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int r = run0 + warp; r <= run1; r += warps) {
-    const size_t slot = (static_cast<size_t>(r) + pair) * rows + head;
-    const float2 ml = *reinterpret_cast<const float2*>(ws.ml + slot * 2);
-    const float4 v = *reinterpret_cast<const float4*>(ws.o + slot * kD + lane * 4);
-    const float mn = fmaxf(M, ml.x), f0 = exp2f((M - mn) * scale), f1 = exp2f((ml.x - mn) * scale);
+  for (int r = run0 + warp; r <= run1; r += BATCH * R) {
+    float2 ml[BATCH];
+    float4 v[BATCH];
+    float mn = M;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const bool there = r + i * R <= run1;
+      const size_t slot = (static_cast<size_t>(r + i * R) + pair) * rows + head;
+      ml[i] = there ? *reinterpret_cast<const float2*>(ws.ml + slot * 2) : make_float2(kNoMax, 0.f);
+      v[i] = there ? *reinterpret_cast<const float4*>(ws.o + slot * kD + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) mn = fmaxf(mn, ml[i].x);
+    const float f0 = exp2f((M - mn) * scale);
     M = mn;
-    L = L * f0 + ml.y * f1;
-    acc.x = acc.x * f0 + v.x * f1; acc.y = acc.y * f0 + v.y * f1;
-    acc.z = acc.z * f0 + v.z * f1; acc.w = acc.w * f0 + v.w * f1;
+    L *= f0;
+    acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float f = exp2f((ml[i].x - mn) * scale);
+      L += ml[i].y * f;
+      acc.x += v[i].x * f; acc.y += v[i].y * f; acc.z += v[i].z * f; acc.w += v[i].w * f;
+    }
   }
-  sm_o[warp][lane] = acc;
-  if (lane == 0) {
-    sm_m[warp] = M;
-    sm_l[warp] = L;
-  }
-  __syncthreads();
-  if (warp != 0) return;
-  for (int w = 0; w < warps; ++w) M = fmaxf(M, sm_m[w]);
-  L = 0.f;
-  acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int w = 0; w < warps; ++w) {
-    const float f = exp2f((sm_m[w] - M) * scale);
-    const float4 v = sm_o[w][lane];
-    L += sm_l[w] * f;
-    acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+  if constexpr (R > 1) {
+    sm_o[warp][lane] = acc;
+    if (lane == 0) {
+      sm_m[warp] = M;
+      sm_l[warp] = L;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    M = kNoMax;
+    L = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < R; ++w) M = fmaxf(M, sm_m[w]);
+#pragma unroll
+    for (int w = 0; w < R; ++w) {
+      const float f = exp2f((sm_m[w] - M) * scale);
+      const float4 v = sm_o[w][lane];
+      L += sm_l[w] * f;
+      acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+    }
   }
   store_out(dst, acc, L);
 }
@@ -763,6 +869,7 @@ int fill(Params& p, const void* q, const void* k_cache, const void* v_cache, con
   p.kv_lens = kv_lens;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.hq = hq; p.hkv = hkv; p.block_size = block_size; p.max_blocks = max_blocks; p.num_blocks = num_blocks;
+  p.max_tokens = static_cast<int>(std::min(static_cast<long long>(max_blocks) * block_size, 0x7ffffff0ll));
   p.scale_log2 = scale * kLog2e;
   p.status = status;
   return 0;
@@ -830,7 +937,7 @@ int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const
     return launch_ok();
   }
   const long long units = static_cast<long long>(max_blocks) * (block_size / kv4::kUnit);
-  if (units * num_seqs * hkv > 0x7fffffffLL || static_cast<long long>(num_seqs) * hkv > 0x7fffffffLL) return XV_ERR_SHAPE;
+  if (units * num_seqs * hkv > 0x7fffffffLL || static_cast<long long>(num_seqs) * hq > 0x7fffffffLL) return XV_ERR_SHAPE;
   if (!workspace || workspace_bytes < xv_kv4_decode_workspace_bytes(num_seqs, hq, hkv, 0, num_sms)) return XV_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return XV_ERR_ALIGN;
   const int ctas = share_ctas(num_sms, nt);
@@ -842,9 +949,14 @@ int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const
   launch_pdl(nt == 1 ? kv4_share_kernel<1> : kv4_share_kernel<2>, dim3(ctas), dim3(kShareWarps * 32), decode_smem(kShareWarps),
              stream, p, ws, num_seqs);
   if (int rc = launch_ok()) return rc;
-  // Few pairs have many partials each: more warps per row.
-  const int threads = num_seqs * hkv <= 64 ? 512 : 64;
-  launch_pdl(kv4_join_kernel, dim3(num_seqs * hkv, hq / hkv), dim3(threads), 0, stream, p, ws, num_seqs, 8 * nt);
+  // Warps per row by the partials that a pair may have, its share of the runs. Both kernels with 16 / 4 / 1 warps a row:
+  // 8 pairs (223 partials) 19.7 / 30.3 / 69.6 us, 32 (56) 27.3 / 29.7 / 40.6, 72 (25) 28.5 / 28.5 / 33.9, 160 (12)
+  // 54.6 / 49.9 / 52.5, 256 (7) 54.1 / 47.5 / 48.2, 512 (4) 81.3 / 69.2 / 68.1, 2048 (1) 187.9 / 144.7 / 138.2.
+  const int partials = ctas * kShareWarps / (num_seqs * hkv) + 1;
+  const unsigned rows = static_cast<unsigned>(num_seqs) * hq;
+  if (partials > 24) launch_pdl(kv4_join_kernel<16, 8>, dim3(rows), dim3(512), 0, stream, p, ws, num_seqs, 8 * nt);
+  else if (partials > 4) launch_pdl(kv4_join_kernel<4, 4>, dim3(rows), dim3(128), 0, stream, p, ws, num_seqs, 8 * nt);
+  else launch_pdl(kv4_join_kernel<1, 4>, dim3((rows + 3) / 4), dim3(128), 0, stream, p, ws, num_seqs, 8 * nt);
   return launch_ok();
 }
 
