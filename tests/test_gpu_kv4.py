@@ -252,6 +252,54 @@ def test_decode_growing_maxima():
     _attend([1, 1], [400, 700], 8, 1, n_decode=2, q_scale=8.0, seed=4)
 
 
+@pytest.mark.parametrize("extra_pages", [1, WIDE])
+@pytest.mark.parametrize("order", [(0, 1, 2), (2, 1, 0), (1, 2, 0)])
+def test_decode_values_of_mixed_magnitude(order, extra_pages):
+    """V rows of 2^-20, 1 and 2^20 times normal values behind rows that are constant, in runs that a warp meets one after
+    the other: the power of two that P * s is held in moves up. A term's rounding is at most half a step of fp16, 2^-11 of
+    it, or of the smallest subnormal, 2^-25 in units that the largest scale met so far is at least 2^2 of: relative to the
+    largest |v| (at least 2^-7 of it is in `mag`, a tenth of the weights being on such rows) 400 * 8 * 2^-27 / 12 is below 2^-18."""
+    hq, hkv, bs, n = 4, 1, 16, 400
+    nb = n // bs
+    g = torch.Generator().manual_seed(31)
+    k, v = (torch.zeros(nb, hkv, bs, kv4.row_bytes(D), dtype=torch.uint8) for _ in range(2))
+    size = torch.tensor([2.0 ** (20 * (order[t // 5 % 3] - 1)) for t in range(n)])[:, None, None]
+    values = torch.randn(n, hkv, D, generator=g) * size
+    values[:7] = 3.0
+    kv4.write_rows(k, torch.arange(n), torch.randn(n, hkv, D, generator=g))
+    kv4.write_rows(v, torch.arange(n), values)
+    q = (torch.randn(1, hq * D, generator=g) * 0.25).bfloat16()
+    table = torch.zeros(1, nb + extra_pages, dtype=torch.int32)
+    table[0, :nb] = torch.arange(nb)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    attn = AttnBatch(torch.tensor([0, 1], **i32), torch.tensor([n], **i32), table.to(DEV), 1, 1, 1, n, 1)
+    out = _ops().paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), attn, D ** -0.5, hq, hkv, D)
+    _cuda().check_status()
+    ref, mag, swing, qk = kv4_ref.attention(q, k, v, [1], [n], table, D ** -0.5, hq)
+    got = out.double().cpu().numpy().reshape(1, hq, D)
+    tol = HALF_BF16 * (np.abs(ref) + swing) + 2 * (2.0 ** -24 * 17 * 8 * qk[..., None] + 2.0 ** -18) * mag
+    assert ((np.abs(got - ref) - tol) <= 0).all()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("extra_pages", [1, WIDE])
+def test_decode_query_head_that_is_not_finite_stays_alone(bad, extra_pages):
+    k, v = _random(8, 2, 16, 3)
+    q = torch.randn(2, 8 * D, generator=torch.Generator().manual_seed(8)).bfloat16()
+    q[0, 2 * D + 5] = 0.0
+    i32 = dict(dtype=torch.int32, device=DEV)
+    table = torch.zeros(2, 4 + extra_pages, **i32)
+    table[0, :4], table[1, :4] = torch.arange(4, **i32), torch.arange(4, 8, **i32)
+    attn = AttnBatch(torch.tensor([0, 1, 2], **i32), torch.tensor([50, 61], **i32), table, 2, 2, 1, 61, 2)
+    clean = _ops().paged_attention(q.to(DEV), k, v, attn, 0.09, 8, 2, D)
+    q[0, 2 * D + 5] = bad
+    out = _ops().paged_attention(q.to(DEV), k, v, attn, 0.09, 8, 2, D)
+    _cuda().check_status()
+    assert not bool(out[0, 2 * D:3 * D].isfinite().any())
+    out[0, 2 * D:3 * D] = clean[0, 2 * D:3 * D]
+    assert torch.equal(out, clean)
+
+
 def test_rows_beyond_the_sequence_may_hold_nan():
     _attend([1, 1, 1, 20, 70], [1, 15, 33, 20, 100], 8, 2, n_decode=3, poison=True)
     _attend([1, 65], [47, 130], 4, 2, bs=48, n_decode=1, poison=True)
