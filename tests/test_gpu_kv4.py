@@ -402,6 +402,12 @@ def test_small_and_large_values():
     _attend([1, 30], [40, 60], 4, 2, n_decode=1, v_scale=2.0 ** 40, q_scale=2.0 ** -40)
 
 
+def test_scores_below_the_smallest_float_leave_equal_weights():
+    """The scale of a score underflows; what the mask takes out still has weight 0, not NaN."""
+    _attend([1, 30, 200], [40, 60, 200], 4, 2, n_decode=1, v_scale=2.0 ** -60, q_scale=2.0 ** -70)
+    _attend([1, 30, 200], [40, 60, 200], 4, 2, n_decode=1, v_scale=2.0 ** -40, q_scale=0.0)
+
+
 def _small(n_decode=2):
     k, v = _random(4, 2, 16, 0)
     i32 = dict(dtype=torch.int32, device=DEV)

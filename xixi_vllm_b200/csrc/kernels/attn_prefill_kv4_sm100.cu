@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   const int row0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * rpu;     // long ones first
   if (row0 >= q_len) return;
   int kv_len = max(p.kv_lens[b], 0);
-  const long long most = static_cast<long long>(p.max_blocks) * p.block_size;
+  const long long most = min(static_cast<long long>(p.max_blocks) * p.block_size, 0x7fffff00ll);   // a tile more stays 32-bit
   if (kv_len > most) {
     if (threadIdx.x == 0) report_status(p.status, kId, kBadIndex);
     kv_len = static_cast<int>(most);
@@ -273,8 +273,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         at[8] = ok ? 0u : 1u;
       }
     };
-    // Largest magnitude of a stored tile: 2^14 .. 2^15 when an exponent is chosen (smaller values of the tile then keep
-    // fp16's precision down to 2^-29 of it), kept while it stays in 2^7 .. 2^15.
+    // Largest magnitude of a stored tile: 2^12 .. 2^13 when an exponent is chosen (smaller values of the tile then keep
+    // fp16's precision down to 2^-26 of it), kept while it stays in 2^7 .. 2^15.
     auto choose = [](int e, uint32_t bits) {
       const int top = static_cast<int>(bits >> 23) - 127;
       if (bits != 0 && (top - e > 14 || top - e < 7)) e = top - 12;
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         mx[c] = fmax3(fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]), fmax3(a[6], a[7], a[8])),
                       fmax3(a[9], __uint_as_float(sr[c][30]), __uint_as_float(sr[c][31])), -INFINITY);
       }
-      const float scale = row_scale * ts.k;
+      const float scale = fmaxf(row_scale * ts.k, 1e-37f);   // never 0: it meets -inf
       const float mt = fmaxf(fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale, kNoMax);
       if (j == 0) {
         m = mt;
