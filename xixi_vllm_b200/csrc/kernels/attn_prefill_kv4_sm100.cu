@@ -45,7 +45,7 @@ constexpr int kBM = 128, kBN = 128;               // lanes of a unit, tokens of 
 constexpr int kHalf = kBN * 128;                  // bytes of 64 channels of a tile
 constexpr int kTileBytes = 2 * kHalf;             // 32 KiB
 constexpr int kNK = 3, kNV = 2;                   // ring slots
-constexpr int kBarBytes = 512 + 2 * kBM * 4;      // barriers and small arrays; a float per lane
+constexpr int kBarBytes = 512;                    // barriers and small arrays
 constexpr int kSmem = (2 + kNK + kNV) * kTileBytes + 1024 + kBarBytes;
 constexpr uint32_t kTmemCols = 512, kTmemUnit = 256, kTmemO = 128;
 constexpr int kId = 12;
@@ -185,7 +185,6 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   uint32_t* red = reinterpret_cast<uint32_t*>(scales + 8);   // [2][12]
   uint32_t* tmem_slot = red + 24;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* row_power = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);      // [2][128]
 
   if (threadIdx.x == 0) {
     for (int u = 0; u < 2; ++u) {
@@ -414,34 +413,50 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     // ---------------- softmax and output: thread r of unit u is query row r / G, head r % G ----------------
     set_regs_up<184>();
     const int u = wg, r = threadIdx.x & 127;
+    const int by_g = 65536 / G + 1;                          // lane / G as a product: exact for 128 lanes and G up to 16
     const int row = row0 + u * rpu + r / G;
     const int pos = pos0 + min(row, q_len - 1);              // lanes without a row follow the last one
-    // Q: a power of two per row keeps it in fp16's range; a negative scale is its sign. Sixteen lanes a row, two rows at a
-    // time, so that the reads are whole lines; the row's power goes to its own lane through shared memory.
+    // Q: a power of two per warp takes its largest element to 2^14 .. 2^15 of fp16, which is exact down to 2^-31 of it; a
+    // negative scale is its sign. Sixteen lanes a row, two rows at a time, so that the reads are whole lines.
+    float q_power;
     {
       const int c = lane & 15;
       uint4 v[16];                                           // all reads in flight at once
       {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4), rr = qr_ / G, hh = qr_ - rr * G;
+          const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4), rr = (qr_ * by_g) >> 16, hh = qr_ - rr * G;
           const int qrow = row0 + u * rpu + rr;
           const bool there = rr < rpu && qrow < q_len;
           v[i] = there ? __ldg(reinterpret_cast<const uint4*>(
                                    p.q + (static_cast<size_t>(q_begin + qrow) * p.hq + hk * G + hh) * kD) + c)
                        : make_uint4(0u, 0u, 0u, 0u);
         }
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          top = __vmaxu2(__vmaxu2(__vmaxu2(top, v[i].x & 0x7fff7fffu), __vmaxu2(v[i].y & 0x7fff7fffu, v[i].z & 0x7fff7fffu)),
+                         v[i].w & 0x7fff7fffu);
+        uint32_t most = max(top >> 16, top & 0xffffu);
+        if (__any_sync(0xffffffffu, most >= 0x7f80u)) {      // infinities and NaN do not choose the other rows' power
+          most = 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
+              most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+            }
+          }
+        }
+        const int e = max(-100, min(100, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14));
+        const float f = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
+        q_power = pow2(e);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4);
           const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};       // channels 0 1, 2 3, 4 5, 6 7 of the word
-          uint32_t top = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-#pragma unroll
-          for (int k = 1; k < 16; k <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, k));
-          const int e = max(-100, min(100, static_cast<int>(top >> 7) - 127));
-          const float f = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
           float x[8];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -450,14 +465,12 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
           }
           st_shared_v4(chunk_at(row_start(smem_u32(q_s) + u * kTileBytes, qr_), c), pack_f16(x[0], x[4]), pack_f16(x[1], x[5]),
                        pack_f16(x[2], x[6]), pack_f16(x[3], x[7]));
-          if (c == 0) row_power[u * kBM + qr_] = pow2(e);
         }
       }
       fence_proxy_async_smem();
       mbar_arrive(&q_full[u]);
-      __syncwarp();                                          // a warp's lanes read their own rows' powers only
     }
-    const float row_scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * row_power[u * kBM + r];
+    const float row_scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * q_power;
     const uint32_t taddr = tmem_base + u * kTmemUnit + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     float m = kNoMax, l = 0.f, vf = 1.f;
     bool ok = true;
@@ -598,7 +611,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const int c = lane & 15;
 #pragma unroll 4
       for (int i = 0; i < 16; ++i) {
-        const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4), rr = qr_ / G, hh = qr_ - rr * G;
+        const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4), rr = (qr_ * by_g) >> 16, hh = qr_ - rr * G;
         const int qrow = row0 + u * rpu + rr;
         if (rr < rpu && qrow < q_len)
           *(reinterpret_cast<uint4*>(p.out + (static_cast<size_t>(q_begin + qrow) * p.hq + hk * G + hh) * kD) + c) =
@@ -660,12 +673,13 @@ int blocks_of(int max_q_len, int hq, int hkv) {
 
 extern "C" {
 
-// Splits of the KV range, from launch-shape constants: only where the CTAs would leave most SMs idle, at least four tiles
-// each.
+// Splits of the KV range, from launch-shape constants: as many as leave every CTA an SM, but no shorter than a tile. Device
+// times with at least four / two / one tile to a split: 61 rows behind 1536 tokens 24.5 / 21.4 / 20.1 us, behind 512
+// 18.4 / 19.7 / 17.8, three times 61 behind 1536 25.8 / 23.1 / 23.1, 16 rows behind 8000 28.8 / 26.7 / 26.7.
 int xv_kv4_prefill_splits(int num_seqs, int max_q_len, int hq, int hkv, int max_tokens_per_seq, int num_sms) {
   if (num_seqs <= 0 || max_q_len <= 0 || hkv <= 0 || hq < hkv || hq / hkv > 16) return 1;
   const long long ctas = static_cast<long long>(num_seqs) * hkv * blocks_of(max_q_len, hq, hkv);
-  const long long by_sms = num_sms / ctas, by_len = max_tokens_per_seq / (4 * kBN);
+  const long long by_sms = num_sms / ctas, by_len = (max_tokens_per_seq + kBN - 1ll) / kBN;
   return static_cast<int>(std::max(1ll, std::min({by_sms, by_len, 16ll})));
 }
 
