@@ -150,9 +150,9 @@ struct Query {
   uint32_t c[NT][2];
   float unit;                          // a score over what the MMAs make of it
 
-  // `row`: sequence * hq + first query head of the group; `sign`: applied to Q.
-  __device__ __forceinline__ void load(const Params& p, size_t row, int G, float sign, int g, int t) {
-    uint32_t raw[NT][16], top = 0;
+  uint32_t raw[NT][16];
+  // Sends for Q. `row`: sequence * hq + first query head of the group.
+  __device__ __forceinline__ void fetch(const Params& p, size_t row, int G, int g, int t) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const uint4* src = reinterpret_cast<const uint4*>(p.q + (row + nt * 8 + g) * kD + 32 * t);
@@ -161,9 +161,15 @@ struct Query {
         const uint4 r = nt * 8 + g < G ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
         raw[nt][4 * w] = r.x; raw[nt][4 * w + 1] = r.y; raw[nt][4 * w + 2] = r.z; raw[nt][4 * w + 3] = r.w;
       }
+    }
+  }
+  // Makes the operands of what fetch() brought; `sign`: applied to Q.
+  __device__ __forceinline__ void convert(float sign, int t) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = __vmaxu2(top, raw[nt][i] & 0x7fff7fffu);
-    }
     uint32_t most = max(top >> 16, top & 0xffffu);
     if (__any_sync(0xffffffffu, most >= 0x7f80u)) {        // infinities and NaN do not choose the scale of the other heads
       most = 0;
@@ -515,6 +521,8 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
   const int G = p.hq / p.hkv;
   uint8_t* ring_mem = smem + warp * kStages * kSlot;
   grid_dep_wait();
+  Query<NT> q;
+  q.fetch(p, static_cast<size_t>(b) * p.hq + h * G, G, g, t);      // first: everything else hangs on two more reads
   const int kv_len = kv_len_of(p, b);
   const int units = (kv_len + 15) / 16;
   const int per = (units + p.splits * W - 1) / (p.splits * W);
@@ -526,8 +534,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) ring.issue(p);
   const Scale sc(p.scale_log2);
-  Query<NT> q;
-  q.load(p, static_cast<size_t>(b) * p.hq + h * G, G, sc.sign, g, t);
+  q.convert(sc.sign, t);
   const float scale = sc.of(q.unit), lag = kLazy / scale;
   Softmax<NT> st;
   st.clear();
@@ -729,7 +736,8 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
   for (;;) {
     const int n = min(units - first, todo);
     Query<NT> q;
-    q.load(p, static_cast<size_t>(b) * p.hq + h * G, G, sc.sign, g, t);
+    q.fetch(p, static_cast<size_t>(b) * p.hq + h * G, G, g, t);
+    q.convert(sc.sign, t);
     const float scale = sc.of(q.unit), lag = kLazy / scale;
     Softmax<NT> st;
     st.clear();
