@@ -2,10 +2,14 @@
 //
 //   kv4_write_kernel - per-head RMSNorm of q and k, NeoX RoPE, q written in bf16, k and v rounded to bf16 (what a bf16
 //                      cache would hold) and quantised into their slots. Half a warp per head, two heads of one kind at
-//                      a time; a lane holds four channels and their four rotary partners.
+//                      a time; a lane holds four channels and their four rotary partners. A warp takes up to eight such
+//                      pairs, all of them on their way through shared memory at once (cp.async).
 //   kv4_read_kernel  - the bf16 values of a list of slots. A warp per token.
 //
-// Both are bound by memory: the writer moves (hq + 2 hkv) 256 + hq 256 + hkv 144 bytes a token, the reader hkv 2 (72 + 256).
+// Both should be bound by memory: the writer moves (hq + 2 hkv) 256 + hq 256 + hkv 144 bytes a token, the reader
+// hkv 2 (72 + 256). The writer is as much bound by its instructions (3700 a token of 32 + 2 x 8 heads, 70% of the issue
+// slots): 8192 tokens 41.6 us (4.3 TB/s; with one pair sent for ahead in registers 48.5), 997 of 40 + 2 x 8 7.1 us.
+// The reader runs at 5.4 TB/s: 32768 tokens of 8 heads 31.8 us.
 //
 // Quantising is a choice between 16 levels, so K is normalised and rotated in 64 bits from the fp32 row: a value next
 // to a border between two levels then falls the same way wherever the row is computed (five double operations a channel,
@@ -94,10 +98,11 @@ __device__ __forceinline__ void store_row(uint8_t* unit, int r, int c, unsigned 
   }
 }
 
-// Warps of a block of the writer. K's warps take longer than Q's, and a block holds its place until its last one ends:
-// 8192 rows (32 + 2 x 8 heads), written and read back, take 62.7 us with eight warps to a block, 59.6 with two and 57.5
-// with one. 64 registers, for 32 warps an SM, are the best too (28: 59.6 us, 24: 63.4; 40 spill: 76).
+// Warps of a block of the writer, at 64 registers, for 32 warps an SM. A block holds its place until its last warp ends:
+// 8192 rows (32 + 2 x 8 heads), written and read back, took 62.7 us with eight warps to a block, 59.6 with two and 57.5
+// with one; 28 warps an SM 59.6, 24 63.4, 40 (which spill) 76.
 constexpr int kWriteWarps = 1;
+constexpr int kMaxPairs = 8;                  // of heads that a warp takes
 
 // What a launch writes and where.
 struct WriteParams {
@@ -115,7 +120,7 @@ struct WriteParams {
   long long split_stride;
   float eps;
   int splits, max_pos, tokens, hq, hkv, block_size, num_slots;
-  int per_warp;                      // pairs of heads a warp takes
+  int per_warp, kv_per_warp;         // pairs of heads a warp takes: of Q, of K and V
   int q_tasks, tasks;                // warps per token: for Q, and in all
 };
 
@@ -125,15 +130,33 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
   grid_dep_wait();
   constexpr int D = kv4::kD, HALF = D / 2;
   const int warp = blockIdx.x * kWriteWarps + (threadIdx.x >> 5);
-  const int t = warp / p.tasks, task = warp - t * p.tasks;
+  // K's and V's warps first: they take longest.
+  const int kv_tasks = p.tasks - p.q_tasks, kv_warps = p.tokens * kv_tasks;
+  const bool is_q = warp >= kv_warps;
+  const int of = is_q ? p.q_tasks : kv_tasks, at_kind = is_q ? warp - kv_warps : warp;
+  const int t = at_kind / of, task = at_kind - t * of;
   if (t >= p.tokens) return;
   const int lane = threadIdx.x & 31, c = lane & 15, half = lane >> 4;
-  const size_t row0 = static_cast<size_t>(t) * (p.hq + 2 * p.hkv) * D + 4 * c;
+  const size_t row0 = static_cast<size_t>(t) * (p.hq + 2 * p.hkv) * D;
+  // bf16 rows come through shared memory, all of a warp's pairs in flight at once: slot i holds its pair i, a head per half.
+  __shared__ uint4 rows[kWriteWarps][kMaxPairs][32];
+  uint4(&mine)[kMaxPairs][32] = rows[threadIdx.x >> 5];
+  auto send = [&](int i, int h) {
+    if constexpr (!PLANES) cp_async16(&mine[i][lane], p.qkv + row0 + static_cast<size_t>(h) * D + 8 * c);
+  };
 
-  // x[0..3] and x[4..7] of head h
-  auto load = [&](int h, uint2& a, uint2& b) {
-    const size_t off = row0 + static_cast<size_t>(h) * D;
+  auto arrive = [&]() {
+    if constexpr (!PLANES) {
+      cp_async_commit();
+      cp_async_wait<0>();
+      __syncwarp();
+    }
+  };
+
+  // x[0..3] and x[4..7] of head h, the i-th pair of the warp
+  auto load = [&](int i, int h, uint2& a, uint2& b) {
     if constexpr (PLANES) {
+      const size_t off = row0 + static_cast<size_t>(h) * D + 4 * c;
       float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
       for (int s = 0; s < p.splits; ++s) {
         const float4 e = *reinterpret_cast<const float4*>(p.planes + s * p.split_stride + off);
@@ -144,8 +167,9 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
       a = make_uint2(pack_bf16(u.x, u.y), pack_bf16(u.z, u.w));      // as the bf16 GEMM output would have been
       b = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
     } else {
-      a = __ldg(reinterpret_cast<const uint2*>(p.qkv + off));
-      b = __ldg(reinterpret_cast<const uint2*>(p.qkv + off + HALF));
+      const uint2* at = reinterpret_cast<const uint2*>(&mine[i][16 * half]);
+      a = at[c];
+      b = at[16 + c];
     }
   };
   auto unpack = [](const uint2& a, const uint2& b, float (&x)[8]) {
@@ -167,11 +191,12 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
     unpack(__ldg(reinterpret_cast<const uint2*>(nw + 4 * c)), __ldg(reinterpret_cast<const uint2*>(nw + HALF + 4 * c)), w);
   };
 
-  if (task < p.q_tasks) {
+  if (is_q) {
     // ---- Q: heads 2 i + half; a missing second head repeats the first and stores nothing ----
     const int first = task * p.per_warp, last = min(first + p.per_warp, (p.hq + 1) / 2);
-    uint2 a, b, a_next = make_uint2(0u, 0u), b_next = a_next;
-    load(min(2 * first + half, p.hq - 1), a, b);
+    auto head_of = [&](int pair) { return min(2 * pair + half, p.hq - 1); };
+#pragma unroll 2
+    for (int i = first; i < last; ++i) send(i - first, head_of(i));
     rotary(p.q_w);
     float p1[4], p2[4], p3[4], p4[4];                         // w1 cos, w2 sin, w2 cos, w1 sin
 #pragma unroll
@@ -181,9 +206,11 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
       p3[i] = w[4 + i] * cs[i];
       p4[i] = w[i] * sn[i];
     }
+    arrive();
     for (int i = first; i < last; ++i) {
       const int h = 2 * i + half;
-      if (i + 1 < last) load(min(h + 2, p.hq - 1), a_next, b_next);
+      uint2 a, b;
+      load(i - first, head_of(i), a, b);
       float x[8];
       unpack(a, b, x);
       float ss = 0.f;
@@ -201,8 +228,6 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
         *reinterpret_cast<uint2*>(dst + HALF) = make_uint2(pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
       }
-      a = a_next;
-      b = b_next;
     }
     return;
   }
@@ -212,18 +237,20 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
   if (slot >= p.num_slots && lane == 0) report_status(p.status, kIdWrite, kBadIndex);
   if (slot < 0 || slot >= p.num_slots) return;
   const int kv_pairs = (p.hkv + 1) / 2;
-  const int first = (task - p.q_tasks) * p.per_warp, last = min(first + p.per_warp, 2 * kv_pairs);
+  const int first = task * p.kv_per_warp, last = min(first + p.kv_per_warp, 2 * kv_pairs);
   const int place = slot % p.block_size;
   const size_t unit0 = kv4::unit_offset(slot / p.block_size, 0, p.hkv, p.block_size, place);
   const size_t head_bytes = static_cast<size_t>(p.block_size / kv4::kUnit) * kv4::kUnitBytes;
   const unsigned half_mask = half ? 0xffff0000u : 0x0000ffffu;
-  if (first < kv_pairs) rotary(p.k_w);
   auto head_of = [&](int pair) { return min(2 * (pair < kv_pairs ? pair : pair - kv_pairs) + half, p.hkv - 1); };
   auto source = [&](int pair) { return p.hq + (pair < kv_pairs ? 0 : p.hkv) + head_of(pair); };
-  uint2 a, b, a_next = make_uint2(0u, 0u), b_next = a_next;
-  load(source(first), a, b);
+#pragma unroll 2
+  for (int i = first; i < last; ++i) send(i - first, source(i));
+  if (first < kv_pairs) rotary(p.k_w);
+  arrive();
   for (int pair = first; pair < last; ++pair) {
-    if (pair + 1 < last) load(source(pair + 1), a_next, b_next);
+    uint2 a, b;
+    load(pair - first, source(pair), a, b);
     const bool is_k = pair < kv_pairs;
     const int h = head_of(pair);
     const bool there = 2 * (is_k ? pair : pair - kv_pairs) + half < p.hkv;
@@ -247,8 +274,6 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
     } else {
       store_row(p.v_cache + unit0 + h * head_bytes, place % kv4::kUnit, c, half_mask, x, there);
     }
-    a = a_next;
-    b = b_next;
   }
 }
 
@@ -330,12 +355,15 @@ int xv_kv4_write(const void* qkv, const float* partials, int splits, long long s
       misaligned(cos_sin, 16) || misaligned(q_out, 16) || misaligned(k_cache, 16) || misaligned(v_cache, 16))
     return XV_ERR_ALIGN;
   // Pairs of heads per warp: one while that leaves a warp slot for each (short steps are latency), up to eight where it
-  // saves making the token's rotary factors again.
+  // saves making the token's rotary factors again. Below that cap the launch is about one wave, whose end is K's and V's
+  // warps (a pair of K takes twice a pair of Q): they get half as many. 997 rows (40 + 2 x 8 heads) 8.0 -> 7.1 us, but
+  // 8192 rows (32 + 2 x 8) at the cap 41.5 -> 42.6.
   const int q_pairs = (hq + 1) / 2, kv_pairs = 2 * ((hkv + 1) / 2);
   WriteParams p;
-  p.per_warp = static_cast<int>(std::max(1ll, std::min(8ll, static_cast<long long>(tokens) * (q_pairs + kv_pairs) / (148 * 48))));
+  p.per_warp = static_cast<int>(std::max(1ll, std::min<long long>(kMaxPairs, static_cast<long long>(tokens) * (q_pairs + kv_pairs) / (148 * 32))));
   p.q_tasks = (q_pairs + p.per_warp - 1) / p.per_warp;
-  p.tasks = p.q_tasks + (kv_pairs + p.per_warp - 1) / p.per_warp;
+  p.kv_per_warp = p.per_warp == kMaxPairs ? kMaxPairs : (p.per_warp + 1) / 2;
+  p.tasks = p.q_tasks + (kv_pairs + p.kv_per_warp - 1) / p.kv_per_warp;
   const long long blocks = (static_cast<long long>(tokens) * p.tasks + kWriteWarps - 1) / kWriteWarps;
   if (blocks > 0x0fffffffLL) return XV_ERR_SHAPE;
   p.qkv = static_cast<const __nv_bfloat16*>(qkv);
