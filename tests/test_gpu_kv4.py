@@ -402,6 +402,22 @@ def test_small_and_large_values():
     _attend([1, 30], [40, 60], 4, 2, n_decode=1, v_scale=2.0 ** 40, q_scale=2.0 ** -40)
 
 
+@pytest.mark.parametrize("extra_pages", [1, 300])
+def test_rows_before_position_0_and_behind_the_last_sequence_are_zero(extra_pages):
+    out = _attend([1, 40, 150], [9, 25, 130], 4, 2, n_decode=1, extra_pages=extra_pages)
+    assert not out[1:16].any() and not out[41:61].any() and bool(out[16:41].any(-1).all())
+    ops = _ops()
+    q, k, v, attn = _small()
+    padded = torch.cat([q, torch.ones(300, q.shape[1], dtype=q.dtype, device=DEV)])
+    for n_decode in (2, 1, 0):
+        attn.num_decode = n_decode
+        torch.full_like(padded, 7.0)                         # what the allocator may hand out again
+        got = ops.paged_attention(padded, k, v, attn, 0.1, 4, 2, D)
+        assert not got[2:].any()
+        torch.testing.assert_close(got[:2], ops.paged_attention(q, k, v, attn, 0.1, 4, 2, D), rtol=0, atol=0)
+    _cuda().check_status()
+
+
 def test_scores_below_the_smallest_float_leave_equal_weights():
     """The scale of a score underflows; what the mask takes out still has weight 0, not NaN."""
     _attend([1, 30, 200], [40, 60, 200], 4, 2, n_decode=1, v_scale=2.0 ** -60, q_scale=2.0 ** -70)
@@ -443,6 +459,9 @@ def test_refusals():
                       (ValueError, (q, k.cpu(), v.cpu()))):
         with pytest.raises(bad):
             ops.paged_attention(*args, attn, 0.1, 4, 2, D)
+    for bad in (float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="finite"):
+            ops.paged_attention(q, k, v, attn, bad, 4, 2, D)
     with pytest.raises(ValueError, match="16 to one"):
         ops.paged_attention(torch.zeros(2, 34 * D, device=DEV).bfloat16(), k, v, attn, 0.1, 34, 2, D)
     with pytest.raises(ValueError, match="head_dim 128"):

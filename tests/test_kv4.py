@@ -124,6 +124,37 @@ def test_append_then_attend_matches_64_bits():
     np.testing.assert_allclose(out.view(T, hq, d).numpy(), ref, atol=1e-5)
 
 
+def test_what_a_row_does_not_see_cannot_reach_it():
+    """NaN under a negative slot, NaN at later positions of a chunk, rows before position 0 and behind the last sequence."""
+    hq, hkv, d, n = 2, 1, 64, 6
+    k, v = (torch.zeros(2, hkv, 16, kv4.row_bytes(d), dtype=torch.uint8) for _ in range(2))
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(n, hkv, d, generator=g)
+    kv4.write_rows(k, torch.arange(n), x)
+    nan = x.clone()
+    nan[4] = float("nan")
+    q = torch.randn(n + 1, hq * d, generator=g)
+    table = torch.tensor([[0]], dtype=torch.int32)
+    i32 = dict(dtype=torch.int32)
+
+    def run(rows, length=n):
+        attn = AttnBatch(cu_q=torch.tensor([0, rows], **i32), kv_lens=torch.tensor([length], **i32), block_tables=table, num_seqs=1,
+                         num_decode=0, max_q_len=rows, max_kv_len=length, num_tokens=rows)
+        return ops.paged_attention(q, k, v, attn, 0.125, hq, hkv, d)
+
+    kv4.write_rows(v, torch.arange(n), x)
+    clean = run(n)
+    assert not clean[n].any()
+    late = run(n, 4)
+    assert not late[:2].any() and bool(late[2:n].isfinite().all()) and bool(late[2:n].any(-1).all())
+    kv4.write_rows(v, torch.arange(n), nan)
+    out = run(n)
+    assert torch.equal(out[:4], clean[:4]) and bool(out[4:n].isnan().all())
+    kv4.write_rows(k, torch.tensor([0]), torch.full((1, hkv, d), float("nan")))
+    rows, _ = ops.read_cache(k, v, torch.tensor([-1, 0, 1], dtype=torch.int32), d)
+    assert not rows[0].any() and bool(rows[1].isnan().all()) and bool(rows[2].isfinite().all())
+
+
 # ---- the engine with kv_cache_dtype="int4" ----
 
 def _generate(model_dir, prompts, max_tokens=8, **kw):
@@ -188,6 +219,8 @@ def test_pool_sizes_and_reads_its_tokens(tiny_model_dir):
             k, v = p.read_tokens(1, slots)
             assert k.shape == x.shape and torch.equal(k, v)
             assert float((k - x).float().abs().max()) <= (0 if name == "auto" else 0.3)
+            k, v = p.read_tokens(1, torch.tensor([-1, 33], dtype=torch.int32))
+            assert not k[0].any() and not v[0].any() and bool(k[1].any())
     finally:
         groups.destroy_model_parallel()
 

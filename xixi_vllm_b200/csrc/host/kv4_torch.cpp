@@ -13,6 +13,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -233,6 +234,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto* kv_lens = static_cast<const int*>(vector(lens, B, at::kInt, c.dev, "kv_lens"));
     const int* cu_q = np > 0 ? static_cast<const int*>(vector(tensor(a[3], "cu_q"), B + 1, at::kInt, c.dev, "cu_q")) : nullptr;
     const float scale = real(a[9]);
+    if (!std::isfinite(scale)) refuse(PyExc_ValueError, "paged_attention: scale must be finite");
     const int sms = integer(a[13], "num_sms");
     auto* status = static_cast<int*>(vector(tensor(a[14], "status"), 1, at::kInt, c.dev, "status"));
     const c10::cuda::OptionalCUDAGuard guard(c.dev);
@@ -241,6 +243,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       out.zero_();
       return THPVariable_Wrap(std::move(out));
     }
+    if (np == 0 && nd < T) out.narrow(0, nd, T - nd).zero_();           // rows behind the last sequence; else the chunk kernel's
     const auto stream = c10::cuda::getCurrentCUDAStream(c.dev.index()).stream();
     // Workspaces come from torch's allocator, call by call: calls on two streams, or two captured graphs, never share one.
     if (nd > 0) {

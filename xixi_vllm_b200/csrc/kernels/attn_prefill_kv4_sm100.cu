@@ -141,6 +141,12 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   grid_dep_launch();
   grid_dep_wait();
   const int b = p.seq_begin + blockIdx.z / p.splits, split = blockIdx.z % p.splits, hk = blockIdx.y;
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == gridDim.z - 1) {       // rows behind the last sequence
+    const int end = max(p.cu_q[p.seq_begin + gridDim.z / p.splits], 0);
+    const size_t row_chunks = static_cast<size_t>(p.hq) * (kD / 8), last = p.total_rows * row_chunks;
+    for (size_t i = end * row_chunks + threadIdx.x; i < last; i += blockDim.x)
+      reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
   const int q_begin = p.cu_q[b];
   const int q_len = p.cu_q[b + 1] - q_begin;
   if (q_begin < 0 || q_len < 0 || q_len > p.total_rows - q_begin) {

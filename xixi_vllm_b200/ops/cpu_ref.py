@@ -116,7 +116,7 @@ def read_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor
     out = []
     for cache in (k_cache, v_cache):
         rows = kv4.read_rows(cache, slots.clamp_min(0))
-        out.append((rows * (slots >= 0)[:, None, None]).to(torch.bfloat16))
+        out.append(rows.masked_fill((slots < 0)[:, None, None], 0).to(torch.bfloat16))
     return out[0], out[1]
 
 
@@ -158,7 +158,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         kpos = torch.arange(L, device=q.device)[None, :]
         s = s.masked_fill(kpos > qpos, float("-inf"))
         p = torch.softmax(s, dim=-1)
+        if kv4.is_kv4(v_cache):
+            p = p.masked_fill(qpos < 0, 0)          # a row before position 0 sees nothing
+            bad = ~torch.isfinite(v)                # what a row does not see must not reach it as 0 * NaN
+            v = v.masked_fill(bad, 0)
         o = torch.einsum("hgnl,hld->hgnd", p, v)                                        # [Hkv,G,n,D]
+        if kv4.is_kv4(v_cache) and bool(bad.any()):
+            hit = torch.einsum("nl,hld->hnd", (kpos <= qpos).float(), bad.float()) > 0
+            o = o.masked_fill(hit[:, None], float("nan"))
         out[q0:q1] = o.permute(2, 0, 1, 3).reshape(n, num_q_heads * D).to(q.dtype)
     return out
 

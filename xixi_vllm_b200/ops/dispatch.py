@@ -93,7 +93,8 @@ def read_cache(k_cache, v_cache, slots, head_dim):
 
 def paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
     """``attn`` is a ``runtime.staging.AttnBatch`` (cu_q, kv_lens, block_tables, decode split). The caches are bf16
-    pages or, as uint8, pages held in 4 bits (``ops.kv4``)."""
+    pages or, as uint8, pages held in 4 bits (``ops.kv4``). On a 4-bit cache rows of ``q`` behind the last sequence, rows of
+    a sequence without cached tokens and rows before position 0 come out as zeros; ``scale`` is finite."""
     if q.is_cuda:
         return _cuda().paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim)
     return cpu_ref.paged_attention(q, k_cache, v_cache, attn.cu_q, attn.kv_lens, attn.block_tables,

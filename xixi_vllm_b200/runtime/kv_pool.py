@@ -52,13 +52,20 @@ class KVPool:
 
     def read_tokens(self, layer: int, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values ``[T, kv_heads, head_dim]`` of the cached tokens at ``slots`` (int32, on the pool's device),
-        whatever form the pool holds them in: to hand a prefix to another pool, or to inspect it. A slot outside the pool
-        raises on the CPU; on the GPU a 4-bit pool reports it through the status word."""
+        whatever form the pool holds them in: to hand a prefix to another pool, or to inspect it. Rows whose slot is
+        negative are zero. A slot beyond the pool raises on the CPU; on the GPU its row is zero, and a 4-bit pool reports
+        it through the status word."""
         k, v = self.k_cache(layer), self.v_cache(layer)
         if self.int4:
             return ops.read_cache(k, v, slots, self.head_dim)
-        s = slots.long()
-        return k[s // self.block_size, :, s % self.block_size], v[s // self.block_size, :, s % self.block_size]
+        s, end = slots.long(), self.num_blocks_total * self.block_size
+        out = (s < 0)[:, None, None]
+        if self.device.type == "cuda":
+            out = out | (s >= end)[:, None, None]
+            s = s.clamp_max(end - 1)
+        s = s.clamp_min(0)
+        page, place = s // self.block_size, s % self.block_size
+        return k[page, :, place].masked_fill(out, 0), v[page, :, place].masked_fill(out, 0)
 
     @property
     def bytes_per_block(self) -> int:
