@@ -9,11 +9,19 @@
 //   8-11      - dequantisers (thread = token of the tile): 64 bytes of codes and 8 of parameters of K and of V from global
 //               memory, one tile ahead in registers, to fp16 rows in the 128-byte-swizzled shared-memory rings.
 //   12, 13    - one MMA issuer thread per unit: O += P V as soon as P is written, then the next S = Q K^T.
-// Registers move from the issuers' and dequantisers' warpgroups to the softmax ones (setmaxnreg: 2 x 184 + 96 + 48 = 4 x 128).
+//   14, 15    - bring a unit's rows of Q (bulk copies), which the softmax warps convert.
+// Registers move from the issuers' and dequantisers' warpgroups to the softmax ones (setmaxnreg: 2 x 176 + 104 + 56 = 4 x 128).
+//
+// What bounds it: the chain of one unit, S -> softmax -> P -> O += P V -> next S, about 4100 cycles a tile of 128 tokens, of
+// which 1590 are the exponentials (1024 of MUFU), 840 S's way through tensor memory and the maximum, 1030 the two MMAs and
+// the rest hand-over; the other unit's exponentials lie in between. Both units' MMAs are 2050 of it. Beside them the
+// dequantisers' loop (770 instructions a warp) takes 4200 cycles when all SMs are busy. 4 x 2048 rows behind 512 tokens, 32
+// query heads: 273 us, 754 TFLOP/s. Measured against: registers 2 x 184 + 96 + 48 277 us, 2 x 192 + 80 + 48 286,
+// 2 x 168 + 112 + 64 287; Q loaded by the lanes that convert it 285.
 //
 // fp16 operands, not bf16: a dequantised value c + s (n - 8) has more than bf16's 8 bits, and its rounding (2^-12 instead
-// of 2^-9) would otherwise be the largest error of the result. Their range is kept by powers of two: a row of Q is scaled
-// by its largest element, a tile of K or V by an exponent that its dequantisers choose from the tile's parameters (and
+// of 2^-9) would otherwise be the largest error of the result. Their range is kept by powers of two: 32 lanes of Q are scaled
+// by their largest element, a tile of K or V by an exponent that its dequantisers choose from the tile's parameters (and
 // keep while it fits); the scores undo Q's and K's, and V's is carried with the output accumulator.
 // Inside a word the channels are stored in the order 0 4 1 5 2 6 3 7, which is how the nibbles unpack: Q follows it, and
 // the output undoes it for V.
@@ -47,7 +55,7 @@ constexpr int kTileBytes = 2 * kHalf;             // 32 KiB
 constexpr int kNK = 3, kNV = 2;                   // ring slots
 constexpr int kBarBytes = 512;                    // barriers and small arrays
 constexpr int kSmem = (2 + kNK + kNV) * kTileBytes + 1024 + kBarBytes;
-constexpr uint32_t kTmemCols = 512, kTmemUnit = 256, kTmemO = 128;
+constexpr uint32_t kTmemCols = 512, kTmemUnit = 256, kTmemO = 128;       // all of it, so it begins at address 0
 constexpr int kId = 12;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;                      // log2 units
@@ -102,6 +110,18 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+// A contiguous run of bytes (a multiple of 16) from global to this CTA's shared memory, counted in bytes on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 // Two channels of a word, nibbles j and j + 4, as n - 8 in fp16 (exact): even j as 1024 + n, odd j as 1024 + 16 n.
 __device__ __forceinline__ __half2 centred_f16(uint32_t w, bool odd) {
   uint32_t r;
@@ -138,40 +158,6 @@ __device__ __forceinline__ void put_words(uint32_t row_at, int c0, const uint4& 
 
 __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  grid_dep_launch();
-  grid_dep_wait();
-  const int b = p.seq_begin + blockIdx.z / p.splits, split = blockIdx.z % p.splits, hk = blockIdx.y;
-  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == gridDim.z - 1) {       // rows behind the last sequence
-    const int end = max(p.cu_q[p.seq_begin + gridDim.z / p.splits], 0);
-    const size_t row_chunks = static_cast<size_t>(p.hq) * (kD / 8), last = p.total_rows * row_chunks;
-    for (size_t i = end * row_chunks + threadIdx.x; i < last; i += blockDim.x)
-      reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0u, 0u, 0u, 0u);
-  }
-  const int q_begin = p.cu_q[b];
-  const int q_len = p.cu_q[b + 1] - q_begin;
-  if (q_begin < 0 || q_len < 0 || q_len > p.total_rows - q_begin) {
-    if (threadIdx.x == 0) report_status(p.status, kId, kBadIndex);
-    return;
-  }
-  const int G = p.hq / p.hkv;
-  const int rpu = kBM / G;                                   // query rows of a unit
-  const int row0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * rpu;     // long ones first
-  if (row0 >= q_len) return;
-  int kv_len = max(p.kv_lens[b], 0);
-  const long long most = min(static_cast<long long>(p.max_blocks) * p.block_size, 0x7fffff00ll);   // a tile more stays 32-bit
-  if (kv_len > most) {
-    if (threadIdx.x == 0) report_status(p.status, kId, kBadIndex);
-    kv_len = static_cast<int>(most);
-  }
-  const int pos0 = kv_len - q_len;                           // position of query row 0; rows before position 0 see nothing
-  const int rows_here = min(2 * rpu, q_len - row0);
-  const int n_kv = max(0, min(kv_len, pos0 + row0 + rows_here));
-  // This CTA's run of tiles.
-  const int all_tiles = (n_kv + kBN - 1) / kBN, per_split = (all_tiles + p.splits - 1) / p.splits;
-  const int tile0 = min(split * per_split, all_tiles), n_tiles = min(per_split, all_tiles - tile0);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int wg = warp >> 2;
-
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
   uint8_t* smem = smem_raw + pad;
   uint8_t* q_s = smem;                                       // [2 units]
@@ -187,11 +173,16 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   uint64_t* p_ready = s_full + 2;                            // [2] P written (and O rescaled)
   uint64_t* o_done = p_ready + 2;                            // [2]
   uint64_t* xu_done = o_done + 2;                            // [2] a unit's exponentials of the tile are over
-  TileScale* scales = reinterpret_cast<TileScale*>(xu_done + 2);         // [8], by tile (20 barriers before it: 16-byte aligned)
+  uint64_t* q_raw = xu_done + 2;                             // [2] a unit's rows as they are in memory
+  TileScale* scales = reinterpret_cast<TileScale*>(q_raw + 2);           // [8], by tile (22 barriers before it: 16-byte aligned)
   uint32_t* red = reinterpret_cast<uint32_t*>(scales + 8);   // [2][12]
   uint32_t* tmem_slot = red + 24;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wg = warp >> 2;
 
+  // Under the launch before: the barriers. (Tensor memory waits until that launch has ended: it may want all of it.)
+  grid_dep_launch();
   if (threadIdx.x == 0) {
     for (int u = 0; u < 2; ++u) {
       mbar_init(&q_full[u], 128);
@@ -199,6 +190,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       mbar_init(&p_ready[u], 128);
       mbar_init(&o_done[u], 1);
       mbar_init(&xu_done[u], 128);
+      mbar_init(&q_raw[u], 1);
     }
     for (int s = 0; s < kNK; ++s) {
       mbar_init(&k_full[s], 128);
@@ -211,18 +203,42 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 12) {
-    tmem_alloc(tmem_slot, kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before_sync();
   __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_slot;
+  grid_dep_wait();
+
+  const int b = p.seq_begin + blockIdx.z / p.splits, split = blockIdx.z % p.splits, hk = blockIdx.y;
+  const int q_begin = p.cu_q[b], q_end = p.cu_q[b + 1];
+  int kv_len = max(p.kv_lens[b], 0);
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == gridDim.z - 1) {       // rows behind the last sequence
+    const size_t row_chunks = static_cast<size_t>(p.hq) * (kD / 8), last = p.total_rows * row_chunks;
+    for (size_t i = max(q_end, 0) * row_chunks + threadIdx.x; i < last; i += blockDim.x)
+      reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  const int q_len = q_end - q_begin;
+  if (q_begin < 0 || q_len < 0 || q_len > p.total_rows - q_begin) {
+    if (threadIdx.x == 0) report_status(p.status, kId, kBadIndex);
+    return;
+  }
+  const int G = p.hq / p.hkv;
+  const int rpu = kBM / G;                                   // query rows of a unit
+  const int row0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * rpu;     // long ones first
+  if (row0 >= q_len) return;
+  const long long most = min(static_cast<long long>(p.max_blocks) * p.block_size, 0x7fffff00ll);   // a tile more stays 32-bit
+  if (kv_len > most) {
+    if (threadIdx.x == 0) report_status(p.status, kId, kBadIndex);
+    kv_len = static_cast<int>(most);
+  }
+  const int pos0 = kv_len - q_len;                           // position of query row 0; rows before position 0 see nothing
+  const int rows_here = min(2 * rpu, q_len - row0);
+  const int n_kv = max(0, min(kv_len, pos0 + row0 + rows_here));
+  // This CTA's run of tiles.
+  const int all_tiles = (n_kv + kBN - 1) / kBN, per_split = (all_tiles + p.splits - 1) / p.splits;
+  const int tile0 = min(split * per_split, all_tiles), n_tiles = min(per_split, all_tiles - tile0);
+  auto rows_of = [&](int u) { return max(0, min(rpu, q_len - row0 - u * rpu)); };
 
   if (wg == 2) {
     // ---------------- dequantisers ----------------
-    set_regs_down<96>();
+    set_regs_down<104>();
     const int row = threadIdx.x & 127;
     const int upp = p.block_size / kv4::kUnit;
     const int* table = p.block_tables + static_cast<size_t>(b) * p.max_blocks;
@@ -323,6 +339,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       }
       const int ks = j % kNK, vs = j % kNV;
       const uint2 vp_now = vp;
+      if (j == 1 || j == 2) ok = ok && __all_sync(0xffffffffu, mbar_wait(&q_full[j - 1], 0));    // Q's rows lie in these slots
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&k_empty[ks], ((j / kNK) & 1) ^ 1) && *abort_flag == 0);
       if (ok) {
         const float f = pow2(-ek);
@@ -359,14 +376,34 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     // ---------------- MMA issuers: one warp per unit, one elected lane issues ----------------
     // The whole warp walks the loop, so that descriptors stay in uniform registers: a lone lane took about 120 cycles an
     // MMA, twice what the MMA itself takes.
-    set_regs_down<48>();
-    const int u = __shfl_sync(0xffffffffu, warp, 0) - 12;
-    if (u < 2 && n_tiles > 0) {
+    set_regs_down<56>();
+    const int role = __shfl_sync(0xffffffffu, warp, 0) - 12;             // 0, 1: MMA issuers; 2, 3: Q's copies
+    if (role >= 2) {
+      const int u = role - 2;
+      // ---- Q: a unit's rows of all its heads, contiguous in memory row by row, into a K slot that is free until tile 1 + u ----
+      const int rows = rows_of(u);
+      const uint32_t bytes = static_cast<uint32_t>(G) * kD * 2;
+      if (lane == 0) mbar_expect_tx(&q_raw[u], rows * bytes);
+      __syncwarp();
+      const __nv_bfloat16* src = p.q + (static_cast<size_t>(q_begin + row0 + u * rpu) * p.hq + hk * G) * kD;
+      for (int i = lane; i < rows; i += 32)
+        bulk_load(k_ring + (1 + u) * kTileBytes + i * bytes, src + static_cast<size_t>(i) * p.hq * kD, bytes, &q_raw[u]);
+    } else {
+      if (role == 0) {
+        tmem_alloc(tmem_slot, kTmemCols);
+        tmem_relinquish();
+      }
+      tc_fence_before_sync();
+      named_barrier(2, 64);
+      tc_fence_after_sync();
+    }
+    if (role < 2 && n_tiles > 0) {
+      const int u = role;
       const uint32_t idesc_s = idesc_f16(kBM, kBN), idesc_o = idesc_f16(kBM, kD) | (1u << 16);
       const uint64_t q_desc = umma_desc_sw128(smem_u32(q_s) + u * kTileBytes);
       const uint64_t k_desc0 = umma_desc_sw128(smem_u32(k_ring)), v_desc0 = umma_desc_sw128_mn(smem_u32(v_ring), kHalf, 1024);
-      const uint32_t s_tmem = tmem_base + u * kTmemUnit, o_tmem = s_tmem + kTmemO;
-      bool ok = mbar_wait(&q_full[u], 0);
+      const uint32_t s_tmem = u * kTmemUnit, o_tmem = s_tmem + kTmemO;
+      bool ok = *tmem_slot == 0 && mbar_wait(&q_full[u], 0);
       int reason = kWaitFullTimeout;
       int ks = 0, vs = 0;                                     // ring slots and their phases
       uint32_t kph = 0, vph = 0;
@@ -417,70 +454,63 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     }
   } else {
     // ---------------- softmax and output: thread r of unit u is query row r / G, head r % G ----------------
-    set_regs_up<184>();
+    set_regs_up<176>();
     const int u = wg, r = threadIdx.x & 127;
     const int by_g = 65536 / G + 1;                          // lane / G as a product: exact for 128 lanes and G up to 16
     const int row = row0 + u * rpu + r / G;
     const int pos = pos0 + min(row, q_len - 1);              // lanes without a row follow the last one
     // Q: a power of two per warp takes its largest element to 2^14 .. 2^15 of fp16, which is exact down to 2^-31 of it; a
-    // negative scale is its sign. Sixteen lanes a row, two rows at a time, so that the reads are whole lines.
-    float q_power;
-    {
-      const int c = lane & 15;
-      uint4 v[16];                                           // all reads in flight at once
-      {
+    // negative scale is its sign. The rows come by bulk copies (as loads by the lanes that convert them they took 3500
+    // cycles to arrive, a sixth of a short CTA's life); sixteen lanes convert a row, two rows at a time.
+    float q_power = 1.f;
+    bool ok = __all_sync(0xffffffffu, mbar_wait(&q_raw[u], 0));
+    if (!ok) mbar_wait(&q_raw[u], 0);                        // the copies must not outlive the CTA
+    if (ok) {
+      const int c = lane & 15, first = (warp & 3) * 32 + (lane >> 4), lanes = rows_of(u) * G;
+      const uint32_t raw = smem_u32(k_ring) + (1 + u) * kTileBytes + c * 16;
+      uint4 v[16];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        v[i] = first + 2 * i < lanes ? ld_shared_v4(raw + (first + 2 * i) * 256) : make_uint4(0u, 0u, 0u, 0u);
+        top = __vmaxu2(__vmaxu2(__vmaxu2(top, v[i].x & 0x7fff7fffu), __vmaxu2(v[i].y & 0x7fff7fffu, v[i].z & 0x7fff7fffu)),
+                       v[i].w & 0x7fff7fffu);
+      }
+      uint32_t most = max(top >> 16, top & 0xffffu);
+      if (__any_sync(0xffffffffu, most >= 0x7f80u)) {        // infinities and NaN do not choose the other rows' power
+        most = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4), rr = (qr_ * by_g) >> 16, hh = qr_ - rr * G;
-          const int qrow = row0 + u * rpu + rr;
-          const bool there = rr < rpu && qrow < q_len;
-          v[i] = there ? __ldg(reinterpret_cast<const uint4*>(
-                                   p.q + (static_cast<size_t>(q_begin + qrow) * p.hq + hk * G + hh) * kD) + c)
-                       : make_uint4(0u, 0u, 0u, 0u);
-        }
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          top = __vmaxu2(__vmaxu2(__vmaxu2(top, v[i].x & 0x7fff7fffu), __vmaxu2(v[i].y & 0x7fff7fffu, v[i].z & 0x7fff7fffu)),
-                         v[i].w & 0x7fff7fffu);
-        uint32_t most = max(top >> 16, top & 0xffffu);
-        if (__any_sync(0xffffffffu, most >= 0x7f80u)) {      // infinities and NaN do not choose the other rows' power
-          most = 0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
-              most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-            }
-          }
-        }
-        const int e = max(-100, min(100, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14));
-        const float f = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
-        q_power = pow2(e);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4);
-          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};       // channels 0 1, 2 3, 4 5, 6 7 of the word
-          float x[8];
+          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            x[2 * k] = __uint_as_float(w[k] << 16) * f;
-            x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u) * f;
+            const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
+            most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
           }
-          st_shared_v4(chunk_at(row_start(smem_u32(q_s) + u * kTileBytes, qr_), c), pack_f16(x[0], x[4]), pack_f16(x[1], x[5]),
-                       pack_f16(x[2], x[6]), pack_f16(x[3], x[7]));
         }
+      }
+      const int e = max(-100, min(100, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14));
+      const float f = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
+      q_power = pow2(e);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};         // channels 0 1, 2 3, 4 5, 6 7 of the word
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[2 * k] = __uint_as_float(w[k] << 16) * f;
+          x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u) * f;
+        }
+        st_shared_v4(chunk_at(row_start(smem_u32(q_s) + u * kTileBytes, first + 2 * i), c), pack_f16(x[0], x[4]), pack_f16(x[1], x[5]),
+                     pack_f16(x[2], x[6]), pack_f16(x[3], x[7]));
       }
       fence_proxy_async_smem();
       mbar_arrive(&q_full[u]);
     }
     const float row_scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * q_power;
-    const uint32_t taddr = tmem_base + u * kTmemUnit + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t taddr = u * kTmemUnit + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     float m = kNoMax, l = 0.f, vf = 1.f;
-    bool ok = true;
-    for (int j = 0; j < n_tiles; ++j) {
+    for (int j = 0; ok && j < n_tiles; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[u], j & 1) && *abort_flag == 0);
       if (!ok) break;
       tc_fence_after_sync();
@@ -578,38 +608,55 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const size_t slot = (((static_cast<size_t>(blockIdx.z / p.splits) * gridDim.y + hk) * gridDim.x + blockIdx.x) * p.splits + split) *
                               (2 * kBM) + u * kBM + r;
       *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(m, l);
-      for (int ch = 0; ch < kD / 16 && n_tiles > 0; ++ch) {  // a split without tiles leaves no output, only m = kNoMax, l = 0
-        uint32_t o[16];
-        tmem_ld16(taddr + kTmemO + ch * 16, o);
-        tmem_ld_wait();
-        tmem_ld_fence_regs(o);
+      // Through the unit's Q tile (all its MMAs are over) half the channels at a time, so that the writes are whole lines. A
+      // split without tiles leaves no output, only m = kNoMax, l = 0.
+      const uint32_t tile = smem_u32(q_s) + u * kTileBytes;
+      const size_t slot0 = slot - r;
+#pragma unroll 1
+      for (int half = 0; half < 2 && n_tiles > 0; ++half) {
+#pragma unroll 1
+        for (int ch = 0; ch < 2; ++ch) {
+          uint32_t o[32];
+          tmem_ld32(taddr + kTmemO + half * 64 + ch * 32, o);
+          tmem_ld_wait();
+          tmem_ld_fence_regs(o);
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {                        // words of channels 0 4 1 5 2 6 3 7
-          auto x = [&](int i) { return __uint_as_float(o[8 * w + i]) * vf; };
-          float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * kD + ch * 16 + 8 * w);
-          dst[0] = make_float4(x(0), x(2), x(4), x(6));
-          dst[1] = make_float4(x(1), x(3), x(5), x(7));
+          for (int w = 0; w < 4; ++w) {                      // words of channels 0 4 1 5 2 6 3 7
+            auto x = [&](int i) { return __float_as_uint(__uint_as_float(o[8 * w + i]) * vf); };
+            const int k = ch * 8 + 2 * w;
+            st_shared_v4(tile + r * 256 + ((k ^ (r & 15)) << 4), x(0), x(2), x(4), x(6));
+            st_shared_v4(tile + r * 256 + (((k + 1) ^ (r & 15)) << 4), x(1), x(3), x(5), x(7));
+          }
         }
+        __syncwarp();
+        const int c = lane & 15;
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          const int at = (warp & 3) * 32 + 2 * i + (lane >> 4);
+          *(reinterpret_cast<uint4*>(p.ws_o + (slot0 + at) * kD + half * 64) + c) = ld_shared_v4(tile + at * 256 + ((c ^ (at & 15)) << 4));
+        }
+        __syncwarp();
       }
     } else if (ok) {
       tc_fence_after_sync();
       const float inv = l == 0.f ? 0.f : vf / l;
       // Rows leave through the unit's Q tile (all its MMAs are over), so that the writes are whole lines.
       const uint32_t at = row_start(smem_u32(q_s) + u * kTileBytes, r);
-#pragma unroll 2
-      for (int ch = 0; ch < kD / 16; ++ch) {
-        uint32_t o[16];
+#pragma unroll 1
+      for (int ch = 0; ch < kD / 32; ++ch) {
+        uint32_t o[32];
         if (n_tiles > 0) {
-          tmem_ld16(taddr + kTmemO + ch * 16, o);
+          tmem_ld32(taddr + kTmemO + ch * 32, o);
           tmem_ld_wait();
+          tmem_ld_fence_regs(o);
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = 0u;
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {                        // words of channels 0 4 1 5 2 6 3 7
+        for (int w = 0; w < 4; ++w) {                        // words of channels 0 4 1 5 2 6 3 7
           auto x = [&](int i) { return l == 0.f ? 0.f : __uint_as_float(o[8 * w + i]) * inv; };
-          st_shared_v4(chunk_at(at, 2 * ch + w), pack_bf16(x(0), x(2)), pack_bf16(x(4), x(6)), pack_bf16(x(1), x(3)),
+          st_shared_v4(chunk_at(at, 4 * ch + w), pack_bf16(x(0), x(2)), pack_bf16(x(4), x(6)), pack_bf16(x(1), x(3)),
                        pack_bf16(x(5), x(7)));
         }
       }
@@ -633,7 +680,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   __syncthreads();
   if (warp == 12) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, kTmemCols);
+    tmem_dealloc(*tmem_slot, kTmemCols);
   }
 }
 
