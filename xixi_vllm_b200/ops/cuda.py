@@ -386,10 +386,14 @@ def _kv4_calls():
     return _calls
 
 
+def _kv4_state(cache):
+    return _states.get(cache.get_device()) or _state(cache)      # the short way: these calls take 5 us in all
+
+
 def _kv4_write(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads, num_kv_heads, head_dim):
     global launch_count
     launch_count += 1
-    calls, status = _calls or _kv4_calls(), _state(k_cache).status
+    calls, status = _calls or _kv4_calls(), _kv4_state(k_cache).status
     if isinstance(qkv, SplitKPartial):
         T, cols = qkv.shape
         if cols != (num_q_heads + 2 * num_kv_heads) * head_dim:
@@ -404,12 +408,12 @@ def read_cache(k_cache, v_cache, slots, head_dim):
     """bf16 rows of a 4-bit cache (see ``dispatch.read_cache``). A slot beyond the cache gives zeros and status 5."""
     global launch_count
     launch_count += 1
-    return (_calls or _kv4_calls()).read(k_cache, v_cache, slots, head_dim, _state(k_cache).status)
+    return (_calls or _kv4_calls()).read(k_cache, v_cache, slots, head_dim, _kv4_state(k_cache).status)
 
 
 def _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
     global launch_count
-    st, n, n_d = _state(k_cache), attn.num_seqs, attn.num_decode
+    st, n, n_d = _kv4_state(k_cache), attn.num_seqs, attn.num_decode
     launch_count += (n_d > 0) + (n > n_d)
     return (_calls or _kv4_calls()).attention(q, k_cache, v_cache, attn.cu_q, attn.kv_lens, attn.block_tables, n, n_d,
                                               attn.max_q_len, scale, num_q_heads, num_kv_heads, head_dim, st.num_sms, st.status)
