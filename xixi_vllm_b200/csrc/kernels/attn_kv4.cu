@@ -51,16 +51,6 @@ struct Params {
   float scale_log2;
 };
 
-// Page of a block-table entry; an entry outside the cache is recorded and replaced by page 0.
-__device__ __forceinline__ int page_of(const Params& p, int b, int entry) {
-  int blk = __ldg(p.block_tables + static_cast<size_t>(b) * p.max_blocks + entry);
-  if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) {
-    report_status(p.status, kIdDecode, kBadIndex);
-    blk = 0;
-  }
-  return blk;
-}
-
 // Cached tokens of a sequence, never more than its block table can name.
 __device__ __forceinline__ int kv_len_of(const Params& p, int b) {
   const int n = p.kv_lens[b];
@@ -430,75 +420,83 @@ struct Softmax {
   }
 };
 
-// A warp's ring of slots in shared memory and the walk over the units of one (sequence, KV head) that fills it. A unit in
-// a slot: K's 1152 bytes, then V's; five cp.async of 16 bytes a lane (K's codes, V's codes, both parameter blocks by half
-// a warp). Pages are looked up 32 at a time, one batch ahead of use.
+// A warp's ring of slots in shared memory and the walk over units of one (sequence, KV head) that fills it. Slot k takes the
+// units first + k stride and the next one, below `end`. A unit in a slot: K's 1152 bytes, then V's; five cp.async of 16 bytes
+// a lane (K's codes, V's codes, both parameter blocks by half a warp). Pages are looked up 32 units at a time, one batch
+// ahead of use; a lane turns its entry into the unit's number in the cache.
 struct Ring {
   uint32_t dst, slot, p_to;
   int lane;
-  // units still to fetch, and where they are
-  const uint8_t *k_src, *v_src, *p_src;      // this lane's 16 bytes of K's codes, V's codes and the parameters in page 0
-  uint32_t page_bytes;
-  int b, left, place, upp, page0, page_i, last_page, pages, pages_next;
+  const uint8_t *k_src, *v_src, *p_src;      // this lane's 16 bytes of K's codes, V's codes and the parameters in unit 0
+  const int* table;
+  int first, stride, end, k, slots, upp, hkv, h;
+  uint32_t units, units_next;
 
-  __device__ __forceinline__ void init(uint8_t* ring, int lane_, int upp_, int hkv) {
+  __device__ __forceinline__ void init(const Params& p, uint8_t* ring, int lane_) {
     lane = lane_;
-    upp = upp_;
+    upp = p.block_size / kv4::kUnit;
+    hkv = p.hkv;
     dst = smem_u32(ring) + lane * 16;
     p_to = kv4::kParBase + (lane < 8 ? 0 : kv4::kUnitBytes - 128);
-    slot = 0;
-    left = 0;
-    page_bytes = static_cast<uint32_t>(hkv) * upp * kv4::kUnitBytes;
-  }
-  __device__ __forceinline__ int lookup(const Params& p, int i) const {
-    return page_of(p, b, min(page0 + i, last_page));
-  }
-  // n units from `first` on of the `units` that sequence b has.
-  __device__ __forceinline__ void start(const Params& p, int b_, int h, int first, int n, int units) {
-    b = b_;
-    left = n;
-    page0 = first / upp;
-    place = first - page0 * upp;
-    last_page = max(0, (units - 1) / upp);
-    page_i = 0;
-    const size_t head = static_cast<size_t>(h) * upp * kv4::kUnitBytes + lane * 16;
-    k_src = p.k_cache + head;
-    v_src = p.v_cache + head;
+    k_src = p.k_cache + lane * 16;
+    v_src = p.v_cache + lane * 16;
     p_src = (lane < 8 ? k_src : v_src - 128) + kv4::kParBase;
-    if (n > 0) {
-      pages = lookup(p, lane);
-      pages_next = lookup(p, 32 + lane);
-    }
+    slot = 0;
+    k = slots = 0;
   }
-  // The next kPair units (or what is left of them) into the next slot; one commit group per call, empty ones included.
+  // The walk, but for its end; sends for the first entries, which end() checks.
+  __device__ __forceinline__ int begin(const Params& p, int b, int h_, int first_, int stride_) {
+    h = h_;
+    first = first_;
+    stride = stride_;
+    table = p.block_tables + static_cast<size_t>(b) * p.max_blocks;
+    return entry(p, 0);
+  }
+  __device__ __forceinline__ int unit_of(int slot0) const { return first + (slot0 + (lane >> 1)) * stride + (lane & 1); }
+  __device__ __forceinline__ int entry(const Params& p, int slot0) const {
+    return __ldg(table + min(unit_of(slot0) / upp, p.max_blocks - 1));
+  }
+  __device__ __forceinline__ uint32_t number(const Params& p, int slot0, int blk) const {
+    const int unit = unit_of(slot0);
+    if (static_cast<unsigned>(blk) >= static_cast<unsigned>(p.num_blocks)) {
+      if (unit < end) report_status(p.status, kIdDecode, kBadIndex);     // entries behind the sequence may be anything
+      blk = 0;
+    }
+    return (static_cast<uint32_t>(blk) * hkv + h) * upp + unit % upp;
+  }
+  __device__ __forceinline__ void until(const Params& p, int end_, int entry0) {
+    end = end_;
+    k = 0;
+    slots = first < end ? (end - first + stride - 1) / stride : 0;
+    units = number(p, 0, entry0);
+    if (slots > 16) units_next = number(p, 16, entry(p, 16));
+  }
+  // The next slot, if there is one; one commit group per call, empty ones included.
   __device__ __forceinline__ void issue(const Params& p) {
+    if (k < slots) {
+      const int unit0 = first + k * stride;
 #pragma unroll
-    for (int u = 0; u < kPair; ++u) {
-      if (left > 0) {
-        if (place == upp) {
-          place = 0;
-          if ((++page_i & 31) == 0) {
-            pages = pages_next;
-            pages_next = lookup(p, page_i + 32 + lane);
-          }
-        }
-        const uint32_t blk = __shfl_sync(0xffffffffu, pages, page_i & 31);
-        const uint64_t at = static_cast<uint64_t>(blk) * page_bytes + static_cast<uint32_t>(place * kv4::kUnitBytes);
+      for (int u = 0; u < kPair; ++u) {
+        const uint64_t at = static_cast<uint64_t>(__shfl_sync(0xffffffffu, units, (2 * k + u) & 31)) * kv4::kUnitBytes;
         const uint32_t to = dst + slot * kSlot + u * kUnitSlot;
-        cp_async16_u32(to, k_src + at);
-        cp_async16_u32(to + 512, k_src + at + 512);
-        cp_async16_u32(to + kv4::kUnitBytes, v_src + at);
-        cp_async16_u32(to + kv4::kUnitBytes + 512, v_src + at + 512);
-        if (lane < 16)
-          cp_async16_u32(to + p_to, p_src + at);
-        ++place;
-        --left;
+        if (unit0 + u < end) {
+          cp_async16_u32(to, k_src + at);
+          cp_async16_u32(to + 512, k_src + at + 512);
+          cp_async16_u32(to + kv4::kUnitBytes, v_src + at);
+          cp_async16_u32(to + kv4::kUnitBytes + 512, v_src + at + 512);
+          if (lane < 16) cp_async16_u32(to + p_to, p_src + at);
+        }
+      }
+      if ((++k & 15) == 0) {
+        units = units_next;
+        if (k + 16 < slots) units_next = number(p, k + 16, entry(p, k + 16));
       }
     }
     cp_async_commit();
     slot = slot == kStages - 1 ? 0 : slot + 1;
   }
 };
+static_assert(kPair == 2, "a lookup of 32 lanes serves 16 slots");
 
 // A negative scale is Q's sign, so the running maxima need not know it; zero becomes a scale too small to matter.
 struct Scale {
@@ -523,14 +521,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
   grid_dep_wait();
   Query<NT> q;
   q.fetch(p, static_cast<size_t>(b) * p.hq + h * G, G, g, t);      // first: everything else hangs on two more reads
-  const int kv_len = kv_len_of(p, b);
-  const int units = (kv_len + 15) / 16;
-  const int per = (units + p.splits * W - 1) / (p.splits * W);
-  const int first = min((split * W + warp) * per, units);
-  const int n = min(per, units - first);
+  // Slots are dealt to the warps in turn: which pages a warp reads first does not hang on the length.
+  const int first = (split * W + warp) * kPair, stride = p.splits * W * kPair;
   Ring ring;
-  ring.init(ring_mem, lane, p.block_size / kv4::kUnit, p.hkv);
-  ring.start(p, b, h, first, n, units);
+  ring.init(p, ring_mem, lane);
+  const int entry0 = ring.begin(p, b, h, first, stride);
+  const int kv_len = kv_len_of(p, b);
+  ring.until(p, (kv_len + 15) / 16, entry0);
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) ring.issue(p);
   const Scale sc(p.scale_log2);
@@ -541,8 +538,8 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
 
   const int tok = token_of_row(g);
   const uint8_t* at = ring_mem;
-  int mine = min(kv_len - first * 16, n * 16);           // tokens of this warp still to come
-  for (int i = 0; i < n; i += kPair, mine -= 16 * kPair) {
+  int mine = kv_len - first * 16;                        // tokens from the slot's first on
+  for (; mine > 0; mine -= 16 * stride) {
     cp_async_wait<kStages - 2>();
     __syncwarp();                        // everyone's part of the slot has landed, and everyone has read the slot filled next
     ring.issue(p);
@@ -706,7 +703,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
   }
 
   Ring ring;
-  ring.init(ring_mem, lane, p.block_size / kv4::kUnit, p.hkv);
+  ring.init(p, ring_mem, lane);
   const Scale sc(p.scale_log2);
   const int tok = token_of_row(g);
   const uint8_t* at = ring_mem;
@@ -715,10 +712,11 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
   auto fetch_pair = [&](int start) {
     const int n = min(f_units - start, f_todo);
     f_todo -= n;
-    ring.start(p, f_b, f_h, start, n, f_units);
+    const int entry0 = ring.begin(p, f_b, f_h, start, kPair);
+    ring.until(p, start + n, entry0);
   };
   auto fetch = [&]() {
-    if (ring.left == 0 && f_todo > 0) {
+    if (ring.k == ring.slots && f_todo > 0) {
       if (++f_h == p.hkv) {
         f_h = 0;
         do f_units = (kv_len_of(p, ++f_b) + 15) / 16;
@@ -935,7 +933,7 @@ int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const
                     scale, status))
     return rc;
   if (hq / hkv > 16 || hkv > 65535 || num_seqs > 65535 || splits < 0 || splits > 8) return XV_ERR_SHAPE;
-  if (static_cast<long long>(hkv) * block_size * kv4::kRow > 0xffffffffLL) return XV_ERR_SHAPE;    // bytes of a page: 32-bit
+  if (static_cast<long long>(num_blocks) * hkv * (block_size / kv4::kUnit) > 0xffffffffLL) return XV_ERR_SHAPE;     // units: 32-bit numbers
   if (int rc = allow_decode_kernels()) return rc;
   p.splits = splits;
   const int nt = hq / hkv > 8 ? 2 : 1;
