@@ -906,14 +906,19 @@ extern "C" {
 
 // How a decode launch divides its work, from launch-shape constants only (never from sequence lengths), so that a captured
 // graph keeps its shape: 1, 2, 4 or 8 CTAs (one cluster) per (sequence, KV head) as long as they are one wave of three an
-// SM, or 0 for even shares where a CTA could get more than 2048 tokens. Device times, clusters of 1 / 2 / 4 / 8 against
-// shares: 256 pairs of up to 1280 tokens 13.0 / 14.7 / 18.3 / 32.2 against 15.8 us; 72 pairs of up to 3001 19.9 / 14.0 /
-// 11.6 / 14.0 against 18.9; 8 pairs of 2000 14.4 / 10.5 / 6.9 / 5.7 against 9.2, of 40960 246 / 128 / 66 / 36 against 22.5.
+// SM and get 128 tokens each, or 0 for even shares. Device times, clusters of 1 / 2 / 4 / 8 against shares:
+//   8 pairs of 2000 tokens 13.2 / 9.7 / 6.4 / 5.3 against 9.6 us, of 40960 228 / 118 / 62 / 33 against 19.7
+//   72 pairs of up to 3001 18.7 / 13.2 / 10.7 / 13.1 against 15.8, 256 of up to 1280 11.4 / 15.0 / 17.0 / 29.9 against 14.8
+// Two CTAs repay their join from about 1280 tokens on (8 pairs of 300 4.2 / 5.4 / 4.2, 128 of up to 1200 8.5 / 8.9).
+// Shares pay where a CTA could get more than 2048 tokens (a tail that they do not have), until so many pairs wait for a place
+// that the tail no longer counts: pairs of up to 4096, 320 of them 32.3 (one CTA each) against 27.5, 768 67.0 against
+// 61.4, 1024 80.6 against 78.5, 1600 109.0 against 112.1, 2048 135.6 against 138.2.
 int xv_kv4_decode_splits(int num_seqs, int hkv, int num_sms, int max_tokens_per_seq) {
   const long long pairs = static_cast<long long>(num_seqs) * hkv;
   int s = 1;
   while (s < 8 && pairs * 2 * s <= 3 * num_sms && max_tokens_per_seq / (2 * s) >= 128) s *= 2;
-  return max_tokens_per_seq / s > 2048 ? 0 : s;
+  if (s == 2 && max_tokens_per_seq < 1280) s = 1;
+  return max_tokens_per_seq / s > 2048 && pairs < 4 * 3 * num_sms ? 0 : s;
 }
 
 long long xv_kv4_decode_workspace_bytes(int num_seqs, int hq, int hkv, int splits, int num_sms) {
