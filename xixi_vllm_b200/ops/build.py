@@ -101,7 +101,7 @@ def build_torch(force: bool = False) -> str:
                     "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
                     "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
                     "-I", os.path.join(CSRC, "kernels"), "-o", tmp, TORCH_SRC,
-                    "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], check=True)
+                    "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"], check=True)
     os.replace(tmp, TORCH_LIB)
     return TORCH_LIB
 

@@ -341,8 +341,17 @@ def resolve_token_refs(ids, prev) -> None:
 def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads,
                        num_kv_heads, head_dim, prefill_begin: int = 0):
     if k_cache.dtype is torch.uint8:
-        return _kv4_write(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads, num_kv_heads,
-                          head_dim)
+        global launch_count
+        launch_count += 1
+        calls, status = _calls or _kv4_calls(), _kv4_state(k_cache).status
+        if isinstance(qkv, SplitKPartial):
+            T, cols = qkv.shape
+            if cols != (num_q_heads + 2 * num_kv_heads) * head_dim:
+                raise ValueError(f"qk_norm_rope_cache: {cols} columns for {num_q_heads} query and {num_kv_heads} KV heads")
+            return calls.write(None, qkv.ws, qkv.splits, T, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache,
+                               num_q_heads, num_kv_heads, head_dim, status)
+        return calls.write(qkv, None, 0, 0, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads,
+                           num_kv_heads, head_dim, status)
     if isinstance(qkv, SplitKPartial):
         _bf16(q_w, k_w, k_cache, v_cache)
         T = qkv.shape[0]
@@ -390,33 +399,11 @@ def _kv4_state(cache):
     return _states.get(cache.get_device()) or _state(cache)      # the short way: these calls take 5 us in all
 
 
-def _kv4_write(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads, num_kv_heads, head_dim):
-    global launch_count
-    launch_count += 1
-    calls, status = _calls or _kv4_calls(), _kv4_state(k_cache).status
-    if isinstance(qkv, SplitKPartial):
-        T, cols = qkv.shape
-        if cols != (num_q_heads + 2 * num_kv_heads) * head_dim:
-            raise ValueError(f"qk_norm_rope_cache: {cols} columns for {num_q_heads} query and {num_kv_heads} KV heads")
-        return calls.write(None, qkv.ws, qkv.splits, T, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache,
-                           num_q_heads, num_kv_heads, head_dim, status)
-    return calls.write(qkv, None, 0, 0, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads,
-                       num_kv_heads, head_dim, status)
-
-
 def read_cache(k_cache, v_cache, slots, head_dim):
     """bf16 rows of a 4-bit cache (see ``dispatch.read_cache``). A slot beyond the cache gives zeros and status 5."""
     global launch_count
     launch_count += 1
     return (_calls or _kv4_calls()).read(k_cache, v_cache, slots, head_dim, _kv4_state(k_cache).status)
-
-
-def _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
-    global launch_count
-    st, n, n_d = _kv4_state(k_cache), attn.num_seqs, attn.num_decode
-    launch_count += (n_d > 0) + (n > n_d)
-    return (_calls or _kv4_calls()).attention(q, k_cache, v_cache, attn.cu_q, attn.kv_lens, attn.block_tables, n, n_d,
-                                              attn.max_q_len, scale, num_q_heads, num_kv_heads, head_dim, st.num_sms, st.status)
 
 
 def decode_splits(num_seqs: int, num_kv_heads: int, num_sms: int, max_blocks_tokens: int) -> int:
@@ -448,7 +435,12 @@ def prefill_pair_heads(on: bool) -> None:
 def paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
     """Decode rows (the first ``attn.num_decode`` sequences) and prefill chunks of one packed batch."""
     if k_cache.dtype is torch.uint8:
-        return _kv4_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim)
+        global launch_count
+        st, n, n_d = _kv4_state(k_cache), attn.num_seqs, attn.num_decode
+        launch_count += (n_d > 0) + (n > n_d)
+        return (_calls or _kv4_calls()).attention(
+            q, k_cache, v_cache, attn.cu_q, attn.kv_lens, attn.block_tables, n, n_d, attn.max_q_len, scale, num_q_heads,
+            num_kv_heads, head_dim, st.num_sms, st.status)
     _bf16(q, k_cache, v_cache)
     st = _state(q)
     L = lib()
