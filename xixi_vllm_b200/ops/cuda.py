@@ -3,7 +3,9 @@
 Tensors are passed as raw device pointers together with the current CUDA stream; outputs
 are allocated with torch so they live in its caching allocator (and in CUDA-graph pools
 during capture). Only bf16 activations and weights are supported on the GPU. A missing
-library raises: there is no silent fallback to library kernels.
+library raises: there is no silent fallback to library kernels. The calls on 4-bit caches go through a
+small Python extension instead of ctypes (``_xv_torch.so``, ``csrc/host/kv4_torch.cpp``): one C function
+checks, allocates and launches.
 
 ``XV_GEMM=cublas`` in the environment swaps the GEMM for ``torch.matmul`` (cuBLAS); it
 exists to A/B the hand-written kernel and to bisect numerical differences.
