@@ -698,19 +698,33 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_prefill_join_kernel(const
   const int row = (blocks - 1 - block) * 2 * rpu + u * rpu + r / G;
   if (r >= rpu * G || row >= q_len) return;
   const size_t slot = ((static_cast<size_t>(blockIdx.z) * gridDim.y + hk) * blocks + block) * p.splits * (2 * kBM) + i % (2 * kBM);
-  float M = kNoMax;
-  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.ws_ml[(slot + s * (2 * kBM)) * 2]);
-  float L = 0.f;
+  constexpr int kBatch = 8;                                  // splits in flight: the kernel is a chain of L2 round trips
+  float M = kNoMax, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
-    const size_t at = slot + s * (2 * kBM);
-    const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + at * 2);
-    if (ml.x == kNoMax && ml.y == 0.f) continue;             // saw nothing, and may have written nothing
-    const float f = exp2f(ml.x - M);
-    const float4 v = *reinterpret_cast<const float4*>(p.ws_o + at * kD + lane * 4);
-    L += ml.y * f;
-    acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+  for (int s0 = 0; s0 < p.splits; s0 += kBatch) {
+    float2 ml[kBatch];
+    float4 v[kBatch];
+    float mn = M;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const size_t at = slot + static_cast<size_t>(s0 + i) * (2 * kBM);
+      const bool there = s0 + i < p.splits;
+      ml[i] = there ? *reinterpret_cast<const float2*>(p.ws_ml + at * 2) : make_float2(kNoMax, 0.f);
+      v[i] = there ? *reinterpret_cast<const float4*>(p.ws_o + at * kD + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) mn = fmaxf(mn, ml[i].x);
+    const float f0 = exp2f(M - mn);
+    M = mn;
+    L *= f0;
+    acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (ml[i].x == kNoMax && ml[i].y == 0.f) continue;     // saw nothing, and may have written nothing
+      const float f = exp2f(ml[i].x - M);
+      L += ml[i].y * f;
+      acc.x += v[i].x * f; acc.y += v[i].y * f; acc.z += v[i].z * f; acc.w += v[i].w * f;
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(q_begin + row) * p.hq + hk * G + r % G) * kD + lane * 4) =
