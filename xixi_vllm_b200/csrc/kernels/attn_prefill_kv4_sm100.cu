@@ -9,7 +9,7 @@
 //   8-11      - dequantisers (thread = token of the tile): 64 bytes of codes and 8 of parameters of K and of V from global
 //               memory, one tile ahead in registers, to fp16 rows in the 128-byte-swizzled shared-memory rings.
 //   12, 13    - one MMA issuer thread per unit: O += P V as soon as P is written, then the next S = Q K^T.
-//   14, 15    - bring a unit's rows of Q (bulk copies), which the softmax warps convert.
+//   14, 15    - fill up the warpgroup.
 // Registers move from the issuers' and dequantisers' warpgroups to the softmax ones (setmaxnreg: 2 x 176 + 104 + 56 = 4 x 128).
 //
 // What bounds it: the chain of one unit, S -> softmax -> P -> O += P V -> next S, about 4100 cycles a tile of 128 tokens, of
@@ -74,6 +74,10 @@ struct Params {
   float* ws_ml;                                   // [CTA][split][256 lanes][2]: maximum (log2 units), sum
   int seq_begin, hq, hkv, block_size, max_blocks, num_blocks, total_rows, splits;
   float scale_log2;
+  int G, rpu, by_g;                               // heads to a KV head, rows of a unit; 65536 / G + 1: lane / G is a product
+  uint32_t inv_splits;                            // 2^32 / splits + 1, or 0 for one split
+  // n / splits; exact for n splits < 2^32.
+  __device__ __forceinline__ int by_splits(int n) const { return inv_splits ? __umulhi(n, inv_splits) : n; }
 };
 
 struct alignas(16) TileScale {                    // of one tile: K and V are stored divided by k and v
@@ -206,7 +210,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   __syncthreads();
   grid_dep_wait();
 
-  const int b = p.seq_begin + blockIdx.z / p.splits, split = blockIdx.z % p.splits, hk = blockIdx.y;
+  const int z = p.by_splits(blockIdx.z), split = blockIdx.z - z * p.splits, b = p.seq_begin + z, hk = blockIdx.y;
   const int q_begin = p.cu_q[b], q_end = p.cu_q[b + 1];
   int kv_len = max(p.kv_lens[b], 0);
   if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == gridDim.z - 1) {       // rows behind the last sequence
@@ -219,8 +223,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     if (threadIdx.x == 0) report_status(p.status, kId, kBadIndex);
     return;
   }
-  const int G = p.hq / p.hkv;
-  const int rpu = kBM / G;                                   // query rows of a unit
+  const int G = p.G, rpu = p.rpu;                            // heads of a KV head; query rows of a unit
   const int row0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * rpu;     // long ones first
   if (row0 >= q_len) return;
   const long long most = min(static_cast<long long>(p.max_blocks) * p.block_size, 0x7fffff00ll);   // a tile more stays 32-bit
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   const int rows_here = min(2 * rpu, q_len - row0);
   const int n_kv = max(0, min(kv_len, pos0 + row0 + rows_here));
   // This CTA's run of tiles.
-  const int all_tiles = (n_kv + kBN - 1) / kBN, per_split = (all_tiles + p.splits - 1) / p.splits;
+  const int all_tiles = (n_kv + kBN - 1) / kBN, per_split = p.by_splits(all_tiles + p.splits - 1);
   const int tile0 = min(split * per_split, all_tiles), n_tiles = min(per_split, all_tiles - tile0);
   auto rows_of = [&](int u) { return max(0, min(rpu, q_len - row0 - u * rpu)); };
 
@@ -377,18 +380,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     // The whole warp walks the loop, so that descriptors stay in uniform registers: a lone lane took about 120 cycles an
     // MMA, twice what the MMA itself takes.
     set_regs_down<56>();
-    const int role = __shfl_sync(0xffffffffu, warp, 0) - 12;             // 0, 1: MMA issuers; 2, 3: Q's copies
-    if (role >= 2) {
-      const int u = role - 2;
-      // ---- Q: a unit's rows of all its heads, contiguous in memory row by row, into a K slot that is free until tile 1 + u ----
-      const int rows = rows_of(u);
-      const uint32_t bytes = static_cast<uint32_t>(G) * kD * 2;
-      if (lane == 0) mbar_expect_tx(&q_raw[u], rows * bytes);
-      __syncwarp();
-      const __nv_bfloat16* src = p.q + (static_cast<size_t>(q_begin + row0 + u * rpu) * p.hq + hk * G) * kD;
-      for (int i = lane; i < rows; i += 32)
-        bulk_load(k_ring + (1 + u) * kTileBytes + i * bytes, src + static_cast<size_t>(i) * p.hq * kD, bytes, &q_raw[u]);
-    } else {
+    const int role = __shfl_sync(0xffffffffu, warp, 0) - 12;             // 0, 1: MMA issuers
+    if (role < 2) {
       if (role == 0) {
         tmem_alloc(tmem_slot, kTmemCols);
         tmem_relinquish();
@@ -456,32 +449,44 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     // ---------------- softmax and output: thread r of unit u is query row r / G, head r % G ----------------
     set_regs_up<176>();
     const int u = wg, r = threadIdx.x & 127;
-    const int by_g = 65536 / G + 1;                          // lane / G as a product: exact for 128 lanes and G up to 16
-    const int row = row0 + u * rpu + r / G;
+    const int by_g = p.by_g, row = row0 + u * rpu + ((r * by_g) >> 16);
     const int pos = pos0 + min(row, q_len - 1);              // lanes without a row follow the last one
     // Q: a power of two per warp takes its largest element to 2^14 .. 2^15 of fp16, which is exact down to 2^-31 of it; a
-    // negative scale is its sign. The rows come by bulk copies (as loads by the lanes that convert them they took 3500
-    // cycles to arrive, a sixth of a short CTA's life); sixteen lanes convert a row, two rows at a time.
+    // negative scale is its sign. A unit's rows of all its heads are contiguous in memory row by row; bulk copies bring them
+    // into a K slot that is free until tile 1 + u. All four warps send their share: a copy takes its warp 67 cycles (one warp
+    // for all of them 2160; loads by the lanes that convert 3500). Sixteen lanes convert a row, two rows at a time, in
+    // loops that are mostly rolled: code that a CTA runs once waits for its instructions.
     float q_power = 1.f;
+    {
+      const uint32_t bytes = static_cast<uint32_t>(G) * kD * 2;
+      const int rows = rows_of(u);
+      if (r == 0) mbar_expect_tx(&q_raw[u], rows * bytes);
+      const __nv_bfloat16* src = p.q + (static_cast<size_t>(q_begin + row0 + u * rpu) * p.hq + hk * G) * kD;
+      for (int i = (warp & 3) + 4 * lane; i < rows; i += 128)
+        bulk_load(k_ring + (1 + u) * kTileBytes + i * bytes, src + static_cast<size_t>(i) * p.hq * kD, bytes, &q_raw[u]);
+      __syncwarp();
+    }
     bool ok = __all_sync(0xffffffffu, mbar_wait(&q_raw[u], 0));
     if (!ok) mbar_wait(&q_raw[u], 0);                        // the copies must not outlive the CTA
     if (ok) {
       const int c = lane & 15, first = (warp & 3) * 32 + (lane >> 4), lanes = rows_of(u) * G;
       const uint32_t raw = smem_u32(k_ring) + (1 + u) * kTileBytes + c * 16;
-      uint4 v[16];
+      auto piece = [&](int i) {
+        return first + 2 * i < lanes ? ld_shared_v4(raw + (first + 2 * i) * 256) : make_uint4(0u, 0u, 0u, 0u);
+      };
       uint32_t top = 0;
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < 16; ++i) {
-        v[i] = first + 2 * i < lanes ? ld_shared_v4(raw + (first + 2 * i) * 256) : make_uint4(0u, 0u, 0u, 0u);
-        top = __vmaxu2(__vmaxu2(__vmaxu2(top, v[i].x & 0x7fff7fffu), __vmaxu2(v[i].y & 0x7fff7fffu, v[i].z & 0x7fff7fffu)),
-                       v[i].w & 0x7fff7fffu);
+        const uint4 v = piece(i);
+        top = __vmaxu2(__vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, v.z & 0x7fff7fffu)), v.w & 0x7fff7fffu);
       }
       uint32_t most = max(top >> 16, top & 0xffffu);
       if (__any_sync(0xffffffffu, most >= 0x7f80u)) {        // infinities and NaN do not choose the other rows' power
         most = 0;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 16; ++i) {
-          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+          const uint4 v = piece(i);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
@@ -492,9 +497,10 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const int e = max(-100, min(100, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14));
       const float f = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
       q_power = pow2(e);
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < 16; ++i) {
-        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};         // channels 0 1, 2 3, 4 5, 6 7 of the word
+        const uint4 v = piece(i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};          // channels 0 1, 2 3, 4 5, 6 7 of the word
         float x[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -605,7 +611,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[u], (n_tiles - 1) & 1) && *abort_flag == 0);
     if (ok && p.splits > 1) {
       tc_fence_after_sync();
-      const size_t slot = (((static_cast<size_t>(blockIdx.z / p.splits) * gridDim.y + hk) * gridDim.x + blockIdx.x) * p.splits + split) *
+      const size_t slot = (((static_cast<size_t>(z) * gridDim.y + hk) * gridDim.x + blockIdx.x) * p.splits + split) *
                               (2 * kBM) + u * kBM + r;
       *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(m, l);
       // Through the unit's Q tile (all its MMAs are over) half the channels at a time, so that the writes are whole lines. A
@@ -740,14 +746,15 @@ int blocks_of(int max_q_len, int hq, int hkv) {
 
 extern "C" {
 
-// Splits of the KV range, from launch-shape constants: as many as leave every CTA an SM, but no shorter than a tile. Device
-// times with at least four / two / one tile to a split: 61 rows behind 1536 tokens 24.5 / 21.4 / 20.1 us, behind 512
-// 18.4 / 19.7 / 17.8, three times 61 behind 1536 25.8 / 23.1 / 23.1, 16 rows behind 8000 28.8 / 26.7 / 26.7.
+// Splits of the KV range, from launch-shape constants: as many as leave every CTA an SM, but no shorter than a tile, and only
+// from four tiles on. Device times: 8 CTAs of 1 tile 10.0 us whole, 12.6 in two; of 5 tiles 18.3 whole, 13.4 in five; of
+// 13 35.0 whole, 15.0 in 13 or more; 24 of 13 35.4 whole, 19.0 in six, 27.0 in eight (more than the SMs); 40 of 3 14.1 whole,
+// 16.6 in three; 80 of 26 63.1 whole, 79.4 in two, 63.2 in three.
 int xv_kv4_prefill_splits(int num_seqs, int max_q_len, int hq, int hkv, int max_tokens_per_seq, int num_sms) {
   if (num_seqs <= 0 || max_q_len <= 0 || hkv <= 0 || hq < hkv || hq / hkv > 16) return 1;
   const long long ctas = static_cast<long long>(num_seqs) * hkv * blocks_of(max_q_len, hq, hkv);
   const long long by_sms = num_sms / ctas, by_len = (max_tokens_per_seq + kBN - 1ll) / kBN;
-  return static_cast<int>(std::max(1ll, std::min({by_sms, by_len, 16ll})));
+  return by_len < 4 ? 1 : static_cast<int>(std::max(1ll, std::min({by_sms, by_len, 16ll})));
 }
 
 long long xv_kv4_prefill_workspace_bytes(int num_seqs, int max_q_len, int hq, int hkv, int splits) {
@@ -792,6 +799,10 @@ int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, cons
   p.scale_log2 = scale * kLog2e;
   const int blocks = blocks_of(max_q_len, hq, hkv);
   p.splits = splits;
+  p.G = hq / hkv;
+  p.rpu = kBM / p.G;
+  p.by_g = 65536 / p.G + 1;                       // exact for 128 lanes and G up to 16
+  p.inv_splits = splits > 1 ? static_cast<uint32_t>((1ull << 32) / splits) + 1 : 0u;
   p.ws_o = static_cast<float*>(workspace);
   p.ws_ml = splits > 1 ? p.ws_o + static_cast<size_t>(num_seqs) * hkv * blocks * splits * (2 * kBM) * kD : nullptr;
   launch_pdl(kv4_prefill_tc_kernel, dim3(blocks, hkv, num_seqs * splits), dim3(512), kSmem, stream, p);
