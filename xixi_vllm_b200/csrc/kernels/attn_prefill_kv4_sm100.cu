@@ -454,8 +454,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     // Q: a power of two per warp takes its largest element to 2^14 .. 2^15 of fp16, which is exact down to 2^-31 of it; a
     // negative scale is its sign. A unit's rows of all its heads are contiguous in memory row by row; bulk copies bring them
     // into a K slot that is free until tile 1 + u. All four warps send their share: a copy takes its warp 67 cycles (one warp
-    // for all of them 2160; loads by the lanes that convert 3500). Sixteen lanes convert a row, two rows at a time, in
-    // loops that are mostly rolled: code that a CTA runs once waits for its instructions.
+    // for all of them 2160; loads by the lanes that convert 3500). Sixteen lanes convert a row, two rows at a time.
     float q_power = 1.f;
     {
       const uint32_t bytes = static_cast<uint32_t>(G) * kD * 2;
@@ -471,22 +470,22 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     if (ok) {
       const int c = lane & 15, first = (warp & 3) * 32 + (lane >> 4), lanes = rows_of(u) * G;
       const uint32_t raw = smem_u32(k_ring) + (1 + u) * kTileBytes + c * 16;
-      auto piece = [&](int i) {
-        return first + 2 * i < lanes ? ld_shared_v4(raw + (first + 2 * i) * 256) : make_uint4(0u, 0u, 0u, 0u);
-      };
-      uint32_t top = 0;
-#pragma unroll 4
-      for (int i = 0; i < 16; ++i) {
-        const uint4 v = piece(i);
-        top = __vmaxu2(__vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, v.z & 0x7fff7fffu)), v.w & 0x7fff7fffu);
-      }
+      uint4 v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        v[i] = first + 2 * i < lanes ? ld_shared_v4(raw + (first + 2 * i) * 256) : make_uint4(0u, 0u, 0u, 0u);
+      uint32_t tops[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        tops[i & 3] = __vmaxu2(__vmaxu2(tops[i & 3], __vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu)),
+                               __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
+      const uint32_t top = __vmaxu2(__vmaxu2(tops[0], tops[1]), __vmaxu2(tops[2], tops[3]));
       uint32_t most = max(top >> 16, top & 0xffffu);
       if (__any_sync(0xffffffffu, most >= 0x7f80u)) {        // infinities and NaN do not choose the other rows' power
         most = 0;
-#pragma unroll 1
+#pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const uint4 v = piece(i);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
@@ -497,10 +496,9 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const int e = max(-100, min(100, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14));
       const float f = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
       q_power = pow2(e);
-#pragma unroll 4
+#pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const uint4 v = piece(i);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};          // channels 0 1, 2 3, 4 5, 6 7 of the word
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};         // channels 0 1, 2 3, 4 5, 6 7 of the word
         float x[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -620,15 +618,17 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const size_t slot0 = slot - r;
 #pragma unroll 1
       for (int half = 0; half < 2 && n_tiles > 0; ++half) {
-#pragma unroll 1
+        uint32_t o[2][32];
+        tmem_ld32(taddr + kTmemO + half * 64, o[0]);
+        tmem_ld32(taddr + kTmemO + half * 64 + 32, o[1]);
+        tmem_ld_wait();
+        tmem_ld_fence_regs(o[0]);
+        tmem_ld_fence_regs(o[1]);
+#pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
-          uint32_t o[32];
-          tmem_ld32(taddr + kTmemO + half * 64 + ch * 32, o);
-          tmem_ld_wait();
-          tmem_ld_fence_regs(o);
 #pragma unroll
           for (int w = 0; w < 4; ++w) {                      // words of channels 0 4 1 5 2 6 3 7
-            auto x = [&](int i) { return __float_as_uint(__uint_as_float(o[8 * w + i]) * vf); };
+            auto x = [&](int i) { return __float_as_uint(__uint_as_float(o[ch][8 * w + i]) * vf); };
             const int k = ch * 8 + 2 * w;
             st_shared_v4(tile + r * 256 + ((k ^ (r & 15)) << 4), x(0), x(2), x(4), x(6));
             st_shared_v4(tile + r * 256 + (((k + 1) ^ (r & 15)) << 4), x(1), x(3), x(5), x(7));
@@ -636,11 +636,15 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         }
         __syncwarp();
         const int c = lane & 15;
-#pragma unroll 4
+        uint4 v[16];
+#pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int at = (warp & 3) * 32 + 2 * i + (lane >> 4);
-          *(reinterpret_cast<uint4*>(p.ws_o + (slot0 + at) * kD + half * 64) + c) = ld_shared_v4(tile + at * 256 + ((c ^ (at & 15)) << 4));
+          v[i] = ld_shared_v4(tile + at * 256 + ((c ^ (at & 15)) << 4));
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          *(reinterpret_cast<uint4*>(p.ws_o + (slot0 + (warp & 3) * 32 + 2 * i + (lane >> 4)) * kD + half * 64) + c) = v[i];
         __syncwarp();
       }
     } else if (ok) {
@@ -648,33 +652,41 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const float inv = l == 0.f ? 0.f : vf / l;
       // Rows leave through the unit's Q tile (all its MMAs are over), so that the writes are whole lines.
       const uint32_t at = row_start(smem_u32(q_s) + u * kTileBytes, r);
-#pragma unroll 1
-      for (int ch = 0; ch < kD / 32; ++ch) {
-        uint32_t o[32];
-        if (n_tiles > 0) {
-          tmem_ld32(taddr + kTmemO + ch * 32, o);
-          tmem_ld_wait();
-          tmem_ld_fence_regs(o);
-        } else {
+      uint32_t o[4][32];
+      if (n_tiles > 0) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
-        }
+        for (int ch = 0; ch < 4; ++ch) tmem_ld32(taddr + kTmemO + ch * 32, o[ch]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) tmem_ld_fence_regs(o[ch]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) o[i >> 5][i & 31] = 0u;
+      }
+#pragma unroll
+      for (int ch = 0; ch < 4; ++ch) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {                        // words of channels 0 4 1 5 2 6 3 7
-          auto x = [&](int i) { return l == 0.f ? 0.f : __uint_as_float(o[8 * w + i]) * inv; };
+          auto x = [&](int i) { return l == 0.f ? 0.f : __uint_as_float(o[ch][8 * w + i]) * inv; };
           st_shared_v4(chunk_at(at, 4 * ch + w), pack_bf16(x(0), x(2)), pack_bf16(x(4), x(6)), pack_bf16(x(1), x(3)),
                        pack_bf16(x(5), x(7)));
         }
       }
       __syncwarp();
       const int c = lane & 15;
-#pragma unroll 4
-      for (int i = 0; i < 16; ++i) {
-        const int qr_ = (warp & 3) * 32 + 2 * i + (lane >> 4), rr = (qr_ * by_g) >> 16, hh = qr_ - rr * G;
-        const int qrow = row0 + u * rpu + rr;
-        if (rr < rpu && qrow < q_len)
-          *(reinterpret_cast<uint4*>(p.out + (static_cast<size_t>(q_begin + qrow) * p.hq + hk * G + hh) * kD) + c) =
-              *reinterpret_cast<const uint4*>(q_s + u * kTileBytes + (chunk_at(row_start(0u, qr_), c)));
+#pragma unroll 1
+      for (int i0 = 0; i0 < 16; i0 += 8) {                   // eight reads, then eight writes: the compiler keeps their order
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          v[i] = ld_shared_v4(chunk_at(row_start(smem_u32(q_s) + u * kTileBytes, (warp & 3) * 32 + 2 * (i0 + i) + (lane >> 4)), c));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int qr_ = (warp & 3) * 32 + 2 * (i0 + i) + (lane >> 4), rr = (qr_ * by_g) >> 16, hh = qr_ - rr * G;
+          const int qrow = row0 + u * rpu + rr;
+          if (rr < rpu && qrow < q_len)
+            *(reinterpret_cast<uint4*>(p.out + (static_cast<size_t>(q_begin + qrow) * p.hq + hk * G + hh) * kD) + c) = v[i];
+        }
       }
     } else if (lane == 0) {
       report_status(p.status, kId, kWaitAccumTimeout);
