@@ -252,6 +252,16 @@ def test_decode_growing_maxima():
     _attend([1, 1], [400, 700], 8, 1, n_decode=2, q_scale=8.0, seed=4)
 
 
+def test_decode_values_near_zero_of_a_large_step():
+    """Rows that one token dominates, where codes of 8 and small centres make outputs a thousandth of a step: nothing of the
+    8 that comes off may be left."""
+    _attend([1] * 20, [9, 0, 11, 9, 2, 7, 15, 6, 3, 18, 11, 12, 14, 4, 11, 12, 3, 8, 3, 3], 24, 3, bs=64, n_decode=20, seed=84421,
+            q_scale=4.0, extra_pages=300)
+    _attend([1] * 20, [16, 156, 81, 98, 52, 181, 75, 24, 111, 1, 89, 23, 104, 39, 28, 136, 187, 45, 192, 87], 48, 3, bs=128,
+            n_decode=20, seed=990221, q_scale=4.0)
+    _attend([1] * 64, [1] * 64, 8, 8, n_decode=64, seed=5)
+
+
 @pytest.mark.parametrize("extra_pages", [1, WIDE])
 @pytest.mark.parametrize("order", [(0, 1, 2), (2, 1, 0), (1, 2, 0)])
 def test_decode_values_of_mixed_magnitude(order, extra_pages):
