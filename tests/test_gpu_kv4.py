@@ -131,6 +131,25 @@ def test_write_matches_the_cpu_backend_byte_for_byte():
         torch.testing.assert_close(kv4.read_rows(a.cpu(), live), kv4.read_rows(b, live), rtol=0, atol=0, equal_nan=True)
 
 
+@pytest.mark.parametrize("size", [1e-30, 1e-20, 1e-3, 1e15, 1e25, 3e38])
+def test_rows_of_any_size_and_infinite_ones(size):
+    """The sum of squares of a K row leaves fp32, or is lost beside eps (which counts in 64 bits); an infinity makes its own
+    group NaN and, through the norm, zeros of the rest."""
+    T, hq, hkv, bs = 600, 2, 2, 16
+    nb, qkv, qw, kw, cs, pos, slots = _write_case(T, hq, hkv, bs, 12)
+    qkv[:, hq * D:] = (qkv[:, hq * D:].float().clamp(-1, 1) * size).bfloat16()
+    qkv[1, hq * D + 3] = float("inf")
+    qkv[2, hq * D + D] = float("-inf")
+    qkv[4, hq * D] = float("nan")
+    gpu, cpu = _empty(nb, hkv, bs), [c.cpu() for c in _empty(nb, hkv, bs)]
+    _ops().qk_norm_rope_cache(qkv.to(DEV), qw.to(DEV), kw.to(DEV), 1e-6, cs.to(DEV), pos.to(DEV), slots.to(DEV), *gpu, hq, hkv, D)
+    _ops().qk_norm_rope_cache(qkv, qw, kw, 1e-6, cs, pos, slots, *cpu, hq, hkv, D)
+    live = slots[slots >= 0].long()
+    for a, b in zip(gpu, cpu):
+        torch.testing.assert_close(kv4.read_rows(a.cpu(), live), kv4.read_rows(b, live), rtol=0, atol=0, equal_nan=True)
+    assert bool(kv4.read_rows(cpu[0], live).any())
+
+
 def test_bad_slots_and_positions_are_reported_and_not_followed():
     T, hq, hkv, bs = 4, 2, 1, 16
     nb, qkv, qw, kw, cs, pos, slots = _write_case(T, hq, hkv, bs, 5)

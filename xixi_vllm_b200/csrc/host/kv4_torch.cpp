@@ -69,10 +69,10 @@ int integer(PyObject* o, const char* what) {
   return static_cast<int>(v);
 }
 
-float real(PyObject* o) {
+double real(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw Refused{nullptr, ""};
-  return static_cast<float>(v);
+  return v;
 }
 
 void bf16(const at::Tensor& t) {
@@ -167,7 +167,7 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor &qw = tensor(a[4], "q_w"), &kw = tensor(a[5], "k_w"), &cs = tensor(a[7], "cos_sin");
     bf16(qw);
     bf16(kw);
-    const float eps = real(a[6]);
+    const double eps = real(a[6]);
     const void* qwp = vector(qw, d, at::kBFloat16, c.dev, "q_w");
     const void* kwp = vector(kw, d, at::kBFloat16, c.dev, "k_w");
     const auto* csp = static_cast<const float*>(vector(cs, d, at::kFloat, c.dev, "cos_sin"));
@@ -236,7 +236,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto* tables = static_cast<const int*>(vector(bt, static_cast<int64_t>(B) * maxb, at::kInt, c.dev, "block_tables"));
     const auto* kv_lens = static_cast<const int*>(vector(lens, B, at::kInt, c.dev, "kv_lens"));
     const int* cu_q = np > 0 ? static_cast<const int*>(vector(tensor(a[3], "cu_q"), B + 1, at::kInt, c.dev, "cu_q")) : nullptr;
-    const float scale = real(a[9]);
+    const float scale = static_cast<float>(real(a[9]));
     if (!std::isfinite(scale)) refuse(PyExc_ValueError, "paged_attention: scale must be finite");
     const int sms = integer(a[13], "num_sms");
     auto* status = static_cast<int*>(vector(tensor(a[14], "status"), 1, at::kInt, c.dev, "status"));

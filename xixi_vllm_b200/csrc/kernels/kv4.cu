@@ -119,7 +119,7 @@ struct WriteParams {
   uint8_t* v_cache;
   int* status;
   long long split_stride;
-  float eps;
+  double eps;
   int splits, max_pos, tokens, hq, hkv, block_size, num_slots;
   int per_warp, kv_per_warp;         // pairs of heads a warp takes: of Q, of K and V
   int q_tasks, tasks;                // warps per token: for Q, and in all
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
       }
       float sa, sb;
       unpack_f32x2(ss2, sa, sb);
-      const float inv = rsqrtf(half_sum(sa + sb) / static_cast<float>(D) + p.eps);
+      const float inv = rsqrtf(half_sum(sa + sb) / static_cast<float>(D) + static_cast<float>(p.eps));
       const uint64_t inv2 = pack_f32x2(inv, inv);
       float o[8];
 #pragma unroll
@@ -268,9 +268,15 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
       double ss = 0.0;
 #pragma unroll
       for (int k = 0; k < 8; ++k) ss += static_cast<double>(x[k]) * x[k];
-      const double ms = half_sum(ss) * (1.0 / D) + static_cast<double>(p.eps);
-      double inv = rsqrtf(static_cast<float>(ms));            // one Newton step doubles its 22 bits
-      inv = inv + 0.5 * inv * (1.0 - ms * inv * inv);
+      double ms = half_sum(ss) * (1.0 / D) + p.eps;
+      if (ms > 1e38) {                                        // beyond fp32: the row at 2^-100 of its size
+        ms *= 0x1p-200;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] *= 0x1p-100f;
+      }
+      const float about = rsqrtf(static_cast<float>(ms));     // one Newton step doubles its 22 bits; 0 for an infinite row
+      double inv = about;
+      if (about > 0.f) inv += 0.5 * inv * (1.0 - ms * inv * inv);
       float k8[8];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {                           // value times weight is exact in fp32: 8 + 8 bits
@@ -358,7 +364,7 @@ int check_cache(int hkv, int d, int block_size, int num_blocks) {
 extern "C" {
 
 int xv_kv4_write(const void* qkv, const float* partials, int splits, long long split_stride, const void* q_w,
-                 const void* k_w, float eps, const float* cos_sin, int max_pos, const int* positions, const int* slots,
+                 const void* k_w, double eps, const float* cos_sin, int max_pos, const int* positions, const int* slots,
                  void* q_out, void* k_cache, void* v_cache, int tokens, int hq, int hkv, int d, int block_size,
                  int num_blocks, int* status, cudaStream_t stream) {
   if (tokens <= 0) return 0;

@@ -153,7 +153,7 @@ int xv_attn_prefill_tc_profile(const void* q, const void* k_cache, const void* v
 // num_blocks * block_size or more is not written and a position outside cos_sin's max_pos rows uses row 0; both are
 // reported through `status`.
 int xv_kv4_write(const void* qkv, const float* partials, int splits, long long split_stride, const void* q_w,
-                 const void* k_w, float eps, const float* cos_sin, int max_pos, const int* positions, const int* slots,
+                 const void* k_w, double eps, const float* cos_sin, int max_pos, const int* positions, const int* slots,
                  void* q_out, void* k_cache, void* v_cache, int tokens, int hq, int hkv, int d, int block_size,
                  int num_blocks, int* status, cudaStream_t stream);
 // bf16 values [tokens, hkv, d] of the rows at `slots` (negative or out of range: zeros, the latter reported).
@@ -302,6 +302,7 @@ typedef struct XvModelDesc {
                                       // arena's h / residual are received from / sent to the neighbours
   int kv4;                            // 1: k_cache / v_cache hold 4-bit rows (common/kv4.cuh)
   int max_pos;                        // rows of cos_sin
+  double kv4_eps;                     // eps in the 64 bits that K of a 4-bit cache is normalised in
 } XvModelDesc;
 
 typedef struct XvBatchDesc {

@@ -38,7 +38,7 @@ class ModelDesc(ctypes.Structure):
                 ("num_kv_blocks", _i32), ("prefill_tc", _i32), ("tp_push", _i32), ("tp_push_max", _i32),
                 ("tp_one_shot_max", _i32), ("tp_pull_two_shot", _i32), ("tp_defer_row_wait", _i32), ("is_first", _i32),
                 ("is_last", _i32),
-                ("kv4", _i32), ("max_pos", _i32)]
+                ("kv4", _i32), ("max_pos", _i32), ("kv4_eps", ctypes.c_double)]
 
 
 class BatchDesc(ctypes.Structure):
@@ -99,6 +99,7 @@ class NativeForward:
         d.kv4 = 1 if kv.int4 else 0
         d.prefill_tc = int(os.environ.get("XV_ATTN_PREFILL", "tc") != "mma")
         d.eps, d.attn_scale = float(cfg.rms_norm_eps), float(attn0.scale)
+        d.kv4_eps = float(cfg.rms_norm_eps)
         d.gate_up_interleaved = 1 if first.mlp.gate_up_proj.interleave else 0
         if self.is_first:
             d.vocab_start, d.vocab_rows = m.embed_tokens.vocab_start, m.embed_tokens.weight.shape[0]
