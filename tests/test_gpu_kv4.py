@@ -447,6 +447,13 @@ def test_rows_before_position_0_and_behind_the_last_sequence_are_zero(extra_page
     _cuda().check_status()
 
 
+@pytest.mark.parametrize("power", [100, -100])
+@pytest.mark.parametrize("extra_pages", [1, 300, WIDE])
+def test_values_near_the_ends_of_the_range(power, extra_pages):
+    """K and V of 2^100 or 2^-100 times normal values against queries that bring the scores back to size."""
+    _attend([1, 1, 30, 140], [40, 700, 60, 333], 6, 2, n_decode=2, v_scale=2.0 ** power, q_scale=2.0 ** -power, extra_pages=extra_pages)
+
+
 def test_scores_below_the_smallest_float_leave_equal_weights():
     """The scale of a score underflows; what the mask takes out still has weight 0, not NaN."""
     _attend([1, 30, 200], [40, 60, 200], 4, 2, n_decode=1, v_scale=2.0 ** -60, q_scale=2.0 ** -70)

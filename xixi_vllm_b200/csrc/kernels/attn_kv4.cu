@@ -182,7 +182,7 @@ struct Query {
           most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
         }
     }
-    const int e = max(static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14, -80);
+    const int e = max(static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14, -120);
     unit = power_of_two(e) * 16777216.f;                   // the codes are n 2^-24
     const float even = power_of_two(-e) * sign, odd = even * 0.0625f;
 #pragma unroll

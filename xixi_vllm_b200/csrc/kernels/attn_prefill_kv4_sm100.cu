@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     auto choose = [](int e, uint32_t bits) {
       const int top = static_cast<int>(bits >> 23) - 127;
       if (bits != 0 && (top - e > 14 || top - e < 7)) e = top - 12;
-      return max(-100, min(100, e));
+      return max(-120, min(120, e));
     };
     int ek = 0, ev = 0;
     // A wait that runs out is only noted: the four warps leave together, at the barrier of the next tile.
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
           }
         }
       }
-      const int e = max(-100, min(100, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14));
+      const int e = max(-120, min(120, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14));
       const float f = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
       q_power = pow2(e);
 #pragma unroll
