@@ -505,6 +505,12 @@ def test_refusals():
                        torch.zeros(1, 1, 16, 40, dtype=torch.uint8, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV), 64)
     with pytest.raises(ValueError, match="slots"):
         ops.read_cache(k, v, torch.zeros(1, dtype=torch.int64, device=DEV), D)
+    attn.block_tables = torch.zeros(2, 4, dtype=torch.int32, device=DEV)[:, ::2]
+    with pytest.raises(ValueError, match="block_tables"):
+        ops.paged_attention(q, k, v, attn, 0.1, 4, 2, D)
+    attn.block_tables = attn.block_tables.contiguous()
+    with pytest.raises(RuntimeError, match="misaligned"):
+        ops.paged_attention(torch.zeros(2 * 4 * D + 1, device=DEV).bfloat16()[1:].view(2, 4 * D), k, v, attn, 0.1, 4, 2, D)
     attn.kv_lens = attn.kv_lens.long()
     with pytest.raises(ValueError, match="kv_lens"):
         ops.paged_attention(q, k, v, attn, 0.1, 4, 2, D)
@@ -542,6 +548,76 @@ def test_two_streams_and_graph_replay_do_not_share_scratch():
         assert torch.equal(eager, runs[0][3])
         for _, _, out, want, _ in runs:
             assert torch.equal(out, want)
+    _cuda().check_status()
+
+
+def test_split_chunks_on_two_streams_do_not_share_scratch():
+    """Two captured chunk calls whose KV range is split, replayed at the same time on two streams."""
+    ops = _ops()
+    runs = []
+    for seed in (1, 2):
+        k, v = _random(80, 2, 16, seed)
+        g = torch.Generator().manual_seed(seed)
+        q = torch.randn(40, 8 * D, generator=g).bfloat16().to(DEV)
+        i32 = dict(dtype=torch.int32, device=DEV)
+        attn = AttnBatch(torch.tensor([0, 40], **i32), torch.tensor([1200], **i32), torch.randperm(80, generator=g)[None].to(**i32),
+                         1, 0, 40, 1200, 40)
+        want = ops.paged_attention(q, k, v, attn, 0.09, 8, 2, D).clone()
+        torch.cuda.synchronize()
+        gr, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(gr, stream=s):
+            out = ops.paged_attention(q, k, v, attn, 0.09, 8, 2, D)
+        runs.append((gr, s, out, want, (q, k, v, attn)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for gr, s, out, want, _ in runs:
+            with torch.cuda.stream(s):
+                gr.replay()
+        torch.cuda.synchronize()
+        for _, _, out, want, _ in runs:
+            assert torch.equal(out, want)
+    _cuda().check_status()
+
+
+def test_captured_step_follows_its_inputs():
+    """One graph of append, decode attention and read-back on a side stream: every replay takes what the inputs hold then,
+    padded rows (slot -1, no cached tokens) among them."""
+    ops, B, hq, hkv, bs = _ops(), 5, 8, 2, 16
+    k, v = _random(64, hkv, bs, 4)
+    ek, ev = k.clone(), v.clone()
+    g = torch.Generator().manual_seed(4)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    qw, kw = (torch.exp(0.3 * torch.randn(D, generator=g)).bfloat16().to(DEV) for _ in range(2))
+    cs = cpu_ref.build_cos_sin_cache(D, 5000, 1e6).to(DEV)
+    qkv = torch.zeros(B, (hq + 2 * hkv) * D, device=DEV).bfloat16()
+    pos, slots, lens = (torch.zeros(B, **i32) for _ in range(3))
+    slots.fill_(-1)
+    table = torch.arange(60, **i32).view(B, 12).contiguous()
+    attn = AttnBatch(torch.arange(B + 1, **i32), lens, table, B, B, 1, 192, B)
+
+    def step(k, v):
+        q = ops.qk_norm_rope_cache(qkv, qw, kw, 1e-6, cs, pos, slots, k, v, hq, hkv, D)
+        return (ops.paged_attention(q, k, v, attn, 0.09, hq, hkv, D), *ops.read_cache(k, v, slots, D))
+
+    step(k, v)
+    torch.cuda.synchronize()
+    gr, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(gr, stream=s):
+        got = step(k, v)
+    for i in range(6):
+        n = torch.randint(1, 190, (B,), generator=g)
+        live = torch.arange(B) != i % B
+        qkv.copy_(torch.randn(qkv.shape, generator=g))
+        pos.copy_(n)
+        lens.copy_(torch.where(live, n + 1, 0))
+        slots.copy_(torch.where(live, torch.arange(B) * 192 + n, -1))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step(ek, ev)):
+            assert torch.equal(a, b)
+        assert torch.equal(k, ek) and torch.equal(v, ev) and not got[0][i % B].any() and not got[1][i % B].any()
     _cuda().check_status()
 
 
