@@ -13,7 +13,7 @@
 //                        The tensor pipe aligns its sums by a subnormal's nominal exponent, -14: with n 2^-24 a sum of V
 //                        loses what is below 2^-14 of the largest P s, which shows where 8 - 8 should leave 0 (an output
 //                        of 5e-4 was off by 3e-5). So V's even codes are moved to n 2^-20 as well, a shift each (256 sequences
-//                        131 -> 136 us); K's stay (a score loses 1e-5 of max |q| s; both moved: 142).
+//                        131 -> 137 us); K's stay (a score loses 1e-5 of max |q| s; both moved: 143).
 //                        K's lanes own 16-byte pieces of a row, V's lanes pair two tokens with PRMT, so codes go from
 //                        shared memory to MMA operands in registers. Warps are merged through shared memory, splits
 //                        through the cluster's distributed shared memory: one launch, no workspace.
@@ -21,12 +21,13 @@
 //   kv4_join_kernel      partial results of pairs that span runs joined by a second kernel.
 // Prompt chunks: attn_prefill_kv4_sm100.cu.
 //
-// What bounds it: instructions, not memory: 293 of them for the 2304 bytes of 16 tokens of a head, 104 of which take the
-// codes apart. 96 sequences of 2048 tokens, 8 KV heads: 57% of the issue slots, 53% of the ALU, 31% of the tensor pipe,
-// 4.1 TB/s. 256 sequences of 256-4096 tokens 136 us (4.7 TB/s), one of 40960 19.8 us (2.4 TB/s). On the way: codes as bf16
-// integers with shifts and a subtraction 333 instructions and 153 us, a unit at a time 424 and 189, bulk copies in place
-// of cp.async 241. 128 registers, for four CTAs an SM, spill: 149 us. Small batches are a chain of dependent reads (length,
-// page, codes), about 3000 cycles before the first product.
+// What bounds it: instructions, not memory: 293 of them for the 2304 bytes of 16 tokens of a head (271 for groups of up to
+// four query heads, whose columns hold both channel groups: 256 sequences 137 -> 129 us, 32 11.7 -> 11.4), 104 of which
+// take the codes apart. 96 sequences of 2048 tokens, 32 / 8 heads: 57% of the issue slots, 52% of the ALU, 30% of the tensor
+// pipe, 4.3 TB/s. 256 sequences of 256-4096 tokens 129 us (5.0 TB/s), one of 40960 (64 / 8 heads) 19.8 us (2.4 TB/s). On the way:
+// codes as bf16 integers with shifts and a subtraction 333 instructions and 153 us, a unit at a time 424 and 189, bulk copies
+// in place of cp.async 241. 128 registers, for four CTAs an SM, spill: 149 us. Small batches are a chain of dependent
+// reads (length and page, codes), about 2500 cycles before the first product.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -34,6 +35,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <atomic>
 
 #include "../common/kv4.cuh"
@@ -139,9 +141,11 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }       // e in -126 .. 127
 
-// The group's queries as B operands. NT: column tiles of 8 query heads.
-template <int NT>
+// The group's queries as B operands. NT: column tiles of 8 query heads. TWIN (up to four heads): column n + 4 is head n
+// again, columns 0-3 hold its channels of group 0 and zeros, columns 4-7 those of group 1.
+template <int NT, bool TWIN>
 struct Query {
+  static_assert(!TWIN || NT == 1);
   // MMA (word w, half hf) of lane (g, t) multiplies channels 32 t + 8 w + 2 hf + {0, 4, 1, 5}. Q is held in fp16, scaled by
   // a power of two that takes the group's largest value to 2^14 .. 2^15 (exact down to 2^-28 of it); the odd channels meet
   // codes that are 16 times too large and carry another 1 / 16.
@@ -156,16 +160,17 @@ struct Query {
   __device__ __forceinline__ void fetch(const Params& p, size_t row, int G, int g, int t) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (row + nt * 8 + g) * kD + 32 * t);
+      const int head = TWIN ? g & 3 : nt * 8 + g;
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (row + head) * kD + 32 * t);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const uint4 r = nt * 8 + g < G ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
+        const uint4 r = head < G ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
         raw[nt][4 * w] = r.x; raw[nt][4 * w + 1] = r.y; raw[nt][4 * w + 2] = r.z; raw[nt][4 * w + 3] = r.w;
       }
     }
   }
   // Makes the operands of what fetch() brought; `sign`: applied to Q.
-  __device__ __forceinline__ void convert(float sign, int t) {
+  __device__ __forceinline__ void convert(float sign, int g, int t) {
     uint32_t top = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -201,6 +206,7 @@ struct Query {
         for (int hf = 0; hf < 2; ++hf) {
           f[nt][w][hf][0] = pack_f16(x[2 * hf] * even, x[2 * hf + 4] * even);
           f[nt][w][hf][1] = pack_f16(x[2 * hf + 1] * odd, x[2 * hf + 5] * odd);
+          if (TWIN && (w & 1) != (g >> 2)) f[nt][w][hf][0] = f[nt][w][hf][1] = 0u;
         }
       }
 #pragma unroll
@@ -215,6 +221,7 @@ struct Query {
       const float q2 = __bfloat162float(__float2bfloat16(qs - q1)), b2 = __bfloat162float(__float2bfloat16(bs - b1));
       c[nt][0] = t < 2 ? pack_bf16(b1, q1) : pack_bf16(b2, q2);
       c[nt][1] = t < 2 ? pack_bf16(bs - b1 - b2, qs - q1 - q2) : 0u;
+      if (TWIN && g >= 4) c[nt][0] = c[nt][1] = 0u;        // both groups' centres count once
     }
   }
 };
@@ -246,7 +253,7 @@ struct Softmax {
   }
 
   // One slot of kPair units, of which the first `mine` tokens count. lane_k .. lane_v1: this lane's places in the slot.
-  __device__ __forceinline__ void add(const Query<NT>& q, const uint8_t* lane_k, const uint8_t* lane_p, const uint8_t* lane_v0,
+  __device__ __forceinline__ void add(const Query<NT, false>& q, const uint8_t* lane_k, const uint8_t* lane_p, const uint8_t* lane_v0,
                                       const uint8_t* lane_v1, int mine, int tok, int t, float scale, float lag) {
     float x[kPair][NT][4];               // (row g: heads 2t, 2t + 1), (row g + 8: the same)
 #pragma unroll
@@ -422,12 +429,199 @@ struct Softmax {
         m[nt][hd] = m[nt][hd] == kNoMax ? kNoMax : m[nt][hd] * unit;
       }
   }
-  // Channels 16 g + 4 j .. + 3 of head (nt, hd) after finish().
-  __device__ __forceinline__ float4 quad(int nt, int hd, int j) const {
-    const float(&a)[4] = o[nt][j >> 1][2 * (j & 1)], (&b)[4] = o[nt][j >> 1][2 * (j & 1) + 1];
-    return hd ? make_float4(a[1], a[3], b[1], b[3]) : make_float4(a[0], a[2], b[0], b[2]);
+  // After finish(), f(head, first of four channels, their sums, m, l) for what this lane (g, t) holds.
+  template <typename F>
+  __device__ __forceinline__ void each(int g, int t, F f) const {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int hd = 0; hd < 2; ++hd)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float(&a)[4] = o[nt][j >> 1][2 * (j & 1)], (&b)[4] = o[nt][j >> 1][2 * (j & 1) + 1];
+          f(nt * 8 + 2 * t + hd, 16 * g + 4 * j, make_float4(a[hd], a[2 + hd], b[hd], b[2 + hd]), m[nt][hd], l[nt][hd]);
+        }
   }
 };
+
+// The same for up to four heads on the columns of Query<1, true>: a lane has one group (t >> 1) of heads 2 (t & 1) + {0, 1}, so
+// parameters, products with them and the operands of the second MMA are half as many; scores are the sum over lane pairs.
+struct TwinSoftmax {
+  float o[2][4][4];                // as Softmax::o; valid where [group] is the lane's own
+  float cen[2], off[4];            // of the lane's group
+  float m[2], l[2];
+  float vs, v_most;
+
+  __device__ __forceinline__ void clear() {
+    vs = 1.f;
+    v_most = 0.f;
+#pragma unroll
+    for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[gr][i][0] = o[gr][i][1] = o[gr][i][2] = o[gr][i][3] = 0.f;
+    cen[0] = cen[1] = 0.f;
+    off[0] = off[1] = off[2] = off[3] = 0.f;
+    m[0] = m[1] = kNoMax;
+    l[0] = l[1] = 0.f;
+  }
+
+  __device__ __forceinline__ void add(const Query<1, true>& q, const uint8_t* lane_k, const uint8_t* lane_p, const uint8_t* lane_v0,
+                                      const uint8_t* lane_v1, int mine, int tok, int t, float scale, float lag) {
+    const uint8_t* lane_s = lane_p + (t >> 1) * 4;       // the lane's group's parameters
+    const uint8_t* lane_c = lane_p + (t & 1) * 4;        // those that the centres' MMA takes from it
+    float x[kPair][4];
+#pragma unroll
+    for (int u = 0; u < kPair; ++u) {
+      const uint4 k0 = *reinterpret_cast<const uint4*>(lane_k + u * kUnitSlot);
+      const uint4 k1 = *reinterpret_cast<const uint4*>(lane_k + u * kUnitSlot + 8 * 64);
+      const uint32_t s0 = *reinterpret_cast<const uint32_t*>(lane_s + u * kUnitSlot);
+      const uint32_t s1 = *reinterpret_cast<const uint32_t*>(lane_s + u * kUnitSlot + 64);
+      const uint32_t w0 = *reinterpret_cast<const uint32_t*>(lane_c + u * kUnitSlot);
+      const uint32_t w1 = *reinterpret_cast<const uint32_t*>(lane_c + u * kUnitSlot + 64);
+      const uint32_t ka[4] = {k0.x, k0.y, k0.z, k0.w}, kb[4] = {k1.x, k1.y, k1.z, k1.w};
+      const uint32_t ac[4] = {w0, w1, w0, w1};
+      float s[4], sc[4];
+      mma_bf16(sc, ac, q.c[0][0], q.c[0][1]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const uint32_t wa = ka[w] >> (8 * hf), wb = kb[w] >> (8 * hf);
+          const uint32_t a[4] = {wa & kLow, wb & kLow, wa & kHigh, wb & kHigh};
+          if (w == 0 && hf == 0) mma_first(s, a, q.f[0][w][hf][0], q.f[0][w][hf][1]);
+          else mma_more(s, a, q.f[0][w][hf][0], q.f[0][w][hf][1]);
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[u][e] = fmaf(kv4::par_s(e < 2 ? s0 : s1), s[e], sc[e]);
+        x[u][e] += __shfl_xor_sync(0xffffffffu, x[u][e], 2);
+      }
+    }
+    const bool ragged = mine < 16 * kPair;               // warp-uniform
+    uint32_t vp[kPair][2];                               // V's parameters of this lane's tokens and group
+    float s_most = 0.f;
+#pragma unroll
+    for (int u = 0; u < kPair; ++u) {
+      vp[u][0] = *reinterpret_cast<const uint32_t*>(lane_s + u * kUnitSlot + kv4::kUnitBytes);
+      vp[u][1] = *reinterpret_cast<const uint32_t*>(lane_s + u * kUnitSlot + kv4::kUnitBytes + 64);
+      if (ragged) {                                      // as in Softmax
+        if (16 * u + tok >= mine) {
+          x[u][0] = x[u][1] = -CUDART_INF_F;
+          vp[u][0] = 0u;
+        }
+        if (16 * u + tok + 8 >= mine) {
+          x[u][2] = x[u][3] = -CUDART_INF_F;
+          vp[u][1] = 0u;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) s_most = fmaxf(s_most, fabsf(kv4::par_s(vp[u][r])));
+    }
+    bool grow = s_most > v_most;
+    float mx[2];
+#pragma unroll
+    for (int hd = 0; hd < 2; ++hd) {
+      mx[hd] = fmaxf(fmaxf(x[0][hd], x[0][2 + hd]), fmaxf(x[1][hd], x[1][2 + hd]));
+      grow |= mx[hd] > m[hd] + lag;
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+      float back = 1.f;                                  // of the sums of P * s
+#pragma unroll
+      for (int d = 2; d <= 16; d <<= 1) s_most = fmaxf(s_most, __shfl_xor_sync(0xffffffffu, s_most, d));
+      if (s_most > v_most) {
+        const int e = min(max((__float_as_int(s_most) >> 23) - 127 - 2, -120), 119);
+        const float now = power_of_two(-e);
+        back = now / vs;
+        vs = now;
+        v_most = power_of_two(e + 7);
+      }
+#pragma unroll
+      for (int hd = 0; hd < 2; ++hd) {
+        float mn = fmaxf(m[hd], mx[hd]);
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 4));
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 8));
+        mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 16));
+        const float cr = exp2f((m[hd] - mn) * scale);
+        m[hd] = mn;
+        l[hd] *= cr;
+        cen[hd] *= cr;
+        off[hd] *= cr * back;
+#pragma unroll
+        for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            o[gr][j][hd] *= cr * back;
+            o[gr][j][2 + hd] *= cr * back;
+          }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kPair; ++u) {
+      uint2 vw[4];                                       // tokens of rows 2t, 2t + 1, then the same 8 further
+      vw[0] = *reinterpret_cast<const uint2*>(lane_v0 + u * kUnitSlot);
+      vw[1] = *reinterpret_cast<const uint2*>(lane_v1 + u * kUnitSlot);
+      vw[2] = *reinterpret_cast<const uint2*>(lane_v0 + u * kUnitSlot + 8 * 64);
+      vw[3] = *reinterpret_cast<const uint2*>(lane_v1 + u * kUnitSlot + 8 * 64);
+      float pr[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][e], scale, -m[e & 1] * scale));
+      l[0] += pr[0] + pr[2];
+      l[1] += pr[1] + pr[3];
+      const float v0 = kv4::par_s(vp[u][0]) * vs, v1 = kv4::par_s(vp[u][1]) * vs;
+      const float c0 = kv4::par_c(vp[u][0]), c1 = kv4::par_c(vp[u][1]);
+      const uint32_t p0 = movmatrix_trans(pack_f16(pr[0] * v0, pr[1] * v0)), p1 = movmatrix_trans(pack_f16(pr[2] * v1, pr[3] * v1));
+      cen[0] = fmaf(pr[0], c0, fmaf(pr[2], c1, cen[0]));
+      cen[1] = fmaf(pr[1], c0, fmaf(pr[3], c1, cen[1]));
+      const uint32_t a8[4] = {kMinus8, kMinus8, kMinus8, kMinus8};
+      mma_more(off, a8, p0, p1);
+#pragma unroll
+      for (int gr = 0; gr < 2; ++gr) {
+        const uint32_t w0 = gr ? vw[0].y : vw[0].x, w1 = gr ? vw[1].y : vw[1].x, w2 = gr ? vw[2].y : vw[2].x,
+                       w3 = gr ? vw[3].y : vw[3].x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                    // byte of the word: channels 2 i, 2 i + 1
+          const uint32_t u0 = __byte_perm(w0, w1, 0x4400 + 0x1111 * i), u1 = __byte_perm(w2, w3, 0x4400 + 0x1111 * i);
+          const uint32_t a[4] = {(u0 << 4) & kHigh, u0 & kHigh, (u1 << 4) & kHigh, u1 & kHigh};
+          mma_more(o[gr][i], a, p0, p1);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish(float unit) {
+    const float back = 1.f / vs;
+#pragma unroll
+    for (int hd = 0; hd < 2; ++hd) {
+#pragma unroll
+      for (int x = 4; x <= 16; x <<= 1) {
+        l[hd] += __shfl_xor_sync(0xffffffffu, l[hd], x);
+        cen[hd] += __shfl_xor_sync(0xffffffffu, cen[hd], x);
+      }
+#pragma unroll
+      for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[gr][i][hd] = fmaf(fmaf(o[gr][i][hd], 1048576.f, off[hd]), back, cen[hd]);                    // n 2^-20
+          o[gr][i][2 + hd] = fmaf(fmaf(o[gr][i][2 + hd], 1048576.f, off[hd]), back, cen[hd]);
+        }
+      m[hd] = m[hd] == kNoMax ? kNoMax : m[hd] * unit;
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(int g, int t, F f) const {
+    const bool second = t >= 2;
+#pragma unroll
+    for (int hd = 0; hd < 2; ++hd)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        auto own = [&](int i, int e) { return second ? o[1][i][e] : o[0][i][e]; };
+        f(2 * (t & 1) + hd, 16 * g + 8 * (t >> 1) + 4 * j,
+          make_float4(own(2 * j, hd), own(2 * j, 2 + hd), own(2 * j + 1, hd), own(2 * j + 1, 2 + hd)), m[hd], l[hd]);
+      }
+  }
+};
+template <int NT, bool TWIN>
+using SoftmaxOf = std::conditional_t<TWIN, TwinSoftmax, Softmax<NT>>;
 
 // A warp's ring of slots in shared memory and the walk over units of one (sequence, KV head) that fills it. Slot k takes the
 // units first + k stride and the next one, below `end`. A unit in a slot: K's 1152 bytes, then V's; five cp.async of 16 bytes
@@ -515,8 +709,8 @@ struct Scale {
   __device__ __forceinline__ float of(float unit) const { return fmaxf(scale * unit, 1e-36f); }
 };
 
-// A cluster of CTAs, one per KV split, per (sequence, KV head). NT: column tiles of 8 query heads; W: warps.
-template <int NT, int W>
+// A cluster of CTAs, one per KV split, per (sequence, KV head). NT, TWIN: as in Query; W: warps.
+template <int NT, int W, bool TWIN>
 __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sm_m[W][8 * NT], sm_l[W][8 * NT];
@@ -528,7 +722,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
   const int G = p.hq / p.hkv;
   uint8_t* ring_mem = smem + warp * kStages * kSlot;
   grid_dep_wait();
-  Query<NT> q;
+  Query<NT, TWIN> q;
   q.fetch(p, static_cast<size_t>(b) * p.hq + h * G, G, g, t);      // first: everything else hangs on two more reads
   // Slots are dealt to the warps in turn: which pages a warp reads first does not hang on the length.
   const int first = (split * W + warp) * kPair, stride = p.splits * W * kPair;
@@ -540,9 +734,9 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) ring.issue(p);
   const Scale sc(p.scale_log2);
-  q.convert(sc.sign, t);
+  q.convert(sc.sign, g, t);
   const float scale = sc.of(q.unit), lag = kLazy / scale;
-  Softmax<NT> st;
+  SoftmaxOf<NT, TWIN> st;
   st.clear();
 
   const int tok = token_of_row(g);
@@ -564,21 +758,14 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
   float* sm_o = reinterpret_cast<float*>(smem);                    // [warp][8 NT][128]
   float* part_o = sm_o + W * 8 * NT * kD;                          // [8 NT][128]
   static_assert((W + 1) * 8 * NT * kD * 4 <= decode_smem(W));
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int hd = 0; hd < 2; ++hd) {
-      const int head = nt * 8 + 2 * t + hd;
-      if (head < G) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<float4*>(&sm_o[(warp * 8 * NT + head) * kD + 16 * g + 4 * j]) = st.quad(nt, hd, j);
-        if (g == 0) {
-          sm_m[warp][head] = st.m[nt][hd];
-          sm_l[warp][head] = st.l[nt][hd];
-        }
-      }
+  st.each(g, t, [&](int head, int channel, const float4& v, float m, float l) {
+    if (head >= G) return;
+    *reinterpret_cast<float4*>(&sm_o[(warp * 8 * NT + head) * kD + channel]) = v;
+    if (channel == 0) {
+      sm_m[warp][head] = m;
+      sm_l[warp][head] = l;
     }
+  });
   __syncthreads();
   // Four channels a thread. Sums stay unnormalised until the last join.
   for (int idx = threadIdx.x; idx < G * (kD / 4); idx += blockDim.x) {
@@ -636,7 +823,7 @@ struct Shares {
 };
 constexpr int kShareWarps = 4, kMinRun = 4;
 
-template <int NT>
+template <int NT, bool TWIN>
 __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_kernel(const Params p, const Shares ws, int num_seqs) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int T = kShareWarps * 32;
@@ -742,11 +929,11 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
 
   for (;;) {
     const int n = min(units - first, todo);
-    Query<NT> q;
+    Query<NT, TWIN> q;
     q.fetch(p, static_cast<size_t>(b) * p.hq + h * G, G, g, t);
-    q.convert(sc.sign, t);
+    q.convert(sc.sign, g, t);
     const float scale = sc.of(q.unit), lag = kLazy / scale;
-    Softmax<NT> st;
+    SoftmaxOf<NT, TWIN> st;
     st.clear();
     int mine = min(kv_len - first * 16, n * 16);
     for (int i = 0; i < n; i += kPair, mine -= 16 * kPair) {
@@ -761,24 +948,15 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
     const bool whole = n == units;
     const int pair = b * p.hkv + h;
     const size_t slot = static_cast<size_t>(run) + pair;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int hd = 0; hd < 2; ++hd) {
-        const int head = nt * 8 + 2 * t + hd;
-        if (head < G) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 v = st.quad(nt, hd, j);
-            if (whole)
-              store_out(p.out + (static_cast<size_t>(pair) * G + head) * kD + 16 * g + 4 * j, v, st.l[nt][hd]);
-            else
-              *reinterpret_cast<float4*>(ws.o + (slot * 8 * NT + head) * kD + 16 * g + 4 * j) = v;
-          }
-          if (!whole && g == 0)
-            *reinterpret_cast<float2*>(ws.ml + (slot * 8 * NT + head) * 2) = make_float2(st.m[nt][hd], st.l[nt][hd]);
-        }
+    st.each(g, t, [&](int head, int channel, const float4& v, float m, float l) {
+      if (head >= G) return;
+      if (whole) {
+        store_out(p.out + (static_cast<size_t>(pair) * G + head) * kD + channel, v, l);
+      } else {
+        *reinterpret_cast<float4*>(ws.o + (slot * 8 * NT + head) * kD + channel) = v;
+        if (channel == 0) *reinterpret_cast<float2*>(ws.ml + (slot * 8 * NT + head) * 2) = make_float2(m, l);
       }
+    });
     todo -= n;
     if (todo == 0) break;
     first = 0;
@@ -897,10 +1075,12 @@ int allow_decode_kernels() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return XV_ERR_LAUNCH;
   if (done[dev].load(std::memory_order_acquire)) return 0;
   const auto at = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  if (cudaFuncSetAttribute(kv4_decode_kernel<1, 4>, at, decode_smem(4)) != cudaSuccess ||
-      cudaFuncSetAttribute(kv4_decode_kernel<2, 4>, at, decode_smem(4)) != cudaSuccess ||
-      cudaFuncSetAttribute(kv4_share_kernel<1>, at, decode_smem(kShareWarps)) != cudaSuccess ||
-      cudaFuncSetAttribute(kv4_share_kernel<2>, at, decode_smem(kShareWarps)) != cudaSuccess)
+  if (cudaFuncSetAttribute(kv4_decode_kernel<1, 4, true>, at, decode_smem(4)) != cudaSuccess ||
+      cudaFuncSetAttribute(kv4_decode_kernel<1, 4, false>, at, decode_smem(4)) != cudaSuccess ||
+      cudaFuncSetAttribute(kv4_decode_kernel<2, 4, false>, at, decode_smem(4)) != cudaSuccess ||
+      cudaFuncSetAttribute(kv4_share_kernel<1, true>, at, decode_smem(kShareWarps)) != cudaSuccess ||
+      cudaFuncSetAttribute(kv4_share_kernel<1, false>, at, decode_smem(kShareWarps)) != cudaSuccess ||
+      cudaFuncSetAttribute(kv4_share_kernel<2, false>, at, decode_smem(kShareWarps)) != cudaSuccess)
     return XV_ERR_LAUNCH;
   done[dev].store(true, std::memory_order_release);
   return 0;
@@ -951,8 +1131,9 @@ int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const
   if (int rc = allow_decode_kernels()) return rc;
   p.splits = splits;
   const int nt = hq / hkv > 8 ? 2 : 1;
+  const bool twin = hq / hkv <= 4;             // half the columns would be idle
   if (splits > 0) {
-    launch_pdl_cluster(nt == 1 ? kv4_decode_kernel<1, 4> : kv4_decode_kernel<2, 4>, dim3(splits, hkv, num_seqs), dim3(4 * 32),
+    launch_pdl_cluster(twin ? kv4_decode_kernel<1, 4, true> : nt == 1 ? kv4_decode_kernel<1, 4, false> : kv4_decode_kernel<2, 4, false>, dim3(splits, hkv, num_seqs), dim3(4 * 32),
                        decode_smem(4), stream, splits, p);
     return launch_ok();
   }
@@ -966,7 +1147,7 @@ int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const
   const size_t slots = static_cast<size_t>(ctas) * kShareWarps + static_cast<size_t>(num_seqs) * hkv;
   ws.ml = ws.o + slots * 8 * nt * kD;
   ws.begin = reinterpret_cast<int*>(ws.ml + slots * 8 * nt * 2);
-  launch_pdl(nt == 1 ? kv4_share_kernel<1> : kv4_share_kernel<2>, dim3(ctas), dim3(kShareWarps * 32), decode_smem(kShareWarps),
+  launch_pdl(twin ? kv4_share_kernel<1, true> : nt == 1 ? kv4_share_kernel<1, false> : kv4_share_kernel<2, false>, dim3(ctas), dim3(kShareWarps * 32), decode_smem(kShareWarps),
              stream, p, ws, num_seqs);
   if (int rc = launch_ok()) return rc;
   // Warps per row by the partials that a pair may have, its share of the runs. Both kernels with 16 / 4 / 1 warps a row:

@@ -7,7 +7,7 @@
 //   kv4_read_kernel  - the bf16 values of a list of slots. A warp per token.
 //
 // Both should be bound by memory: the writer moves (hq + 2 hkv) 256 + hq 256 + hkv 144 bytes a token, the reader
-// hkv 2 (72 + 256). The writer is as much bound by its instructions (3700 a token of 32 + 2 x 8 heads, 70% of the issue
+// hkv 2 (72 + 256). The writer is as much bound by its instructions (3500 a token of 32 + 2 x 8 heads, 67% of the issue
 // slots): 8192 tokens 41.0 us (4.3 TB/s; with one pair sent for ahead in registers 48.5), 997 of 40 + 2 x 8 7.0 us.
 // The reader runs at the copy rate: 32768 tokens of 8 heads 26.1 us (6.6 TB/s).
 //
