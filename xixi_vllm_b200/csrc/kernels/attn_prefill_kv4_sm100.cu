@@ -16,8 +16,8 @@
 // which 1590 are the exponentials (1024 of MUFU), 840 S's way through tensor memory and the maximum, 1030 the two MMAs and
 // the rest hand-over; the other unit's exponentials lie in between. Both units' MMAs are 2050 of it. Beside them the
 // dequantisers' loop (770 instructions a warp) takes 4200 cycles when all SMs are busy. 4 x 2048 rows behind 512 tokens, 32
-// query heads: 273 us, 754 TFLOP/s. Measured against: registers 2 x 184 + 96 + 48 277 us, 2 x 192 + 80 + 48 286,
-// 2 x 168 + 112 + 64 287; Q loaded by the lanes that convert it 285.
+// query heads: 268 us, 769 TFLOP/s. On the way: Q loaded by the lanes that convert it 285; then, at 273 with these
+// registers, 277 with 2 x 184 + 96 + 48, 286 with 2 x 192 + 80 + 48, 287 with 2 x 168 + 112 + 64.
 //
 // fp16 operands, not bf16: a dequantised value c + s (n - 8) has more than bf16's 8 bits, and its rounding (2^-12 instead
 // of 2^-9) would otherwise be the largest error of the result. Their range is kept by powers of two: 32 lanes of Q are scaled
