@@ -15,8 +15,8 @@
 // What bounds it: the chain of one unit, S -> softmax -> P -> O += P V -> next S, about 4100 cycles a tile of 128 tokens, of
 // which 1590 are the exponentials (1024 of MUFU), 840 S's way through tensor memory and the maximum, 1030 the two MMAs and
 // the rest hand-over; the other unit's exponentials lie in between. Both units' MMAs are 2050 of it. Beside them the
-// dequantisers' loop (770 instructions a warp) takes 4200 cycles when all SMs are busy. 4 x 2048 rows behind 512 tokens, 32
-// query heads: 268 us, 769 TFLOP/s. On the way: Q loaded by the lanes that convert it 285; then, at 273 with these
+// dequantisers' loop (770 instructions a warp) takes as long when all SMs are busy. 4 x 2048 rows behind 512 tokens, 32
+// query heads: 261 us, 790 TFLOP/s. On the way: Q loaded by the lanes that convert it 285; then, at 273 with these
 // registers, 277 with 2 x 184 + 96 + 48, 286 with 2 x 192 + 80 + 48, 287 with 2 x 168 + 112 + 64.
 //
 // fp16 operands, not bf16: a dequantised value c + s (n - 8) has more than bf16's 8 bits, and its rounding (2^-12 instead
@@ -320,10 +320,11 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     }
     for (int j = 0; j < n_tiles; ++j) {
       named_barrier(1, 128);
-      const uint32_t* seen = red + (j & 1) * 12;
-      if ((seen[8] | seen[9] | seen[10] | seen[11]) != 0u) break;
-      ek = choose(ek, max(max(seen[0], seen[1]), max(seen[2], seen[3])));
-      ev = choose(ev, max(max(seen[4], seen[5]), max(seen[6], seen[7])));
+      const uint4* seen = reinterpret_cast<const uint4*>(red + (j & 1) * 12);       // of the four warps: K, V, gave up
+      const uint4 k4 = seen[0], v4 = seen[1], out = seen[2];
+      if ((out.x | out.y | out.z | out.w) != 0u) break;
+      ek = choose(ek, max(max(k4.x, k4.y), max(k4.z, k4.w)));
+      ev = choose(ev, max(max(v4.x, v4.y), max(v4.z, v4.w)));
       if (row == 0) {
         TileScale sc;
         sc.k = pow2(ek);
@@ -353,7 +354,12 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         fence_proxy_async_smem();
         mbar_arrive(&k_full[ks]);
       }
-      if (more) load_codes(kc, code);
+      if (more) {                                            // here, so that its reductions end under V's conversion
+        load_codes(kc, code);
+        kp = kp_next;
+        vp = vp_next;
+        admit(j + 1, ok);
+      }
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&v_empty[vs], ((j / kNV) & 1) ^ 1) && *abort_flag == 0);
       if (ok) {
         const float f = pow2(-ev);
@@ -364,12 +370,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         fence_proxy_async_smem();
         mbar_arrive(&v_full[vs]);
       }
-      if (more) {
-        load_codes(vc, code + v_off);
-        kp = kp_next;
-        vp = vp_next;
-        admit(j + 1, ok);
-      }
+      if (more) load_codes(vc, code + v_off);
     }
     if (!ok && lane == 0) {
       report_status(p.status, kId, kWaitEmptyTimeout);
