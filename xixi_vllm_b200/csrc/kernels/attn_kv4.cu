@@ -24,7 +24,7 @@
 // What bounds it: instructions, not memory: 293 of them for the 2304 bytes of 16 tokens of a head (271 for groups of up to
 // four query heads, whose columns hold both channel groups: 256 sequences 137 -> 129 us, 32 11.7 -> 11.4), 104 of which
 // take the codes apart. 96 sequences of 2048 tokens, 32 / 8 heads: 57% of the issue slots, 52% of the ALU, 30% of the tensor
-// pipe, 4.3 TB/s. 256 sequences of 256-4096 tokens 129 us (5.0 TB/s), one of 40960 (64 / 8 heads) 19.8 us (2.4 TB/s). On the way:
+// pipe, 4.3 TB/s. 256 sequences of 256-4096 tokens 128 us (5.1 TB/s), one of 40960 (64 / 8 heads) 19.8 us (2.4 TB/s). On the way:
 // codes as bf16 integers with shifts and a subtraction 333 instructions and 153 us, a unit at a time 424 and 189, bulk copies
 // in place of cp.async 241. 128 registers, for four CTAs an SM, spill: 149 us. Small batches are a chain of dependent
 // reads (length and page, codes), about 2500 cycles before the first product.
