@@ -1,0 +1,138 @@
+"""Calls on 4-bit caches at the ends of what they take: magnitudes, scales, values that are not finite, launch bounds."""
+import numpy as np
+import pytest
+import torch
+
+import kv4_ref
+from test_gpu_kv4 import D, DEV, HALF_BF16, WIDE, _cuda, _ops
+from xixi_vllm_b200.ops import kv4
+from xixi_vllm_b200.runtime.staging import AttnBatch
+
+pytestmark = pytest.mark.gpu
+SCALE = D ** -0.5
+I32 = dict(dtype=torch.int32, device=DEV)
+
+
+class Case:
+    """One packed batch on pages of 16 tokens, made on the CPU: k, v ``[sequence][tokens, hkv, D]``, q ``[rows, hq, D]``."""
+
+    def __init__(self, q_lens, kv_lens, hq, hkv, n_decode=0, extra_pages=1, seed=0, crowd=0):
+        """``crowd``: so many one-token sequences more, which make a launch of chunks too large for its range to be split."""
+        q_lens, kv_lens = q_lens + [1] * crowd, kv_lens + [1] * crowd
+        self.q_lens, self.kv_lens, self.hq, self.hkv, self.n_decode = q_lens, kv_lens, hq, hkv, n_decode
+        g = torch.Generator().manual_seed(seed)
+        per = max(1, max(-(-n // 16) for n in kv_lens))
+        self.table = torch.zeros(len(kv_lens), per + extra_pages, dtype=torch.int32)
+        self.table[:, :per] = torch.arange(len(kv_lens) * per).view(-1, per)
+        self.pages = len(kv_lens) * per
+        self.k, self.v = ([torch.randn(n, hkv, D, generator=g) for n in kv_lens] for _ in range(2))
+        self.q = torch.randn(sum(q_lens), hq, D, generator=g)
+
+    def attn(self):
+        cu = torch.tensor([0] + list(np.cumsum(self.q_lens)))
+        return AttnBatch(cu.to(**I32), torch.tensor(self.kv_lens, **I32), self.table.to(DEV), len(self.kv_lens), self.n_decode,
+                         max(self.q_lens), max(self.kv_lens), sum(self.q_lens))
+
+    def caches(self):
+        out = []
+        for values in (self.k, self.v):
+            c = torch.zeros(self.pages, self.hkv, 16, kv4.row_bytes(D), dtype=torch.uint8)
+            for b, x in enumerate(values):
+                slots = self.table[b, torch.arange(len(x)) // 16] * 16 + torch.arange(len(x)) % 16
+                kv4.write_rows(c, slots, x)
+            out.append(c)
+        return out
+
+    def run(self, scale=SCALE):
+        k, v = self.caches()
+        q = self.q.bfloat16().flatten(1)
+        out = _ops().paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), self.attn(), scale, self.hq, self.hkv, D)
+        _cuda().check_status()
+        return out.view(-1, self.hq, D).cpu()
+
+    def reference(self, scale):
+        """64-bit outputs ``[rows, hq, D]`` and how far a call may be from them. A decode score is an fp32 sum of at most 2 * 64
+        products no larger than 17 times those of q and k, so it is off by 2^-24 * 17 * 8 of sum |q| |k|; P s is rounded to
+        fp16 and the output to bf16 (both held to bf16's bound). A chunk's K, V and P are rounded to fp16 once each, 2^-11.
+        An error d of token j's score moves p_j by p_j (e^d - 1), in the numerator and in the sum. What falls below fp16's
+        smallest number, and fp32 sums, are 2^-18 of sum p |v| at these lengths."""
+        k_cache, v_cache = self.caches()
+        q = self.q.bfloat16().double().numpy() * scale
+        ref, tol = np.zeros(q.shape), np.zeros(q.shape)
+        at = 0
+        for b, (n, L) in enumerate(zip(self.q_lens, self.kv_lens)):
+            slots = [int(self.table[b, t // 16]) * 16 + t % 16 for t in range(L)]
+            k, (v, codes) = kv4_ref.rows(k_cache, slots)[0], kv4_ref.rows(v_cache, slots)
+            for h in range(self.hq):
+                hk = h // (self.hq // self.hkv)
+                x = q[at:at + n, h]
+                s = x @ k[:, hk].T
+                s[np.arange(L) > (L - n + np.arange(n))[:, None]] = -np.inf
+                p = np.exp(s - s.max(-1, keepdims=True))
+                p /= p.sum(-1, keepdims=True)
+                decode = np.arange(b, b + n)[:, None] < self.n_decode
+                with np.errstate(over="ignore", invalid="ignore"):
+                    moved = np.where(p > 0, p * np.expm1(np.minimum(np.where(decode, 2.0 ** -24 * 17 * 8, 2.0 ** -11) * (np.abs(x) @ np.abs(k[:, hk]).T), 700)), 0)
+                out, mag, swing = p @ v[:, hk], p @ np.abs(v[:, hk]), p @ np.abs(codes[:, hk])
+                ref[at:at + n, h] = out
+                rounded = np.where(decode, HALF_BF16 * swing, 2.0 ** -10 * (mag + swing))
+                tol[at:at + n, h] = (HALF_BF16 * np.abs(out) + rounded + 2.0 ** -18 * mag + moved @ np.abs(v[:, hk]) +
+                                     moved.sum(-1, keepdims=True) * np.abs(out))
+            at += n
+        return ref, tol
+
+    def check(self, scale=SCALE):
+        got = self.run(scale).double().numpy()
+        ref, tol = self.reference(scale)
+        bad = ~(np.abs(got - ref) <= tol)                    # NaN is bad
+        assert not bad.any(), (bad.sum(), np.argwhere(bad)[:4].tolist(), got[bad][:4], ref[bad][:4], tol[bad][:4])
+        return got
+
+
+@pytest.mark.parametrize("extra_pages", [1, WIDE])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (7, 1), (16, 1)])
+def test_decode_head_of_any_finite_size_stays_alone(hq, hkv, extra_pages):
+    """Query heads of 2^120 beside ordinary ones and beside heads of 2^-100: each head has its own power of two."""
+    c = Case([1, 1], [40, 700], hq, hkv, n_decode=2, extra_pages=extra_pages, seed=3)
+    c.q[:, 1] *= 2.0 ** 120
+    c.q[:, 2] *= 2.0 ** -100
+    got = c.check()
+    # one token has all of the large head's weight: its scores are 2^100 and more apart
+    vals, swing = kv4_ref.rows(c.caches()[1], [(int(c.table[1, t // 16])) * 16 + t % 16 for t in range(700)])
+    k, _ = kv4_ref.rows(c.caches()[0], [(int(c.table[1, t // 16])) * 16 + t % 16 for t in range(700)])
+    s = k[:, 0] @ c.q[1, 1].bfloat16().double().numpy()
+    first, second = np.argsort(s)[::-1][:2]
+    assert s[first] - s[second] > 2.0 ** -12 * np.abs(k[first, 0]) @ np.abs(c.q[1, 1].double().numpy())
+    want, sw = vals[first, 0], np.abs(swing[first, 0])
+    assert (np.abs(got[1, 1] - want) <= HALF_BF16 * (np.abs(want) + sw) + 2.0 ** -18 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("power", [124, 110, -110, -118])
+@pytest.mark.parametrize("extra_pages", [1, WIDE])
+def test_decode_queries_at_the_ends_of_the_range(power, extra_pages):
+    """Queries of 2^124 down to 2^-118 times normal values on keys that bring the scores back to size."""
+    c = Case([1, 1], [40, 700], 6, 2, n_decode=2, extra_pages=extra_pages, seed=4)
+    c.q.clamp_(-4, 4).mul_(2.0 ** power)
+    c.q[:, ::2].abs_()                                       # their sum leaves fp32
+    c.k = [k * 2.0 ** -min(power, 120) for k in c.k]
+    c.check(SCALE * 2.0 ** (-power + min(power, 120)))
+
+
+@pytest.mark.parametrize("extra_pages", [1, WIDE])
+def test_decode_scores_beyond_2_to_the_30(extra_pages):
+    """Weights are 1 and 0 there: the maximum's own exponent has to be 0, not what rounding leaves of it."""
+    c = Case([1, 1], [40, 700], 6, 2, n_decode=2, extra_pages=extra_pages, seed=15)
+    c.q *= 2.0 ** 31
+    assert not np.isnan(c.run().double().numpy()).any()
+    c.q.mul_(2.0 ** 8)
+    k, v = c.caches()
+    at = [int(c.table[1, t // 16]) * 16 + t % 16 for t in range(700)]
+    (keys, _), (vals, swing) = kv4_ref.rows(k, at), kv4_ref.rows(v, at)
+    got = c.run().double().numpy()[1]
+    for h in range(6):
+        q = c.q[1, h].bfloat16().double().numpy()
+        s = keys[:, h // 3] @ q
+        first, second = np.argsort(s)[::-1][:2]
+        if s[first] - s[second] > 2.0 ** -12 * (np.abs(keys[first, h // 3]) @ np.abs(q)):       # well apart: fp32 sums see it
+            want, sw = vals[first, h // 3], np.abs(swing[first, h // 3])
+            assert (np.abs(got[h] - want) <= HALF_BF16 * (np.abs(want) + sw) + 2.0 ** -18 * np.abs(want)).all()

@@ -35,8 +35,9 @@
 #include <math_constants.h>
 
 #include <algorithm>
-#include <type_traits>
 #include <atomic>
+#include <cmath>
+#include <type_traits>
 
 #include "../common/kv4.cuh"
 #include "../common/launch.cuh"
@@ -49,7 +50,7 @@ using namespace xv;
 
 constexpr int kD = kv4::kD;
 constexpr int kIdDecode = 10;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
 
 struct Params {
   const __nv_bfloat16* q;
@@ -61,7 +62,8 @@ struct Params {
   int* status;
   int hq, hkv, block_size, max_blocks, num_blocks, splits;
   int max_tokens;                        // that a block table can name; 32-bit sums of a unit more must not wrap
-  float scale_log2;
+  float scale, sign;                     // of a score, times log2 e: sign * scale * 2^scale_exp, scale in 1/4 .. 1/2
+  int scale_exp;
 };
 
 // Cached tokens of a sequence, never more than its block table can name.
@@ -146,14 +148,19 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 template <int NT, bool TWIN>
 struct Query {
   static_assert(!TWIN || NT == 1);
-  // MMA (word w, half hf) of lane (g, t) multiplies channels 32 t + 8 w + 2 hf + {0, 4, 1, 5}. Q is held in fp16, scaled by
-  // a power of two that takes the group's largest value to 2^14 .. 2^15 (exact down to 2^-28 of it); the odd channels meet
+  // MMA (word w, half hf) of lane (g, t) multiplies channels 32 t + 8 w + 2 hf + {0, 4, 1, 5}. Q is held in fp16, every head
+  // scaled by a power of two that takes its largest value to 2^14 .. 2^15 (exact down to 2^-28 of it); the odd channels meet
   // codes that are 16 times too large and carry another 1 / 16.
   uint32_t f[NT][4][2][2];
   // The centres' share of a score, sum over groups of c_g Qs_g - 8 s_g Qs_g with Qs_g the group's sum of Q, is one more
   // MMA: its A operand is the parameter words as stored, its B operand {-8 Qs_g, Qs_g} as three bf16 terms (24 bits).
   uint32_t c[NT][2];
-  float unit;                          // a score over what the MMAs make of it
+  // What the MMAs and K's parameters make of a score, times power, is the score in log2 units. power joins the head's power of
+  // two, the codes' 2^-24 and the exponent of the softmax's scale, whose mantissa is in lift, by which K's steps and the
+  // centres' operand are multiplied. A power of two, so that x power - m power is 0 for the largest x however large the scores
+  // are. It stays in 2^-100 .. 2^120: where a head's would be larger (queries from 2^107 on at ordinary scales) lift takes the
+  // rest for all heads of the group, where it would be smaller the head's Q is scaled down. For heads 2t, 2t + 1 of each tile.
+  float power[NT][2], lift;
 
   uint32_t raw[NT][16];
   // Sends for Q. `row`: sequence * hq + first query head of the group.
@@ -169,43 +176,54 @@ struct Query {
       }
     }
   }
-  // Makes the operands of what fetch() brought; `sign`: applied to Q.
-  __device__ __forceinline__ void convert(float sign, int g, int t) {
-    uint32_t top = 0;
+  // Makes the operands of what fetch() brought.
+  __device__ __forceinline__ void convert(const Params& p, int g, int t) {
+    int e[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = __vmaxu2(top, raw[nt][i] & 0x7fff7fffu);
-    uint32_t most = max(top >> 16, top & 0xffffu);
-    if (__any_sync(0xffffffffu, most >= 0x7f80u)) {        // infinities and NaN do not choose the scale of the other heads
-      most = 0;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      uint32_t most = max(top >> 16, top & 0xffffu);
+      if (most >= 0x7f80u) {                               // infinities and NaN do not choose a power
+        most = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const uint32_t lo = raw[nt][i] & 0x7fffu, hi = (raw[nt][i] >> 16) & 0x7fffu;
           most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
         }
+      }
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      e[nt] = max(static_cast<int>(most >> 7) - 127 - 14, -120);
     }
-    const int e = max(static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14, -120);
-    unit = power_of_two(e) * 16777216.f;                   // the codes are n 2^-24
-    const float even = power_of_two(-e) * sign, odd = even * 0.0625f;
+    const int top_e = __reduce_max_sync(0xffffffffu, NT == 2 ? max(e[0], e[NT - 1]) : e[0]), rest = p.scale_exp + 24;
+    const int over = min(max(top_e + rest - 120, 0), 120);
+    lift = p.scale * power_of_two(over);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      e[nt] = max(e[nt], over - rest - 100);
+#pragma unroll
+      for (int hd = 0; hd < 2; ++hd)                       // a lane's scores are those of heads 2t + hd, whose rows lanes g = 2t + hd have
+        power[nt][hd] = power_of_two(min(__shfl_sync(0xffffffffu, e[nt], 8 * t + 4 * hd) + rest - over, 127));
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float by = power_of_two(-e[nt]) * p.sign;
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         float x[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[2 * i] = __uint_as_float(raw[nt][4 * w + i] << 16);
-          x[2 * i + 1] = __uint_as_float(raw[nt][4 * w + i] & 0xffff0000u);
+          x[2 * i] = __uint_as_float(raw[nt][4 * w + i] << 16) * by;
+          x[2 * i + 1] = __uint_as_float(raw[nt][4 * w + i] & 0xffff0000u) * by;
           sum[w & 1] += x[2 * i] + x[2 * i + 1];
         }
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          f[nt][w][hf][0] = pack_f16(x[2 * hf] * even, x[2 * hf + 4] * even);
-          f[nt][w][hf][1] = pack_f16(x[2 * hf + 1] * odd, x[2 * hf + 5] * odd);
+          f[nt][w][hf][0] = pack_f16(x[2 * hf], x[2 * hf + 4]);
+          f[nt][w][hf][1] = pack_f16(x[2 * hf + 1] * 0.0625f, x[2 * hf + 5] * 0.0625f);
           if (TWIN && (w & 1) != (g >> 2)) f[nt][w][hf][0] = f[nt][w][hf][1] = 0u;
         }
       }
@@ -216,7 +234,7 @@ struct Query {
       }
       // Lane (g, t) holds K rows 2t, 2t + 1 of B (first register) and 2t + 8, 2t + 9 (second): group t & 1; the first
       // term for t < 2, the second for t >= 2, the third in the second register for t < 2.
-      const float qs = ((t & 1) ? sum[1] : sum[0]) * even * 5.9604644775390625e-08f, bs = -8.f * qs;      // 2^-24
+      const float qs = ((t & 1) ? sum[1] : sum[0]) * 5.9604644775390625e-08f * lift, bs = -8.f * qs;      // 2^-24
       const float q1 = __bfloat162float(__float2bfloat16(qs)), b1 = __bfloat162float(__float2bfloat16(bs));
       const float q2 = __bfloat162float(__float2bfloat16(qs - q1)), b2 = __bfloat162float(__float2bfloat16(bs - b1));
       c[nt][0] = t < 2 ? pack_bf16(b1, q1) : pack_bf16(b2, q2);
@@ -232,7 +250,7 @@ struct Softmax {
   float o[NT][2][4][4];            // [group][MMA]: rows g, g + 8 = channels 16 g + 8 group + 2 i + {0, 1}; heads 2t, 2t+1
   float cen[NT][2][2];             // sum of P * centre, this lane's tokens
   float off[NT][4];                // sum of -8 P * s, rounded as it is in o: group 0 (heads 2t, 2t + 1), group 1
-  float m[NT][2], l[NT][2];        // running maximum of the unscaled scores (may lag), sum of P of this lane's tokens
+  float m[NT][2], l[NT][2];        // running maximum of the products (may lag), sum of P of this lane's tokens
   float vs, v_most;                // power of two that V's scales are multiplied by; the largest scale that it allows
 
   __device__ __forceinline__ void clear() {
@@ -254,7 +272,7 @@ struct Softmax {
 
   // One slot of kPair units, of which the first `mine` tokens count. lane_k .. lane_v1: this lane's places in the slot.
   __device__ __forceinline__ void add(const Query<NT, false>& q, const uint8_t* lane_k, const uint8_t* lane_p, const uint8_t* lane_v0,
-                                      const uint8_t* lane_v1, int mine, int tok, int t, float scale, float lag) {
+                                      const uint8_t* lane_v1, int mine, int tok, int t) {
     float x[kPair][NT][4];               // (row g: heads 2t, 2t + 1), (row g + 8: the same)
 #pragma unroll
     for (int u = 0; u < kPair; ++u) {
@@ -281,13 +299,12 @@ struct Softmax {
             else mma_more(s[nt][w & 1], a, q.f[nt][w][hf][0], q.f[nt][w][hf][1]);
           }
         }
+      const float ks[2][2] = {{kv4::par_s(kp0.x) * q.lift, kv4::par_s(kp0.y) * q.lift},
+                              {kv4::par_s(kp1.x) * q.lift, kv4::par_s(kp1.y) * q.lift}};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint2 kp = e < 2 ? kp0 : kp1;
-          x[u][nt][e] = fmaf(kv4::par_s(kp.x), s[nt][0][e], fmaf(kv4::par_s(kp.y), s[nt][1][e], sc[nt][e]));
-        }
+        for (int e = 0; e < 4; ++e) x[u][nt][e] = fmaf(ks[e >> 1][0], s[nt][0][e], fmaf(ks[e >> 1][1], s[nt][1][e], sc[nt][e]));
     }
     const bool ragged = mine < 16 * kPair;               // warp-uniform
     if (ragged) {
@@ -319,7 +336,7 @@ struct Softmax {
 #pragma unroll
       for (int hd = 0; hd < 2; ++hd) {
         mx[nt][hd] = fmaxf(fmaxf(x[0][nt][hd], x[0][nt][2 + hd]), fmaxf(x[1][nt][hd], x[1][nt][2 + hd]));
-        grow |= mx[nt][hd] > m[nt][hd] + lag;
+        grow |= (mx[nt][hd] - m[nt][hd]) * q.power[nt][hd] > kLazy;
       }
     if (__any_sync(0xffffffffu, grow)) {
       float back = 1.f;                  // of the sums of P * s
@@ -341,7 +358,7 @@ struct Softmax {
           mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 4));
           mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 8));
           mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 16));
-          const float cr = exp2f((m[nt][hd] - mn) * scale);
+          const float cr = exp2f((m[nt][hd] - mn) * q.power[nt][hd]);
           m[nt][hd] = mn;
           l[nt][hd] *= cr;
 #pragma unroll
@@ -377,7 +394,7 @@ struct Softmax {
       for (int nt = 0; nt < NT; ++nt) {
         float pr[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][nt][e], scale, -m[nt][e & 1] * scale));
+        for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][nt][e], q.power[nt][e & 1], -m[nt][e & 1] * q.power[nt][e & 1]));
         l[nt][0] += pr[0] + pr[2];
         l[nt][1] += pr[1] + pr[3];
 #pragma unroll
@@ -406,8 +423,9 @@ struct Softmax {
     }
   }
 
-  // Sums over the lanes of equal t; the centres join the outputs. Then every lane holds, for its two heads, 16 channels.
-  __device__ __forceinline__ void finish(float unit) {
+  // Sums over the lanes of equal t; the centres join the outputs, the maximum turns to log2 units. Then every lane holds, for
+  // its two heads, 16 channels.
+  __device__ __forceinline__ void finish(const Query<NT, false>& q) {
     const float back = 1.f / vs;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -426,7 +444,7 @@ struct Softmax {
             o[nt][gr][i][hd] = fmaf(fmaf(o[nt][gr][i][hd], 1048576.f, off[nt][2 * gr + hd]), back, cen[nt][gr][hd]);      // n 2^-20
             o[nt][gr][i][2 + hd] = fmaf(fmaf(o[nt][gr][i][2 + hd], 1048576.f, off[nt][2 * gr + hd]), back, cen[nt][gr][hd]);
           }
-        m[nt][hd] = m[nt][hd] == kNoMax ? kNoMax : m[nt][hd] * unit;
+        m[nt][hd] = m[nt][hd] == kNoMax ? kNoMax : m[nt][hd] * q.power[nt][hd];
       }
   }
   // After finish(), f(head, first of four channels, their sums, m, l) for what this lane (g, t) holds.
@@ -466,7 +484,7 @@ struct TwinSoftmax {
   }
 
   __device__ __forceinline__ void add(const Query<1, true>& q, const uint8_t* lane_k, const uint8_t* lane_p, const uint8_t* lane_v0,
-                                      const uint8_t* lane_v1, int mine, int tok, int t, float scale, float lag) {
+                                      const uint8_t* lane_v1, int mine, int tok, int t) {
     const uint8_t* lane_s = lane_p + (t >> 1) * 4;       // the lane's group's parameters
     const uint8_t* lane_c = lane_p + (t & 1) * 4;        // those that the centres' MMA takes from it
     float x[kPair][4];
@@ -491,9 +509,10 @@ struct TwinSoftmax {
           if (w == 0 && hf == 0) mma_first(s, a, q.f[0][w][hf][0], q.f[0][w][hf][1]);
           else mma_more(s, a, q.f[0][w][hf][0], q.f[0][w][hf][1]);
         }
+      const float ks[2] = {kv4::par_s(s0) * q.lift, kv4::par_s(s1) * q.lift};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[u][e] = fmaf(kv4::par_s(e < 2 ? s0 : s1), s[e], sc[e]);
+        x[u][e] = fmaf(ks[e >> 1], s[e], sc[e]);
         x[u][e] += __shfl_xor_sync(0xffffffffu, x[u][e], 2);
       }
     }
@@ -522,7 +541,7 @@ struct TwinSoftmax {
 #pragma unroll
     for (int hd = 0; hd < 2; ++hd) {
       mx[hd] = fmaxf(fmaxf(x[0][hd], x[0][2 + hd]), fmaxf(x[1][hd], x[1][2 + hd]));
-      grow |= mx[hd] > m[hd] + lag;
+      grow |= (mx[hd] - m[hd]) * q.power[0][hd] > kLazy;
     }
     if (__any_sync(0xffffffffu, grow)) {
       float back = 1.f;                                  // of the sums of P * s
@@ -541,7 +560,7 @@ struct TwinSoftmax {
         mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 4));
         mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 8));
         mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 16));
-        const float cr = exp2f((m[hd] - mn) * scale);
+        const float cr = exp2f((m[hd] - mn) * q.power[0][hd]);
         m[hd] = mn;
         l[hd] *= cr;
         cen[hd] *= cr;
@@ -564,7 +583,7 @@ struct TwinSoftmax {
       vw[3] = *reinterpret_cast<const uint2*>(lane_v1 + u * kUnitSlot + 8 * 64);
       float pr[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][e], scale, -m[e & 1] * scale));
+      for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][e], q.power[0][e & 1], -m[e & 1] * q.power[0][e & 1]));
       l[0] += pr[0] + pr[2];
       l[1] += pr[1] + pr[3];
       const float v0 = kv4::par_s(vp[u][0]) * vs, v1 = kv4::par_s(vp[u][1]) * vs;
@@ -588,7 +607,7 @@ struct TwinSoftmax {
     }
   }
 
-  __device__ __forceinline__ void finish(float unit) {
+  __device__ __forceinline__ void finish(const Query<1, true>& q) {
     const float back = 1.f / vs;
 #pragma unroll
     for (int hd = 0; hd < 2; ++hd) {
@@ -604,7 +623,7 @@ struct TwinSoftmax {
           o[gr][i][hd] = fmaf(fmaf(o[gr][i][hd], 1048576.f, off[hd]), back, cen[hd]);                    // n 2^-20
           o[gr][i][2 + hd] = fmaf(fmaf(o[gr][i][2 + hd], 1048576.f, off[hd]), back, cen[hd]);
         }
-      m[hd] = m[hd] == kNoMax ? kNoMax : m[hd] * unit;
+      m[hd] = m[hd] == kNoMax ? kNoMax : m[hd] * q.power[0][hd];
     }
   }
   template <typename F>
@@ -704,14 +723,6 @@ struct Ring {
 };
 static_assert(kPair == 2, "a lookup of 32 lanes serves 16 slots");
 
-// A negative scale is Q's sign, so the running maxima need not know it; zero becomes a scale too small to matter.
-struct Scale {
-  float scale, sign;
-  __device__ __forceinline__ explicit Scale(float s) : scale(fmaxf(fabsf(s), 1e-30f)), sign(s < 0.f ? -1.f : 1.f) {}
-  // For scores in units of Query::unit.
-  __device__ __forceinline__ float of(float unit) const { return fmaxf(scale * unit, 1e-36f); }
-};
-
 // A cluster of CTAs, one per KV split, per (sequence, KV head). NT, TWIN: as in Query; W: warps.
 template <int NT, int W, bool TWIN>
 __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_kernel(const Params p) {
@@ -736,9 +747,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
   ring.until(p, (kv_len + 15) / 16, entry0);
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) ring.issue(p);
-  const Scale sc(p.scale_log2);
-  q.convert(sc.sign, g, t);
-  const float scale = sc.of(q.unit), lag = kLazy / scale;
+  q.convert(p, g, t);
   SoftmaxOf<NT, TWIN> st;
   st.clear();
 
@@ -750,13 +759,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
     __syncwarp();                        // everyone's part of the slot has landed, and everyone has read the slot filled next
     ring.issue(p);
     st.add(q, at + tok * 64 + t * 16, at + kv4::kParBase + tok * 8, at + kv4::kUnitBytes + token_of_row(2 * t) * 64 + g * 8,
-           at + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8, mine, tok, t, scale, lag);
+           at + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8, mine, tok, t);
     at = at == ring_mem + (kStages - 1) * kSlot ? ring_mem : at + kSlot;
   }
   cp_async_wait<0>();
 
   // The warps meet in the (now idle) ring.
-  st.finish(q.unit);
+  st.finish(q);
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(smem);                    // [warp][8 NT][128]
   float* part_o = sm_o + W * 8 * NT * kD;                          // [8 NT][128]
@@ -780,7 +789,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float f = exp2f((sm_m[w][r] - M) * sc.scale);
+      const float f = exp2f(sm_m[w][r] - M);
       const float4 v = *reinterpret_cast<const float4*>(&sm_o[(w * 8 * NT + r) * kD + d]);
       L += sm_l[w][r] * f;
       acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
@@ -805,7 +814,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
     for (int c = 0; c < p.splits; ++c) M = fmaxf(M, ld_cluster_f32(map_to_cta(sm + r * 4, c)));
     float L = 0.f, acc = 0.f;
     for (int c = 0; c < p.splits; ++c) {
-      const float f = exp2f((ld_cluster_f32(map_to_cta(sm + r * 4, c)) - M) * sc.scale);
+      const float f = exp2f(ld_cluster_f32(map_to_cta(sm + r * 4, c)) - M);
       L += ld_cluster_f32(map_to_cta(sl + r * 4, c)) * f;
       acc += ld_cluster_f32(map_to_cta(so + idx * 4, c)) * f;
     }
@@ -821,7 +830,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 12 / W : 8 / W) kv4_decode_k
 // same order, so the partial of (run w, pair x) has the slot w + x and a pair's slots are consecutive.
 struct Shares {
   float* o;         // [slot][8 NT][128]
-  float* ml;        // [slot][8 NT][2]: running maximum (unscaled), sum
+  float* ml;        // [slot][8 NT][2]: running maximum (log2 units), sum
   int* begin;       // [seq + 1]: units of one head before the sequence; then the units per run
 };
 constexpr int kShareWarps = 4, kMinRun = 4;
@@ -903,7 +912,6 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
 
   Ring ring;
   ring.init(p, ring_mem, lane);
-  const Scale sc(p.scale_log2);
   const int tok = token_of_row(g);
   const uint8_t* at = ring_mem;
   // The fetching side runs kStages - 1 slots ahead and may already be in the next pair.
@@ -934,8 +942,7 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
     const int n = min(units - first, todo);
     Query<NT, TWIN> q;
     q.fetch(p, static_cast<size_t>(b) * p.hq + h * G, G, g, t);
-    q.convert(sc.sign, g, t);
-    const float scale = sc.of(q.unit), lag = kLazy / scale;
+    q.convert(p, g, t);
     SoftmaxOf<NT, TWIN> st;
     st.clear();
     int mine = min(kv_len - first * 16, n * 16);
@@ -944,10 +951,10 @@ __global__ void __launch_bounds__(kShareWarps * 32, NT == 1 ? 3 : 2) kv4_share_k
       __syncwarp();
       fetch();
       st.add(q, at + tok * 64 + t * 16, at + kv4::kParBase + tok * 8, at + kv4::kUnitBytes + token_of_row(2 * t) * 64 + g * 8,
-             at + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8, mine, tok, t, scale, lag);
+             at + kv4::kUnitBytes + token_of_row(2 * t + 1) * 64 + g * 8, mine, tok, t);
       at = at == ring_mem + (kStages - 1) * kSlot ? ring_mem : at + kSlot;
     }
-    st.finish(q.unit);
+    st.finish(q);
     const bool whole = n == units;
     const int pair = b * p.hkv + h;
     const size_t slot = static_cast<size_t>(run) + pair;
@@ -998,7 +1005,6 @@ __global__ void __launch_bounds__(R == 1 ? 128 : R * 32) kv4_join_kernel(const P
   const long long from = static_cast<long long>(before) * p.hkv + static_cast<long long>(h) * units;
   const int run0 = static_cast<int>(from / per), run1 = static_cast<int>((from + units - 1) / per);
   if (run0 == run1) return;                    // written by its run
-  const float scale = Scale(p.scale_log2).scale;
   float M = kNoMax, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int r = run0 + warp; r <= run1; r += BATCH * R) {
@@ -1014,13 +1020,13 @@ __global__ void __launch_bounds__(R == 1 ? 128 : R * 32) kv4_join_kernel(const P
     }
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) mn = fmaxf(mn, ml[i].x);
-    const float f0 = exp2f((M - mn) * scale);
+    const float f0 = exp2f(M - mn);
     M = mn;
     L *= f0;
     acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
-      const float f = exp2f((ml[i].x - mn) * scale);
+      const float f = exp2f(ml[i].x - mn);
       L += ml[i].y * f;
       acc.x += v[i].x * f; acc.y += v[i].y * f; acc.z += v[i].z * f; acc.w += v[i].w * f;
     }
@@ -1040,7 +1046,7 @@ __global__ void __launch_bounds__(R == 1 ? 128 : R * 32) kv4_join_kernel(const P
     for (int w = 0; w < R; ++w) M = fmaxf(M, sm_m[w]);
 #pragma unroll
     for (int w = 0; w < R; ++w) {
-      const float f = exp2f((sm_m[w] - M) * scale);
+      const float f = exp2f(sm_m[w] - M);
       const float4 v = sm_o[w][lane];
       L += sm_l[w] * f;
       acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
@@ -1066,7 +1072,11 @@ int fill(Params& p, const void* q, const void* k_cache, const void* v_cache, con
   p.out = static_cast<__nv_bfloat16*>(out);
   p.hq = hq; p.hkv = hkv; p.block_size = block_size; p.max_blocks = max_blocks; p.num_blocks = num_blocks;
   p.max_tokens = static_cast<int>(std::min(static_cast<long long>(max_blocks) * block_size, 0x7ffffff0ll));
-  p.scale_log2 = scale * kLog2e;
+  // A negative scale is Q's sign, so the running maxima need not know it; zero becomes a scale too small to matter.
+  const double s = std::max(std::abs(static_cast<double>(scale)) * kLog2e, 1e-30);
+  p.scale = static_cast<float>(0.5 * std::frexp(s, &p.scale_exp));      // below 1: K's largest steps stay in fp32
+  p.scale_exp += 1;
+  p.sign = scale < 0.f ? -1.f : 1.f;
   p.status = status;
   return 0;
 }
