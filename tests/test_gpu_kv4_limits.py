@@ -136,3 +136,22 @@ def test_decode_scores_beyond_2_to_the_30(extra_pages):
         if s[first] - s[second] > 2.0 ** -12 * (np.abs(keys[first, h // 3]) @ np.abs(q)):       # well apart: fp32 sums see it
             want, sw = vals[first, h // 3], np.abs(swing[first, h // 3])
             assert (np.abs(got[h] - want) <= HALF_BF16 * (np.abs(want) + sw) + 2.0 ** -18 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-33, -1e-33, 2.0 ** -120, 1e30])
+@pytest.mark.parametrize("extra_pages,crowd", [(1, 0), (300, 0), (1, 160), (WIDE, 0)])
+def test_scales_of_any_size(scale, extra_pages, crowd):
+    """Zero leaves equal weights whatever the scores; a scale of 1e-33 is not a larger one."""
+    c = Case([1, 1, 30, 200], [40, 700, 60, 333], 6, 2, n_decode=2, extra_pages=extra_pages, seed=5, crowd=crowd)
+    size = 2.0 ** 110 if scale == 0 else 0.1 / abs(scale)
+    c.q *= size ** 0.5
+    c.k = [k * size ** 0.5 for k in c.k]
+    c.check(scale)
+
+
+@pytest.mark.parametrize("qp,kp,scale", [(-110, 120, 2.0 ** -13), (-100, 60, 2.0 ** 37), (100, -110, 2.0 ** 7), (100, -60, 2.0 ** -43)])
+def test_products_of_scale_query_and_key_powers(qp, kp, scale):
+    c = Case([1, 30, 200], [40, 60, 333], 6, 2, n_decode=1, seed=6)
+    c.q *= 2.0 ** qp
+    c.k = [k * 2.0 ** kp for k in c.k]
+    c.check(scale)

@@ -1072,11 +1072,11 @@ int fill(Params& p, const void* q, const void* k_cache, const void* v_cache, con
   p.out = static_cast<__nv_bfloat16*>(out);
   p.hq = hq; p.hkv = hkv; p.block_size = block_size; p.max_blocks = max_blocks; p.num_blocks = num_blocks;
   p.max_tokens = static_cast<int>(std::min(static_cast<long long>(max_blocks) * block_size, 0x7ffffff0ll));
-  // A negative scale is Q's sign, so the running maxima need not know it; zero becomes a scale too small to matter.
-  const double s = std::max(std::abs(static_cast<double>(scale)) * kLog2e, 1e-30);
+  // The scale's sign is Q's, so the running maxima need not know it; a scale of 0 is a Q of 0.
+  const double s = scale == 0.f ? 1.0 : std::abs(static_cast<double>(scale)) * kLog2e;
   p.scale = static_cast<float>(0.5 * std::frexp(s, &p.scale_exp));      // below 1: K's largest steps stay in fp32
   p.scale_exp += 1;
-  p.sign = scale < 0.f ? -1.f : 1.f;
+  p.sign = scale == 0.f ? 0.f : scale < 0.f ? -1.f : 1.f;
   p.status = status;
   return 0;
 }

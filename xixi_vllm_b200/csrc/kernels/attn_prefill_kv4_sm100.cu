@@ -37,6 +37,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdint>
 
 #include "../common/kv4.cuh"
@@ -57,7 +58,7 @@ constexpr int kBarBytes = 512;                    // barriers and small arrays
 constexpr int kSmem = (2 + kNK + kNV) * kTileBytes + 1024 + kBarBytes;
 constexpr uint32_t kTmemCols = 512, kTmemUnit = 256, kTmemO = 128;       // all of it, so it begins at address 0
 constexpr int kId = 12;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
 constexpr float kLazy = 8.f;                      // log2 units
 constexpr float kNoMax = -3.0e38f;
 
@@ -73,15 +74,17 @@ struct Params {
   float* ws_o;                                    // [CTA][split][256 lanes][128] unnormalised outputs, when splits > 1
   float* ws_ml;                                   // [CTA][split][256 lanes][2]: maximum (log2 units), sum
   int seq_begin, hq, hkv, block_size, max_blocks, num_blocks, total_rows, splits;
-  float scale_log2;
+  float scale, sign;                              // of a score, times log2 e: sign * scale * 2^scale_exp, scale in 1 .. 2
+  int scale_exp;
   int G, rpu, by_g;                               // heads to a KV head, rows of a unit; 65536 / G + 1: lane / G is a product
   uint32_t inv_splits;                            // 2^32 / splits + 1, or 0 for one split
   // n / splits; exact for n splits < 2^32.
   __device__ __forceinline__ int by_splits(int n) const { return inv_splits ? __umulhi(n, inv_splits) : n; }
 };
 
-struct alignas(16) TileScale {                    // of one tile: K and V are stored divided by k and v
-  float k, v, v_inv, unused;
+struct alignas(16) TileScale {                    // of one tile: K and V are stored divided by 2^k and v
+  int k;
+  float v, v_inv, unused;
 };
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -327,7 +330,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       ev = choose(ev, max(max(v4.x, v4.y), max(v4.z, v4.w)));
       if (row == 0) {
         TileScale sc;
-        sc.k = pow2(ek);
+        sc.k = ek;
         sc.v = pow2(ev);
         sc.v_inv = pow2(-ev);
         sc.unused = 0.f;
@@ -452,11 +455,11 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     const int u = wg, r = threadIdx.x & 127;
     const int by_g = p.by_g, row = row0 + u * rpu + ((r * by_g) >> 16);
     const int pos = pos0 + min(row, q_len - 1);              // lanes without a row follow the last one
-    // Q: a power of two per warp takes its largest element to 2^14 .. 2^15 of fp16, which is exact down to 2^-31 of it; a
-    // negative scale is its sign. A unit's rows of all its heads are contiguous in memory row by row; bulk copies bring them
+    // Q: a power of two per warp takes its largest element to 2^14 .. 2^15 of fp16, which is exact down to 2^-31 of it; the
+    // scale's sign is Q's, and a scale of 0 a Q of 0. A unit's rows of all its heads are contiguous in memory row by row; bulk copies bring them
     // into a K slot that is free until tile 1 + u. All four warps send their share: a copy takes its warp 67 cycles (one warp
     // for all of them 2160; loads by the lanes that convert 3500). Sixteen lanes convert a row, two rows at a time.
-    float q_power = 1.f;
+    int q_exp = 0;
     {
       const uint32_t bytes = static_cast<uint32_t>(G) * kD * 2;
       const int rows = rows_of(u);
@@ -495,8 +498,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         }
       }
       const int e = max(-120, min(120, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14));
-      const float f = p.scale_log2 < 0.f ? -pow2(-e) : pow2(-e);
-      q_power = pow2(e);
+      const float f = p.sign * pow2(-e);
+      q_exp = e;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};         // channels 0 1, 2 3, 4 5, 6 7 of the word
@@ -512,7 +515,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       fence_proxy_async_smem();
       mbar_arrive(&q_full[u]);
     }
-    const float row_scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * q_power;
+    const int row_exp = p.scale_exp + q_exp;
     const uint32_t taddr = u * kTmemUnit + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     float m = kNoMax, l = 0.f, vf = 1.f;
     for (int j = 0; ok && j < n_tiles; ++j) {
@@ -542,7 +545,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         mx[c] = fmax3(fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]), fmax3(a[6], a[7], a[8])),
                       fmax3(a[9], __uint_as_float(sr[c][30]), __uint_as_float(sr[c][31])), -INFINITY);
       }
-      const float scale = fmaxf(row_scale * ts.k, 1e-37f);   // never 0: it meets -inf
+      // |S| is below 2^37: what a scale below 2^-100 makes of it is nothing. Never 0: it meets -inf.
+      const float scale = p.scale * pow2(max(-100, min(126, row_exp + ts.k)));
       const float mt = fmaxf(fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale, kNoMax);
       if (j == 0) {
         m = mt;
@@ -809,7 +813,10 @@ int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, cons
   p.status = status;
   p.seq_begin = seq_begin; p.hq = hq; p.hkv = hkv; p.block_size = block_size; p.max_blocks = max_blocks;
   p.num_blocks = num_blocks; p.total_rows = total_rows;
-  p.scale_log2 = scale * kLog2e;
+  const double s = scale == 0.f ? 1.0 : std::abs(static_cast<double>(scale)) * kLog2e;
+  p.scale = static_cast<float>(2.0 * std::frexp(s, &p.scale_exp));
+  p.scale_exp -= 1;
+  p.sign = scale == 0.f ? 0.f : scale < 0.f ? -1.f : 1.f;
   const int blocks = blocks_of(max_q_len, hq, hkv);
   p.splits = splits;
   p.G = hq / hkv;
