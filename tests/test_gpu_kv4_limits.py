@@ -155,3 +155,49 @@ def test_products_of_scale_query_and_key_powers(qp, kp, scale):
     c.q *= 2.0 ** qp
     c.k = [k * 2.0 ** kp for k in c.k]
     c.check(scale)
+
+
+@pytest.mark.parametrize("crowd", [0, 160])
+def test_chunk_scores_beyond_2_to_the_30(crowd):
+    """As for decode rows. A row whose best score is well apart from the next is that token's value."""
+    c = Case([70, 30], [70, 560], 6, 2, extra_pages=300, crowd=crowd, seed=16)
+    c.q *= 2.0 ** 31
+    assert not np.isnan(c.run().double().numpy()).any()
+    c.q *= 2.0 ** 8
+    got, at, seen = c.run().double().numpy(), 0, 0
+    k_cache, v_cache = c.caches()
+    for b, (n, L) in enumerate(zip(c.q_lens[:2], c.kv_lens)):
+        slots = [int(c.table[b, t // 16]) * 16 + t % 16 for t in range(L)]
+        keys, vals = kv4_ref.rows(k_cache, slots)[0], kv4_ref.rows(v_cache, slots)[0]
+        for i in range(n):
+            for h in range(6):
+                q = c.q[at + i, h].bfloat16().double().numpy()
+                s = keys[:L - n + i + 1, h // 3] @ q
+                best = int(np.argmax(s))
+                rest = np.delete(s, best)
+                if len(rest) == 0 or s[best] - rest.max() > 2.0 ** -10 * 2 * (np.abs(keys[:L - n + i + 1, h // 3]) @ np.abs(q)).max():
+                    want = vals[best, h // 3]                # V rounded to fp16 once, P exact, the output to bf16
+                    assert (np.abs(got[at + i, h] - want) <= (HALF_BF16 + 2.0 ** -11) * np.abs(want) + 2.0 ** -11 * np.abs(want).max()).all()
+                    seen += 1
+        at += n
+    assert seen > 100
+
+
+@pytest.mark.parametrize("crowd", [0, 160])
+@pytest.mark.parametrize("first,second", [(10, 500), (500, 10), (300, 20)])
+def test_chunk_scores_around_2_to_the_24(first, second, crowd):
+    """Two tokens of 1.01 and 0.9 times 2^24 in log2 units, in different tiles (and CTAs): rows beyond 2^24 leave the scale's
+    mantissa out, which must not turn their order."""
+    c = Case([30], [560], 4, 1, extra_pages=300, crowd=crowd, seed=17)
+    c.q = torch.ones_like(c.q)
+    for b, k in enumerate(c.k):
+        k.mul_(0.0)
+    c.k[0][first], c.k[0][second] = 1.0, 0.9
+    one = float(kv4_ref.rows(c.caches()[0], [int(c.table[0, first // 16]) * 16 + first % 16])[0].sum())
+    target = 1.01 * 2.0 ** 24 / np.log2(np.e)
+    size = max((1.0, 1.0625, 1.25, 1.5, 1.75), key=lambda a: np.frexp(target * np.log2(np.e) / (one * a))[0])
+    assert np.frexp(target * np.log2(np.e) / (one * size))[0] > 0.85
+    c.q *= size
+    got = c.run(target / (one * size)).double().numpy()[:30]
+    want = kv4_ref.rows(c.caches()[1], [int(c.table[0, first // 16]) * 16 + first % 16])[0][0, 0]
+    assert (np.abs(got - want) <= (HALF_BF16 + 2.0 ** -11) * np.abs(want) + 2.0 ** -11 * np.abs(want).max()).all()

@@ -518,6 +518,11 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     const int row_exp = p.scale_exp + q_exp;
     const uint32_t taddr = u * kTmemUnit + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     float m = kNoMax, l = 0.f, vf = 1.f;
+    // S scale - m leaves what rounding took from m, 2^-24 of it: of scores of 2^30 more than an exponential may see. Rows whose
+    // maximum is beyond 2^24 leave the scale's mantissa out, so that the product with a power of two is exact. Their weights
+    // are those of the largest score and of its equals, whatever the mantissa: others as near are within S's own rounding.
+    float mantissa = p.scale;
+    auto is_huge = [](float x) { return fabsf(x) > 16777216.f && x != kNoMax; };
     for (int j = 0; ok && j < n_tiles; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[u], j & 1) && *abort_flag == 0);
       if (!ok) break;
@@ -546,10 +551,17 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
                       fmax3(a[9], __uint_as_float(sr[c][30]), __uint_as_float(sr[c][31])), -INFINITY);
       }
       // |S| is below 2^37: what a scale below 2^-100 makes of it is nothing. Never 0: it meets -inf.
-      const float scale = p.scale * pow2(max(-100, min(126, row_exp + ts.k)));
-      const float mt = fmaxf(fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale, kNoMax);
+      const float unit = pow2(max(-100, min(126, row_exp + ts.k)));
+      float scale = mantissa * unit;
+      const float top = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+      const float mt = fmaxf(top * scale, kNoMax);
       if (j == 0) {
         m = mt;
+        if (is_huge(m)) {
+          mantissa = 1.f;
+          scale = unit;
+          m = top * scale;
+        }
         vf = ts.v;
       } else {
         const bool need = mt > m + kLazy || ts.v != vf;
@@ -557,7 +569,14 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
           ok = __all_sync(0xffffffffu, mbar_wait(&o_done[u], (j - 1) & 1));
           if (!ok) break;
           tc_fence_after_sync();
-          const float m_new = need ? fmaxf(m, mt) : m;
+          float m_new = need ? fmaxf(m, mt) : m;
+          const float want = is_huge(m_new) ? 1.f : p.scale;
+          if (want != mantissa) {
+            m *= want / mantissa;
+            mantissa = want;
+            scale = mantissa * unit;
+            m_new = fmaxf(m, top * scale);
+          }
           const float down = exp2f(m - m_new);
           l *= down;
           m = m_new;
@@ -616,7 +635,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       tc_fence_after_sync();
       const size_t slot = (((static_cast<size_t>(z) * gridDim.y + hk) * gridDim.x + blockIdx.x) * p.splits + split) *
                               (2 * kBM) + u * kBM + r;
-      *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(m, l);
+      *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(mantissa == p.scale ? m : m * p.scale, l);
       // Through the unit's Q tile (all its MMAs are over) half the channels at a time, so that the writes are whole lines. A
       // split without tiles leaves no output, only m = kNoMax, l = 0.
       const uint32_t tile = smem_u32(q_s) + u * kTileBytes;
