@@ -201,3 +201,13 @@ def test_chunk_scores_around_2_to_the_24(first, second, crowd):
     got = c.run(target / (one * size)).double().numpy()[:30]
     want = kv4_ref.rows(c.caches()[1], [int(c.table[0, first // 16]) * 16 + first % 16])[0][0, 0]
     assert (np.abs(got - want) <= (HALF_BF16 + 2.0 ** -11) * np.abs(want) + 2.0 ** -11 * np.abs(want).max()).all()
+
+
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (3, 1), (16, 1)])
+@pytest.mark.parametrize("crowd", [0, 160])
+def test_chunk_row_of_any_finite_size_stays_alone(hq, hkv, crowd):
+    c = Case([40, 33], [40, 633], hq, hkv, extra_pages=300, crowd=crowd, seed=7)
+    c.q[5, 1] *= 2.0 ** 120
+    c.q[50, 0] *= 2.0 ** 60
+    c.q[9] *= 2.0 ** -90
+    c.check()

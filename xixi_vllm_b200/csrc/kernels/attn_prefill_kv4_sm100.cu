@@ -20,8 +20,8 @@
 // registers, 277 with 2 x 184 + 96 + 48, 286 with 2 x 192 + 80 + 48, 287 with 2 x 168 + 112 + 64.
 //
 // fp16 operands, not bf16: a dequantised value c + s (n - 8) has more than bf16's 8 bits, and its rounding (2^-12 instead
-// of 2^-9) would otherwise be the largest error of the result. Their range is kept by powers of two: 32 lanes of Q are scaled
-// by their largest element, a tile of K or V by an exponent that its dequantisers choose from the tile's parameters (and
+// of 2^-9) would otherwise be the largest error of the result. Their range is kept by powers of two: a row of Q is scaled
+// by its largest element, a tile of K or V by an exponent that its dequantisers choose from the tile's parameters (and
 // keep while it fits); the scores undo Q's and K's, and V's is carried with the output accumulator.
 // Inside a word the channels are stored in the order 0 4 1 5 2 6 3 7, which is how the nibbles unpack: Q follows it, and
 // the output undoes it for V.
@@ -455,8 +455,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     const int u = wg, r = threadIdx.x & 127;
     const int by_g = p.by_g, row = row0 + u * rpu + ((r * by_g) >> 16);
     const int pos = pos0 + min(row, q_len - 1);              // lanes without a row follow the last one
-    // Q: a power of two per warp takes its largest element to 2^14 .. 2^15 of fp16, which is exact down to 2^-31 of it; the
-    // scale's sign is Q's, and a scale of 0 a Q of 0. A unit's rows of all its heads are contiguous in memory row by row; bulk copies bring them
+    // Q: a power of two per row (and head) takes its largest element to 2^14 .. 2^15 of fp16, which is exact down to 2^-31 of
+    // it; the scale's sign is Q's, and a scale of 0 a Q of 0. A unit's rows of all its heads are contiguous in memory row by row; bulk copies bring them
     // into a K slot that is free until tile 1 + u. All four warps send their share: a copy takes its warp 67 cycles (one warp
     // for all of them 2160; loads by the lanes that convert 3500). Sixteen lanes convert a row, two rows at a time.
     int q_exp = 0;
@@ -478,31 +478,48 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         v[i] = first + 2 * i < lanes ? ld_shared_v4(raw + (first + 2 * i) * 256) : make_uint4(0u, 0u, 0u, 0u);
-      uint32_t tops[4] = {0u, 0u, 0u, 0u};
+      // Largest magnitude of each row, rows i and i + 8 in one word; then sixteen lanes' words in steps that halve what a lane
+      // keeps, so that lanes 2k and 2k + 1 of a half warp end with rows k and k + 8.
+      auto top_of = [](const uint4& r) {
+        const uint32_t m2 = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+        return max(m2 >> 16, m2 & 0xffffu);
+      };
+      uint32_t tops[8], any = 0u;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        tops[i & 3] = __vmaxu2(__vmaxu2(tops[i & 3], __vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu)),
-                               __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
-      const uint32_t top = __vmaxu2(__vmaxu2(tops[0], tops[1]), __vmaxu2(tops[2], tops[3]));
-      uint32_t most = max(top >> 16, top & 0xffffu);
-      if (__any_sync(0xffffffffu, most >= 0x7f80u)) {        // infinities and NaN do not choose the other rows' power
-        most = 0;
+      for (int i = 0; i < 8; ++i) {
+        tops[i] = top_of(v[i]) | top_of(v[i + 8]) << 16;
+        any = __vmaxu2(any, tops[i]);
+      }
+      if (__any_sync(0xffffffffu, __vmaxu2(any, 0x7f7f7f7fu) != 0x7f7f7f7fu)) {      // infinities and NaN do not choose a power
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+          uint32_t most = 0u;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
             most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
           }
+          tops[i & 7] = i < 8 ? most : tops[i & 7] | most << 16;
         }
       }
-      const int e = max(-120, min(120, static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7) - 127 - 14));
-      const float f = p.sign * pow2(-e);
-      q_exp = e;
+#pragma unroll
+      for (int step = 8, n = 4; step >= 2; step >>= 1, n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const bool up = lane & step;
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, up ? tops[i] : tops[i + n], step);
+          tops[i] = __vmaxu2(up ? tops[i + n] : tops[i], other);
+        }
+      tops[0] = __vmaxu2(tops[0], __shfl_xor_sync(0xffffffffu, tops[0], 1));
+      // This thread's row is number 2 i + half of its warp: i = lane / 2, half = lane & 1.
+      const uint32_t word = __shfl_sync(0xffffffffu, tops[0], 16 * (lane & 1) + 2 * ((lane >> 1) & 7));
+      q_exp = max(-120, static_cast<int>((lane < 16 ? word & 0xffffu : word >> 16) >> 7) - 127 - 14);
+      const float f_own = p.sign * pow2(-q_exp);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};         // channels 0 1, 2 3, 4 5, 6 7 of the word
+        const float f = __shfl_sync(0xffffffffu, f_own, 2 * i + (lane >> 4));
         float x[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
