@@ -211,3 +211,11 @@ def test_chunk_row_of_any_finite_size_stays_alone(hq, hkv, crowd):
     c.q[50, 0] *= 2.0 ** 60
     c.q[9] *= 2.0 ** -90
     c.check()
+
+
+@pytest.mark.parametrize("crowd", [0, 160])
+def test_small_values_over_a_long_context(crowd):
+    c = Case([1, 100], [1100, 1500], 4, 1, n_decode=1, extra_pages=300, crowd=crowd, seed=10)
+    c.v = [v * 2.0 ** -112 for v in c.v]
+    c.q *= 0.3
+    c.check()

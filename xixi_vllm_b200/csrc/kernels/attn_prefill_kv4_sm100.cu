@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       }
     } else if (ok) {
       tc_fence_after_sync();
-      const float inv = l == 0.f ? 0.f : vf / l;
+      const float inv = l == 0.f ? 0.f : 1.f / l;            // times vf it may leave fp32: small values, many tokens
       // Rows leave through the unit's Q tile (all its MMAs are over), so that the writes are whole lines.
       const uint32_t at = row_start(smem_u32(q_s) + u * kTileBytes, r);
       uint32_t o[4][32];
@@ -708,7 +708,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       for (int ch = 0; ch < 4; ++ch) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {                        // words of channels 0 4 1 5 2 6 3 7
-          auto x = [&](int i) { return l == 0.f ? 0.f : __uint_as_float(o[ch][8 * w + i]) * inv; };
+          auto x = [&](int i) { return l == 0.f ? 0.f : __uint_as_float(o[ch][8 * w + i]) * inv * vf; };
           st_shared_v4(chunk_at(at, 4 * ch + w), pack_bf16(x(0), x(2)), pack_bf16(x(4), x(6)), pack_bf16(x(1), x(3)),
                        pack_bf16(x(5), x(7)));
         }
