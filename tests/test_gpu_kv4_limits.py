@@ -219,3 +219,25 @@ def test_small_values_over_a_long_context(crowd):
     c.v = [v * 2.0 ** -112 for v in c.v]
     c.q *= 0.3
     c.check()
+
+
+@pytest.mark.parametrize("powers", [(20, -110), (0, -120, 0), (100, -20, -110, 60), (-110, 20), (10, -40, -10, -100)])
+@pytest.mark.parametrize("crowd", [0, 160])
+def test_chunk_values_whose_tiles_differ_by_any_power(powers, crowd):
+    """128 tokens each of V at 2^p: the accumulator's unit must never take it out of fp32."""
+    n = 128 * len(powers)
+    c = Case([100], [n], 4, 1, extra_pages=300, crowd=crowd, seed=8)
+    c.v[0] *= torch.tensor([2.0 ** powers[t // 128] for t in range(n)])[:, None, None]
+    c.check()
+
+
+@pytest.mark.parametrize("crowd", [0, 160])
+def test_chunk_small_values_behind_large_ones_that_no_longer_count(crowd):
+    """Later keys score about 200 higher, so the weights of the first 256 tokens, whose values are 2^80, are 2^-250 and less."""
+    c = Case([100], [512], 4, 1, seed=9, crowd=crowd)
+    c.q = 2.5 * (c.q.abs() + 0.5)
+    c.k[0][256:] = c.k[0][256:].abs() + 2
+    c.k[0][:256] = -c.k[0][:256].abs() - 2
+    c.v[0][:256] *= 2.0 ** 80
+    c.v[0][256:] *= 2.0 ** -30
+    c.check()

@@ -22,7 +22,7 @@
 // fp16 operands, not bf16: a dequantised value c + s (n - 8) has more than bf16's 8 bits, and its rounding (2^-12 instead
 // of 2^-9) would otherwise be the largest error of the result. Their range is kept by powers of two: a row of Q is scaled
 // by its largest element, a tile of K or V by an exponent that its dequantisers choose from the tile's parameters (and
-// keep while it fits); the scores undo Q's and K's, and V's is carried with the output accumulator.
+// keep while it fits); the scores undo Q's and K's, and V's is carried with the output accumulator, row by row.
 // Inside a word the channels are stored in the order 0 4 1 5 2 6 3 7, which is how the nibbles unpack: Q follows it, and
 // the output undoes it for V.
 //
@@ -82,9 +82,8 @@ struct Params {
   __device__ __forceinline__ int by_splits(int n) const { return inv_splits ? __umulhi(n, inv_splits) : n; }
 };
 
-struct alignas(16) TileScale {                    // of one tile: K and V are stored divided by 2^k and v
-  int k;
-  float v, v_inv, unused;
+struct alignas(8) TileScale {                     // of one tile: K and V are stored divided by 2^k and 2^v
+  int k, v;
 };
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -181,7 +180,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   uint64_t* o_done = p_ready + 2;                            // [2]
   uint64_t* xu_done = o_done + 2;                            // [2] a unit's exponentials of the tile are over
   uint64_t* q_raw = xu_done + 2;                             // [2] a unit's rows as they are in memory
-  TileScale* scales = reinterpret_cast<TileScale*>(q_raw + 2);           // [8], by tile (22 barriers before it: 16-byte aligned)
+  TileScale* scales = reinterpret_cast<TileScale*>(q_raw + 2);           // [8], by tile
   uint32_t* red = reinterpret_cast<uint32_t*>(scales + 8);   // [2][12]
   uint32_t* tmem_slot = red + 24;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -331,9 +330,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       if (row == 0) {
         TileScale sc;
         sc.k = ek;
-        sc.v = pow2(ev);
-        sc.v_inv = pow2(-ev);
-        sc.unused = 0.f;
+        sc.v = ev;
         scales[j & 7] = sc;
       }
       const bool more = j + 1 < n_tiles;
@@ -534,7 +531,12 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     }
     const int row_exp = p.scale_exp + q_exp;
     const uint32_t taddr = u * kTmemUnit + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    float m = kNoMax, l = 0.f, vf = 1.f;
+    float m = kNoMax, l = 0.f;
+    // A row's O is in units of 2^unit_v, the current tile's power, but no more than 2^60 below 2^most_v, which bounds what O
+    // holds (|O| < 2^54 2^most_v: 2^31 tokens, P up to 2^8, V up to 2^15), so that no change of units takes it out of fp32.
+    // P of a tile that is smaller still is scaled down instead: next to what O holds the tile is nothing.
+    int unit_v = 0, least_v = 0;                             // least_v = most_v - 60
+    float most_v = 0.f;
     // S scale - m leaves what rounding took from m, 2^-24 of it: of scores of 2^30 more than an exponential may see. Rows whose
     // maximum is beyond 2^24 leave the scale's mantissa out, so that the product with a power of two is exact. Their weights
     // are those of the largest score and of its equals, whatever the mantissa: others as near are within S's own rounding.
@@ -579,9 +581,11 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
           scale = unit;
           m = top * scale;
         }
-        vf = ts.v;
+        unit_v = ts.v;
+        most_v = static_cast<float>(ts.v);
+        least_v = ts.v - 60;
       } else {
-        const bool need = mt > m + kLazy || ts.v != vf;
+        const bool need = mt > m + kLazy || max(ts.v, least_v) != unit_v;
         if (__any_sync(0xffffffffu, need)) {
           ok = __all_sync(0xffffffffu, mbar_wait(&o_done[u], (j - 1) & 1));
           if (!ok) break;
@@ -594,11 +598,14 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
             scale = mantissa * unit;
             m_new = fmaxf(m, top * scale);
           }
-          const float down = exp2f(m - m_new);
-          l *= down;
+          const float grown = m - m_new;
+          l *= exp2f(grown);
           m = m_new;
-          const float alpha = down * (vf * ts.v_inv);
-          vf = ts.v;
+          most_v = fmaxf(most_v + grown, static_cast<float>(ts.v));
+          least_v = static_cast<int>(most_v) - 60;
+          const int to = max(ts.v, least_v);
+          const float alpha = exp2f(grown + static_cast<float>(unit_v - to));
+          unit_v = to;
           const uint64_t alpha2 = pack_f32x2(alpha, alpha);
 #pragma unroll 1
           for (int ch = 0; ch < kD / 16; ++ch) {
@@ -622,7 +629,9 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         ok = __all_sync(0xffffffffu, u == 1 ? mbar_wait(&xu_done[0], j & 1) : mbar_wait(&xu_done[1], (j - 1) & 1));
         if (!ok) break;
       }
-      const uint64_t scale2 = pack_f32x2(scale, scale), negm2 = pack_f32x2(-m, -m);
+      const int below = max(ts.v - unit_v, -60);             // 0 but for tiles below least_v
+      const float less = static_cast<float>(below);
+      const uint64_t scale2 = pack_f32x2(scale, scale), negm2 = pack_f32x2(-m + less, -m + less);
       uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -640,7 +649,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       {
         float a, c;
         unpack_f32x2(add_f32x2(sums[0], sums[1]), a, c);
-        l += a + c;
+        l += (a + c) * pow2(-below);
       }
       mbar_arrive(&xu_done[u]);
       tmem_st_wait();
@@ -653,6 +662,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const size_t slot = (((static_cast<size_t>(z) * gridDim.y + hk) * gridDim.x + blockIdx.x) * p.splits + split) *
                               (2 * kBM) + u * kBM + r;
       *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(mantissa == p.scale ? m : m * p.scale, l);
+      const float vf = pow2(unit_v);
       // Through the unit's Q tile (all its MMAs are over) half the channels at a time, so that the writes are whole lines. A
       // split without tiles leaves no output, only m = kNoMax, l = 0.
       const uint32_t tile = smem_u32(q_s) + u * kTileBytes;
@@ -690,6 +700,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       }
     } else if (ok) {
       tc_fence_after_sync();
+      const float vf = pow2(unit_v);
       const float inv = l == 0.f ? 0.f : 1.f / l;            // times vf it may leave fp32: small values, many tokens
       // Rows leave through the unit's Q tile (all its MMAs are over), so that the writes are whole lines.
       const uint32_t at = row_start(smem_u32(q_s) + u * kTileBytes, r);
