@@ -241,3 +241,20 @@ def test_chunk_small_values_behind_large_ones_that_no_longer_count(crowd):
     c.v[0][:256] *= 2.0 ** 80
     c.v[0][256:] *= 2.0 ** -30
     c.check()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("crowd", [0, 160])
+def test_chunk_query_row_that_is_not_finite_is_nan_and_stays_alone(bad, sign, crowd):
+    """Also where all its scores are -inf: a softmax of those is NaN, not zeros."""
+    c = Case([40, 3], [40, 600], 4, 2, extra_pages=300, crowd=crowd, seed=11)
+    for k in c.k:
+        k[..., 5] = sign * (k[..., 5].abs() + 1)
+    c.q[7, 2, 5] = c.q[41, 0, 5] = 0.0
+    clean = c.run()
+    c.q[7, 2, 5] = c.q[41, 0, 5] = bad
+    out = c.run()
+    assert not bool(out[7, 2].isfinite().any()) and not bool(out[41, 0].isfinite().any())
+    out[7, 2], out[41, 0] = clean[7, 2], clean[41, 0]
+    assert torch.equal(out, clean)

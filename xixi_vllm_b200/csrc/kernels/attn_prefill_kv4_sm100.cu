@@ -487,16 +487,19 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         tops[i] = top_of(v[i]) | top_of(v[i + 8]) << 16;
         any = __vmaxu2(any, tops[i]);
       }
-      if (__any_sync(0xffffffffu, __vmaxu2(any, 0x7f7f7f7fu) != 0x7f7f7f7fu)) {      // infinities and NaN do not choose a power
+      // Infinities and NaN do not choose a power, and are NaN: a row of scores that are all -inf has no softmax.
+      if (__any_sync(0xffffffffu, __vmaxu2(any, 0x7f7f7f7fu) != 0x7f7f7f7fu)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+          uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
           uint32_t most = 0u;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t lo = w[k] & 0x7fffu, hi = (w[k] >> 16) & 0x7fffu;
             most = max(most, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+            w[k] |= (lo < 0x7f80u ? 0u : 0x7fffu) | (hi < 0x7f80u ? 0u : 0x7fff0000u);
           }
+          v[i] = make_uint4(w[0], w[1], w[2], w[3]);
           tops[i & 7] = i < 8 ? most : tops[i & 7] | most << 16;
         }
       }
