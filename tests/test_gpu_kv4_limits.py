@@ -258,3 +258,20 @@ def test_chunk_query_row_that_is_not_finite_is_nan_and_stays_alone(bad, sign, cr
     assert not bool(out[7, 2].isfinite().any()) and not bool(out[41, 0].isfinite().any())
     out[7, 2], out[41, 0] = clean[7, 2], clean[41, 0]
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("q_len,n_decode,extra_pages", [(1, 1, 1), (1, 1, WIDE), (40, 0, 1), (200, 0, 1), (40, 0, 300)])
+def test_values_that_are_not_finite_reach_the_channels_of_their_group(q_len, n_decode, extra_pages):
+    """One channel of a V row is infinite: its group's half of the row is held as NaN, and the rows that see it are NaN
+    there; the other half is as if the group held zeros."""
+    c = Case([q_len], [q_len + 600], 4, 1, n_decode=n_decode, extra_pages=extra_pages, seed=12)
+    at = 600 + q_len // 2
+    of = torch.arange(D) // 8 % 2 == 1
+    c.v[0][at, 0, of] = 0.0
+    clean = c.run()
+    c.v[0][at, 0, 9] = float("inf")
+    out = c.run()
+    first = q_len // 2
+    assert bool(out[first:, :, of].isnan().all())
+    out[first:, :, of] = clean[first:, :, of]
+    assert torch.equal(out, clean)

@@ -26,17 +26,20 @@
 // Inside a word the channels are stored in the order 0 4 1 5 2 6 3 7, which is how the nibbles unpack: Q follows it, and
 // the output undoes it for V.
 //
-// Rows that do not see a token never meet its values: its score is replaced by -inf, P is 0 there, and V of a token whose
-// parameters are not finite is stored as 0 with its K made NaN, so that exactly the rows that see it become NaN.
+// Rows that do not see a token never meet its values: its score is replaced by -inf, P is 0 there, and a group of V whose
+// parameters are not finite is stored as 0. The first token of each group that had such is kept; the rows that see it
+// become NaN in that group's channels at the end.
 // Every wait is bounded; one that runs out records a status code, the CTA stops issuing work, frees its tensor memory and
 // returns.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <math_constants.h>
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 
@@ -182,7 +185,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   uint64_t* q_raw = xu_done + 2;                             // [2] a unit's rows as they are in memory
   TileScale* scales = reinterpret_cast<TileScale*>(q_raw + 2);           // [8], by tile
   uint32_t* red = reinterpret_cast<uint32_t*>(scales + 8);   // [2][12]
-  uint32_t* tmem_slot = red + 24;
+  int* first_bad = reinterpret_cast<int*>(red + 24);         // [2 groups of V]: the first token whose values are not finite
+  uint32_t* tmem_slot = red + 26;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wg = warp >> 2;
@@ -207,6 +211,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       mbar_init(&v_empty[s], 2);
     }
     *abort_flag = 0;
+    first_bad[0] = first_bad[1] = INT_MAX;
     mbar_fence_init();
   }
   __syncthreads();
@@ -278,14 +283,18 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     };
     uint4 kc[4], vc[4];
     uint2 kp, vp, kp_next = make_uint2(0u, 0u), vp_next = make_uint2(0u, 0u);
-    // What counts of tile j's parameters (a V that is not finite makes K not finite instead), and the tile's largest
+    // What counts of tile j's parameters (values of V that are not finite are noted and count as 0), and the tile's largest
     // possible magnitudes, left in `red` for everyone.
     auto admit = [&](int j, bool ok) {
       if ((tile0 + j) * kBN + row >= n_kv) kp = vp = make_uint2(0u, 0u);
       auto finite = [](uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; };
-      if (!finite(vp.x) || !finite(vp.y)) {
-        vp = make_uint2(0u, 0u);
-        kp = make_uint2(0x7fff7fffu, 0x7fff7fffu);
+      if (!finite(vp.x)) {
+        atomicMin(first_bad, (tile0 + j) * kBN + row);
+        vp.x = 0u;
+      }
+      if (!finite(vp.y)) {
+        atomicMin(first_bad + 1, (tile0 + j) * kBN + row);
+        vp.y = 0u;
       }
       auto bound = [](uint2 w) {
         return fmaxf(fabsf(kv4::par_c(w.x)) + 8.f * fabsf(kv4::par_s(w.x)), fabsf(kv4::par_c(w.y)) + 8.f * fabsf(kv4::par_s(w.y)));
@@ -665,7 +674,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const size_t slot = (((static_cast<size_t>(z) * gridDim.y + hk) * gridDim.x + blockIdx.x) * p.splits + split) *
                               (2 * kBM) + u * kBM + r;
       *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(mantissa == p.scale ? m : m * p.scale, l);
-      const float vf = pow2(unit_v);
+      const float vf0 = pos >= first_bad[0] ? CUDART_NAN_F : pow2(unit_v), vf1 = pos >= first_bad[1] ? CUDART_NAN_F : pow2(unit_v);
       // Through the unit's Q tile (all its MMAs are over) half the channels at a time, so that the writes are whole lines. A
       // split without tiles leaves no output, only m = kNoMax, l = 0.
       const uint32_t tile = smem_u32(q_s) + u * kTileBytes;
@@ -682,7 +691,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         for (int ch = 0; ch < 2; ++ch) {
 #pragma unroll
           for (int w = 0; w < 4; ++w) {                      // words of channels 0 4 1 5 2 6 3 7
-            auto x = [&](int i) { return __float_as_uint(__uint_as_float(o[ch][8 * w + i]) * vf); };
+            auto x = [&](int i) { return __float_as_uint(__uint_as_float(o[ch][8 * w + i]) * ((w & 1) ? vf1 : vf0)); };
             const int k = ch * 8 + 2 * w;
             st_shared_v4(tile + r * 256 + ((k ^ (r & 15)) << 4), x(0), x(2), x(4), x(6));
             st_shared_v4(tile + r * 256 + (((k + 1) ^ (r & 15)) << 4), x(1), x(3), x(5), x(7));
@@ -703,8 +712,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       }
     } else if (ok) {
       tc_fence_after_sync();
-      const float vf = pow2(unit_v);
-      const float inv = l == 0.f ? 0.f : 1.f / l;            // times vf it may leave fp32: small values, many tokens
+      const float vf0 = pos >= first_bad[0] ? CUDART_NAN_F : pow2(unit_v), vf1 = pos >= first_bad[1] ? CUDART_NAN_F : pow2(unit_v);
+      const float inv = l == 0.f ? 0.f : 1.f / l;            // times 2^unit_v it may leave fp32: small values, many tokens
       // Rows leave through the unit's Q tile (all its MMAs are over), so that the writes are whole lines.
       const uint32_t at = row_start(smem_u32(q_s) + u * kTileBytes, r);
       uint32_t o[4][32];
@@ -722,7 +731,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       for (int ch = 0; ch < 4; ++ch) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {                        // words of channels 0 4 1 5 2 6 3 7
-          auto x = [&](int i) { return l == 0.f ? 0.f : __uint_as_float(o[ch][8 * w + i]) * inv * vf; };
+          auto x = [&](int i) { return l == 0.f ? 0.f : __uint_as_float(o[ch][8 * w + i]) * inv * ((w & 1) ? vf1 : vf0); };
           st_shared_v4(chunk_at(at, 4 * ch + w), pack_bf16(x(0), x(2)), pack_bf16(x(4), x(6)), pack_bf16(x(1), x(3)),
                        pack_bf16(x(5), x(7)));
         }
