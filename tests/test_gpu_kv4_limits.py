@@ -275,3 +275,13 @@ def test_values_that_are_not_finite_reach_the_channels_of_their_group(q_len, n_d
     assert bool(out[first:, :, of].isnan().all())
     out[first:, :, of] = clean[first:, :, of]
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("power", [124, 110, -110, -118])
+@pytest.mark.parametrize("crowd", [0, 160])
+def test_chunk_queries_at_the_ends_of_the_range(power, crowd):
+    c = Case([30, 140], [60, 333], 6, 2, extra_pages=300, seed=4, crowd=crowd)
+    c.q.clamp_(-4, 4).mul_(2.0 ** power)
+    c.q[:, ::2].abs_()
+    c.k = [k * 2.0 ** -min(power, 120) for k in c.k]
+    c.check(SCALE * 2.0 ** (-power + min(power, 120)))

@@ -142,10 +142,23 @@ __device__ __forceinline__ __half2 centred_f16(uint32_t w, bool odd) {
   return __hsub2(*reinterpret_cast<const __half2*>(&r), __floats2half2_rn(1032.f, 1032.f));
 }
 
+// a b and a b + c where a or c may be subnormal, which the library's fast-math flags take for 0: the centre of a group that
+// is small throughout (its step is never subnormal).
+__device__ __forceinline__ float mul_whole(float a, float b) {
+  float d;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float fma_whole(float a, float b, float c) {
+  float d;
+  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // A group's parameters as fp16 pairs, the tile's power of two taken out.
 struct Pair {
   __half2 s, c;
-  __device__ __forceinline__ Pair(uint32_t w, float f) : s(__float2half2_rn(kv4::par_s(w) * f)), c(__float2half2_rn(kv4::par_c(w) * f)) {}
+  __device__ __forceinline__ Pair(uint32_t w, float f) : s(__float2half2_rn(kv4::par_s(w) * f)), c(__float2half2_rn(mul_whole(kv4::par_c(w), f))) {}
 };
 
 // 16 of a row's 64 code bytes as fp16 c + s (n - 8) into chunks c0 .. c0 + 3: words of even index belong to group 0.
@@ -297,9 +310,10 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         vp.y = 0u;
       }
       auto bound = [](uint2 w) {
-        return fmaxf(fabsf(kv4::par_c(w.x)) + 8.f * fabsf(kv4::par_s(w.x)), fabsf(kv4::par_c(w.y)) + 8.f * fabsf(kv4::par_s(w.y)));
+        return max(__float_as_uint(fma_whole(8.f, kv4::par_s(w.x & 0x7fffu), kv4::par_c(w.x & 0x7fff0000u))),
+                   __float_as_uint(fma_whole(8.f, kv4::par_s(w.y & 0x7fffu), kv4::par_c(w.y & 0x7fff0000u))));
       };
-      const uint32_t kb = __float_as_uint(finite(kp.x) && finite(kp.y) ? bound(kp) : 0.f), vb = __float_as_uint(bound(vp));
+      const uint32_t kb = finite(kp.x) && finite(kp.y) ? bound(kp) : 0u, vb = bound(vp);
       const uint32_t kw = __reduce_max_sync(0xffffffffu, kb), vw = __reduce_max_sync(0xffffffffu, vb);
       if (lane == 0) {
         uint32_t* at = red + (j & 1) * 12 + (warp & 3);
