@@ -285,3 +285,63 @@ def test_chunk_queries_at_the_ends_of_the_range(power, crowd):
     c.q[:, ::2].abs_()
     c.k = [k * 2.0 ** -min(power, 120) for k in c.k]
     c.check(SCALE * 2.0 ** (-power + min(power, 120)))
+
+
+def test_chunks_without_rows_and_chunks_beyond_max_q_len():
+    """Rows that no chunk covers are zeros whatever max_q_len says; a chunk that is longer than it is reported and comes
+    out as zeros, its neighbours untouched."""
+    ops, cuda = _ops(), _cuda()
+    for extra_pages in (1, 300):
+        c = Case([1, 5, 70, 9], [30, 45, 600, 9], 4, 2, n_decode=1, extra_pages=extra_pages, seed=13)
+        k, v = (x.to(DEV) for x in c.caches())
+        q = torch.cat([c.q, torch.ones(300, 4, D)]).bfloat16().flatten(1).to(DEV)
+        want = ops.paged_attention(q, k, v, c.attn(), SCALE, 4, 2, D)
+        assert bool(want[:85].any(-1).all()) and not want[85:].any()
+        for most in (0, 1, 8, 9, 64, 69):
+            torch.full_like(q, 7.0)                          # what the allocator may hand out again
+            attn = c.attn()
+            attn.max_q_len = most
+            got = ops.paged_attention(q, k, v, attn, SCALE, 4, 2, D)
+            with pytest.raises(RuntimeError, match="status 5"):
+                cuda.check_status()
+            at = 0
+            for n in c.q_lens:
+                if n == 1 or n <= most:
+                    torch.testing.assert_close(got[at:at + n], want[at:at + n], rtol=2 * HALF_BF16, atol=2.0 ** -8)
+                else:
+                    assert not got[at:at + n].any()
+                at += n
+            assert not got[85:].any()
+        for most in (0, 2 ** 31 - 1):                        # empty chunks only; a bound far above any row count
+            attn = c.attn()
+            if most == 0:
+                attn.cu_q = torch.tensor([0, 1, 1, 1, 1], **I32)
+            attn.max_q_len = most
+            torch.full_like(q, 7.0)
+            got = ops.paged_attention(q, k, v, attn, SCALE, 4, 2, D)
+            cuda.check_status()
+            torch.testing.assert_close(got, want if most else torch.cat([want[:1], torch.zeros_like(want[1:])]),
+                                       rtol=2 * HALF_BF16, atol=2.0 ** -8)
+        attn.max_q_len = -1
+        with pytest.raises(ValueError, match="max_q_len"):
+            ops.paged_attention(q, k, v, attn, SCALE, 4, 2, D)
+        attn = c.attn()
+        attn.cu_q = torch.tensor([0, 1, 6, 76, 2000], **I32)          # beyond the rows of q
+        torch.full_like(q, 7.0)
+        got = ops.paged_attention(q, k, v, attn, SCALE, 4, 2, D)
+        with pytest.raises(RuntimeError, match="status 5"):
+            cuda.check_status()
+        torch.testing.assert_close(got[:76], want[:76], rtol=2 * HALF_BF16, atol=2.0 ** -8)
+        assert not got[76:].any()
+        attn.cu_q = torch.tensor([0, 4, 9, 79, 88], **I32)            # three rows between the decode row and the chunks
+        torch.full_like(q, 7.0)
+        moved = torch.cat([q[:1], torch.ones_like(q[:3]), q[1:-3]])
+        got = ops.paged_attention(moved, k, v, attn, SCALE, 4, 2, D)
+        cuda.check_status()
+        assert torch.equal(got[:1], want[:1]) and torch.equal(got[4:88], want[1:85]) and not got[1:4].any() and not got[88:].any()
+        attn.cu_q = torch.tensor([0, 0, 6, 76, 85], **I32)            # the first chunk begins on the decode row
+        torch.full_like(q, 7.0)
+        got = ops.paged_attention(q, k, v, attn, SCALE, 4, 2, D)
+        with pytest.raises(RuntimeError, match="status 5"):
+            cuda.check_status()
+        assert torch.equal(got[:1], want[:1]) and torch.equal(got[6:], want[6:]) and not got[1:6].any()

@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdint>
@@ -222,9 +223,11 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
              static_cast<long long>(hq) * d, c.dev.str().c_str(), shape_of(q).c_str(), q.device().str().c_str());
     if (hq <= 0 || hq % hkv || hq / hkv > 16)
       refuse(PyExc_ValueError, "paged_attention: %d query heads over %d KV heads (at most 16 to one)", hq, hkv);
-    const int B = integer(a[6], "num_seqs"), nd = integer(a[7], "num_decode"), mq = integer(a[8], "max_q_len");
+    const int B = integer(a[6], "num_seqs"), nd = integer(a[7], "num_decode"), most = integer(a[8], "max_q_len");
     const int np = B - nd;
     const int64_t T = q.size(0);
+    if (most < 0) refuse(PyExc_ValueError, "paged_attention: max_q_len = %d", most);
+    const int mq = static_cast<int>(std::min<int64_t>(most, T));       // no chunk has more rows than q
     if (nd < 0 || np < 0 || nd > T || T > INT32_MAX || bt.dim() != 2 || bt.size(0) < B || bt.size(1) > INT32_MAX)
       refuse(PyExc_ValueError, "paged_attention: %d decode rows and %d chunks for %lld query rows and a block table of %s", nd, np,
              static_cast<long long>(T), shape_of(bt).c_str());
@@ -242,7 +245,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto* status = static_cast<int*>(vector(tensor(a[14], "status"), 1, at::kInt, c.dev, "status"));
     const c10::cuda::OptionalCUDAGuard guard(c.dev);
     at::Tensor out = fresh({T, q.size(1)}, at::kBFloat16, c.dev);
-    if (maxb == 0 || c.blocks == 0) {                                   // nothing is cached: every row is empty
+    if (T == 0 || maxb == 0 || c.blocks == 0) {                         // nothing is cached: every row is empty
       out.zero_();
       return THPVariable_Wrap(std::move(out));
     }

@@ -76,7 +76,7 @@ struct Params {
   int* status;
   float* ws_o;                                    // [CTA][split][256 lanes][128] unnormalised outputs, when splits > 1
   float* ws_ml;                                   // [CTA][split][256 lanes][2]: maximum (log2 units), sum
-  int seq_begin, hq, hkv, block_size, max_blocks, num_blocks, total_rows, splits;
+  int seq_begin, num_seqs, max_q_len, hq, hkv, block_size, max_blocks, num_blocks, total_rows, splits;
   float scale, sign;                              // of a score, times log2 e: sign * scale * 2^scale_exp, scale in 1 .. 2
   int scale_exp;
   int G, rpu, by_g;                               // heads to a KV head, rows of a unit; 65536 / G + 1: lane / G is a product
@@ -84,6 +84,17 @@ struct Params {
   // n / splits; exact for n splits < 2^32.
   __device__ __forceinline__ int by_splits(int n) const { return inv_splits ? __umulhi(n, inv_splits) : n; }
 };
+
+// Whether a chunk's rows are rows of Q behind the decode rows, and no more than the launch has CTAs for.
+__device__ __forceinline__ bool rows_fine(const Params& p, int q_begin, int q_end) {
+  return q_begin >= p.seq_begin && q_end >= q_begin && q_end <= p.total_rows && q_end - q_begin <= p.max_q_len;
+}
+// Clears 16-byte pieces of output rows: `pieces` from piece `at` on of each row in [from, to), by `workers` threads.
+__device__ __forceinline__ void clear_rows(const Params& p, int from, int to, int at, int pieces, int worker, int workers) {
+  const size_t row = static_cast<size_t>(p.hq) * (kD / 8), all = from < to ? static_cast<size_t>(to - from) * pieces : 0;
+  for (size_t i = worker; i < all; i += workers)
+    reinterpret_cast<uint4*>(p.out)[(from + i / pieces) * row + at + i % pieces] = make_uint4(0u, 0u, 0u, 0u);
+}
 
 struct alignas(8) TileScale {                     // of one tile: K and V are stored divided by 2^k and 2^v
   int k, v;
@@ -233,14 +244,18 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   const int z = p.by_splits(blockIdx.z), split = blockIdx.z - z * p.splits, b = p.seq_begin + z, hk = blockIdx.y;
   const int q_begin = p.cu_q[b], q_end = p.cu_q[b + 1];
   int kv_len = max(p.kv_lens[b], 0);
-  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && blockIdx.z == gridDim.z - 1) {       // rows behind the last sequence
-    const size_t row_chunks = static_cast<size_t>(p.hq) * (kD / 8), last = p.total_rows * row_chunks;
-    for (size_t i = max(q_end, 0) * row_chunks + threadIdx.x; i < last; i += blockDim.x)
-      reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && (z == 0 || z == p.num_seqs - 1) && split == 0) {      // rows of no chunk
+    const int pieces = p.hq * (kD / 8), threads = blockDim.x;
+    if (z == 0) clear_rows(p, p.seq_begin, min(q_begin, p.total_rows), 0, pieces, threadIdx.x, threads);
+    if (z == p.num_seqs - 1) clear_rows(p, max(max(q_begin, q_end), p.seq_begin), p.total_rows, 0, pieces, threadIdx.x, threads);
   }
   const int q_len = q_end - q_begin;
-  if (q_begin < 0 || q_len < 0 || q_len > p.total_rows - q_begin) {
+  if (!rows_fine(p, q_begin, q_end)) {
     if (threadIdx.x == 0) report_status(p.status, kId, kBadIndex);
+    const int pieces = p.G * (kD / 8);
+    if (split == 0)
+      clear_rows(p, max(q_begin, p.seq_begin), min(q_end, p.total_rows), hk * pieces, pieces,
+                 blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
     return;
   }
   const int G = p.G, rpu = p.rpu;                            // heads of a KV head; query rows of a unit
@@ -787,7 +802,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_prefill_join_kernel(const
   grid_dep_wait();
   const int b = p.seq_begin + blockIdx.z, hk = blockIdx.y;
   const int q_begin = p.cu_q[b], q_len = p.cu_q[b + 1] - q_begin;
-  if (q_begin < 0 || q_len < 0 || q_len > p.total_rows - q_begin) return;
+  if (!rows_fine(p, q_begin, p.cu_q[b + 1])) return;
   const int G = p.hq / p.hkv, rpu = kBM / G;
   const int i = blockIdx.x * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int block = i / (2 * kBM), u = (i / kBM) & 1, r = i % kBM;
@@ -829,7 +844,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_prefill_join_kernel(const
 
 int blocks_of(int max_q_len, int hq, int hkv) {
   const int rows = 2 * (kBM / (hq / hkv));
-  return (max_q_len + rows - 1) / rows;
+  return std::max(1, static_cast<int>((max_q_len + rows - 1ll) / rows));          // one to clear rows even where all chunks are empty
 }
 
 }  // namespace
@@ -856,10 +871,10 @@ int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, cons
                    const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq, int hkv,
                    int d, int block_size, int max_blocks, int num_blocks, float scale, int splits, void* workspace,
                    long long workspace_bytes, int* status, cudaStream_t stream) {
-  if (num_seqs <= 0 || max_q_len <= 0) return 0;
+  if (num_seqs <= 0) return 0;
   if (d != kD) return XV_ERR_UNSUPPORTED;
   if (hkv <= 0 || hq <= 0 || hq % hkv || hq / hkv > 16 || block_size <= 0 || block_size % kv4::kUnit || max_blocks <= 0 ||
-      num_blocks <= 0 || hkv > 65535 || splits < 1 || static_cast<long long>(num_seqs) * splits > 65535)
+      num_blocks <= 0 || hkv > 65535 || splits < 1 || max_q_len < 0 || static_cast<long long>(num_seqs) * splits > 65535)
     return XV_ERR_SHAPE;
   if (splits > 1 && (!workspace || workspace_bytes < xv_kv4_prefill_workspace_bytes(num_seqs, max_q_len, hq, hkv, splits)))
     return XV_ERR_WORKSPACE;
@@ -884,7 +899,7 @@ int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, cons
   p.kv_lens = kv_lens;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.status = status;
-  p.seq_begin = seq_begin; p.hq = hq; p.hkv = hkv; p.block_size = block_size; p.max_blocks = max_blocks;
+  p.seq_begin = seq_begin; p.num_seqs = num_seqs; p.max_q_len = max_q_len; p.hq = hq; p.hkv = hkv; p.block_size = block_size; p.max_blocks = max_blocks;
   p.num_blocks = num_blocks; p.total_rows = total_rows;
   const double s = scale == 0.f ? 1.0 : std::abs(static_cast<double>(scale)) * kLog2e;
   p.scale = static_cast<float>(2.0 * std::frexp(s, &p.scale_exp));

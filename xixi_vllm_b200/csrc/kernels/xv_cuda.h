@@ -160,7 +160,8 @@ int xv_kv4_write(const void* qkv, const float* partials, int splits, long long s
 int xv_kv4_read(const void* k_cache, const void* v_cache, const int* slots, void* k_out, void* v_out, int tokens, int hkv,
                 int d, int block_size, int num_blocks, int* status, cudaStream_t stream);
 // As xv_attn_decode / xv_attn_prefill. Block-table entries outside [0, num_blocks), lengths beyond the table and query
-// ranges beyond total_rows are reported through `status`, never followed.
+// ranges that reach beyond total_rows, into the decode rows or over more than max_q_len rows are reported through `status`,
+// never followed: rows of such a range are zeros, and so are the rows behind seq_begin that no chunk names.
 // xv_kv4_decode_splits: 1..8 CTAs per (sequence, KV head), joined inside a cluster, or 0: even shares of all tokens, which
 // need xv_kv4_decode_workspace_bytes(...) bytes.
 int xv_kv4_decode_splits(int num_seqs, int hkv, int num_sms, int max_tokens_per_seq);

@@ -93,8 +93,9 @@ def read_cache(k_cache, v_cache, slots, head_dim):
 
 def paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim):
     """``attn`` is a ``runtime.staging.AttnBatch`` (cu_q, kv_lens, block_tables, decode split). The caches are bf16
-    pages or, as uint8, pages held in 4 bits (``ops.kv4``). On a 4-bit cache rows of ``q`` behind the last sequence, rows of
-    a sequence without cached tokens and rows before position 0 come out as zeros; ``scale`` is finite."""
+    pages or, as uint8, pages held in 4 bits (``ops.kv4``). On a 4-bit cache rows of ``q`` that no sequence names, rows of
+    a sequence without cached tokens and rows before position 0 come out as zeros; ``scale`` is finite. On the GPU a chunk
+    that is longer than ``attn.max_q_len`` or reaches beyond ``q`` is reported through the status word and is zeros."""
     if q.is_cuda:
         return _cuda().paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim)
     return cpu_ref.paged_attention(q, k_cache, v_cache, attn.cu_q, attn.kv_lens, attn.block_tables,
