@@ -345,3 +345,19 @@ def test_chunks_without_rows_and_chunks_beyond_max_q_len():
         with pytest.raises(RuntimeError, match="status 5"):
             cuda.check_status()
         assert torch.equal(got[:1], want[:1]) and torch.equal(got[6:], want[6:]) and not got[1:6].any()
+
+
+@pytest.mark.parametrize("power", [60, 110])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("crowd", [0, 160])
+def test_chunk_tokens_far_larger_than_their_neighbours(which, power, crowd):
+    """Two tokens of 2^60 times the others' size inside one tile of a chunk: rows before them do not see them, rows behind
+    them give them no weight (their scores are the lowest) or all of what they are worth."""
+    c = Case([100, 30], [100, 560], 4, 1, extra_pages=300, crowd=crowd, seed=14)
+    c.q = c.q.abs() + 0.5
+    for b, at in ((0, 50), (0, 90), (1, 545)):
+        if which == "k":
+            c.k[b][at] = -(c.k[b][at].abs() + 1) * 2.0 ** power
+        else:
+            c.v[b][at] *= 2.0 ** power
+    c.check()

@@ -22,7 +22,9 @@
 // fp16 operands, not bf16: a dequantised value c + s (n - 8) has more than bf16's 8 bits, and its rounding (2^-12 instead
 // of 2^-9) would otherwise be the largest error of the result. Their range is kept by powers of two: a row of Q is scaled
 // by its largest element, a tile of K or V by an exponent that its dequantisers choose from the tile's parameters (and
-// keep while it fits); the scores undo Q's and K's, and V's is carried with the output accumulator, row by row.
+// keep while it fits); the scores undo Q's and K's, and V's is carried with the output accumulator, row by row. In a tile
+// with tokens 2^20 and more below its largest every token has its own exponent, so that a large one that a row does not see, or
+// gives no weight, costs the row nothing of the others; softmax takes such tiles by a slower way of its own.
 // Inside a word the channels are stored in the order 0 4 1 5 2 6 3 7, which is how the nibbles unpack: Q follows it, and
 // the output undoes it for V.
 //
@@ -58,7 +60,8 @@ constexpr int kHalf = kBN * 128;                  // bytes of 64 channels of a t
 constexpr int kTileBytes = 2 * kHalf;             // 32 KiB
 constexpr int kNK = 3, kNV = 2;                   // ring slots
 constexpr int kBarBytes = 512;                    // barriers and small arrays
-constexpr int kSmem = (2 + kNK + kNV) * kTileBytes + 1024 + kBarBytes;
+constexpr int kPowerBytes = 4 * 2 * kBN;          // [4 tiles][K, V][token]: powers of tokens
+constexpr int kSmem = (2 + kNK + kNV) * kTileBytes + 1024 + kBarBytes + kPowerBytes;
 constexpr uint32_t kTmemCols = 512, kTmemUnit = 256, kTmemO = 128;       // all of it, so it begins at address 0
 constexpr int kId = 12;
 constexpr double kLog2e = 1.4426950408889634;
@@ -96,8 +99,8 @@ __device__ __forceinline__ void clear_rows(const Params& p, int from, int to, in
     reinterpret_cast<uint4*>(p.out)[(from + i / pieces) * row + at + i % pieces] = make_uint4(0u, 0u, 0u, 0u);
 }
 
-struct alignas(8) TileScale {                     // of one tile: K and V are stored divided by 2^k and 2^v
-  int k, v;
+struct alignas(16) TileScale {                    // of one tile: K and V are stored divided by 2^k and 2^v
+  int k, v, own, unused;                          // own: each token has its own k and v
 };
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -189,6 +192,117 @@ __device__ __forceinline__ void put_words(uint32_t row_at, int c0, const uint4& 
   }
 }
 
+// What a lane of the softmax keeps of its row between tiles.
+struct RowState {
+  float m, l;                                     // running maximum in log2 units (it may lag), sum of P
+  // S scale - m leaves what rounding took from m, 2^-24 of it: of scores of 2^30 more than an exponential may see. Rows whose
+  // maximum is beyond 2^24 leave the scale's mantissa out, so that the product with a power of two is exact. Their weights
+  // are those of the largest score and of its equals, whatever the mantissa: others as near are within S's own rounding.
+  float mantissa;
+  // O is in units of 2^unit_v, the current tile's power, but no more than 2^60 below 2^most_v, which bounds what O holds
+  // (|O| < 2^54 2^most_v: 2^31 tokens, P up to 2^8, V up to 2^15), so that no change of units takes it out of fp32. P of a tile
+  // that is smaller still is scaled down instead: next to what O holds the tile is nothing.
+  float most_v;
+  int unit_v, least_v;                            // least_v = most_v - 60
+
+  static __device__ __forceinline__ bool is_huge(float x) { return fabsf(x) > 16777216.f && x != kNoMax; }
+  // To a new maximum and a tile of V in units of 2^tile_v; returns what O is to be multiplied by.
+  __device__ __forceinline__ float settle(const Params& p, float top, float unit, float m_new, int tile_v) {
+    const float want = is_huge(m_new) ? 1.f : p.scale;
+    if (want != mantissa) {
+      m *= want / mantissa;
+      mantissa = want;
+      m_new = fmaxf(m, top * (mantissa * unit));
+    }
+    const float grown = m - m_new;
+    l *= exp2f(grown);
+    m = m_new;
+    most_v = fmaxf(most_v + grown, static_cast<float>(tile_v));
+    least_v = static_cast<int>(most_v) - 60;
+    const int to = max(tile_v, least_v);
+    const float alpha = exp2f(grown + static_cast<float>(unit_v - to));
+    unit_v = to;
+    return alpha;
+  }
+};
+
+__device__ __forceinline__ void rescale(uint32_t taddr, float alpha) {
+  const uint64_t alpha2 = pack_f32x2(alpha, alpha);
+#pragma unroll 1
+  for (int ch = 0; ch < kD / 16; ++ch) {
+    uint32_t o[16];
+    tmem_ld16(taddr + kTmemO + ch * 16, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      float lo, hi;
+      unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), alpha2), lo, hi);
+      o[i] = __float_as_uint(lo);
+      o[i + 1] = __float_as_uint(hi);
+    }
+    tmem_st16(taddr + kTmemO + ch * 16, o);
+  }
+  tmem_st_wait();
+}
+
+// The softmax of a tile whose tokens have powers of their own (own: K's, then V's), of which the row sees the first `seen`: two
+// walks over S, 32 columns at a time. The row's unit of V is the largest of what it sees, and P of the other tokens is scaled
+// down to it. False: a wait ran out.
+__device__ __forceinline__ bool apart_tile(const Params& p, RowState& st, const TileScale ts, const int8_t* own, int seen, float unit,
+                                        uint32_t taddr, int u, int j, uint64_t* o_done, uint64_t* xu_done, uint64_t* p_ready) {
+  auto score = [&](uint32_t x, int i) {
+    return i < seen ? __uint_as_float(x) * pow2(max(own[i] - ts.k, -126)) : __uint_as_float(0xff800000u);
+  };
+  float top = __uint_as_float(0xff800000u);
+  int tile_v = -120;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t x[32];
+    tmem_ld32(taddr + c * 32, x);
+    tmem_ld_wait();
+    tmem_ld_fence_regs(x);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      top = fmaxf(top, score(x[i], c * 32 + i));
+      if (c * 32 + i < seen) tile_v = max(tile_v, static_cast<int>(own[kBN + c * 32 + i]));
+    }
+  }
+  if (j > 0) {
+    if (!__all_sync(0xffffffffu, mbar_wait(&o_done[u], (j - 1) & 1))) return false;
+    tc_fence_after_sync();
+  }
+  const float alpha = st.settle(p, top, unit, fmaxf(st.m, top * (st.mantissa * unit)), tile_v), scale = st.mantissa * unit;
+  if (j > 0) rescale(taddr, alpha);
+  if ((u == 1 || j > 0) && !__all_sync(0xffffffffu, u == 1 ? mbar_wait(&xu_done[0], j & 1) : mbar_wait(&xu_done[1], (j - 1) & 1)))
+    return false;
+  float l = st.l;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t x[32], packed[16];
+    tmem_ld32(taddr + c * 32, x);
+    tmem_ld_wait();
+    tmem_ld_fence_regs(x);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float of[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float y = fmaf(score(x[i + k], c * 32 + i + k), scale, -st.m);
+        l += exp2f(y);
+        of[k] = exp2f(y + static_cast<float>(own[kBN + c * 32 + i + k] - st.unit_v));
+      }
+      packed[i >> 1] = pack_f16(of[0], of[1]);
+    }
+    tmem_st16(taddr + c * 16, packed);            // over scores that have been read
+  }
+  st.l = l;
+  mbar_arrive(&xu_done[u]);
+  tmem_st_wait();
+  tc_fence_before_sync();
+  mbar_arrive(&p_ready[u]);
+  return true;
+}
+
 __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
@@ -211,6 +325,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   uint32_t* red = reinterpret_cast<uint32_t*>(scales + 8);   // [2][12]
   int* first_bad = reinterpret_cast<int*>(red + 24);         // [2 groups of V]: the first token whose values are not finite
   uint32_t* tmem_slot = red + 26;
+  volatile int* again = reinterpret_cast<volatile int*>(red + 28);       // [4 warps]
+  int8_t* powers = reinterpret_cast<int8_t*>(bars) + kBarBytes;          // slot: tile & 3; no tile is more than three ahead
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wg = warp >> 2;
@@ -311,11 +427,22 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     };
     uint4 kc[4], vc[4];
     uint2 kp, vp, kp_next = make_uint2(0u, 0u), vp_next = make_uint2(0u, 0u);
+    auto finite = [](uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; };
+    // Largest possible magnitude of a token's values; 0 for K that is not finite.
+    auto bound = [](uint2 w) {
+      return max(__float_as_uint(fma_whole(8.f, kv4::par_s(w.x & 0x7fffu), kv4::par_c(w.x & 0x7fff0000u))),
+                 __float_as_uint(fma_whole(8.f, kv4::par_s(w.y & 0x7fffu), kv4::par_c(w.y & 0x7fff0000u))));
+    };
+    auto bound_k = [&](uint2 w) { return finite(w.x) && finite(w.y) ? bound(w) : 0u; };
+    // A token below 2^-13 in the tile's units (and not 0) would lose bits to fp16's subnormals; `least`: that as a float's bits.
+    auto least_of = [](int e) { return static_cast<uint32_t>(max(e + 127 - 13, 0)) << 23; };
+    auto small = [](uint32_t bits, uint32_t least) { return bits - 1u < least; };
+    int ek = -10, ev = -10;                                  // what magnitudes of 2 to 8 would choose
+    uint32_t least_k = least_of(ek), least_v = least_k;
     // What counts of tile j's parameters (values of V that are not finite are noted and count as 0), and the tile's largest
     // possible magnitudes, left in `red` for everyone.
     auto admit = [&](int j, bool ok) {
       if ((tile0 + j) * kBN + row >= n_kv) kp = vp = make_uint2(0u, 0u);
-      auto finite = [](uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; };
       if (!finite(vp.x)) {
         atomicMin(first_bad, (tile0 + j) * kBN + row);
         vp.x = 0u;
@@ -324,27 +451,26 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         atomicMin(first_bad + 1, (tile0 + j) * kBN + row);
         vp.y = 0u;
       }
-      auto bound = [](uint2 w) {
-        return max(__float_as_uint(fma_whole(8.f, kv4::par_s(w.x & 0x7fffu), kv4::par_c(w.x & 0x7fff0000u))),
-                   __float_as_uint(fma_whole(8.f, kv4::par_s(w.y & 0x7fffu), kv4::par_c(w.y & 0x7fff0000u))));
-      };
-      const uint32_t kb = finite(kp.x) && finite(kp.y) ? bound(kp) : 0u, vb = bound(vp);
+      const uint32_t kb = bound_k(kp), vb = bound(vp);
       const uint32_t kw = __reduce_max_sync(0xffffffffu, kb), vw = __reduce_max_sync(0xffffffffu, vb);
+      const bool far = __any_sync(0xffffffffu, small(kb, least_k) || small(vb, least_v));
       if (lane == 0) {
         uint32_t* at = red + (j & 1) * 12 + (warp & 3);
         at[0] = kw;
         at[4] = vw;
-        at[8] = ok ? 0u : 1u;
+        at[8] = (ok ? 0u : 1u) | (far ? 2u : 0u);
       }
     };
-    // Largest magnitude of a stored tile: 2^12 .. 2^13 when an exponent is chosen (smaller values of the tile then keep
-    // fp16's precision down to 2^-26 of it), kept while it stays in 2^7 .. 2^15.
+    // Largest magnitude of a stored tile: 2^12 .. 2^13 when an exponent is chosen (where tokens are below 2^-20 of it, each
+    // has its own), kept while it stays in 2^7 .. 2^15.
     auto choose = [](int e, uint32_t bits) {
       const int top = static_cast<int>(bits >> 23) - 127;
       if (bits != 0 && (top - e > 14 || top - e < 7)) e = top - 12;
       return max(-120, min(120, e));
     };
-    int ek = 0, ev = 0;
+    auto own_power = [&](uint32_t bits, uint32_t least, int e, int none) {
+      return bits == 0u ? none : small(bits, least) ? max(-120, static_cast<int>(bits >> 23) - 127 - 12) : e;
+    };
     // A wait that runs out is only noted: the four warps leave together, at the barrier of the next tile.
     bool ok = true;
     if (n_tiles > 0) {
@@ -362,13 +488,26 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       named_barrier(1, 128);
       const uint4* seen = reinterpret_cast<const uint4*>(red + (j & 1) * 12);       // of the four warps: K, V, gave up
       const uint4 k4 = seen[0], v4 = seen[1], out = seen[2];
-      if ((out.x | out.y | out.z | out.w) != 0u) break;
-      ek = choose(ek, max(max(k4.x, k4.y), max(k4.z, k4.w)));
-      ev = choose(ev, max(max(v4.x, v4.y), max(v4.z, v4.w)));
+      const uint32_t flags = out.x | out.y | out.z | out.w;
+      if (flags & 1u) break;
+      bool own = flags & 2u;
+      const int ek_new = choose(ek, max(max(k4.x, k4.y), max(k4.z, k4.w))), ev_new = choose(ev, max(max(v4.x, v4.y), max(v4.z, v4.w)));
+      if (ek_new != ek || ev_new != ev) {                    // alike in the four warps: look again, in the new units
+        ek = ek_new;
+        ev = ev_new;
+        least_k = least_of(ek);
+        least_v = least_of(ev);
+        const bool far = __any_sync(0xffffffffu, small(bound_k(kp), least_k) || small(bound(vp), least_v));
+        if (lane == 0) again[warp & 3] = far;
+        named_barrier(1, 128);
+        own = again[0] | again[1] | again[2] | again[3];
+      }
       if (row == 0) {
         TileScale sc;
         sc.k = ek;
         sc.v = ev;
+        sc.own = own;
+        sc.unused = 0;
         scales[j & 7] = sc;
       }
       const bool more = j + 1 < n_tiles;
@@ -381,10 +520,17 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       }
       const int ks = j % kNK, vs = j % kNV;
       const uint2 vp_now = vp;
+      int token_k = ek, token_v = ev;
+      if (own) {                                             // here: both before S can be ready
+        token_k = own_power(bound_k(kp), least_k, ek, ek);
+        token_v = own_power(bound(vp), least_v, ev, -120);
+        powers[(j & 3) * 2 * kBN + row] = static_cast<int8_t>(token_k);
+        powers[(j & 3) * 2 * kBN + kBN + row] = static_cast<int8_t>(token_v);
+      }
       if (j == 1 || j == 2) ok = ok && __all_sync(0xffffffffu, mbar_wait(&q_full[j - 1], 0));    // Q's rows lie in these slots
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&k_empty[ks], ((j / kNK) & 1) ^ 1) && *abort_flag == 0);
       if (ok) {
-        const float f = pow2(-ek);
+        const float f = pow2(-token_k);
         const Pair g0(kp.x, f), g1(kp.y, f);
         const uint32_t at = row_start(smem_u32(k_ring) + ks * kTileBytes, row);
 #pragma unroll
@@ -400,7 +546,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       }
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&v_empty[vs], ((j / kNV) & 1) ^ 1) && *abort_flag == 0);
       if (ok) {
-        const float f = pow2(-ev);
+        const float f = pow2(-token_v);
         const Pair g0(vp_now.x, f), g1(vp_now.y, f);
         const uint32_t at = row_start(smem_u32(v_ring) + vs * kTileBytes, row);
 #pragma unroll
@@ -572,138 +718,109 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     }
     const int row_exp = p.scale_exp + q_exp;
     const uint32_t taddr = u * kTmemUnit + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    float m = kNoMax, l = 0.f;
-    // A row's O is in units of 2^unit_v, the current tile's power, but no more than 2^60 below 2^most_v, which bounds what O
-    // holds (|O| < 2^54 2^most_v: 2^31 tokens, P up to 2^8, V up to 2^15), so that no change of units takes it out of fp32.
-    // P of a tile that is smaller still is scaled down instead: next to what O holds the tile is nothing.
-    int unit_v = 0, least_v = 0;                             // least_v = most_v - 60
-    float most_v = 0.f;
-    // S scale - m leaves what rounding took from m, 2^-24 of it: of scores of 2^30 more than an exponential may see. Rows whose
-    // maximum is beyond 2^24 leave the scale's mantissa out, so that the product with a power of two is exact. Their weights
-    // are those of the largest score and of its equals, whatever the mantissa: others as near are within S's own rounding.
-    float mantissa = p.scale;
-    auto is_huge = [](float x) { return fabsf(x) > 16777216.f && x != kNoMax; };
-    for (int j = 0; ok && j < n_tiles; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[u], j & 1) && *abort_flag == 0);
-      if (!ok) break;
-      tc_fence_after_sync();
-      uint32_t sr[4][32];                                    // the score row: 128 fp32
-      const TileScale ts = scales[j & 7];
-      const int k0 = (tile0 + j) * kBN;
-      const bool diagonal = k0 + kBN - 1 > pos;
-      float mx[4];
-      tmem_ld32(taddr, sr[0]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {                          // the maximum of one quarter while the next is on its way
-        tmem_ld_wait();
-        tmem_ld_fence_regs(sr[c]);
-        if (c < 3) tmem_ld32(taddr + (c + 1) * 32, sr[c + 1]);
-        if (diagonal) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (k0 + c * 32 + i > pos) sr[c][i] = 0xff800000u;       // -inf
-        }
-        float a[10];
-#pragma unroll
-        for (int i = 0; i < 10; ++i)
-          a[i] = fmax3(__uint_as_float(sr[c][3 * i]), __uint_as_float(sr[c][3 * i + 1]), __uint_as_float(sr[c][3 * i + 2]));
-        mx[c] = fmax3(fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]), fmax3(a[6], a[7], a[8])),
-                      fmax3(a[9], __uint_as_float(sr[c][30]), __uint_as_float(sr[c][31])), -INFINITY);
-      }
-      // |S| is below 2^37: what a scale below 2^-100 makes of it is nothing. Never 0: it meets -inf.
-      const float unit = pow2(max(-100, min(126, row_exp + ts.k)));
-      float scale = mantissa * unit;
-      const float top = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
-      const float mt = fmaxf(top * scale, kNoMax);
-      if (j == 0) {
-        m = mt;
-        if (is_huge(m)) {
-          mantissa = 1.f;
-          scale = unit;
-          m = top * scale;
-        }
-        unit_v = ts.v;
-        most_v = static_cast<float>(ts.v);
-        least_v = ts.v - 60;
-      } else {
-        const bool need = mt > m + kLazy || max(ts.v, least_v) != unit_v;
-        if (__any_sync(0xffffffffu, need)) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&o_done[u], (j - 1) & 1));
-          if (!ok) break;
-          tc_fence_after_sync();
-          float m_new = need ? fmaxf(m, mt) : m;
-          const float want = is_huge(m_new) ? 1.f : p.scale;
-          if (want != mantissa) {
-            m *= want / mantissa;
-            mantissa = want;
-            scale = mantissa * unit;
-            m_new = fmaxf(m, top * scale);
-          }
-          const float grown = m - m_new;
-          l *= exp2f(grown);
-          m = m_new;
-          most_v = fmaxf(most_v + grown, static_cast<float>(ts.v));
-          least_v = static_cast<int>(most_v) - 60;
-          const int to = max(ts.v, least_v);
-          const float alpha = exp2f(grown + static_cast<float>(unit_v - to));
-          unit_v = to;
-          const uint64_t alpha2 = pack_f32x2(alpha, alpha);
-#pragma unroll 1
-          for (int ch = 0; ch < kD / 16; ++ch) {
-            uint32_t o[16];
-            tmem_ld16(taddr + kTmemO + ch * 16, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float lo, hi;
-              unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), alpha2), lo, hi);
-              o[i] = __float_as_uint(lo);
-              o[i + 1] = __float_as_uint(hi);
-            }
-            tmem_st16(taddr + kTmemO + ch * 16, o);
-          }
-          tmem_st_wait();
-        }
-      }
-      // The units take turns on the MUFU pipe, so that one's exponentials run under the rest of the other's chain.
-      if (u == 1 || j > 0) {
-        ok = __all_sync(0xffffffffu, u == 1 ? mbar_wait(&xu_done[0], j & 1) : mbar_wait(&xu_done[1], (j - 1) & 1));
+    RowState st{kNoMax, 0.f, p.scale, 0.f, 0, 0};
+    int j = 0;
+    // The tiles whose tokens have powers of their own are outside the loop of the others: inside it they cost those 1.5%.
+    for (;; ++j) {
+      for (; ok && j < n_tiles; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[u], j & 1) && *abort_flag == 0);
         if (!ok) break;
-      }
-      const int below = max(ts.v - unit_v, -60);             // 0 but for tiles below least_v
-      const float less = static_cast<float>(below);
-      const uint64_t scale2 = pack_f32x2(scale, scale), negm2 = pack_f32x2(-m + less, -m + less);
-      uint64_t sums[2] = {0ull, 0ull};
+        tc_fence_after_sync();
+        const TileScale ts = scales[j & 7];
+        const int k0 = (tile0 + j) * kBN;
+        // |S| is below 2^37: what a scale below 2^-100 makes of it is nothing. Never 0: it meets -inf.
+        const float unit = pow2(max(-100, min(126, row_exp + ts.k)));
+        uint32_t sr[4][32];                                    // the score row: 128 fp32
+        tmem_ld32(taddr, sr[0]);
+        if (ts.own) break;                                   // handled below
+        const bool diagonal = k0 + kBN - 1 > pos;
+        float mx[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t packed[16];
+        for (int c = 0; c < 4; ++c) {                          // the maximum of one quarter while the next is on its way
+          tmem_ld_wait();
+          tmem_ld_fence_regs(sr[c]);
+          if (c < 3) tmem_ld32(taddr + (c + 1) * 32, sr[c + 1]);
+          if (diagonal) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float x0, x1;
-          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1])), scale2, negm2), x0, x1);
-          const float p0 = exp2f(x0), p1 = exp2f(x1);
-          sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(p0, p1));
-          packed[i >> 1] = pack_f16(p0, p1);
+            for (int i = 0; i < 32; ++i)
+              if (k0 + c * 32 + i > pos) sr[c][i] = 0xff800000u;       // -inf
+          }
+          float a[10];
+#pragma unroll
+          for (int i = 0; i < 10; ++i)
+            a[i] = fmax3(__uint_as_float(sr[c][3 * i]), __uint_as_float(sr[c][3 * i + 1]), __uint_as_float(sr[c][3 * i + 2]));
+          mx[c] = fmax3(fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]), fmax3(a[6], a[7], a[8])),
+                        fmax3(a[9], __uint_as_float(sr[c][30]), __uint_as_float(sr[c][31])), -INFINITY);
         }
-        tmem_st16(taddr + c * 16, packed);
+        float scale = st.mantissa * unit;
+        const float top = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+        const float mt = fmaxf(top * scale, kNoMax);
+        if (j == 0) {
+          st.m = mt;
+          if (RowState::is_huge(st.m)) {
+            st.mantissa = 1.f;
+            scale = unit;
+            st.m = top * scale;
+          }
+          st.unit_v = ts.v;
+          st.most_v = static_cast<float>(ts.v);
+          st.least_v = ts.v - 60;
+        } else {
+          const bool need = mt > st.m + kLazy || max(ts.v, st.least_v) != st.unit_v;
+          if (__any_sync(0xffffffffu, need)) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_done[u], (j - 1) & 1));
+            if (!ok) break;
+            tc_fence_after_sync();
+            const float alpha = st.settle(p, top, unit, need ? fmaxf(st.m, mt) : st.m, ts.v);
+            scale = st.mantissa * unit;
+            rescale(taddr, alpha);
+          }
+        }
+        // The units take turns on the MUFU pipe, so that one's exponentials run under the rest of the other's chain.
+        if (u == 1 || j > 0) {
+          ok = __all_sync(0xffffffffu, u == 1 ? mbar_wait(&xu_done[0], j & 1) : mbar_wait(&xu_done[1], (j - 1) & 1));
+          if (!ok) break;
+        }
+        const int below = max(ts.v - st.unit_v, -60);             // 0 but for tiles below least_v
+        const float less = static_cast<float>(below);
+        const uint64_t scale2 = pack_f32x2(scale, scale), negm2 = pack_f32x2(-st.m + less, -st.m + less);
+        uint64_t sums[2] = {0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x0, x1;
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1])), scale2, negm2), x0, x1);
+            const float p0 = exp2f(x0), p1 = exp2f(x1);
+            sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(p0, p1));
+            packed[i >> 1] = pack_f16(p0, p1);
+          }
+          tmem_st16(taddr + c * 16, packed);
+        }
+        {
+          float a, c;
+          unpack_f32x2(add_f32x2(sums[0], sums[1]), a, c);
+          st.l += (a + c) * pow2(-below);
+        }
+        mbar_arrive(&xu_done[u]);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        mbar_arrive(&p_ready[u]);
       }
-      {
-        float a, c;
-        unpack_f32x2(add_f32x2(sums[0], sums[1]), a, c);
-        l += (a + c) * pow2(-below);
-      }
-      mbar_arrive(&xu_done[u]);
-      tmem_st_wait();
-      tc_fence_before_sync();
-      mbar_arrive(&p_ready[u]);
+      if (!ok || j == n_tiles) break;
+      tmem_ld_wait();
+      const TileScale ts = scales[j & 7];
+      ok = apart_tile(p, st, ts, powers + (j & 3) * 2 * kBN, min(kBN, pos - (tile0 + j) * kBN + 1),
+                      pow2(max(-100, min(126, row_exp + ts.k))), taddr, u, j, o_done, xu_done, p_ready);
     }
     if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[u], (n_tiles - 1) & 1) && *abort_flag == 0);
     if (ok && p.splits > 1) {
       tc_fence_after_sync();
       const size_t slot = (((static_cast<size_t>(z) * gridDim.y + hk) * gridDim.x + blockIdx.x) * p.splits + split) *
                               (2 * kBM) + u * kBM + r;
-      *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(mantissa == p.scale ? m : m * p.scale, l);
-      const float vf0 = pos >= first_bad[0] ? CUDART_NAN_F : pow2(unit_v), vf1 = pos >= first_bad[1] ? CUDART_NAN_F : pow2(unit_v);
+      *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(st.mantissa == p.scale ? st.m : st.m * p.scale, st.l);
+      const float vf0 = pos >= first_bad[0] ? CUDART_NAN_F : pow2(st.unit_v), vf1 = pos >= first_bad[1] ? CUDART_NAN_F : pow2(st.unit_v);
       // Through the unit's Q tile (all its MMAs are over) half the channels at a time, so that the writes are whole lines. A
       // split without tiles leaves no output, only m = kNoMax, l = 0.
       const uint32_t tile = smem_u32(q_s) + u * kTileBytes;
@@ -741,8 +858,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       }
     } else if (ok) {
       tc_fence_after_sync();
-      const float vf0 = pos >= first_bad[0] ? CUDART_NAN_F : pow2(unit_v), vf1 = pos >= first_bad[1] ? CUDART_NAN_F : pow2(unit_v);
-      const float inv = l == 0.f ? 0.f : 1.f / l;            // times 2^unit_v it may leave fp32: small values, many tokens
+      const float vf0 = pos >= first_bad[0] ? CUDART_NAN_F : pow2(st.unit_v), vf1 = pos >= first_bad[1] ? CUDART_NAN_F : pow2(st.unit_v);
+      const float inv = st.l == 0.f ? 0.f : 1.f / st.l;            // times 2^unit_v it may leave fp32: small values, many tokens
       // Rows leave through the unit's Q tile (all its MMAs are over), so that the writes are whole lines.
       const uint32_t at = row_start(smem_u32(q_s) + u * kTileBytes, r);
       uint32_t o[4][32];
@@ -760,7 +877,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       for (int ch = 0; ch < 4; ++ch) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {                        // words of channels 0 4 1 5 2 6 3 7
-          auto x = [&](int i) { return l == 0.f ? 0.f : __uint_as_float(o[ch][8 * w + i]) * inv * ((w & 1) ? vf1 : vf0); };
+          auto x = [&](int i) { return st.l == 0.f ? 0.f : __uint_as_float(o[ch][8 * w + i]) * inv * ((w & 1) ? vf1 : vf0); };
           st_shared_v4(chunk_at(at, 4 * ch + w), pack_bf16(x(0), x(2)), pack_bf16(x(4), x(6)), pack_bf16(x(1), x(3)),
                        pack_bf16(x(5), x(7)));
         }
