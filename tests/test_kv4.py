@@ -103,6 +103,48 @@ def test_refusals():
         kv4.row_bytes(72)
 
 
+def test_the_cpu_form_refuses_what_the_kernels_refuse():
+    """Writing and attending, with caches that do not fit each other or the call, scales and pages that mean nothing."""
+    hq, hkv, d, bs = 4, 2, 64, 16
+    k, v = caches(3, hkv, bs, d)
+    i32 = dict(dtype=torch.int32)
+    cs, w = cpu_ref.build_cos_sin_cache(d, 10, 1e4), torch.ones(d)
+    wide = torch.zeros(3, hkv, bs, d)
+
+    def write(k, v, qkv=torch.ones(1, (hq + 2 * hkv) * d), hkv=hkv):
+        return ops.qk_norm_rope_cache(qkv, w, w, 1e-6, cs, torch.zeros(1, **i32), torch.zeros(1, **i32), k, v, hq, hkv, d)
+
+    def attend(k, v, scale=0.1, hq=hq, hkv=hkv, pages=(0, 1), length=20):
+        attn = AttnBatch(torch.tensor([0, 1], **i32), torch.tensor([length], **i32), torch.tensor([pages], **i32), 1, 1, 1, length, 1)
+        return ops.paged_attention(torch.ones(1, 4 * d), k, v, attn, scale, hq, hkv, d)
+
+    write(k, v)
+    assert bool(attend(k, v).isfinite().all())
+    for call in (write, attend):
+        for bad in ((k, wide), (wide, v)):
+            with pytest.raises(TypeError, match="uint8"):
+                call(*bad)
+        with pytest.raises(ValueError, match="one 4-d shape"):
+            call(k, v[:2])
+        with pytest.raises(ValueError, match="expected"):
+            call(k[:, :, :8].contiguous(), v[:, :, :8].contiguous())
+        with pytest.raises(ValueError, match="expected"):
+            call(k, v, hkv=1)
+        with pytest.raises(ValueError, match="contiguous"):
+            call(k.transpose(0, 1).contiguous().transpose(0, 1), v.transpose(0, 1).contiguous().transpose(0, 1))
+    assert not bool(wide.any())
+    with pytest.raises(ValueError, match="qkv of shape"):
+        write(k, v, torch.ones(1, (hq + 2 * hkv) * d + 8))
+    with pytest.raises(ValueError, match="q of shape"):
+        attend(k, v, hq=3)
+    for scale in (float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="finite"):
+            attend(k, v, scale)
+    for pages, length in (((0, 3), 20), ((0, -1), 20), ((0, 1), 33)):
+        with pytest.raises(IndexError, match="pages"):
+            attend(k, v, pages=pages, length=length)
+
+
 def test_append_then_attend_matches_64_bits():
     torch.manual_seed(0)
     hq, hkv, d, bs = 4, 2, 64, 32

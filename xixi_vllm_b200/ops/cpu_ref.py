@@ -124,6 +124,8 @@ def _context(cache: torch.Tensor, blocks: torch.Tensor, length: int) -> torch.Te
     """fp32 ``[kv_heads, length, D]`` of the first ``length`` tokens in ``blocks``."""
     bs = cache.shape[2]
     if kv4.is_kv4(cache):
+        if blocks.numel() * bs < length or bool(((blocks < 0) | (blocks >= cache.shape[0])).any()):
+            raise IndexError(f"pages {blocks.tolist()} for {length} tokens of a cache of {cache.shape[0]} pages")
         slots = (blocks[:, None] * bs + torch.arange(bs, device=cache.device)).flatten()[:length]
         return kv4.read_rows(cache, slots).transpose(0, 1)
     return cache[blocks].permute(1, 0, 2, 3).reshape(cache.shape[1], -1, cache.shape[3])[:, :length].float()

@@ -5,6 +5,8 @@ is missing on a machine with a GPU the call raises instead of falling back.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import cpu_ref, kv4
@@ -78,6 +80,10 @@ def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v
     if qkv.is_cuda:
         return _cuda().qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache,
                                           num_q_heads, num_kv_heads, head_dim, prefill_begin)
+    if kv4.is_kv4(k_cache) or kv4.is_kv4(v_cache):
+        kv4.check_caches(k_cache, v_cache, head_dim, num_kv_heads)
+        if qkv.shape[-1] != (num_q_heads + 2 * num_kv_heads) * head_dim:
+            raise ValueError(f"qk_norm_rope_cache: qkv of shape {tuple(qkv.shape)} for {num_q_heads} query and {num_kv_heads} KV heads")
     return cpu_ref.qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache,
                                       num_q_heads, num_kv_heads, head_dim)
 
@@ -98,6 +104,12 @@ def paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads,
     that is longer than ``attn.max_q_len`` or reaches beyond ``q`` is reported through the status word and is zeros."""
     if q.is_cuda:
         return _cuda().paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim)
+    if kv4.is_kv4(k_cache) or kv4.is_kv4(v_cache):
+        kv4.check_caches(k_cache, v_cache, head_dim, num_kv_heads)
+        if q.shape[-1] != num_q_heads * head_dim or num_q_heads % num_kv_heads:
+            raise ValueError(f"paged_attention: q of shape {tuple(q.shape)} for {num_q_heads} query and {num_kv_heads} KV heads")
+        if not math.isfinite(scale):
+            raise ValueError("paged_attention: scale must be finite")
     return cpu_ref.paged_attention(q, k_cache, v_cache, attn.cu_q, attn.kv_lens, attn.block_tables,
                                    scale, num_q_heads, num_kv_heads, head_dim)
 
