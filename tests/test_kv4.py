@@ -1,4 +1,6 @@
 """4-bit KV cache on the CPU backend: byte format, quantiser, refusals and the engine that uses it."""
+import os
+
 import numpy as np
 import pytest
 import torch
@@ -195,6 +197,31 @@ def test_what_a_row_does_not_see_cannot_reach_it():
     kv4.write_rows(k, torch.tensor([0]), torch.full((1, hkv, d), float("nan")))
     rows, _ = ops.read_cache(k, v, torch.tensor([-1, 0, 1], dtype=torch.int32), d)
     assert not rows[0].any() and bool(rows[1].isnan().all()) and bool(rows[2].isfinite().all())
+
+
+def test_an_extension_of_another_torch_is_built_again(tmp_path, monkeypatch):
+    from xixi_vllm_b200.ops import build
+    lib = tmp_path / "_xv_torch.so"
+    monkeypatch.setattr(build, "TORCH_LIB", str(lib))
+    runs = []
+
+    def compiler(cmd, **kw):
+        runs.append(cmd)
+        mark = next(a for a in cmd if a.startswith("-DXV_BUILT_FOR=")).split('"')[1]
+        with open(cmd[cmd.index("-o") + 1], "wb") as f:
+            f.write(b"code " + mark.encode() + b" code")
+
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    build.build_torch()                                       # not there
+    build.build_torch()                                       # fits
+    assert len(runs) == 1
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    build.build_torch()                                       # newer than its sources, but of another torch
+    build.build_torch()
+    assert len(runs) == 2 and b"torch 1.0.0 " in lib.read_bytes()
+    os.utime(lib, (0, 0))
+    build.build_torch()                                       # older than its sources
+    assert len(runs) == 3
 
 
 # ---- the engine with kv_cache_dtype="int4" ----

@@ -311,4 +311,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_xv_torch", nullptr, -1, methods, 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__xv_torch(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__xv_torch(void) {
+  PyObject* m = PyModule_Create(&module);
+  // The torch and Python that this was compiled against; ops/build.py looks for the text before it loads the file.
+  if (m && PyModule_AddStringConstant(m, "built_for", XV_BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -84,10 +84,25 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
+def _built_for() -> str:
+    """What a Python extension fits: it is compiled against one torch and one Python."""
+    import torch
+
+    return f"xv built for torch {torch.__version__} {sys.implementation.cache_tag};"
+
+
+def _torch_lib_fits() -> bool:
+    """The extension is there, no older than its sources, and carries the mark of this torch and Python."""
+    header = os.path.join(CSRC, "kernels", "xv_cuda.h")
+    if not os.path.isfile(TORCH_LIB) or os.path.getmtime(TORCH_LIB) < max(map(os.path.getmtime, (TORCH_SRC, header))):
+        return False
+    with open(TORCH_LIB, "rb") as f:
+        return _built_for().encode() in f.read()
+
+
 def build_torch(force: bool = False) -> str:
     """Compile the Python extension in-tree with g++ (half a minute: torch's headers)."""
-    header = os.path.join(CSRC, "kernels", "xv_cuda.h")
-    if not force and os.path.isfile(TORCH_LIB) and os.path.getmtime(TORCH_LIB) >= max(map(os.path.getmtime, (TORCH_SRC, header))):
+    if not force and _torch_lib_fits():
         return TORCH_LIB
     import sysconfig
 
@@ -97,6 +112,7 @@ def build_torch(force: bool = False) -> str:
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path())))
     tmp = TORCH_LIB + f".tmp{os.getpid()}"
     subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+                    f'-DXV_BUILT_FOR="{_built_for()}"',
                     "-isystem", os.path.join(root, "include"),
                     "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
                     "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
