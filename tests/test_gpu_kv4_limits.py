@@ -361,3 +361,18 @@ def test_chunk_tokens_far_larger_than_their_neighbours(which, power, crowd):
         else:
             c.v[b][at] *= 2.0 ** power
     c.check()
+
+
+def test_write_does_not_depend_on_how_heads_are_dealt_to_warps(monkeypatch):
+    """One pair of heads a warp up to eight, for a device of many and of few SMs."""
+    from test_gpu_kv4 import _empty, _write_case
+    T, hq, hkv, bs = 33, 40, 9, 32
+    nb, qkv, qw, kw, cs, pos, slots = _write_case(T, hq, hkv, bs, 21, (4,))
+    args = [x.to(DEV) for x in (qkv, qw, kw)] + [1e-6] + [x.to(DEV) for x in (cs, pos, slots)]
+    st, runs = _cuda()._kv4_state(args[0]), []
+    for sms in (1000, 148, 10, 5, 4, 3, 2, 1):
+        monkeypatch.setattr(st, "num_sms", sms)
+        caches = _empty(nb, hkv, bs)
+        runs.append((_ops().qk_norm_rope_cache(*args, *caches, hq, hkv, D), *caches))
+    _cuda().check_status()
+    assert all(torch.equal(a, b) for r in runs[1:] for a, b in zip(r, runs[0]))

@@ -141,9 +141,9 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Device& d
 }
 
 // write(qkv | None, planes | None, splits, rows, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, hq, hkv, d,
-//       status) -> q
+//       num_sms, status) -> q
 PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 16, [&]() -> PyObject* {
+  return guarded(n, 17, [&]() -> PyObject* {
     const int hq = integer(a[12], "num_q_heads"), hkv = integer(a[13], "num_kv_heads"), d = integer(a[14], "head_dim");
     const Caches c(a[10], a[11], d, hkv);
     if (hq < 0) refuse(PyExc_ValueError, "num_q_heads = %d", hq);
@@ -174,13 +174,13 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto* csp = static_cast<const float*>(vector(cs, d, at::kFloat, c.dev, "cos_sin"));
     const auto* pos = static_cast<const int*>(vector(tensor(a[8], "positions"), rows, at::kInt, c.dev, "positions"));
     const auto* slots = static_cast<const int*>(vector(tensor(a[9], "slots"), rows, at::kInt, c.dev, "slots"));
-    auto* status = static_cast<int*>(vector(tensor(a[15], "status"), 1, at::kInt, c.dev, "status"));
+    auto* status = static_cast<int*>(vector(tensor(a[16], "status"), 1, at::kInt, c.dev, "status"));
     const c10::cuda::OptionalCUDAGuard guard(c.dev);
     at::Tensor q = fresh({rows, static_cast<int64_t>(hq) * d}, at::kBFloat16, c.dev);
     if (rows > 0)
       check(fn.write(qkv, planes, splits, rows * cols, qwp, kwp, eps, csp, static_cast<int>(cs.numel() / d), pos, slots, q.data_ptr(),
-                     c.k.data_ptr(), c.v.data_ptr(), static_cast<int>(rows), hq, hkv, d, c.page, c.blocks, status,
-                     c10::cuda::getCurrentCUDAStream(c.dev.index()).stream()),
+                     c.k.data_ptr(), c.v.data_ptr(), static_cast<int>(rows), hq, hkv, d, c.page, c.blocks,
+                     integer(a[15], "num_sms"), status, c10::cuda::getCurrentCUDAStream(c.dev.index()).stream()),
             "kv4_write");
     return THPVariable_Wrap(std::move(q));
   });

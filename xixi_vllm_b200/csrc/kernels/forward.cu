@@ -213,7 +213,7 @@ int xv_qwen3_forward(const XvModelDesc* m, const XvBatchDesc* b, const XvArena* 
       XV_TRY(36, xv_kv4_write(a->qkv, splits > 1 ? static_cast<const float*>(a->gemm_ws) : nullptr, splits,
                               static_cast<long long>(T) * m->qkv_rows, w.q_norm, w.k_norm, m->kv4_eps, m->cos_sin, m->max_pos,
                               b->positions, b->slots, a->q, w.k_cache, w.v_cache, T, m->hq, m->hkv, D, m->block_size,
-                              m->num_kv_blocks, a->status, stream));
+                              m->num_kv_blocks, a->num_sms, a->status, stream));
     } else if (splits > 1) {
       XV_TRY(31, xv_qk_norm_rope_cache_partials(static_cast<const float*>(a->gemm_ws), splits,
                                                 static_cast<long long>(T) * m->qkv_rows, w.q_norm, w.k_norm, m->eps,

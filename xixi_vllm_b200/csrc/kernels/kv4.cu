@@ -366,10 +366,10 @@ extern "C" {
 int xv_kv4_write(const void* qkv, const float* partials, int splits, long long split_stride, const void* q_w,
                  const void* k_w, double eps, const float* cos_sin, int max_pos, const int* positions, const int* slots,
                  void* q_out, void* k_cache, void* v_cache, int tokens, int hq, int hkv, int d, int block_size,
-                 int num_blocks, int* status, cudaStream_t stream) {
+                 int num_blocks, int num_sms, int* status, cudaStream_t stream) {
   if (tokens <= 0) return 0;
   if (int rc = check_cache(hkv, d, block_size, num_blocks)) return rc;
-  if (hq < 0 || max_pos <= 0 || (!qkv && !partials)) return XV_ERR_SHAPE;
+  if (hq < 0 || max_pos <= 0 || num_sms <= 0 || (!qkv && !partials)) return XV_ERR_SHAPE;
   if (misaligned(qkv, 16) || misaligned(partials, 16) || misaligned(q_w, 16) || misaligned(k_w, 16) ||
       misaligned(cos_sin, 16) || misaligned(q_out, 16) || misaligned(k_cache, 16) || misaligned(v_cache, 16))
     return XV_ERR_ALIGN;
@@ -379,7 +379,8 @@ int xv_kv4_write(const void* qkv, const float* partials, int splits, long long s
   // 8192 rows (32 + 2 x 8) at the cap 41.5 -> 42.6.
   const int q_pairs = (hq + 1) / 2, kv_pairs = 2 * ((hkv + 1) / 2);
   WriteParams p;
-  p.per_warp = static_cast<int>(std::max(1ll, std::min<long long>(kMaxPairs, static_cast<long long>(tokens) * (q_pairs + kv_pairs) / (148 * 32))));
+  const long long pairs = static_cast<long long>(tokens) * (q_pairs + kv_pairs), wave = static_cast<long long>(num_sms) * 32;
+  p.per_warp = static_cast<int>(std::max(1ll, std::min<long long>(kMaxPairs, pairs / wave)));
   p.q_tasks = (q_pairs + p.per_warp - 1) / p.per_warp;
   p.kv_per_warp = p.per_warp == kMaxPairs ? kMaxPairs : (p.per_warp + 1) / 2;
   p.tasks = p.q_tasks + (kv_pairs + p.kv_per_warp - 1) / p.kv_per_warp;

@@ -155,7 +155,7 @@ int xv_attn_prefill_tc_profile(const void* q, const void* k_cache, const void* v
 int xv_kv4_write(const void* qkv, const float* partials, int splits, long long split_stride, const void* q_w,
                  const void* k_w, double eps, const float* cos_sin, int max_pos, const int* positions, const int* slots,
                  void* q_out, void* k_cache, void* v_cache, int tokens, int hq, int hkv, int d, int block_size,
-                 int num_blocks, int* status, cudaStream_t stream);
+                 int num_blocks, int num_sms, int* status, cudaStream_t stream);
 // bf16 values [tokens, hkv, d] of the rows at `slots` (negative or out of range: zeros, the latter reported).
 int xv_kv4_read(const void* k_cache, const void* v_cache, const int* slots, void* k_out, void* v_out, int tokens, int hkv,
                 int d, int block_size, int num_blocks, int* status, cudaStream_t stream);

@@ -345,15 +345,15 @@ def qk_norm_rope_cache(qkv, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v
     if k_cache.dtype is torch.uint8:
         global launch_count
         launch_count += 1
-        calls, status = _calls or _kv4_calls(), _kv4_state(k_cache).status
+        calls, st = _calls or _kv4_calls(), _kv4_state(k_cache)
         if isinstance(qkv, SplitKPartial):
             T, cols = qkv.shape
             if cols != (num_q_heads + 2 * num_kv_heads) * head_dim:
                 raise ValueError(f"qk_norm_rope_cache: {cols} columns for {num_q_heads} query and {num_kv_heads} KV heads")
             return calls.write(None, qkv.ws, qkv.splits, T, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache,
-                               num_q_heads, num_kv_heads, head_dim, status)
+                               num_q_heads, num_kv_heads, head_dim, st.num_sms, st.status)
         return calls.write(qkv, None, 0, 0, q_w, k_w, eps, cos_sin, positions, slots, k_cache, v_cache, num_q_heads,
-                           num_kv_heads, head_dim, status)
+                           num_kv_heads, head_dim, st.num_sms, st.status)
     if isinstance(qkv, SplitKPartial):
         _bf16(q_w, k_w, k_cache, v_cache)
         T = qkv.shape[0]
