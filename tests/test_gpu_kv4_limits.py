@@ -376,3 +376,30 @@ def test_write_does_not_depend_on_how_heads_are_dealt_to_warps(monkeypatch):
         runs.append((_ops().qk_norm_rope_cache(*args, *caches, hq, hkv, D), *caches))
     _cuda().check_status()
     assert all(torch.equal(a, b) for r in runs[1:] for a, b in zip(r, runs[0]))
+
+
+# ---- the engine on long contexts ----
+
+@pytest.fixture(scope="module")
+def long_model_dir(tmp_path_factory):
+    from xixi_vllm_b200.models.synth import make_model_dir
+    return make_model_dir(str(tmp_path_factory.mktemp("kv4_long")), "tiny", std=0.08, num_hidden_layers=2, hidden_size=512,
+                          num_attention_heads=4, num_key_value_heads=2, head_dim=128, intermediate_size=1024, vocab_size=2048,
+                          torch_dtype="bfloat16", tie_word_embeddings=False, max_position_embeddings=32768)
+
+
+@pytest.mark.parametrize("lens,context,batched", [((9, 40, 1500), 4096, 256), ((9, 40, 17500, 3000), 20480, 2048)])
+def test_engine_forwards_agree_on_long_contexts(long_model_dir, monkeypatch, lens, context, batched):
+    """Captured decode over wide tables and mixed steps whose chunk lies behind a long prefix: even shares and split chunks, one
+    after the other in the native executor's one scratch buffer, layer by layer. The Python forward gives every call scratch of
+    its own; both capture the same shapes, so the tokens are identical."""
+    from test_gpu_kv4 import _engine, _prompts
+    L = _cuda().lib()
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert L.xv_kv4_prefill_splits(1, batched, 4, 2, max(lens), sms) > 1
+    assert (L.xv_kv4_decode_splits(2, 2, sms, context) == 0) == (context > 16384) == (L.xv_kv4_decode_splits(2, 2, sms, max(lens)) == 0)
+    kw = dict(context_len=context, max_num_batched_tokens=batched, num_kvcache_blocks=1600, enforce_eager=False)
+    prompts = _prompts(lens, 5)
+    native = _engine(long_model_dir, prompts, 40, **kw)
+    monkeypatch.setenv("XV_NATIVE_FORWARD", "0")
+    assert native == _engine(long_model_dir, prompts, 40, **kw)

@@ -224,6 +224,28 @@ def test_an_extension_of_another_torch_is_built_again(tmp_path, monkeypatch):
     assert len(runs) == 3
 
 
+def test_the_native_forwards_scratch_covers_every_step():
+    """Over a grid of head counts, sequences, chunk and table lengths: what a launch asks for is never more than it has."""
+    from xixi_vllm_b200.ops import cuda
+    from xixi_vllm_b200.runtime.native_forward import kv4_scratch_bytes
+    L = cuda.lib()
+    split = shared = 0
+    for hq, hkv in ((1, 1), (4, 2), (5, 1), (16, 1), (12, 1), (32, 8), (40, 8), (8, 8)):
+        for sms in (148, 132, 20):
+            for most in (1, 7, 64, 300):
+                have = kv4_scratch_bytes(L, most, hq, hkv, sms)
+                for n in {1, 2, most // 3 + 1, most}:
+                    for reach in (16, 500, 512, 2100, 5000, 20480, 131072):
+                        splits = L.xv_kv4_decode_splits(n, hkv, sms, reach)
+                        assert L.xv_kv4_decode_workspace_bytes(n, hq, hkv, splits, sms) <= have
+                        shared += splits == 0
+                        for q in (0, 1, 63, 64, 65, 700, 4096):
+                            splits = L.xv_kv4_prefill_splits(n, q, hq, hkv, reach, sms)
+                            assert splits >= 1 and L.xv_kv4_prefill_workspace_bytes(n, q, hq, hkv, splits) <= have
+                            split += splits > 1
+    assert split > 1000 and shared > 500
+
+
 # ---- the engine with kv_cache_dtype="int4" ----
 
 def _generate(model_dir, prompts, max_tokens=8, **kw):

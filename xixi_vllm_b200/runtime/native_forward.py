@@ -53,6 +53,14 @@ class Arena(ctypes.Structure):
                [("gemm_ws_bytes", _i64), ("attn_ws", _vp), ("attn_ws_bytes", _i64), ("status", _vp), ("num_sms", _i32)]
 
 
+def kv4_scratch_bytes(L, max_seqs: int, hq: int, hkv: int, num_sms: int) -> int:
+    """Scratch that any step of up to ``max_seqs`` sequences needs on a 4-bit cache. Decode rows and chunks of a step, and its
+    layers, use the same bytes one after the other. A launch of chunks that splits its KV range has at most as many CTAs as
+    there are SMs."""
+    return max(L.xv_kv4_decode_workspace_bytes(max_seqs, hq, hkv, 0, num_sms),
+               num_sms * L.xv_kv4_prefill_workspace_bytes(1, 1, 1, 1, 2) // 2)
+
+
 class NativeForward:
     def __init__(self, model, kv, *, max_tokens: int, max_samples: int) -> None:
         L = cuda.lib()
@@ -159,9 +167,7 @@ class NativeForward:
             self.t["gu"] = buf(T, 2 * d.inter_local)
         st = cuda._state(self.t["h"])
         if d.kv4:
-            # split chunk launches have at most as many CTAs as there are SMs
-            need = max(L.xv_kv4_decode_workspace_bytes(max_samples, d.hq, d.hkv, 0, st.num_sms),
-                       st.num_sms * L.xv_kv4_prefill_workspace_bytes(1, 1, 1, 1, 2) // 2)
+            need = kv4_scratch_bytes(L, max_samples, d.hq, d.hkv, st.num_sms)
             attn_ws = self.t["attn_ws"] = torch.empty(need, dtype=torch.uint8, device=dev)
         else:
             need = L.xv_attn_decode_workspace_bytes(max_samples, d.hq, d.head_dim, 16)
