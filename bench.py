@@ -69,6 +69,8 @@ def parse_args():
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--tp-comm", default="auto", choices=("auto", "fused", "nccl"),
                     help="tensor-parallel reduction path (fused peer-memory kernels or NCCL)")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=("auto", "int4"),
+                    help="how the KV cache is held: the model's dtype (the headline), or 4 bits a value")
     ap.add_argument("--emulate-tp", type=int, default=1,
                     help="single GPU, model dimensions cut to one rank's shard of this tensor-parallel degree "
                          "(compute share of a rank without any communication; diagnostic, not a benchmark)")
@@ -282,7 +284,7 @@ def run_ours(args) -> None:
                       max_num_seqs=args.max_num_seqs, max_num_batched_tokens=args.max_batched_tokens,
                       kvcache_block_size=16, prefix_backend="none", enforce_eager=args.eager,
                       tp_size=args.gpus // args.pp, pp_size=args.pp, pp_microbatches=args.pp_microbatches,
-                      seed=args.seed, gpu_memory_utilization=0.9, tp_comm=args.tp_comm)
+                      seed=args.seed, gpu_memory_utilization=0.9, tp_comm=args.tp_comm, kv_cache_dtype=args.kv_cache_dtype)
     # rank 0 writes config.json before the others read it
     if world > 1:
         import torch.distributed as dist  # noqa: F401
@@ -302,6 +304,8 @@ def run_ours(args) -> None:
     comm_ran = {"tp_comm_ran": "fused" if hasattr(comm, "symm") else ("nccl" if args.gpus // args.pp > 1 else "none"),
                 "nvls_multicast": bool(getattr(comm, "mc_ptr", 0)),
                 "one_kernel_row_parallel": bool(getattr(comm, "fuse_gemm", False))}
+    if args.kv_cache_dtype != "auto":
+        comm_ran["kv_cache_dtype"] = args.kv_cache_dtype
     parallelism = (f"tp{args.gpus}" if args.pp == 1 else f"tp{args.gpus // args.pp}pp{args.pp}mb{args.pp_microbatches}")
 
     def make_sp(n_out):

@@ -330,3 +330,16 @@ def test_configuration_and_command_lines(tiny_model_dir, tmp_path):
         EngineConfig(model=make_model_dir(str(tmp_path), "tiny", weights=False, head_dim=40), device="cpu", kv_cache_dtype="int4")
     args = run.build_parser().parse_args(["--model", tiny_model_dir, "--device", "cpu", "--kv-cache-dtype", "int4"])
     assert engine_config_from(run.config_from_args(args), tiny_model_dir).kv_cache_dtype == "int4"
+
+
+def test_the_benchmark_takes_the_caches_form(monkeypatch):
+    import importlib.util
+    import sys
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "bench.py")
+    spec = importlib.util.spec_from_file_location("bench_script", path)
+    bench = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(bench)
+    monkeypatch.setattr(sys, "argv", ["bench.py"])
+    assert bench.parse_args().kv_cache_dtype == "auto"
+    monkeypatch.setattr(sys, "argv", ["bench.py", "--mode", "decode", "--kv-cache-dtype", "int4"])
+    assert bench.parse_args().kv_cache_dtype == "int4"
