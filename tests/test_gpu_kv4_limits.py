@@ -403,3 +403,19 @@ def test_engine_forwards_agree_on_long_contexts(long_model_dir, monkeypatch, len
     native = _engine(long_model_dir, prompts, 40, **kw)
     monkeypatch.setenv("XV_NATIVE_FORWARD", "0")
     assert native == _engine(long_model_dir, prompts, 40, **kw)
+
+
+@pytest.mark.parametrize("hq", [4, 6, 16])
+@pytest.mark.parametrize("group", [0, 1])
+@pytest.mark.parametrize("extra_pages", [1, WIDE])
+def test_decode_nan_in_a_group_of_v_stays_in_its_channels(hq, group, extra_pages):
+    """At every number of heads to a KV head: up to four have columns for each group, more of them share."""
+    c = Case([1, 1], [50, 61], hq, 1, n_decode=2, extra_pages=extra_pages, seed=22)
+    of = torch.arange(D) // 8 % 2 == group
+    c.v[0][33, 0, of] = 0.0
+    clean = c.run()
+    c.v[0][33, 0, 8 * group + 3] = float("inf")
+    out = c.run()
+    assert bool(out[0][:, of].isnan().all())
+    out[0][:, of] = clean[0][:, of]
+    assert torch.equal(out, clean)

@@ -251,7 +251,10 @@ struct Softmax {
   float cen[NT][2][2];             // sum of P * centre, this lane's tokens
   float off[NT][4];                // sum of -8 P * s, rounded as it is in o: group 0 (heads 2t, 2t + 1), group 1
   float m[NT][2], l[NT][2];        // running maximum of the products (may lag), sum of P of this lane's tokens
-  float vs, v_most;                // power of two that V's scales are multiplied by; the largest scale that it allows
+  // Power of two that V's scales are multiplied by; the largest scale that it allows. Scaled they are 2^-6 to 2^-1 (and P 2^8
+  // times what it is, which cancels), so that saturation leaves them alone and makes NaN 0: both groups' offsets are one
+  // accumulator, where a NaN of one would reach the other. The centre of such a group is NaN too and stays in its channels.
+  float vs, v_most;
 
   __device__ __forceinline__ void clear() {
     vs = 1.f;
@@ -344,11 +347,11 @@ struct Softmax {
       s_most = fmaxf(s_most, __shfl_xor_sync(0xffffffffu, s_most, 8));
       s_most = fmaxf(s_most, __shfl_xor_sync(0xffffffffu, s_most, 16));
       if (s_most > v_most) {
-        const int e = min(max((__float_as_int(s_most) >> 23) - 127 - 2, -120), 119);
+        const int e = min(max((__float_as_int(s_most) >> 23) - 127 + 6, -112), 126);
         const float now = power_of_two(-e);
         back = now / vs;
         vs = now;
-        v_most = power_of_two(e + 7);
+        v_most = power_of_two(e - 1);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -386,7 +389,7 @@ struct Softmax {
 #pragma unroll
         for (int gr = 0; gr < 2; ++gr) {
           const uint32_t w = gr ? vp[u][r].y : vp[u][r].x;
-          vsc[gr][r] = kv4::par_s(w) * vs;
+          vsc[gr][r] = __saturatef(kv4::par_s(w) * vs);
           vce[gr][r] = kv4::par_c(w);
         }
       uint32_t pf[NT][2][2];             // P * s_g as the B operand of the second product
@@ -394,7 +397,7 @@ struct Softmax {
       for (int nt = 0; nt < NT; ++nt) {
         float pr[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][nt][e], q.power[nt][e & 1], -m[nt][e & 1] * q.power[nt][e & 1]));
+        for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][nt][e], q.power[nt][e & 1], fmaf(-m[nt][e & 1], q.power[nt][e & 1], 8.f)));
         l[nt][0] += pr[0] + pr[2];
         l[nt][1] += pr[1] + pr[3];
 #pragma unroll

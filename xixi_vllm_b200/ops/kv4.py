@@ -7,7 +7,8 @@ of parameters (8 bytes each), so one unit is one aligned run whatever the page s
 * Codes: channel ``2 i`` is the low nibble of byte ``i``, channel ``2 i + 1`` the high one. Eight channels are one 32-bit
   word; a word's parity is its group (``(channel >> 3) & 1``). A rotary pair ``(i, i + head_dim / 2)`` lies in one group,
   so a large rotary pair coarsens only its own group.
-* Parameters of a row: bf16 ``s0, c0, s1, c1``. A channel of group ``g`` stands for ``c_g + s_g * (code - 8)``.
+* Parameters of a row: bf16 ``s0, c0, s1, c1``, steps never negative. A channel of group ``g`` stands for
+  ``c_g + s_g * (code - 8)``.
 
 ``quantize`` fixes the numbers: with ``hi``/``lo`` a group's extremes (fp32 arithmetic on bf16 values)
 ``s = bf16((hi / 2 - lo / 2) / 7.5)``, ``c = bf16(hi / 2 + lo / 2 + s / 2)``, ``code = clamp(rint((x - c) / s) + 8, 0, 15)``.
