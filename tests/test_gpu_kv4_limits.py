@@ -419,3 +419,34 @@ def test_decode_nan_in_a_group_of_v_stays_in_its_channels(hq, group, extra_pages
     assert bool(out[0][:, of].isnan().all())
     out[0][:, of] = clean[0][:, of]
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("crowd", [0, 160])
+def test_chunk_tokens_of_every_size(crowd):
+    """V of 2^-100 to 2^100 token by token, with weights and without; and tokens of 2^-6 between ordinary ones, in a tile with one
+    of 2^22 that the rows before it do not see."""
+    c = Case([100, 30], [100, 560], 4, 1, extra_pages=300, seed=23, crowd=crowd)
+    ordinary = [v.clone() for v in c.v]
+    g = torch.Generator().manual_seed(23)
+    c.v = [v * torch.exp2(torch.rand(len(v), 1, 1, generator=g) * 200 - 100) for v in c.v]
+    c.check()
+    c.q *= 0.0
+    c.check()
+    c.v = ordinary
+    c.v[0][1::2] *= 2.0 ** -6
+    c.v[0][90] *= 2.0 ** 22
+    c.check()
+
+
+@pytest.mark.parametrize("crowd", [0, 160])
+def test_chunk_large_values_without_weight_in_front_of_small_ones(crowd):
+    """Tiles of V of 2^80 (and single tokens of it) whose scores are hundreds below the others': nothing of them may be left,
+    nor anything of the others lost."""
+    c = Case([100], [640], 4, 1, extra_pages=300, seed=24, crowd=crowd)
+    c.q = 2.5 * (c.q.abs() + 0.5)
+    c.k[0] = c.k[0].abs() + 2
+    low = torch.zeros(640, dtype=torch.bool)
+    low[128:256] = low[[300, 520, 560, 600]] = True
+    c.k[0][low] *= -1
+    c.v[0][low] *= 2.0 ** 80
+    c.check()

@@ -23,7 +23,7 @@
 // of 2^-9) would otherwise be the largest error of the result. Their range is kept by powers of two: a row of Q is scaled
 // by its largest element, a tile of K or V by an exponent that its dequantisers choose from the tile's parameters (and
 // keep while it fits); the scores undo Q's and K's, and V's is carried with the output accumulator, row by row. In a tile
-// with tokens 2^20 and more below its largest every token has its own exponent, so that a large one that a row does not see, or
+// with tokens 2^12 (to 2^20) below its largest every token has its own exponent, so that a large one that a row does not see, or
 // gives no weight, costs the row nothing of the others; softmax takes such tiles by a slower way of its own.
 // Inside a word the channels are stored in the order 0 4 1 5 2 6 3 7, which is how the nibbles unpack: Q follows it, and
 // the output undoes it for V.
@@ -199,15 +199,15 @@ struct RowState {
   // maximum is beyond 2^24 leave the scale's mantissa out, so that the product with a power of two is exact. Their weights
   // are those of the largest score and of its equals, whatever the mantissa: others as near are within S's own rounding.
   float mantissa;
-  // O is in units of 2^unit_v, the current tile's power, but no more than 2^60 below 2^most_v, which bounds what O holds
-  // (|O| < 2^54 2^most_v: 2^31 tokens, P up to 2^8, V up to 2^15), so that no change of units takes it out of fp32. P of a tile
-  // that is smaller still is scaled down instead: next to what O holds the tile is nothing.
+  // O is in units of 2^unit_v, the current tile's power, but within 2^60 of 2^most_v: no change of units takes it out of fp32.
+  // 2^most_v is the largest that a tile's weights and V may have added (|O| < 2^54 2^most_v: 2^31 tokens, P up to 2^8, V up to
+  // 2^15). P of a tile in other units than the row's is scaled; next to what O holds, or it itself, that tile is nothing.
   float most_v;
-  int unit_v, least_v;                            // least_v = most_v - 60
+  int unit_v;
 
   static __device__ __forceinline__ bool is_huge(float x) { return fabsf(x) > 16777216.f && x != kNoMax; }
-  // To a new maximum and a tile of V in units of 2^tile_v; returns what O is to be multiplied by.
-  __device__ __forceinline__ float settle(const Params& p, float top, float unit, float m_new, int tile_v) {
+  // To a new maximum; returns the exponent (0 or below) of what all sums are to be multiplied by.
+  __device__ __forceinline__ float raise(const Params& p, float top, float unit, float m_new) {
     const float want = is_huge(m_new) ? 1.f : p.scale;
     if (want != mantissa) {
       m *= want / mantissa;
@@ -217,9 +217,12 @@ struct RowState {
     const float grown = m - m_new;
     l *= exp2f(grown);
     m = m_new;
-    most_v = fmaxf(most_v + grown, static_cast<float>(tile_v));
-    least_v = static_cast<int>(most_v) - 60;
-    const int to = max(tile_v, least_v);
+    return grown;
+  }
+  // To a tile of V in units of 2^tile_v with weights of at most 2^weight; returns what O is to be multiplied by.
+  __device__ __forceinline__ float turn(float grown, int tile_v, float weight) {
+    most_v = fmaxf(fmaxf(most_v + grown, static_cast<float>(tile_v) + fminf(weight, 0.f)), -200.f);
+    const int mid = static_cast<int>(most_v), to = max(mid - 60, min(mid + 60, tile_v));
     const float alpha = exp2f(grown + static_cast<float>(unit_v - to));
     unit_v = to;
     return alpha;
@@ -245,57 +248,64 @@ __device__ __forceinline__ void rescale(uint32_t taddr, float alpha) {
   tmem_st_wait();
 }
 
-// The softmax of a tile whose tokens have powers of their own (own: K's, then V's), of which the row sees the first `seen`: two
-// walks over S, 32 columns at a time. The row's unit of V is the largest of what it sees, and P of the other tokens is scaled
-// down to it. False: a wait ran out.
-__device__ __forceinline__ bool apart_tile(const Params& p, RowState& st, const TileScale ts, const int8_t* own, int seen, float unit,
-                                        uint32_t taddr, int u, int j, uint64_t* o_done, uint64_t* xu_done, uint64_t* p_ready) {
-  auto score = [&](uint32_t x, int i) {
-    return i < seen ? __uint_as_float(x) * pow2(max(own[i] - ts.k, -126)) : __uint_as_float(0xff800000u);
-  };
-  float top = __uint_as_float(0xff800000u);
-  int tile_v = -120;
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    uint32_t x[32];
+// The softmax of a tile whose tokens have powers of their own (own: K's, then V's), of which the row sees the first `seen`: three
+// walks over S, 32 columns at a time: the maximum; the largest of weight times V's power, which is the row's unit; P, each
+// token's scaled to that unit. False: a wait ran out.
+__device__ __forceinline__ bool apart_tile(const Params& p, RowState& st, const int8_t* own, int seen,
+                                           int row_exp, uint32_t taddr, int u, int j, uint64_t* o_done, uint64_t* xu_done,
+                                           uint64_t* p_ready) {
+  uint32_t x[32];
+  auto load = [&](int c) {                        // scores in log2 units but for the scale's mantissa
     tmem_ld32(taddr + c * 32, x);
     tmem_ld_wait();
     tmem_ld_fence_regs(x);
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      top = fmaxf(top, score(x[i], c * 32 + i));
-      if (c * 32 + i < seen) tile_v = max(tile_v, static_cast<int>(own[kBN + c * 32 + i]));
+      const float unit = pow2(max(-126, min(126, row_exp + own[c * 32 + i])));
+      x[i] = c * 32 + i < seen ? __float_as_uint(__uint_as_float(x[i]) * unit) : 0xff800000u;
     }
+  };
+  float top = __uint_as_float(0xff800000u);
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    load(c);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
   }
   if (j > 0) {
     if (!__all_sync(0xffffffffu, mbar_wait(&o_done[u], (j - 1) & 1))) return false;
     tc_fence_after_sync();
   }
-  const float alpha = st.settle(p, top, unit, fmaxf(st.m, top * (st.mantissa * unit)), tile_v), scale = st.mantissa * unit;
+  const float grown = st.raise(p, top, 1.f, fmaxf(st.m, top * st.mantissa)), scale = st.mantissa;
+  float most = -120.f;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    load(c);
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      most = fmaxf(most, fmaf(__uint_as_float(x[i]), scale, -st.m) + static_cast<float>(own[kBN + c * 32 + i]));
+  }
+  const float alpha = st.turn(grown, static_cast<int>(ceilf(fminf(most, 120.f))), 0.f);
   if (j > 0) rescale(taddr, alpha);
   if ((u == 1 || j > 0) && !__all_sync(0xffffffffu, u == 1 ? mbar_wait(&xu_done[0], j & 1) : mbar_wait(&xu_done[1], (j - 1) & 1)))
     return false;
-  float l = st.l;
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
-    uint32_t x[32], packed[16];
-    tmem_ld32(taddr + c * 32, x);
-    tmem_ld_wait();
-    tmem_ld_fence_regs(x);
+    load(c);
+    uint32_t packed[16];
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       float of[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float y = fmaf(score(x[i + k], c * 32 + i + k), scale, -st.m);
-        l += exp2f(y);
+        const float y = fmaf(__uint_as_float(x[i + k]), scale, -st.m);
+        st.l += exp2f(y);
         of[k] = exp2f(y + static_cast<float>(own[kBN + c * 32 + i + k] - st.unit_v));
       }
       packed[i >> 1] = pack_f16(of[0], of[1]);
     }
     tmem_st16(taddr + c * 16, packed);            // over scores that have been read
   }
-  st.l = l;
   mbar_arrive(&xu_done[u]);
   tmem_st_wait();
   tc_fence_before_sync();
@@ -434,8 +444,9 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
                  __float_as_uint(fma_whole(8.f, kv4::par_s(w.y & 0x7fffu), kv4::par_c(w.y & 0x7fff0000u))));
     };
     auto bound_k = [&](uint2 w) { return finite(w.x) && finite(w.y) ? bound(w) : 0u; };
-    // A token below 2^-13 in the tile's units (and not 0) would lose bits to fp16's subnormals; `least`: that as a float's bits.
-    auto least_of = [](int e) { return static_cast<uint32_t>(max(e + 127 - 13, 0)) << 23; };
+    // A token below 2^-5 in the tile's units (and not 0): its smaller channels would lose bits to fp16's subnormals, and P of
+    // large tokens that it leaves little of to their own. `least`: that as a float's bits.
+    auto least_of = [](int e) { return static_cast<uint32_t>(max(e + 127 - 5, 0)) << 23; };
     auto small = [](uint32_t bits, uint32_t least) { return bits - 1u < least; };
     int ek = -10, ev = -10;                                  // what magnitudes of 2 to 8 would choose
     uint32_t least_k = least_of(ek), least_v = least_k;
@@ -461,16 +472,14 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
         at[8] = (ok ? 0u : 1u) | (far ? 2u : 0u);
       }
     };
-    // Largest magnitude of a stored tile: 2^12 .. 2^13 when an exponent is chosen (where tokens are below 2^-20 of it, each
+    // Largest magnitude of a stored tile: 2^12 .. 2^13 when an exponent is chosen (where tokens are below 2^-5, each
     // has its own), kept while it stays in 2^7 .. 2^15.
     auto choose = [](int e, uint32_t bits) {
       const int top = static_cast<int>(bits >> 23) - 127;
       if (bits != 0 && (top - e > 14 || top - e < 7)) e = top - 12;
       return max(-120, min(120, e));
     };
-    auto own_power = [&](uint32_t bits, uint32_t least, int e, int none) {
-      return bits == 0u ? none : small(bits, least) ? max(-120, static_cast<int>(bits >> 23) - 127 - 12) : e;
-    };
+    auto own_power = [](uint32_t bits, int none) { return bits == 0u ? none : max(-120, static_cast<int>(bits >> 23) - 127 - 12); };
     // A wait that runs out is only noted: the four warps leave together, at the barrier of the next tile.
     bool ok = true;
     if (n_tiles > 0) {
@@ -522,8 +531,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const uint2 vp_now = vp;
       int token_k = ek, token_v = ev;
       if (own) {                                             // here: both before S can be ready
-        token_k = own_power(bound_k(kp), least_k, ek, ek);
-        token_v = own_power(bound(vp), least_v, ev, -120);
+        token_k = own_power(bound_k(kp), ek);
+        token_v = own_power(bound(vp), -120);
         powers[(j & 3) * 2 * kBN + row] = static_cast<int8_t>(token_k);
         powers[(j & 3) * 2 * kBN + kBN + row] = static_cast<int8_t>(token_v);
       }
@@ -718,7 +727,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     }
     const int row_exp = p.scale_exp + q_exp;
     const uint32_t taddr = u * kTmemUnit + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    RowState st{kNoMax, 0.f, p.scale, 0.f, 0, 0};
+    RowState st{kNoMax, 0.f, p.scale, 0.f, 0};
     int j = 0;
     // The tiles whose tokens have powers of their own are outside the loop of the others: inside it they cost those 1.5%.
     for (;; ++j) {
@@ -764,16 +773,15 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
           }
           st.unit_v = ts.v;
           st.most_v = static_cast<float>(ts.v);
-          st.least_v = ts.v - 60;
         } else {
-          const bool need = mt > st.m + kLazy || max(ts.v, st.least_v) != st.unit_v;
+          const bool need = mt > st.m + kLazy || ts.v != st.unit_v;
           if (__any_sync(0xffffffffu, need)) {
             ok = __all_sync(0xffffffffu, mbar_wait(&o_done[u], (j - 1) & 1));
             if (!ok) break;
             tc_fence_after_sync();
-            const float alpha = st.settle(p, top, unit, need ? fmaxf(st.m, mt) : st.m, ts.v);
+            const float grown = st.raise(p, top, unit, need ? fmaxf(st.m, mt) : st.m);
             scale = st.mantissa * unit;
-            rescale(taddr, alpha);
+            rescale(taddr, st.turn(grown, ts.v, top * scale - st.m));
           }
         }
         // The units take turns on the MUFU pipe, so that one's exponentials run under the rest of the other's chain.
@@ -781,7 +789,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
           ok = __all_sync(0xffffffffu, u == 1 ? mbar_wait(&xu_done[0], j & 1) : mbar_wait(&xu_done[1], (j - 1) & 1));
           if (!ok) break;
         }
-        const int below = max(ts.v - st.unit_v, -60);             // 0 but for tiles below least_v
+        const int below = max(-60, min(100, ts.v - st.unit_v));    // 0 but for tiles far from most_v
         const float less = static_cast<float>(below);
         const uint64_t scale2 = pack_f32x2(scale, scale), negm2 = pack_f32x2(-st.m + less, -st.m + less);
         uint64_t sums[2] = {0ull, 0ull};
@@ -810,9 +818,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       }
       if (!ok || j == n_tiles) break;
       tmem_ld_wait();
-      const TileScale ts = scales[j & 7];
-      ok = apart_tile(p, st, ts, powers + (j & 3) * 2 * kBN, min(kBN, pos - (tile0 + j) * kBN + 1),
-                      pow2(max(-100, min(126, row_exp + ts.k))), taddr, u, j, o_done, xu_done, p_ready);
+      ok = apart_tile(p, st, powers + (j & 3) * 2 * kBN, min(kBN, pos - (tile0 + j) * kBN + 1), row_exp, taddr, u, j, o_done, xu_done,
+                      p_ready);
     }
     if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[u], (n_tiles - 1) & 1) && *abort_flag == 0);
     if (ok && p.splits > 1) {
