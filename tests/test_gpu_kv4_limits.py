@@ -450,3 +450,25 @@ def test_chunk_large_values_without_weight_in_front_of_small_ones(crowd):
     c.k[0][low] *= -1
     c.v[0][low] *= 2.0 ** 80
     c.check()
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+@pytest.mark.parametrize("power,weight", [(-60, 0), (-80, 0), (-110, 0), (-130, 0), (0, -120), (-40, -90)])
+def test_write_of_small_keys_matches_the_cpu_backend(eps, power, weight):
+    """K rows whose squares, and products with the weights, leave fp32; without an eps the norm brings them back to size."""
+    from test_gpu_kv4 import _empty, _write_case
+    T, hq, hkv, bs = 65, 2, 3, 16
+    nb, qkv, qw, kw, cs, pos, slots = _write_case(T, hq, hkv, bs, 31)
+    k = qkv[:, hq * D:(hq + hkv) * D]
+    k.copy_((k.double() * 2.0 ** power).bfloat16())
+    kw = (kw.double() * 2.0 ** weight).bfloat16()
+    gpu = _empty(nb, hkv, bs)
+    cpu = [c.cpu() for c in gpu]
+    _ops().qk_norm_rope_cache(*[x.to(DEV) for x in (qkv, qw, kw)], eps, *[x.to(DEV) for x in (cs, pos, slots)], *gpu, hq, hkv, D)
+    _ops().qk_norm_rope_cache(qkv, qw, kw, eps, cs, pos, slots, *cpu, hq, hkv, D)
+    _cuda().check_status()
+    a, b = (kv4.read_rows(c.cpu(), slots.long()) for c in (gpu[0], cpu[0]))
+    assert bool(b.isfinite().all()) and bool(b.any())
+    # at this step the quantiser's own last bit below 2^-102 is left out of it
+    quantum = 2.0 ** -100 if float(b.abs().max()) < 2.0 ** -90 else 0.0
+    assert float((a - b).abs().max()) <= quantum

@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "../common/kv4.cuh"
@@ -36,6 +37,22 @@ __device__ __forceinline__ float round_bf16(float x) { return __bfloat162float(_
 
 __device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// Conversions and products that keep subnormal numbers, which the library's fast-math flags take for 0.
+__device__ __forceinline__ double widen(float x) {
+  double d;
+  asm("cvt.f64.f32 %0, %1;" : "=d"(d) : "f"(x));
+  return d;
+}
+__device__ __forceinline__ float narrow(double x) {
+  float f;
+  asm("cvt.rn.f32.f64 %0, %1;" : "=f"(f) : "d"(x));
+  return f;
+}
+__device__ __forceinline__ float mul_whole(float a, float b) {
+  float d;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 // Sum over the 16 lanes of half a warp.
 template <typename T>
 __device__ __forceinline__ T half_sum(T v) {
@@ -254,7 +271,14 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
   auto source = [&](int pair) { return p.hq + (pair < kv_pairs ? 0 : p.hkv) + head_of(pair); };
 #pragma unroll 2
   for (int i = first; i < last; ++i) send(i - first, source(i));
-  if (first < kv_pairs) rotary(p.k_w);
+  bool small_w = false;
+  if (first < kv_pairs) {
+    rotary(p.k_w);
+    float least = FLT_MAX;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) least = fminf(least, fabsf(w[k]));
+    small_w = __any_sync(0xffffffffu, least < 0x1p-40f);
+  }
   arrive();
   for (int pair = first; pair < last; ++pair) {
     uint2 a, b;
@@ -267,22 +291,33 @@ __global__ void __launch_bounds__(kWriteWarps * 32, 32 / kWriteWarps) kv4_write_
     if (is_k) {
       double ss = 0.0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) ss += static_cast<double>(x[k]) * x[k];
-      double ms = half_sum(ss) * (1.0 / D) + p.eps;
+      for (int k = 0; k < 8; ++k) ss += widen(x[k]) * widen(x[k]);
+      ss = half_sum(ss);
+      double ms = ss * (1.0 / D) + p.eps;
       if (ms > 1e38) {                                        // beyond fp32: the row at 2^-100 of its size
         ms *= 0x1p-200;
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] *= 0x1p-100f;
+      } else if (ms < 1e-30) {                                // below it (without an eps): the row at 2^100 of its size
+        ms *= 0x1p200;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = mul_whole(x[k], 0x1p100f);
       }
       const float about = rsqrtf(static_cast<float>(ms));     // one Newton step doubles its 22 bits; 0 for an infinite row
       double inv = about;
       if (about > 0.f) inv += 0.5 * inv * (1.0 - ms * inv * inv);
       float k8[8];
+      auto rotate = [&](int k, double u, double v) {
+        const double cd = cs[k], sd = sn[k];
+        k8[k] = round_bf16(narrow((u * cd - v * sd) * inv));
+        k8[4 + k] = round_bf16(narrow((v * cd + u * sd) * inv));
+      };
+      if (small_w || __any_sync(0xffffffffu, ss < 0x1p-120)) {       // products that may leave fp32
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {                           // value times weight is exact in fp32: 8 + 8 bits
-        const double u = x[k] * w[k], v = x[4 + k] * w[4 + k], cd = cs[k], sd = sn[k];
-        k8[k] = round_bf16(static_cast<float>((u * cd - v * sd) * inv));
-        k8[4 + k] = round_bf16(static_cast<float>((v * cd + u * sd) * inv));
+        for (int k = 0; k < 4; ++k) rotate(k, widen(x[k]) * widen(w[k]), widen(x[4 + k]) * widen(w[4 + k]));
+      } else {                                                // value times weight is exact in fp32: 8 + 8 bits
+#pragma unroll
+        for (int k = 0; k < 4; ++k) rotate(k, x[k] * w[k], x[4 + k] * w[4 + k]);
       }
       store_row(p.k_cache + unit0 + h * head_bytes, place % kv4::kUnit, c, half_mask, k8, there);
     } else {
