@@ -472,3 +472,24 @@ def test_write_of_small_keys_matches_the_cpu_backend(eps, power, weight):
     # at this step the quantiser's own last bit below 2^-102 is left out of it
     quantum = 2.0 ** -100 if float(b.abs().max()) < 2.0 ** -90 else 0.0
     assert float((a - b).abs().max()) <= quantum
+
+
+@pytest.mark.parametrize("power", [-63, -64, -66, -95, -104, -118, -124, -127, -131])
+def test_write_of_small_values_matches_the_cpu_backend(power):
+    """Groups whose quotients' remainders, steps or centres are below fp32's smallest normal number."""
+    from test_gpu_kv4 import _empty, _write_case
+    T, hq, hkv, bs = 600, 0, 2, 16
+    nb, qkv, qw, kw, cs, pos, slots = _write_case(T, hq, hkv, bs, 32)
+    g = torch.Generator().manual_seed(32)
+    v = qkv[:, hkv * D:]
+    v.copy_((torch.randn(v.shape, generator=g).double() * 2.0 ** power).bfloat16())
+    v[100:200].abs_()
+    v[200:300, ::2] = 0.0
+    v[300:310] = v[300:310, :1]                                # constant groups
+    gpu = _empty(nb, hkv, bs)
+    cpu = [c.cpu() for c in gpu]
+    _ops().qk_norm_rope_cache(*[x.to(DEV) for x in (qkv, qw, kw)], 1e-6, *[x.to(DEV) for x in (cs, pos, slots)], *gpu, hq, hkv, D)
+    _ops().qk_norm_rope_cache(qkv, qw, kw, 1e-6, cs, pos, slots, *cpu, hq, hkv, D)
+    _cuda().check_status()
+    for a, b in zip(gpu, cpu):
+        assert torch.equal(a.cpu(), b)

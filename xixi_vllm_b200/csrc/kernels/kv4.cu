@@ -53,6 +53,16 @@ __device__ __forceinline__ float mul_whole(float a, float b) {
   asm("mul.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
+__device__ __forceinline__ float max_whole(float a, float b) {
+  float d;
+  asm("max.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float min_whole(float a, float b) {
+  float d;
+  asm("min.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 // Sum over the 16 lanes of half a warp.
 template <typename T>
 __device__ __forceinline__ T half_sum(T v) {
@@ -62,7 +72,7 @@ __device__ __forceinline__ T half_sum(T v) {
 }
 
 // a / b rounded correctly, from the correctly rounded 1 / b: one step of the remainder on the product (P. Markstein,
-// IBM J. Res. Dev. 34, 1990). Below 2^-102 the remainder underflows and the last bit may be off.
+// IBM J. Res. Dev. 34, 1990). The remainder must not underflow: a is 2^-102 at least.
 __device__ __forceinline__ float quotient(float a, float b, float r_b) {
   const float q = __fmul_rn(a, r_b);
   return __fmaf_rn(__fmaf_rn(-q, b, a), r_b, q);
@@ -74,33 +84,44 @@ __device__ __forceinline__ float quotient(float a, float b, float r_b) {
 // Stores one row of bf16 values. ops/kv4.py fixes the arithmetic; the explicit _rn forms keep it under the library's
 // fast-math flags. A code is the quotient (x - centre) / step rounded to even, and ties are common (both are bf16), so
 // the quotient has to be the correctly rounded one.
-__device__ __forceinline__ void store_row(uint8_t* unit, int r, int c, unsigned half_mask, const float (&x)[8], bool there) {
-  float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-  float mn = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
+__device__ __forceinline__ void store_row(uint8_t* unit, int r, int c, unsigned half_mask, float (&x)[8], bool there) {
+  float mx = max_whole(max_whole(max_whole(x[0], x[1]), max_whole(x[2], x[3])), max_whole(max_whole(x[4], x[5]), max_whole(x[6], x[7])));
+  float mn = min_whole(min_whole(min_whole(x[0], x[1]), min_whole(x[2], x[3])), min_whole(min_whole(x[4], x[5]), min_whole(x[6], x[7])));
   float odd = 0.f;                                            // NaN if any value is NaN or infinite
 #pragma unroll
   for (int i = 0; i < 8; ++i) odd = __fmaf_rn(x[i], 0.f, odd);
 #pragma unroll
   for (int o = 1; o <= 8; o <<= 1) {
     if (o == 2) continue;                                     // lane bit 1 is the group
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = max_whole(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mn = min_whole(mn, __shfl_xor_sync(0xffffffffu, mn, o));
   }
   const uint32_t not_fine = __ballot_sync(0xffffffffu, !(odd == 0.f));
   const bool bad = (not_fine & half_mask & ((c & 2) ? 0xccccccccu : 0x33333333u)) != 0;
-  float s = round_bf16(quotient(__fsub_rn(0.5f * mx, 0.5f * mn), 7.5f, 1.f / 7.5f));
+  // Groups below 2^-64 are taken at 2^64 of their size, where nothing underflows; step and centre come back rounded as they
+  // would have been (a centre may be subnormal).
+  const bool small = fmaxf(fabsf(mx), fabsf(mn)) < 0x1p-64f;
+  const float up = small ? 0x1p64f : 1.f, down = small ? 0x1p-64f : 1.f;
+  if (__any_sync(0xffffffffu, small)) {
+    mx = mul_whole(mx, up);
+    mn = mul_whole(mn, up);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = mul_whole(x[i], up);
+  }
+  float s = round_bf16(mul_whole(quotient(__fsub_rn(0.5f * mx, 0.5f * mn), 7.5f, 1.f / 7.5f), down));
   if (s < 1.17549435e-38f) s = 0.f;
-  const float cen = round_bf16(__fadd_rn(__fadd_rn(0.5f * mx, 0.5f * mn), 0.5f * s));
+  const float step = s * up;
+  const float cen = round_bf16(mul_whole(__fadd_rn(__fadd_rn(0.5f * mx, 0.5f * mn), 0.5f * step), down)), mid = mul_whole(cen, up);
   // 1 / s is rounded correctly too: the step leaves an error of 2^-42, and no reciprocal of an 8-bit s is within 2^-33 of a tie.
-  const float r0 = __fdividef(1.f, s);
-  const float r_s = s > 0.f ? __fmaf_rn(__fmaf_rn(-s, r0, 1.f), r0, r0) : 0.f;
+  const float r0 = __fdividef(1.f, step);
+  const float r_s = s > 0.f ? __fmaf_rn(__fmaf_rn(-step, r0, 1.f), r0, r0) : 0.f;
   // 1.5 2^23 + 8: adding it rounds to an integer, even on ties, and leaves code = integer + 8 in the low bits.
   constexpr float kRound = 12582920.f;
   constexpr uint32_t kBits = 0x4B400000u;                     // of 1.5 2^23
   uint32_t code[2] = {0u, 0u};
 #pragma unroll
   for (int i = 7; i >= 0; --i) {
-    const float t = quotient(__fsub_rn(x[i], cen), s, r_s);
+    const float t = quotient(__fsub_rn(x[i], mid), step, r_s);
     const float m = __fadd_rn(fminf(fmaxf(t, -8.f), 7.f), kRound);
     code[i >> 2] = code[i >> 2] * 16u + __float_as_uint(m);   // the constant part of four of them comes off at the end
   }
