@@ -493,3 +493,20 @@ def test_write_of_small_values_matches_the_cpu_backend(power):
     _cuda().check_status()
     for a, b in zip(gpu, cpu):
         assert torch.equal(a.cpu(), b)
+
+
+def test_long_padding_is_cleared():
+    """Thousands of rows behind one short chunk, and behind chunks of which one is long."""
+    for q_lens, most in (([61], 61), ([300] + [1] * 40, 300), ([5, 3], 4000)):
+        c = Case(q_lens, [n + 20 for n in q_lens], 4, 2, n_decode=0, seed=33)
+        k, v = (x.to(DEV) for x in c.caches())
+        rows = sum(q_lens)
+        q = torch.cat([c.q, torch.ones(9000 - rows, 4, D)]).bfloat16().flatten(1).to(DEV)
+        want = c.run().flatten(1).to(DEV)
+        torch.full_like(q, 7.0)                              # what the allocator may hand out again
+        attn = c.attn()
+        attn.max_q_len = most
+        got = _ops().paged_attention(q, k, v, attn, SCALE, 4, 2, D)
+        _cuda().check_status()
+        torch.testing.assert_close(got[:rows], want, rtol=2 * HALF_BF16, atol=2.0 ** -8)
+        assert not got[rows:].any()

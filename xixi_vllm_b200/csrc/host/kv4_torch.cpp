@@ -249,7 +249,9 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       out.zero_();
       return THPVariable_Wrap(std::move(out));
     }
-    if (np == 0 && nd < T) out.narrow(0, nd, T - nd).zero_();           // rows behind the last sequence; else the chunk kernel's
+    // Rows that are behind the last sequence however long the chunks are; the chunk kernel clears what else there is.
+    const int64_t used = std::min(T, nd + static_cast<int64_t>(np) * mq);
+    if (used < T) out.narrow(0, used, T - used).zero_();
     const auto stream = c10::cuda::getCurrentCUDAStream(c.dev.index()).stream();
     // Workspaces come from torch's allocator, call by call: calls on two streams, or two captured graphs, never share one.
     if (nd > 0) {
@@ -267,7 +269,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       at::Tensor ws;
       if (need > 0) ws = fresh({need}, at::kByte, c.dev);
       check(fn.prefill(q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), tables, cu_q, kv_lens, out.data_ptr(), nd, np, mq,
-                       static_cast<int>(T), hq, hkv, d, c.page, maxb, c.blocks, scale, splits, need > 0 ? ws.data_ptr() : nullptr, need,
+                       static_cast<int>(T), static_cast<int>(used), hq, hkv, d, c.page, maxb, c.blocks, scale, splits, need > 0 ? ws.data_ptr() : nullptr, need,
                        status, stream),
             "kv4_prefill");
     }

@@ -79,7 +79,7 @@ struct Params {
   int* status;
   float* ws_o;                                    // [CTA][split][256 lanes][128] unnormalised outputs, when splits > 1
   float* ws_ml;                                   // [CTA][split][256 lanes][2]: maximum (log2 units), sum
-  int seq_begin, num_seqs, max_q_len, hq, hkv, block_size, max_blocks, num_blocks, total_rows, splits;
+  int seq_begin, num_seqs, max_q_len, clear_to, hq, hkv, block_size, max_blocks, num_blocks, total_rows, splits;
   float scale, sign;                              // of a score, times log2 e: sign * scale * 2^scale_exp, scale in 1 .. 2
   int scale_exp;
   int G, rpu, by_g;                               // heads to a KV head, rows of a unit; 65536 / G + 1: lane / G is a product
@@ -93,7 +93,7 @@ __device__ __forceinline__ bool rows_fine(const Params& p, int q_begin, int q_en
   return q_begin >= p.seq_begin && q_end >= q_begin && q_end <= p.total_rows && q_end - q_begin <= p.max_q_len;
 }
 // Clears 16-byte pieces of output rows: `pieces` from piece `at` on of each row in [from, to), by `workers` threads.
-__device__ __forceinline__ void clear_rows(const Params& p, int from, int to, int at, int pieces, int worker, int workers) {
+__device__ __forceinline__ void clear_rows(const Params& p, int from, int to, int at, int pieces, size_t worker, size_t workers) {
   const size_t row = static_cast<size_t>(p.hq) * (kD / 8), all = from < to ? static_cast<size_t>(to - from) * pieces : 0;
   for (size_t i = worker; i < all; i += workers)
     reinterpret_cast<uint4*>(p.out)[(from + i / pieces) * row + at + i % pieces] = make_uint4(0u, 0u, 0u, 0u);
@@ -370,10 +370,14 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   const int z = p.by_splits(blockIdx.z), split = blockIdx.z - z * p.splits, b = p.seq_begin + z, hk = blockIdx.y;
   const int q_begin = p.cu_q[b], q_end = p.cu_q[b + 1];
   int kv_len = max(p.kv_lens[b], 0);
-  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && (z == 0 || z == p.num_seqs - 1) && split == 0) {      // rows of no chunk
-    const int pieces = p.hq * (kD / 8), threads = blockDim.x;
-    if (z == 0) clear_rows(p, p.seq_begin, min(q_begin, p.total_rows), 0, pieces, threadIdx.x, threads);
-    if (z == p.num_seqs - 1) clear_rows(p, max(max(q_begin, q_end), p.seq_begin), p.total_rows, 0, pieces, threadIdx.x, threads);
+  {                                                          // rows of no chunk: behind the last, by all; before the first
+    const int last = p.seq_begin + p.num_seqs, from = max(max(p.cu_q[last - 1], p.cu_q[last]), p.seq_begin);
+    const size_t block = (static_cast<size_t>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+    if (from < p.clear_to)
+      clear_rows(p, from, p.clear_to, 0, p.hq * (kD / 8), block * blockDim.x + threadIdx.x,
+                 static_cast<size_t>(gridDim.x) * gridDim.y * gridDim.z * blockDim.x);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
+      clear_rows(p, p.seq_begin, min(q_begin, p.total_rows), 0, p.hq * (kD / 8), threadIdx.x, blockDim.x);
   }
   const int q_len = q_end - q_begin;
   if (!rows_fine(p, q_begin, q_end)) {
@@ -992,13 +996,13 @@ long long xv_kv4_prefill_workspace_bytes(int num_seqs, int max_q_len, int hq, in
 }
 
 int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_q,
-                   const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq, int hkv,
+                   const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int clear_to, int hq, int hkv,
                    int d, int block_size, int max_blocks, int num_blocks, float scale, int splits, void* workspace,
                    long long workspace_bytes, int* status, cudaStream_t stream) {
   if (num_seqs <= 0) return 0;
   if (d != kD) return XV_ERR_UNSUPPORTED;
   if (hkv <= 0 || hq <= 0 || hq % hkv || hq / hkv > 16 || block_size <= 0 || block_size % kv4::kUnit || max_blocks <= 0 ||
-      num_blocks <= 0 || hkv > 65535 || splits < 1 || max_q_len < 0 || static_cast<long long>(num_seqs) * splits > 65535)
+      num_blocks <= 0 || hkv > 65535 || splits < 1 || max_q_len < 0 || clear_to > total_rows || static_cast<long long>(num_seqs) * splits > 65535)
     return XV_ERR_SHAPE;
   if (splits > 1 && (!workspace || workspace_bytes < xv_kv4_prefill_workspace_bytes(num_seqs, max_q_len, hq, hkv, splits)))
     return XV_ERR_WORKSPACE;
@@ -1023,7 +1027,8 @@ int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, cons
   p.kv_lens = kv_lens;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.status = status;
-  p.seq_begin = seq_begin; p.num_seqs = num_seqs; p.max_q_len = max_q_len; p.hq = hq; p.hkv = hkv; p.block_size = block_size; p.max_blocks = max_blocks;
+  p.seq_begin = seq_begin; p.num_seqs = num_seqs; p.max_q_len = max_q_len; p.clear_to = clear_to;
+  p.hq = hq; p.hkv = hkv; p.block_size = block_size; p.max_blocks = max_blocks;
   p.num_blocks = num_blocks; p.total_rows = total_rows;
   const double s = scale == 0.f ? 1.0 : std::abs(static_cast<double>(scale)) * kLog2e;
   p.scale = static_cast<float>(2.0 * std::frexp(s, &p.scale_exp));

@@ -230,7 +230,7 @@ int xv_qwen3_forward(const XvModelDesc* m, const XvBatchDesc* b, const XvArena* 
                                  a->attn_ws, a->attn_ws_bytes, a->status, stream));
       if (n_pre > 0)
         XV_TRY(38, xv_kv4_prefill(a->q, w.k_cache, w.v_cache, b->block_tables, b->cu_q, b->kv_lens, a->attn, n_dec, n_pre,
-                                  b->max_q_len, T, m->hq, m->hkv, D, m->block_size, b->max_blocks, m->num_kv_blocks,
+                                  b->max_q_len, T, T, m->hq, m->hkv, D, m->block_size, b->max_blocks, m->num_kv_blocks,
                                   m->attn_scale, splits_pre, a->attn_ws, a->attn_ws_bytes, a->status, stream));
     } else {
       if (n_dec > 0)

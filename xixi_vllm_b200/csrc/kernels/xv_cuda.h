@@ -161,7 +161,7 @@ int xv_kv4_read(const void* k_cache, const void* v_cache, const int* slots, void
                 int d, int block_size, int num_blocks, int* status, cudaStream_t stream);
 // As xv_attn_decode / xv_attn_prefill. Block-table entries outside [0, num_blocks), lengths beyond the table and query
 // ranges that reach beyond total_rows, into the decode rows or over more than max_q_len rows are reported through `status`,
-// never followed: rows of such a range are zeros, and so are the rows behind seq_begin that no chunk names.
+// never followed: rows of such a range are zeros, and so are the rows from seq_begin to clear_to that no chunk names.
 // xv_kv4_decode_splits: 1..8 CTAs per (sequence, KV head), joined inside a cluster, or 0: even shares of all tokens, which
 // need xv_kv4_decode_workspace_bytes(...) bytes.
 int xv_kv4_decode_splits(int num_seqs, int hkv, int num_sms, int max_tokens_per_seq);
@@ -175,7 +175,7 @@ int xv_kv4_decode(const void* q, const void* k_cache, const void* v_cache, const
 int xv_kv4_prefill_splits(int num_seqs, int max_q_len, int hq, int hkv, int max_tokens_per_seq, int num_sms);
 long long xv_kv4_prefill_workspace_bytes(int num_seqs, int max_q_len, int hq, int hkv, int splits);
 int xv_kv4_prefill(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_q,
-                   const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int hq, int hkv,
+                   const int* kv_lens, void* out, int seq_begin, int num_seqs, int max_q_len, int total_rows, int clear_to, int hq, int hkv,
                    int d, int block_size, int max_blocks, int num_blocks, float scale, int splits, void* workspace,
                    long long workspace_bytes, int* status, cudaStream_t stream);
 
