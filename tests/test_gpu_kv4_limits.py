@@ -510,3 +510,30 @@ def test_long_padding_is_cleared():
         _cuda().check_status()
         torch.testing.assert_close(got[:rows], want, rtol=2 * HALF_BF16, atol=2.0 ** -8)
         assert not got[rows:].any()
+
+
+@pytest.mark.parametrize("hq", [4, 6, 16])
+@pytest.mark.parametrize("power", [30, 75])
+@pytest.mark.parametrize("extra_pages", [1, WIDE])
+def test_decode_large_values_without_weight(hq, power, extra_pages):
+    """V of 2^30 and 2^75 at tokens that all heads but one give no weight: those heads see nothing of it, in nor beside their sums."""
+    c = Case([1, 1], [70, 700], hq, 1, n_decode=2, extra_pages=extra_pages, seed=25)
+    for b, k in enumerate(c.k):
+        at = [3, 40] if b == 0 else [5, 330, 331, 650]
+        k[at] = 0.0
+        k[at, :, 0] = -40.0                                  # channel 0 decides: far below for heads with a positive q
+        c.v[b][at] *= 2.0 ** power
+        c.q[b, :, 0] = 100.0
+        c.q[b, 1, 0] = -1.0                                  # and far above for head 1
+        k[[i for i in range(len(k)) if i not in at], :, 0] = 0.0
+    c.check()
+
+
+@pytest.mark.parametrize("hq", [4, 6])
+@pytest.mark.parametrize("extra_pages", [1, WIDE])
+def test_decode_large_values_of_many_tokens(hq, extra_pages):
+    """Sums over 1500 tokens of V of 2^112: scaled sums and centres must stay in fp32."""
+    c = Case([1, 1], [70, 1500], hq, 1, n_decode=2, extra_pages=extra_pages, seed=26)
+    c.q *= 0.1
+    c.v = [(v.abs() + 1) * 2.0 ** 112 for v in c.v]
+    c.check()

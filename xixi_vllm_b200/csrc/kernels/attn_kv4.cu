@@ -245,22 +245,61 @@ struct Query {
 };
 
 // Running state of the softmax over the tokens a warp has seen.
+// How V's steps and P are scaled on their way to fp16. A step is multiplied by vs, one power of two for a warp, to 2^-6 .. 2^-1;
+// saturation leaves that alone and makes NaN 0. (With more than four heads both groups' offsets are one accumulator, where a
+// NaN of one would reach the other; the centre of such a group is NaN as well and stays in its channels.) P is multiplied by
+// 2^k: 2^8, or where steps are far apart each head's own, so that the largest P s of what it gives weight is 4 .. 8: a token that
+// a head gives none does not decide how the others are held. Both cancel at the end.
+struct Scaling {
+  float vs = 0.f, most = 0.f;            // no step yet; steps above `most` need a look: with a P of 2^8 they might leave fp16
+
+  // To a larger step; returns what sums of P * s are to be multiplied by.
+  __device__ __forceinline__ float fit(float step) {
+    if (step == 0.f || (vs != 0.f && step * vs <= 0.5f)) return 1.f;
+    const float now = power_of_two(-min(max((__float_as_int(step) >> 23) - 127 + 6, -112), 126));
+    const float back = vs == 0.f ? 1.f : now / vs;
+    vs = now;
+    return back;
+  }
+  // Whether a slot is more than ordinary: `low`, this lane's smallest step that is not 0, is far below the slot's largest, the
+  // steps so far are, or P is not at 2^8.
+  static __device__ __forceinline__ bool apart(float low, float step, float back, bool other_k) {
+    return __any_sync(0xffffffffu, low * 1024.f < step || back < 0.00390625f || other_k);
+  }
+  // A head's k for a slot whose largest P s and P |c| are given, where the sums so far are multiplied by `shrunk`. Beyond scores
+  // of 2^20 rounding would take its part of it.
+  __device__ __forceinline__ float next_k(float k, float shrunk, float ps, float pc, float score) const {
+    auto ilog = [](float x) { return static_cast<float>((__float_as_int(x) >> 23) - 127); };
+    float to = fminf(k - log2f(shrunk), 90.f);             // what they leave room for
+    if (ps > 0.f) to = fminf(to, 2.f - ilog(ps * vs));
+    if (pc > 0.f) to = fminf(to, 100.f - ilog(pc));        // the centres' sums stay in fp32
+    if (fabsf(score) > 1048576.f) to = fminf(to, 8.f);
+    return fmaxf(floorf(to), 0.f);
+  }
+  __device__ __forceinline__ void limit(float most_k) {
+    if (vs != 0.f) most = exp2f(fminf(-1.f, 7.f - most_k)) / vs;
+  }
+  __device__ __forceinline__ float back() const { return vs == 0.f ? 0.f : 1.f / vs; }
+};
+// |s| and |c| of a parameter word; its step as a candidate for the smallest that is not 0.
+__device__ __forceinline__ float low_s(uint32_t w) { return (w & 0x7fffu) == 0u ? CUDART_INF_F : fabsf(kv4::par_s(w)); }
+__device__ __forceinline__ float abs_s(uint32_t w) { return fabsf(kv4::par_s(w)); }
+__device__ __forceinline__ float abs_c(uint32_t w) { return fabsf(kv4::par_c(w)); }
+
 template <int NT>
 struct Softmax {
   float o[NT][2][4][4];            // [group][MMA]: rows g, g + 8 = channels 16 g + 8 group + 2 i + {0, 1}; heads 2t, 2t+1
   float cen[NT][2][2];             // sum of P * centre, this lane's tokens
   float off[NT][4];                // sum of -8 P * s, rounded as it is in o: group 0 (heads 2t, 2t + 1), group 1
   float m[NT][2], l[NT][2];        // running maximum of the products (may lag), sum of P of this lane's tokens
-  // Power of two that V's scales are multiplied by; the largest scale that it allows. Scaled they are 2^-6 to 2^-1 (and P 2^8
-  // times what it is, which cancels), so that saturation leaves them alone and makes NaN 0: both groups' offsets are one
-  // accumulator, where a NaN of one would reach the other. The centre of such a group is NaN too and stays in its channels.
-  float vs, v_most;
+  float k[NT][2];
+  Scaling v;
 
   __device__ __forceinline__ void clear() {
-    vs = 1.f;
-    v_most = 0.f;
+    v = Scaling();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      k[nt][0] = k[nt][1] = 8.f;
 #pragma unroll
       for (int gr = 0; gr < 2; ++gr) {
 #pragma unroll
@@ -332,7 +371,7 @@ struct Softmax {
 #pragma unroll
       for (int r = 0; r < 2; ++r) s_most = fmaxf(s_most, fmaxf(fabsf(kv4::par_s(vp[u][r].x)), fabsf(kv4::par_s(vp[u][r].y))));
     }
-    bool grow = s_most > v_most;
+    bool grow = s_most > v.most;
     float mx[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -342,17 +381,19 @@ struct Softmax {
         grow |= (mx[nt][hd] - m[nt][hd]) * q.power[nt][hd] > kLazy;
       }
     if (__any_sync(0xffffffffu, grow)) {
-      float back = 1.f;                  // of the sums of P * s
       s_most = fmaxf(s_most, __shfl_xor_sync(0xffffffffu, s_most, 4));
       s_most = fmaxf(s_most, __shfl_xor_sync(0xffffffffu, s_most, 8));
       s_most = fmaxf(s_most, __shfl_xor_sync(0xffffffffu, s_most, 16));
-      if (s_most > v_most) {
-        const int e = min(max((__float_as_int(s_most) >> 23) - 127 + 6, -112), 126);
-        const float now = power_of_two(-e);
-        back = now / vs;
-        vs = now;
-        v_most = power_of_two(e - 1);
-      }
+      const float back = v.fit(s_most);
+      float low = CUDART_INF_F, shrunk[NT][2];
+      bool other_k = false;
+#pragma unroll
+      for (int u = 0; u < kPair; ++u)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) low = fminf(low, fminf(low_s(vp[u][r].x), low_s(vp[u][r].y)));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) other_k |= k[nt][0] != 8.f || k[nt][1] != 8.f;
+      const bool apart = Scaling::apart(low, s_most, back, other_k);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -363,6 +404,7 @@ struct Softmax {
           mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 16));
           const float cr = exp2f((m[nt][hd] - mn) * q.power[nt][hd]);
           m[nt][hd] = mn;
+          shrunk[nt][hd] = cr * back;
           l[nt][hd] *= cr;
 #pragma unroll
           for (int gr = 0; gr < 2; ++gr) {
@@ -375,6 +417,44 @@ struct Softmax {
             }
           }
         }
+      float most_k = 8.f;
+      if (__builtin_expect(apart, false)) {
+        most_k = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int hd = 0; hd < 2; ++hd) {
+            float ps = 0.f, pc = 0.f;
+#pragma unroll
+            for (int u = 0; u < kPair; ++u)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const float pr = exp2f((x[u][nt][2 * r + hd] - m[nt][hd]) * q.power[nt][hd]);
+                ps = fmaxf(ps, pr * fmaxf(abs_s(vp[u][r].x), abs_s(vp[u][r].y)));
+                pc = fmaxf(pc, pr * fmaxf(abs_c(vp[u][r].x), abs_c(vp[u][r].y)));
+              }
+#pragma unroll
+            for (int d = 4; d <= 16; d <<= 1) {
+              ps = fmaxf(ps, __shfl_xor_sync(0xffffffffu, ps, d));
+              pc = fmaxf(pc, __shfl_xor_sync(0xffffffffu, pc, d));
+            }
+            const float to = v.next_k(k[nt][hd], shrunk[nt][hd], ps, pc, m[nt][hd] * q.power[nt][hd]), up = exp2f(to - k[nt][hd]);
+            k[nt][hd] = to;
+            most_k = fmaxf(most_k, to);
+            l[nt][hd] *= up;
+#pragma unroll
+            for (int gr = 0; gr < 2; ++gr) {
+              cen[nt][gr][hd] *= up;
+              off[nt][2 * gr + hd] *= up;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                o[nt][gr][j][hd] *= up;
+                o[nt][gr][j][2 + hd] *= up;
+              }
+            }
+          }
+      }
+      v.limit(most_k);
     }
 #pragma unroll
     for (int u = 0; u < kPair; ++u) {
@@ -389,7 +469,7 @@ struct Softmax {
 #pragma unroll
         for (int gr = 0; gr < 2; ++gr) {
           const uint32_t w = gr ? vp[u][r].y : vp[u][r].x;
-          vsc[gr][r] = __saturatef(kv4::par_s(w) * vs);
+          vsc[gr][r] = __saturatef(kv4::par_s(w) * v.vs);
           vce[gr][r] = kv4::par_c(w);
         }
       uint32_t pf[NT][2][2];             // P * s_g as the B operand of the second product
@@ -397,7 +477,7 @@ struct Softmax {
       for (int nt = 0; nt < NT; ++nt) {
         float pr[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][nt][e], q.power[nt][e & 1], fmaf(-m[nt][e & 1], q.power[nt][e & 1], 8.f)));
+        for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][nt][e], q.power[nt][e & 1], fmaf(-m[nt][e & 1], q.power[nt][e & 1], k[nt][e & 1])));
         l[nt][0] += pr[0] + pr[2];
         l[nt][1] += pr[1] + pr[3];
 #pragma unroll
@@ -429,11 +509,15 @@ struct Softmax {
   // Sums over the lanes of equal t; the centres join the outputs, the maximum turns to log2 units. Then every lane holds, for
   // its two heads, 16 channels.
   __device__ __forceinline__ void finish(const Query<NT, false>& q) {
-    const float back = 1.f / vs;
+    const float back = v.back();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int hd = 0; hd < 2; ++hd) {
+        const float down = exp2f(-k[nt][hd]);
+        l[nt][hd] *= down;
+        cen[nt][0][hd] *= down;
+        cen[nt][1][hd] *= down;
 #pragma unroll
         for (int x = 4; x <= 16; x <<= 1) {
           l[nt][hd] += __shfl_xor_sync(0xffffffffu, l[nt][hd], x);
@@ -444,8 +528,8 @@ struct Softmax {
         for (int gr = 0; gr < 2; ++gr)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            o[nt][gr][i][hd] = fmaf(fmaf(o[nt][gr][i][hd], 1048576.f, off[nt][2 * gr + hd]), back, cen[nt][gr][hd]);      // n 2^-20
-            o[nt][gr][i][2 + hd] = fmaf(fmaf(o[nt][gr][i][2 + hd], 1048576.f, off[nt][2 * gr + hd]), back, cen[nt][gr][hd]);
+            o[nt][gr][i][hd] = fmaf(fmaf(o[nt][gr][i][hd], 1048576.f, off[nt][2 * gr + hd]) * down, back, cen[nt][gr][hd]);      // n 2^-20
+            o[nt][gr][i][2 + hd] = fmaf(fmaf(o[nt][gr][i][2 + hd], 1048576.f, off[nt][2 * gr + hd]) * down, back, cen[nt][gr][hd]);
           }
         m[nt][hd] = m[nt][hd] == kNoMax ? kNoMax : m[nt][hd] * q.power[nt][hd];
       }
@@ -471,11 +555,12 @@ struct TwinSoftmax {
   float o[2][4][4];                // as Softmax::o; valid where [group] is the lane's own
   float cen[2], off[4];            // of the lane's group
   float m[2], l[2];
-  float vs, v_most;
+  float k[2];
+  Scaling v;
 
   __device__ __forceinline__ void clear() {
-    vs = 1.f;
-    v_most = 0.f;
+    v = Scaling();
+    k[0] = k[1] = 8.f;
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr)
 #pragma unroll
@@ -539,7 +624,7 @@ struct TwinSoftmax {
 #pragma unroll
       for (int r = 0; r < 2; ++r) s_most = fmaxf(s_most, fabsf(kv4::par_s(vp[u][r])));
     }
-    bool grow = s_most > v_most;
+    bool grow = s_most > v.most;
     float mx[2];
 #pragma unroll
     for (int hd = 0; hd < 2; ++hd) {
@@ -547,16 +632,12 @@ struct TwinSoftmax {
       grow |= (mx[hd] - m[hd]) * q.power[0][hd] > kLazy;
     }
     if (__any_sync(0xffffffffu, grow)) {
-      float back = 1.f;                                  // of the sums of P * s
 #pragma unroll
       for (int d = 2; d <= 16; d <<= 1) s_most = fmaxf(s_most, __shfl_xor_sync(0xffffffffu, s_most, d));
-      if (s_most > v_most) {
-        const int e = min(max((__float_as_int(s_most) >> 23) - 127 - 2, -120), 119);
-        const float now = power_of_two(-e);
-        back = now / vs;
-        vs = now;
-        v_most = power_of_two(e + 7);
-      }
+      const float back = v.fit(s_most);
+      float shrunk[2];
+      const float low = fminf(fminf(low_s(vp[0][0]), low_s(vp[0][1])), fminf(low_s(vp[1][0]), low_s(vp[1][1])));
+      const bool apart = Scaling::apart(low, s_most, back, k[0] != 8.f || k[1] != 8.f);
 #pragma unroll
       for (int hd = 0; hd < 2; ++hd) {
         float mn = fmaxf(m[hd], mx[hd]);
@@ -565,6 +646,7 @@ struct TwinSoftmax {
         mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 16));
         const float cr = exp2f((m[hd] - mn) * q.power[0][hd]);
         m[hd] = mn;
+        shrunk[hd] = cr * back;
         l[hd] *= cr;
         cen[hd] *= cr;
         off[hd] *= cr * back;
@@ -576,6 +658,41 @@ struct TwinSoftmax {
             o[gr][j][2 + hd] *= cr * back;
           }
       }
+      float most_k = 8.f;
+      if (__builtin_expect(apart, false)) {
+        most_k = 0.f;
+#pragma unroll
+        for (int hd = 0; hd < 2; ++hd) {
+          float ps = 0.f, pc = 0.f;
+#pragma unroll
+          for (int u = 0; u < kPair; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float pr = exp2f((x[u][2 * r + hd] - m[hd]) * q.power[0][hd]);
+              ps = fmaxf(ps, pr * abs_s(vp[u][r]));
+              pc = fmaxf(pc, pr * abs_c(vp[u][r]));
+            }
+#pragma unroll
+          for (int d = 2; d <= 16; d <<= 1) {              // the two groups of a head are of one k: their lanes share l
+            ps = fmaxf(ps, __shfl_xor_sync(0xffffffffu, ps, d));
+            pc = fmaxf(pc, __shfl_xor_sync(0xffffffffu, pc, d));
+          }
+          const float to = v.next_k(k[hd], shrunk[hd], ps, pc, m[hd] * q.power[0][hd]), up = exp2f(to - k[hd]);
+          k[hd] = to;
+          most_k = fmaxf(most_k, to);
+          l[hd] *= up;
+          cen[hd] *= up;
+          off[hd] *= up;
+#pragma unroll
+          for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o[gr][j][hd] *= up;
+              o[gr][j][2 + hd] *= up;
+            }
+        }
+      }
+      v.limit(most_k);
     }
 #pragma unroll
     for (int u = 0; u < kPair; ++u) {
@@ -586,10 +703,10 @@ struct TwinSoftmax {
       vw[3] = *reinterpret_cast<const uint2*>(lane_v1 + u * kUnitSlot + 8 * 64);
       float pr[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][e], q.power[0][e & 1], -m[e & 1] * q.power[0][e & 1]));
+      for (int e = 0; e < 4; ++e) pr[e] = exp2f(fmaf(x[u][e], q.power[0][e & 1], fmaf(-m[e & 1], q.power[0][e & 1], k[e & 1])));
       l[0] += pr[0] + pr[2];
       l[1] += pr[1] + pr[3];
-      const float v0 = kv4::par_s(vp[u][0]) * vs, v1 = kv4::par_s(vp[u][1]) * vs;
+      const float v0 = kv4::par_s(vp[u][0]) * v.vs, v1 = kv4::par_s(vp[u][1]) * v.vs;
       const float c0 = kv4::par_c(vp[u][0]), c1 = kv4::par_c(vp[u][1]);
       const uint32_t p0 = movmatrix_trans(pack_f16(pr[0] * v0, pr[1] * v0)), p1 = movmatrix_trans(pack_f16(pr[2] * v1, pr[3] * v1));
       cen[0] = fmaf(pr[0], c0, fmaf(pr[2], c1, cen[0]));
@@ -611,9 +728,12 @@ struct TwinSoftmax {
   }
 
   __device__ __forceinline__ void finish(const Query<1, true>& q) {
-    const float back = 1.f / vs;
+    const float back = v.back();
 #pragma unroll
     for (int hd = 0; hd < 2; ++hd) {
+      const float down = exp2f(-k[hd]);
+      l[hd] *= down;
+      cen[hd] *= down;
 #pragma unroll
       for (int x = 4; x <= 16; x <<= 1) {
         l[hd] += __shfl_xor_sync(0xffffffffu, l[hd], x);
@@ -623,8 +743,8 @@ struct TwinSoftmax {
       for (int gr = 0; gr < 2; ++gr)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          o[gr][i][hd] = fmaf(fmaf(o[gr][i][hd], 1048576.f, off[hd]), back, cen[hd]);                    // n 2^-20
-          o[gr][i][2 + hd] = fmaf(fmaf(o[gr][i][2 + hd], 1048576.f, off[hd]), back, cen[hd]);
+          o[gr][i][hd] = fmaf(fmaf(o[gr][i][hd], 1048576.f, off[hd]) * down, back, cen[hd]);             // n 2^-20
+          o[gr][i][2 + hd] = fmaf(fmaf(o[gr][i][2 + hd], 1048576.f, off[hd]) * down, back, cen[hd]);
         }
       m[hd] = m[hd] == kNoMax ? kNoMax : m[hd] * q.power[0][hd];
     }
