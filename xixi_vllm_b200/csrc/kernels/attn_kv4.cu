@@ -21,10 +21,12 @@
 //   kv4_join_kernel      partial results of pairs that span runs joined by a second kernel.
 // Prompt chunks: attn_prefill_kv4_sm100.cu.
 //
-// What bounds it: instructions, not memory: 293 of them for the 2304 bytes of 16 tokens of a head (271 for groups of up to
-// four query heads, whose columns hold both channel groups: 256 sequences 137 -> 129 us, 32 11.7 -> 11.4), 104 of which
-// take the codes apart. 96 sequences of 2048 tokens, 32 / 8 heads: 57% of the issue slots, 52% of the ALU, 30% of the tensor
-// pipe, 4.3 TB/s. 256 sequences of 256-4096 tokens 128 us (5.1 TB/s), one of 40960 (64 / 8 heads) 19.8 us (2.4 TB/s). On the way:
+// What bounds it: instructions, not memory: 275 of them for the 2304 bytes of 16 tokens of a head (some 20 more for groups of
+// more than four query heads; up to four have columns for both channel groups: 256 sequences 137 -> 129 us, 32 11.7 -> 11.4),
+// 104 of which take the codes apart. 96 sequences of 2048 tokens, 32 / 8 heads: 58% of the issue slots, 52% of the ALU, 30%
+// of the tensor pipe, 4.2 TB/s. 256 sequences of 256-4096 tokens 147 us in a stream (4.4 TB/s), 139 with L2 flushed, 129 in
+// a graph, whose passes find part of the cache in L2; one of 40960 (64 / 8 heads) 22.1 us in a stream, 27.7 with L2 flushed
+// (1.7 TB/s). Groups of 16 heads: 32 sequences of 128-1280 18.2 us (128 / 8 heads), 256 215. On the way:
 // codes as bf16 integers with shifts and a subtraction 333 instructions and 153 us, a unit at a time 424 and 189, bulk copies
 // in place of cp.async 241. 128 registers, for four CTAs an SM, spill: 149 us. Small batches are a chain of dependent
 // reads (length and page, codes), about 2500 cycles before the first product.

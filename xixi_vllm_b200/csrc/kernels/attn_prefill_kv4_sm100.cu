@@ -15,9 +15,11 @@
 // What bounds it: the chain of one unit, S -> softmax -> P -> O += P V -> next S, about 4100 cycles a tile of 128 tokens, of
 // which 1590 are the exponentials (1024 of MUFU), 840 S's way through tensor memory and the maximum, 1030 the two MMAs and
 // the rest hand-over; the other unit's exponentials lie in between. Both units' MMAs are 2050 of it. Beside them the
-// dequantisers' loop (770 instructions a warp) takes as long when all SMs are busy. 4 x 2048 rows behind 512 tokens, 32
-// query heads: 261 us, 790 TFLOP/s. On the way: Q loaded by the lanes that convert it 285; then, at 273 with these
-// registers, 277 with 2 x 184 + 96 + 48, 286 with 2 x 192 + 80 + 48, 287 with 2 x 168 + 112 + 64.
+// dequantisers' loop takes as long when all SMs are busy. (Stamps of an earlier step, 261 us; powers for every row, and for
+// tokens where they are far apart, took it to 271.) 4 x 2048 rows behind 512 tokens, 32 query heads: 280 us in a stream, 271 in
+// a graph, 737 and 760 TFLOP/s; 737 us if every tile is one whose tokens have powers of their own. On the way: Q loaded by the
+// lanes that convert it 285; then, at 273 with these registers, 277 with 2 x 184 + 96 + 48, 286 with 2 x 192 + 80 + 48, 287
+// with 2 x 168 + 112 + 64.
 //
 // fp16 operands, not bf16: a dequantised value c + s (n - 8) has more than bf16's 8 bits, and its rounding (2^-12 instead
 // of 2^-9) would otherwise be the largest error of the result. Their range is kept by powers of two: a row of Q is scaled
@@ -172,7 +174,8 @@ __device__ __forceinline__ float fma_whole(float a, float b, float c) {
 // A group's parameters as fp16 pairs, the tile's power of two taken out.
 struct Pair {
   __half2 s, c;
-  __device__ __forceinline__ Pair(uint32_t w, float f) : s(__float2half2_rn(kv4::par_s(w) * f)), c(__float2half2_rn(mul_whole(kv4::par_c(w), f))) {}
+  __device__ __forceinline__ Pair(uint32_t w, float f)
+      : s(__float2half2_rn(kv4::par_s(w) * f)), c(__float2half2_rn(mul_whole(kv4::par_c(w), f))) {}
 };
 
 // 16 of a row's 64 code bytes as fp16 c + s (n - 8) into chunks c0 .. c0 + 3: words of even index belong to group 0.
@@ -341,7 +344,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wg = warp >> 2;
 
-  // Under the launch before: the barriers. (Tensor memory waits until that launch has ended: it may want all of it.)
+  // Before the wait for the launch before: the barriers, under what is left of launch latency (the trigger that would let blocks
+  // start earlier is compiled out, ptx.cuh). Tensor memory comes after it: that launch may want all of it.
   grid_dep_launch();
   if (threadIdx.x == 0) {
     for (int u = 0; u < 2; ++u) {
@@ -504,7 +508,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const uint32_t flags = out.x | out.y | out.z | out.w;
       if (flags & 1u) break;
       bool own = flags & 2u;
-      const int ek_new = choose(ek, max(max(k4.x, k4.y), max(k4.z, k4.w))), ev_new = choose(ev, max(max(v4.x, v4.y), max(v4.z, v4.w)));
+      const int ek_new = choose(ek, max(max(k4.x, k4.y), max(k4.z, k4.w)));
+      const int ev_new = choose(ev, max(max(v4.x, v4.y), max(v4.z, v4.w)));
       if (ek_new != ek || ev_new != ev) {                    // alike in the four warps: look again, in the new units
         ek = ek_new;
         ev = ev_new;
@@ -650,9 +655,10 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
     const int by_g = p.by_g, row = row0 + u * rpu + ((r * by_g) >> 16);
     const int pos = pos0 + min(row, q_len - 1);              // lanes without a row follow the last one
     // Q: a power of two per row (and head) takes its largest element to 2^14 .. 2^15 of fp16, which is exact down to 2^-31 of
-    // it; the scale's sign is Q's, and a scale of 0 a Q of 0. A unit's rows of all its heads are contiguous in memory row by row; bulk copies bring them
-    // into a K slot that is free until tile 1 + u. All four warps send their share: a copy takes its warp 67 cycles (one warp
-    // for all of them 2160; loads by the lanes that convert 3500). Sixteen lanes convert a row, two rows at a time.
+    // it; the scale's sign is Q's, and a scale of 0 a Q of 0. A unit's rows of all its heads are contiguous in memory row by
+    // row; bulk copies bring them into a K slot that is free until tile 1 + u. All four warps send their share: a copy takes
+    // its warp 67 cycles (one warp for all of them 2160; loads by the lanes that convert 3500). Sixteen lanes convert a row,
+    // two rows at a time.
     int q_exp = 0;
     {
       const uint32_t bytes = static_cast<uint32_t>(G) * kD * 2;
@@ -675,8 +681,9 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       // Largest magnitude of each row, rows i and i + 8 in one word; then sixteen lanes' words in steps that halve what a lane
       // keeps, so that lanes 2k and 2k + 1 of a half warp end with rows k and k + 8.
       auto top_of = [](const uint4& r) {
-        const uint32_t m2 = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
-        return max(m2 >> 16, m2 & 0xffffu);
+        const uint32_t a = __vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu), b = __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu);
+        const uint32_t two = __vmaxu2(a, b);
+        return max(two >> 16, two & 0xffffu);
       };
       uint32_t tops[8], any = 0u;
 #pragma unroll
@@ -831,7 +838,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       const size_t slot = (((static_cast<size_t>(z) * gridDim.y + hk) * gridDim.x + blockIdx.x) * p.splits + split) *
                               (2 * kBM) + u * kBM + r;
       *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(st.mantissa == p.scale ? st.m : st.m * p.scale, st.l);
-      const float vf0 = pos >= first_bad[0] ? CUDART_NAN_F : pow2(st.unit_v), vf1 = pos >= first_bad[1] ? CUDART_NAN_F : pow2(st.unit_v);
+      const float vf0 = pos >= first_bad[0] ? CUDART_NAN_F : pow2(st.unit_v);
+      const float vf1 = pos >= first_bad[1] ? CUDART_NAN_F : pow2(st.unit_v);
       // Through the unit's Q tile (all its MMAs are over) half the channels at a time, so that the writes are whole lines. A
       // split without tiles leaves no output, only m = kNoMax, l = 0.
       const uint32_t tile = smem_u32(q_s) + u * kTileBytes;
@@ -869,7 +877,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prefill_tc_kernel(const Params p) 
       }
     } else if (ok) {
       tc_fence_after_sync();
-      const float vf0 = pos >= first_bad[0] ? CUDART_NAN_F : pow2(st.unit_v), vf1 = pos >= first_bad[1] ? CUDART_NAN_F : pow2(st.unit_v);
+      const float vf0 = pos >= first_bad[0] ? CUDART_NAN_F : pow2(st.unit_v);
+      const float vf1 = pos >= first_bad[1] ? CUDART_NAN_F : pow2(st.unit_v);
       const float inv = st.l == 0.f ? 0.f : 1.f / st.l;            // times 2^unit_v it may leave fp32: small values, many tokens
       // Rows leave through the unit's Q tile (all its MMAs are over), so that the writes are whole lines.
       const uint32_t at = row_start(smem_u32(q_s) + u * kTileBytes, r);

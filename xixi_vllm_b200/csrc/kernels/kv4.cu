@@ -7,13 +7,14 @@
 //   kv4_read_kernel  - the bf16 values of a list of slots. A warp per token.
 //
 // Both should be bound by memory: the writer moves (hq + 2 hkv) 256 + hq 256 + hkv 144 bytes a token, the reader
-// hkv 2 (72 + 256). The writer is as much bound by its instructions (3500 a token of 32 + 2 x 8 heads, 67% of the issue
-// slots): 8192 tokens 41.0 us (4.3 TB/s; with one pair sent for ahead in registers 48.5), 997 of 40 + 2 x 8 7.0 us.
-// The reader runs at the copy rate: 32768 tokens of 8 heads 26.1 us (6.6 TB/s).
+// hkv 2 (72 + 256). The writer is as much bound by its instructions (3600 a token of 32 + 2 x 8 heads, 66% of the issue
+// slots): 8192 tokens 42 us (4.2 TB/s; with one pair sent for ahead in registers 48.5), 997 of 40 + 2 x 8 7.1 us; from four
+// split-K planes 32 tokens 2.9 us. The reader: 32768 tokens of 8 heads 30.2 us in a stream (5.7 TB/s) and 34.8 with L2
+// flushed; 26.2 in a graph, where the 38 MB that it reads stay in L2.
 //
 // Quantising is a choice between 16 levels, so K is normalised and rotated in 64 bits from the fp32 row: a value next
-// to a border between two levels then falls the same way wherever the row is computed (five double operations a channel,
-// for the K heads only).
+// to a border between two levels then falls the same way wherever the row is computed (five double operations a channel and
+// their conversions, for the K heads only).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -385,7 +386,7 @@ kv4_read_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__
   const uint8_t* par = unit + kv4::kParBase + (place % kv4::kUnit) * kv4::kParRow + (c & 1) * 4;
   const size_t head_bytes = static_cast<size_t>(block_size / kv4::kUnit) * kv4::kUnitBytes;
   // Eight rows' reads in flight, then four, then one. The values leave L2 first: nothing here reads them again. 32768 tokens of
-  // 8 heads take 26.1 us; with plain stores 29.7, with four rows in flight 26.9, with both 32.0.
+  // 8 heads in a graph take 26.1 us; with plain stores 29.7, with four rows in flight 26.9, with both 32.0.
   int h = 0;
   auto rows = [&](auto n) {
     constexpr int N = decltype(n)::value;
