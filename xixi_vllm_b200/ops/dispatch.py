@@ -101,7 +101,8 @@ def paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads,
     """``attn`` is a ``runtime.staging.AttnBatch`` (cu_q, kv_lens, block_tables, decode split). The caches are bf16
     pages or, as uint8, pages held in 4 bits (``ops.kv4``). On a 4-bit cache rows of ``q`` that no sequence names, rows of
     a sequence without cached tokens and rows before position 0 come out as zeros; ``scale`` is finite. On the GPU a chunk
-    that is longer than ``attn.max_q_len`` or reaches beyond ``q`` is reported through the status word and is zeros."""
+    that is longer than ``attn.max_q_len`` or reaches beyond ``q`` is reported through the status word and is zeros. Finite
+    values of any size are taken; a row with a score beyond fp32 is NaN."""
     if q.is_cuda:
         return _cuda().paged_attention(q, k_cache, v_cache, attn, scale, num_q_heads, num_kv_heads, head_dim)
     if kv4.is_kv4(k_cache) or kv4.is_kv4(v_cache):
